@@ -1,4 +1,5 @@
-"""ctypes binding of ``libmarathon_kvshift.so`` (C ABI: include/marathon_kvshift.h).
+"""ctypes binding of ``libmarathon_kvshift.so`` (C ABI: include/marathon_kvshift.h and
+include/marathon_kvscaled.h).
 
 The library is built in-tree by :func:`marathon_amd.build.build_library` and loaded
 from ``marathon_amd/_lib/``.  There is deliberately no fallback: if the library is
@@ -49,6 +50,9 @@ MKV_ABI_VERSION = (3 << 16) | 5
 MKV_ORDER_NONE = 0
 MKV_ORDER_DST_PAGE = 1
 MKV_NOALLOC_SCRATCH_BYTES = 16 << 20
+MKV_SCALE_MIN_EXP = -100
+MKV_SCALE_MAX_EXP = 100
+MKV_MAX_REQUESTS = 4096
 
 ERROR_NAMES = {
     MKV_ERR_ARG: "MKV_ERR_ARG",
@@ -70,6 +74,11 @@ EXPORTED = (
     "mkv_rope_tables",
     "mkv_last_error",
     "mkv_abi_version",
+    "mkv_step_slots",
+    "mkv_store_scaled",
+    "mkv_attend_scaled",
+    "mkv_attend_workspace_size",
+    "mkv_shift_scaled",
 )
 
 
@@ -154,6 +163,82 @@ class ShiftDesc(ctypes.Structure):
 assert ctypes.sizeof(Side) == 88 and ctypes.sizeof(ShiftDesc) == 288
 
 
+class ScaledCacheDesc(ctypes.Structure):
+    """mkv_scaled_cache_t (72 bytes)."""
+
+    _fields_ = [
+        ("k_base", ctypes.c_void_p),
+        ("v_base", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("num_blocks", ctypes.c_int64),
+        ("block_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("token_stride", ctypes.c_int64),
+        ("block_size", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("head_size", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class AttendDesc(ctypes.Structure):
+    """mkv_attend_desc_t (216 bytes)."""
+
+    _fields_ = [
+        ("cache", ScaledCacheDesc),
+        ("q", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("block_tables", ctypes.c_void_p),
+        ("starts", ctypes.c_void_p),
+        ("lens", ctypes.c_void_p),
+        ("error_flags", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+        ("q_token_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("out_token_stride", ctypes.c_int64),
+        ("out_head_stride", ctypes.c_int64),
+        ("table_stride", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        ("table_width", ctypes.c_int32),
+        ("requests", ctypes.c_int32),
+        ("q_heads", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("max_new", ctypes.c_int32),
+        ("max_len", ctypes.c_int32),
+        ("softmax_scale", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class ScaledShiftDesc(ctypes.Structure):
+    """mkv_scaled_shift_desc_t (248 bytes)."""
+
+    _fields_ = [
+        ("src", ScaledCacheDesc),
+        ("dst", ScaledCacheDesc),
+        ("src_layers", ctypes.c_void_p),
+        ("dst_layers", ctypes.c_void_p),
+        ("spans", ctypes.c_void_p),
+        ("unit_starts", ctypes.c_void_p),
+        ("tables", ctypes.c_void_p),
+        ("src_table", ctypes.c_void_p),
+        ("dst_table", ctypes.c_void_p),
+        ("error_flags", ctypes.c_void_p),
+        ("src_table_len", ctypes.c_int64),
+        ("dst_table_len", ctypes.c_int64),
+        ("units", ctypes.c_int64),
+        ("n_spans", ctypes.c_int32),
+        ("layers", ctypes.c_int32),
+        ("rotary", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+assert ctypes.sizeof(ScaledCacheDesc) == 72 and ctypes.sizeof(AttendDesc) == 216
+assert ctypes.sizeof(ScaledShiftDesc) == 248
+
+
 class KVShiftError(RuntimeError):
     """A non-MKV_OK status from the library."""
 
@@ -184,6 +269,22 @@ def _bind(cdll: ctypes.CDLL) -> ctypes.CDLL:
     f = cdll.mkv_rope_tables
     f.restype = ctypes.c_int
     f.argtypes = [vp, i32, vp, i32, vp]
+    f = cdll.mkv_step_slots
+    f.restype = ctypes.c_int
+    f.argtypes = [vp, vp, i32, vp, i64, i32, vp, i64, vp, i32, vp, vp, vp, vp, i64, vp, vp, vp]
+    f = cdll.mkv_store_scaled
+    f.restype = ctypes.c_int
+    f.argtypes = [ctypes.POINTER(ScaledCacheDesc), vp, i64, i64, vp, i64, i64, i64, i32, vp, i64,
+                  i32, vp, vp, i32, vp, vp]
+    f = cdll.mkv_attend_scaled
+    f.restype = ctypes.c_int
+    f.argtypes = [ctypes.POINTER(AttendDesc), vp]
+    f = cdll.mkv_attend_workspace_size
+    f.restype = ctypes.c_int64
+    f.argtypes = [ctypes.POINTER(AttendDesc)]
+    f = cdll.mkv_shift_scaled
+    f.restype = ctypes.c_int
+    f.argtypes = [ctypes.POINTER(ScaledShiftDesc), vp]
     cdll.mkv_last_error.restype = ctypes.c_char_p
     cdll.mkv_last_error.argtypes = []
     cdll.mkv_abi_version.restype = ctypes.c_int32

@@ -1,7 +1,7 @@
 """In-tree build of the HIP library (gfx950 only) and of its CPython binding.
 
 ``python -m marathon_amd.build`` (or ``__graft_entry__.build()``) compiles
-``csrc/kvshift.hip`` into ``_lib/libmarathon_kvshift.so`` with hipcc.  It always
+the sources of ``csrc`` (:data:`SRCS`) into ``_lib/libmarathon_kvshift.so`` with hipcc.  It always
 recompiles: the build is a few seconds and a stale library is worse than a slow one.
 :func:`build_binding` compiles ``csrc/binding.cpp``, the per-layer call's path from torch
 tensors, into ``_lib/marathon_binding.so`` with g++.
@@ -20,6 +20,8 @@ import sysconfig
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 SRC = os.path.join(HERE, "csrc", "kvshift.hip")
+#: The library's sources: the shift path, and the block-scaled cache's kernels.
+SRCS = [SRC, *(os.path.join(HERE, "csrc", n) for n in ("scaled_cache.hip", "scaled_attend.hip"))]
 INCLUDE = os.path.join(ROOT, "include")
 OUT_DIR = os.path.join(HERE, "_lib")
 OUT = os.path.join(OUT_DIR, "libmarathon_kvshift.so")
@@ -57,11 +59,12 @@ def hipcc() -> str:
     raise RuntimeError("hipcc not found (expected /opt/rocm/bin/hipcc)")
 
 
-def _compile(src: str, out: str, verbose: bool, extra: list | None = None) -> str:
+def _compile(src: str | list, out: str, verbose: bool, extra: list | None = None) -> str:
     os.makedirs(os.path.dirname(out), exist_ok=True)
     tmp = out + ".tmp"
+    srcs = [src] if isinstance(src, str) else src
     cmd = [hipcc(), *HIPCC_FLAGS, *(extra or []), f"-I{INCLUDE}",
-           f"-I{os.path.join(HERE, 'csrc')}", src, "-o", tmp]
+           f"-I{os.path.join(HERE, 'csrc')}", *srcs, "-o", tmp]
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
@@ -89,7 +92,7 @@ def build_library(verbose: bool = False) -> str:
     for d in extra:
         if not d[2:].startswith("MKV_"):
             raise ValueError(f"{DEFINES_ENV}: {d[2:]!r} is not an MKV_ tuning knob")
-    out = _compile(SRC, OUT, verbose, extra)
+    out = _compile(SRCS, OUT, verbose, extra)
     # beside the library, what it was built with (bench.py reports it)
     with open(DEFINES_FILE, "w") as f:
         f.write(" ".join(d[2:] for d in extra) + "\n")

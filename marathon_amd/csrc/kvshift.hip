@@ -2084,6 +2084,15 @@ int scratch_of(hipStream_t st, void** out) {
 
 extern "C" const char* mkv_last_error(void) { return g_err; }
 
+// The library's other sources record their errors here too.
+__attribute__((visibility("hidden"))) int mkv_fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof g_err, fmt, ap);
+  va_end(ap);
+  return code;
+}
+
 extern "C" int32_t mkv_abi_version(void) { return MKV_ABI_VERSION; }
 
 extern "C" int mkv_rope_tables(const int32_t* deltas, int32_t n_spans, const float* inv_freq,

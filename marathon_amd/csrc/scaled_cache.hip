@@ -1,0 +1,709 @@
+// scaled_cache.hip -- the block-scaled 8-bit cache's slots, store and shift for gfx950.
+//
+// None of the three has matrix work; each reads its input once and writes its output once.
+//
+//   * step_slots: a handful of integers a request and 12 bytes a token.  Bound by latency, so
+//     it is one launch: every workgroup makes the prefix sums of all requests for itself in
+//     LDS (a few thousand requests at most) instead of waiting for a launch that does.
+//   * store and shift: one wave holds 16 rows of one (block, KV head) in registers, 16 values
+//     of K and of V a lane, so that a block's largest value is known before its first code is
+//     written and nothing is read twice.  A lane's 16 values are 16 bytes of codes: every
+//     cache access moves 16 bytes a lane.  Blocks of 32 tokens and more take a wave for each
+//     16 rows, which exchange their largest values through LDS.
+
+#include "scaled_cache.h"
+
+#include "fp8_e4m3.h"
+
+#pragma clang fp contract(off)
+
+namespace {
+
+using namespace mkv_scaled;
+
+// ------------------------------------------------------------------------- step slots
+
+constexpr int kSlotThreads = 1024;
+
+struct SlotParams {
+  const int32_t* held;
+  const int32_t* fresh;
+  int32_t* tables;
+  int64_t table_stride;
+  const int32_t* free_blocks;
+  const int32_t* free_at;
+  int32_t* starts;
+  int32_t* lens;
+  int64_t* slots;
+  int32_t* positions;
+  int32_t* free_at_out;
+  int32_t* flags;
+  int64_t free_len;
+  int64_t max_tokens;
+  int32_t requests;
+  int32_t table_width;
+  int32_t block_size;
+};
+
+__device__ __forceinline__ int64_t blocks_of(int64_t tokens, int bs) { return (tokens + bs - 1) / bs; }
+
+// The last r in [0, n) with a[r] <= at, by halves in LDS; a[0] = 0 <= at.
+__device__ __forceinline__ int owner(const int32_t* a, int n, int at) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a[mid] <= at) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+__global__ __launch_bounds__(kSlotThreads) void step_slots_kernel(SlotParams p) {
+  __shared__ int32_t s_start[MKV_MAX_REQUESTS + 1];  // new tokens before request r
+  __shared__ int32_t s_block[MKV_MAX_REQUESTS + 1];  // fresh blocks before request r
+  __shared__ int64_t s_wave[2][kSlotThreads / 64];
+  __shared__ int32_t s_bad;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int n = p.requests, bs = p.block_size;
+  if (tid == 0) s_bad = 0;
+  __syncthreads();
+  // prefix sums over the requests, a stretch of kSlotThreads at a time
+  int64_t tokens = 0, blocks = 0;
+  for (int base = 0; base < n; base += kSlotThreads) {
+    const int r = base + tid;
+    int64_t held = 0, add = 0, need = 0;
+    if (r < n) {
+      held = p.held[r];
+      add = p.fresh[r];
+      if (held < 0 || add < 0 || held + add > INT32_MAX ||
+          blocks_of(held + add, bs) > p.table_width) {
+        s_bad = 1;
+        held = add = 0;
+      }
+      need = blocks_of(held + add, bs) - blocks_of(held, bs);
+    }
+    int64_t a = add, b = need;  // inclusive within the wave
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t ua = __shfl_up(a, d), ub = __shfl_up(b, d);
+      if (lane >= d) {
+        a += ua;
+        b += ub;
+      }
+    }
+    if (lane == 63) {
+      s_wave[0][wave] = a;
+      s_wave[1][wave] = b;
+    }
+    __syncthreads();
+    for (int w = 0; w < kSlotThreads / 64; ++w) {
+      if (w == wave) {
+        a += tokens;
+        b += blocks;
+      }
+      tokens += s_wave[0][w];
+      blocks += s_wave[1][w];
+    }
+    if (r < n) {
+      // sums past 32 bits are refused below, before anything reads these
+      s_start[r] = static_cast<int32_t>(a - add);
+      s_block[r] = static_cast<int32_t>(b - need);
+    }
+    __syncthreads();
+  }
+  const int64_t at = p.free_at[0];
+  const bool bad = s_bad != 0 || tokens > p.max_tokens || at < 0 ||
+                   at + blocks > p.free_len;
+  const int64_t gtid = static_cast<int64_t>(blockIdx.x) * kSlotThreads + tid;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kSlotThreads;
+  if (blockIdx.x == 0) {
+    if (tid == 0) {
+      p.free_at_out[0] = static_cast<int32_t>(bad ? at : at + blocks);
+      p.starts[n] = bad ? 0 : static_cast<int32_t>(tokens);
+      if (bad) raise(p.flags, MKV_FLAG_DST_RANGE);
+    }
+    for (int r = tid; r < n; r += kSlotThreads) {
+      p.starts[r] = bad ? 0 : s_start[r];
+      p.lens[r] = p.held[r] + (bad ? 0 : p.fresh[r]);
+    }
+  }
+  if (!bad) {  // table entries of the fresh blocks
+    for (int64_t j = gtid; j < blocks; j += step) {
+      const int r = owner(s_block, n, static_cast<int>(j));
+      const int64_t col = blocks_of(p.held[r], bs) + (j - s_block[r]);
+      p.tables[r * p.table_stride + col] = p.free_blocks[at + j];
+    }
+  }
+  for (int64_t t = gtid; t < p.max_tokens; t += step) {
+    int64_t slot = -1;
+    int32_t pos = 0;
+    if (!bad && t < tokens) {
+      const int r = owner(s_start, n, static_cast<int>(t));
+      const int held = p.held[r];
+      pos = held + static_cast<int>(t) - s_start[r];
+      const int64_t b = pos / bs, before = blocks_of(held, bs);
+      // a fresh block's id comes from the free list: other workgroups may be writing its entry
+      const int64_t id = b < before ? p.tables[r * p.table_stride + b]
+                                    : p.free_blocks[at + s_block[r] + (b - before)];
+      slot = id < 0 ? -1 : id * bs + pos % bs;
+    }
+    p.slots[t] = slot;
+    p.positions[t] = pos;
+  }
+}
+
+// ----------------------------------------------------------------- rows and their scales
+
+constexpr uint32_t kInfBits = 0x7F800000u;
+// 448 * 2^MKV_SCALE_MAX_EXP: beyond it even the largest scale saturates
+constexpr uint32_t kTopBits = (static_cast<uint32_t>(MKV_SCALE_MAX_EXP + 8 + 127) << 23) | 0x600000u;
+
+// The exponent of the scale for a largest |x| with these bits (finite): 448 = 1.75 * 2^8.
+__device__ __forceinline__ int exponent_for(uint32_t bits) {
+  if (bits == 0) return MKV_SCALE_MIN_EXP;
+  const int e = static_cast<int>(bits >> 23) - 127 - 8 + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+  return min(max(e, MKV_SCALE_MIN_EXP), MKV_SCALE_MAX_EXP);
+}
+
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+
+// The larger of a lane's bits and every other lane's.
+__device__ __forceinline__ uint32_t wave_max(uint32_t m) {
+  for (int d = 32; d > 0; d >>= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), d)));
+  return m;
+}
+
+// 16 values to 16 codes under 2^e.  Values fit 448 * 2^e unless `wild`: then infinities and
+// what is larger saturate, and NaNs become 0x7F.
+__device__ __forceinline__ u32x4 encode16(const float* x, int e, bool wild) {
+  const float s = pow2(-e);
+  u32x4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float q[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) q[j] = x[4 * i + j] * s;
+    if (wild) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) q[j] = mkv_fp8::clamp448(q[j]);
+    }
+    w[i] = mkv_fp8::encode4(q);
+    if (wild) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (x[4 * i + j] != x[4 * i + j]) w[i] = mkv_fp8::with_nan(w[i], j);
+    }
+  }
+  return w;
+}
+
+__device__ __forceinline__ void decode16(u32x4 w, float s, float* x) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    mkv_fp8::decode4(w[i], x + 4 * i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[4 * i + j] *= s;
+  }
+}
+
+// Where a lane stands in its wave's 16 rows of one (block, head): rows of D values in chunks
+// of 16, as many rows a pass as the wave's 64 lanes cover.
+template <int D>
+struct Rows {
+  static constexpr int kChunks = D / 16;
+  static constexpr int kPerPass = 64 / kChunks;
+  static constexpr int kPasses = 16 / kPerPass;
+};
+
+// The largest finite |x| (bits) of K and of V over the rows of a (block, head), which `parts`
+// waves share, and whether any value there needs care: an infinity, a NaN, or one that
+// saturates under the largest scale.
+struct Largest {
+  uint32_t k, v, wild;
+};
+
+__device__ __forceinline__ uint32_t finite_bits(float x) {
+  const uint32_t b = abs_bits(x);
+  return b >= kInfBits ? 0u : b;
+}
+
+// Over a wave's values, N times 16 a lane of each.
+template <int N>
+__device__ __forceinline__ Largest largest(const float (*k)[16], const float (*v)[16]) {
+  Largest m = {0, 0, 0};
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      m.k = max(m.k, abs_bits(k[u][i]));
+      m.v = max(m.v, abs_bits(v[u][i]));
+    }
+  }
+  m.k = wave_max(m.k);
+  m.v = wave_max(m.v);
+  if (max(m.k, m.v) > kTopBits) {
+    m = {0, 0, 1};
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        m.k = max(m.k, finite_bits(k[u][i]));
+        m.v = max(m.v, finite_bits(v[u][i]));
+      }
+    }
+    m.k = wave_max(m.k);
+    m.v = wave_max(m.v);
+  }
+  return m;
+}
+
+// Exchange between the waves of one (block, head); every wave of the workgroup calls it.
+__device__ __forceinline__ Largest across(Largest m, int parts, uint32_t (*lds)[3], int wave) {
+  if (parts == 1) return m;
+  __syncthreads();  // the last exchange has been read
+  if ((threadIdx.x & 63) == 0) {
+    lds[wave][0] = m.k;
+    lds[wave][1] = m.v;
+    lds[wave][2] = m.wild;
+  }
+  __syncthreads();
+  const int first = wave - wave % parts;
+  for (int i = 0; i < parts; ++i) {
+    m.k = max(m.k, lds[first + i][0]);
+    m.v = max(m.v, lds[first + i][1]);
+    m.wild |= lds[first + i][2];
+  }
+  return m;
+}
+
+// Waves of a workgroup, and how they share (block, head) pairs.
+constexpr int kMaxWaves = 8;
+int waves_of(int bs_shift) { return bs_shift == 7 ? 8 : 4; }
+
+// ------------------------------------------------------------------------------- store
+
+struct StoreParams {
+  DevCache c;
+  DevStep s;
+  const char* k;
+  const char* v;
+  int64_t k_token, k_head, v_token, v_head;  // bytes
+  int64_t tokens;
+  int32_t group;  // tokens a workgroup looks through for blocks that begin there
+};
+
+// 16 values of element type ET at p.
+template <int ET>
+__device__ __forceinline__ void load16(const char* p, float* x) {
+  if constexpr (ET == MKV_F32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const u32x4 w = reinterpret_cast<const u32x4*>(p)[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[4 * i + j] = __uint_as_float(w[j]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const u32x4 w = reinterpret_cast<const u32x4*>(p)[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (ET == MKV_BF16) {
+          x[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
+          x[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+        } else {
+          typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+          const uint32_t pair = w[j];  // (a bit cast of w[j] itself takes element 0)
+          const h2 h = __builtin_bit_cast(h2, pair);
+          x[8 * i + 2 * j] = static_cast<float>(h[0]);
+          x[8 * i + 2 * j + 1] = static_cast<float>(h[1]);
+        }
+      }
+    }
+  }
+}
+
+// A workgroup's waves take the heads of the blocks that begin, for their request and step,
+// among `group` consecutive tokens: the first token of a request and those at a block's first
+// row lead a block.  group 1: a workgroup a token, most of which lead nothing in a prefill.
+template <int ET, int D>
+__global__ __launch_bounds__(64 * kMaxWaves) void store_kernel(StoreParams p) {
+  using R = Rows<D>;
+  constexpr int kBytes = ET == MKV_F32 ? 4 : 2;
+  __shared__ uint32_t s_max[kMaxWaves][3];
+  const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);
+  const int bs = 1 << p.c.bs_shift, parts = bs >> 4;
+  const int heads_here = (blockDim.x >> 6) / parts;
+  const int head = blockIdx.y * heads_here + wave / parts, part = wave % parts;
+  const bool active = head < p.c.heads;
+  const int chunk = lane % R::kChunks, sub = lane / R::kChunks;
+  int64_t t = static_cast<int64_t>(blockIdx.x) * p.group;
+  const int64_t end = min(t + p.group, p.tokens);
+  while (t < end) {  // the same steps in every wave of the workgroup
+    const int32_t* starts = p.s.starts;
+    const int r = last_at_most(p.s.requests, t, [starts](int i) { return starts[i]; });
+    if (r < 0) {  // before the first request
+      const int64_t first = p.s.requests > 0 ? starts[0] : end;
+      t = first > t ? first : end;
+      continue;
+    }
+    const int64_t s0 = starts[r], s1 = starts[r + 1];
+    if (t < s0 || t >= s1) break;  // behind the last request, or starts that descend
+    const int64_t first_pos = p.s.lens[r] - (s1 - s0);
+    const int64_t pos = first_pos + (t - s0);
+    if (s0 < 0 || s1 > p.tokens || first_pos < 0) {
+      if (t == s0 && lane == 0 && wave == 0) raise(p.s.flags, MKV_FLAG_SPAN);
+      t = s1;
+      continue;
+    }
+    const int off = static_cast<int>(pos & (bs - 1));
+    if (t != s0 && off != 0) {  // a block that an earlier token leads
+      t = min(t + bs - off, s1);
+      continue;
+    }
+    const int n = static_cast<int>(min(static_cast<int64_t>(bs - off), s1 - t));
+    const int64_t col = pos >> p.c.bs_shift;
+    int64_t id = -1;
+    if (col < p.s.table_width) id = p.s.tables[r * p.s.table_stride + col];
+    if (id < 0 || id >= p.c.num_blocks) {
+      if (lane == 0 && wave == 0) raise(p.s.flags, MKV_FLAG_DST_RANGE);
+      t += n;
+      continue;
+    }
+    // this wave's rows of the block, and the largest of their new values
+    float k[R::kPasses][16], v[R::kPasses][16];
+#pragma unroll
+    for (int u = 0; u < R::kPasses; ++u) {
+      const int row = part * 16 + u * R::kPerPass + sub;
+      const bool fresh = active && row >= off && row < off + n;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) k[u][i] = v[u][i] = 0.0f;
+      if (fresh) {
+        const int64_t at = t + row - off;
+        load16<ET>(p.k + at * p.k_token + head * p.k_head + chunk * 16 * kBytes, k[u]);
+        load16<ET>(p.v + at * p.v_token + head * p.v_head + chunk * 16 * kBytes, v[u]);
+      }
+    }
+    const Largest most = across(largest<R::kPasses>(k, v), parts, s_max, wave);
+    const bool wild = most.wild != 0;
+    int ek = exponent_for(most.k), ev = exponent_for(most.v);
+    if (active) {
+      uint8_t* scale = p.c.scales + (id * p.c.heads + head) * 2;
+      char* kb = p.c.k + id * p.c.bstride + head * p.c.hstride + chunk * 16;
+      char* vb = p.c.v + id * p.c.bstride + head * p.c.hstride + chunk * 16;
+      if (off > 0) {  // rows [0, off) stay, under the larger scale
+        const int ok = scale_exp(scale[0]), ov = scale_exp(scale[1]);
+        const int nk = max(ek, ok), nv = max(ev, ov);
+#pragma unroll
+        for (int u = 0; u < R::kPasses; ++u) {
+          const int row = part * 16 + u * R::kPerPass + sub;
+          if (row >= off) continue;
+          float x[16];
+          if (nk > ok) {
+            u32x4* w = reinterpret_cast<u32x4*>(kb + row * p.c.tstride);
+            decode16(*w, 1.0f, x);
+            *w = encode16(x, nk - ok > 126 ? 126 : nk - ok, true);
+          }
+          if (nv > ov) {
+            u32x4* w = reinterpret_cast<u32x4*>(vb + row * p.c.tstride);
+            decode16(*w, 1.0f, x);
+            *w = encode16(x, nv - ov > 126 ? 126 : nv - ov, true);
+          }
+        }
+        ek = nk;
+        ev = nv;
+      }
+#pragma unroll
+      for (int u = 0; u < R::kPasses; ++u) {
+        const int row = part * 16 + u * R::kPerPass + sub;
+        if (row < off || row >= off + n) continue;
+        *reinterpret_cast<u32x4*>(kb + row * p.c.tstride) = encode16(k[u], ek, wild);
+        *reinterpret_cast<u32x4*>(vb + row * p.c.tstride) = encode16(v[u], ev, wild);
+      }
+    }
+    if (parts > 1) __syncthreads();  // every wave has read the old scale
+    if (active && part == 0 && lane == 0)
+      *reinterpret_cast<uint16_t*>(p.c.scales + (id * p.c.heads + head) * 2) =
+          static_cast<uint16_t>((ek + 127) | ((ev + 127) << 8));
+    t += n;
+  }
+}
+
+// ------------------------------------------------------------------------------- shift
+
+struct MoveParams {
+  DevCache src;  // geometry; the layers' bases come from the arrays below
+  DevCache dst;
+  const uint64_t* src_layers;
+  const uint64_t* dst_layers;
+  const mkv_span_t* spans;
+  const int64_t* unit_starts;
+  const float* tables;
+  const int32_t* src_table;
+  const int32_t* dst_table;
+  int32_t* flags;
+  int64_t src_table_len;
+  int64_t dst_table_len;
+  int32_t n_spans;
+  int32_t rotary;
+};
+
+// A workgroup makes one destination block of `heads_here` heads and one layer.
+template <int D>
+__global__ __launch_bounds__(64 * kMaxWaves) void move_kernel(MoveParams p) {
+  using R = Rows<D>;
+  __shared__ uint32_t s_max[kMaxWaves][3];
+  const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);
+  const int dbs = 1 << p.dst.bs_shift, parts = dbs >> 4;
+  const int heads_here = (blockDim.x >> 6) / parts;
+  const int head = blockIdx.y * heads_here + wave / parts, part = wave % parts;
+  const bool active = head < p.dst.heads;
+  const int chunk = lane % R::kChunks, sub = lane / R::kChunks;
+  const int64_t unit = blockIdx.x;
+  const int64_t* us = p.unit_starts;
+  const int s = last_at_most(p.n_spans, unit, [us](int i) { return us[i]; });
+  if (s < 0) return;
+  const mkv_span_t sp = p.spans[s];
+  const int64_t first = (unit - us[s]) << p.dst.bs_shift;  // the block's first row in its span
+  const int n = static_cast<int>(min(static_cast<int64_t>(dbs), sp.n_tokens - first));
+  const bool aligned = sp.dst_pos >= 0 && (sp.dst_pos & (dbs - 1)) == 0;
+  if (n <= 0 || first < 0 || !aligned) {
+    if (threadIdx.x == 0 && !aligned) raise(p.flags, MKV_FLAG_SPAN);
+    return;
+  }
+  const int64_t dcol = sp.dst_index + ((sp.dst_pos + first) >> p.dst.bs_shift);
+  int64_t id = -1;
+  if (dcol >= 0 && dcol < p.dst_table_len) id = p.dst_table[dcol];
+  if (id < 0 || id >= p.dst.num_blocks) {
+    if (threadIdx.x == 0) raise(p.flags, MKV_FLAG_DST_RANGE);
+    return;
+  }
+  const uint64_t* sl = p.src_layers + 3 * static_cast<int64_t>(blockIdx.z);
+  const uint64_t* dl = p.dst_layers + 3 * static_cast<int64_t>(blockIdx.z);
+  const char* sk = reinterpret_cast<const char*>(sl[0]);
+  const char* sv = reinterpret_cast<const char*>(sl[1]);
+  const uint8_t* ss = reinterpret_cast<const uint8_t*>(sl[2]);
+
+  u32x4 kw[R::kPasses], vw[R::kPasses];
+  int scale[R::kPasses];
+  bool there[R::kPasses];
+#pragma unroll
+  for (int u = 0; u < R::kPasses; ++u) {
+    const int row = part * 16 + u * R::kPerPass + sub;
+    there[u] = false;
+    kw[u] = vw[u] = u32x4{0, 0, 0, 0};
+    scale[u] = 127 | (127 << 8);
+    if (active && row < n) {
+      const int64_t pos = sp.src_pos + first + row;
+      const int64_t col = sp.src_index + (pos >> p.src.bs_shift);
+      int64_t from = -1;
+      if (pos >= 0 && col >= 0 && col < p.src_table_len) from = p.src_table[col];
+      if (from >= 0 && from < p.src.num_blocks) {
+        there[u] = true;
+        const int64_t at = from * p.src.bstride + head * p.src.hstride +
+                           (pos & ((1 << p.src.bs_shift) - 1)) * p.src.tstride + chunk * 16;
+        kw[u] = *reinterpret_cast<const u32x4*>(sk + at);
+        vw[u] = *reinterpret_cast<const u32x4*>(sv + at);
+        scale[u] = *reinterpret_cast<const uint16_t*>(ss + (from * p.src.heads + head) * 2);
+      } else if (chunk == 0) {
+        raise(p.flags, MKV_FLAG_SRC_RANGE);
+      }
+    }
+  }
+  const bool turn = sp.delta != 0 && p.rotary > 0;
+  const int half = p.rotary >> 5;  // chunks to a lane's partner
+  const bool turned = turn && chunk < 2 * half;
+  const int partner = chunk < half ? lane + half : lane - half;
+  float cs[16], sn[16];
+  if (turned) {
+    const float* t = p.tables + static_cast<int64_t>(s) * 2 * p.rotary + chunk * 16;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      cs[i] = t[i];
+      sn[i] = t[p.rotary + i];
+    }
+  }
+  float k[R::kPasses][16], v[R::kPasses][16];
+#pragma unroll
+  for (int u = 0; u < R::kPasses; ++u) {
+    const float fk = pow2(scale_exp(scale[u] & 0xFF)), fv = pow2(scale_exp(scale[u] >> 8));
+    decode16(kw[u], fk, k[u]);
+    decode16(vw[u], fv, v[u]);
+    if (turn) {
+      u32x4 w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __shfl(static_cast<int>(kw[u][i]), turned ? partner : lane);
+      float y[16];
+      decode16(w, fk, y);
+      if (turned) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float a = k[u][i] * cs[i], b = y[i] * sn[i];
+          k[u][i] = a + b;
+        }
+      }
+    }
+  }
+  const Largest most = across(largest<R::kPasses>(k, v), parts, s_max, wave);
+  const bool wild = most.wild != 0;
+  if (!active) return;
+  const int ek = exponent_for(most.k), ev = exponent_for(most.v);
+  const int64_t to = id * p.dst.bstride + head * p.dst.hstride + chunk * 16;
+#pragma unroll
+  for (int u = 0; u < R::kPasses; ++u) {
+    if (!there[u]) continue;
+    const int64_t at = to + (part * 16 + u * R::kPerPass + sub) * p.dst.tstride;
+    *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(dl[0]) + at) = encode16(k[u], ek, wild);
+    *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(dl[1]) + at) = encode16(v[u], ev, wild);
+  }
+  if (part == 0 && lane == 0)
+    *reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(dl[2]) + (id * p.dst.heads + head) * 2) =
+        static_cast<uint16_t>((ek + 127) | ((ev + 127) << 8));
+}
+
+template <int ET>
+void store_launch(int d, dim3 grid, int threads, const StoreParams& p, hipStream_t s) {
+  if (d == 64)
+    store_kernel<ET, 64><<<grid, threads, 0, s>>>(p);
+  else if (d == 128)
+    store_kernel<ET, 128><<<grid, threads, 0, s>>>(p);
+  else
+    store_kernel<ET, 256><<<grid, threads, 0, s>>>(p);
+}
+
+}  // namespace
+
+// ------------------------------------------------------------------------- entry points
+
+extern "C" int mkv_step_slots(const int32_t* held, const int32_t* fresh, int32_t requests,
+                              int32_t* block_tables, int64_t table_stride, int32_t table_width,
+                              const int32_t* free_blocks, int64_t free_len,
+                              const int32_t* free_at, int32_t block_size, int32_t* starts,
+                              int32_t* lens, int64_t* slots, int32_t* positions,
+                              int64_t max_tokens, int32_t* free_at_out, int32_t* error_flags,
+                              void* stream) {
+  const char* who = "mkv_step_slots";
+  if (requests < 0 || requests > MKV_MAX_REQUESTS)
+    return mkv_fail(MKV_ERR_ARG, "%s: requests %d outside [0, %d]", who, requests,
+                    MKV_MAX_REQUESTS);
+  if (block_size <= 0) return mkv_fail(MKV_ERR_ARG, "%s: block_size %d", who, block_size);
+  if (table_width < 0 || table_stride < 0 || free_len < 0 || max_tokens < 0 ||
+      max_tokens > INT32_MAX || free_len > INT32_MAX)
+    return mkv_fail(MKV_ERR_ARG, "%s: a size is negative or past 32 bits", who);
+  if (free_at == nullptr || free_at_out == nullptr || starts == nullptr ||
+      (requests > 0 && (held == nullptr || fresh == nullptr || lens == nullptr)) ||
+      (max_tokens > 0 && (slots == nullptr || positions == nullptr)) ||
+      (requests > 0 && table_width > 0 && block_tables == nullptr) ||
+      (free_len > 0 && free_blocks == nullptr))
+    return mkv_fail(MKV_ERR_ARG, "%s: a pointer is NULL", who);
+  if (free_at == free_at_out)
+    return mkv_fail(MKV_ERR_ARG, "%s: free_at_out is free_at itself", who);
+  const SlotParams p = {held,   fresh,    block_tables, table_stride, free_blocks, free_at,
+                        starts, lens,     slots,        positions,    free_at_out, error_flags,
+                        free_len, max_tokens, requests, table_width,  block_size};
+  const int64_t want = (max_tokens + kSlotThreads - 1) / kSlotThreads;
+  const int grid = static_cast<int>(want < 1 ? 1 : want > 256 ? 256 : want);
+  step_slots_kernel<<<grid, kSlotThreads, 0, static_cast<hipStream_t>(stream)>>>(p);
+  return launched(who);
+}
+
+extern "C" int mkv_store_scaled(const mkv_scaled_cache_t* cache, const void* k,
+                                int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                                int64_t v_token_stride, int64_t v_head_stride, int64_t tokens,
+                                int32_t dtype, const int32_t* block_tables,
+                                int64_t table_stride, int32_t table_width,
+                                const int32_t* starts, const int32_t* lens, int32_t requests,
+                                int32_t* error_flags, void* stream) {
+  const char* who = "mkv_store_scaled";
+  if (cache == nullptr) return mkv_fail(MKV_ERR_ARG, "%s: cache is NULL", who);
+  StoreParams p;
+  int rc = check_cache(who, *cache, true, &p.c);
+  if (rc == MKV_OK)
+    rc = check_step(who, block_tables, table_stride, table_width, starts, lens, requests,
+                    error_flags, &p.s);
+  if (rc != MKV_OK) return rc;
+  if (dtype != MKV_BF16 && dtype != MKV_F16 && dtype != MKV_F32)
+    return mkv_fail(MKV_ERR_DTYPE, "%s: dtype %d is not bf16, fp16 or fp32", who, dtype);
+  if (tokens < 0 || tokens > INT32_MAX)
+    return mkv_fail(MKV_ERR_ARG, "%s: tokens %lld", who, (long long)tokens);
+  if (tokens == 0 || requests == 0) return MKV_OK;
+  if (k == nullptr || v == nullptr) return mkv_fail(MKV_ERR_ARG, "%s: k or v is NULL", who);
+  const int64_t eb = dtype == MKV_F32 ? 4 : 2;
+  const int64_t most = INT64_MAX / 16 / (tokens + cache->heads);
+  if (k_token_stride < 0 || k_head_stride < 0 || v_token_stride < 0 || v_head_stride < 0 ||
+      k_token_stride > most || k_head_stride > most || v_token_stride > most ||
+      v_head_stride > most)
+    return mkv_fail(MKV_ERR_ARG, "%s: a stride of k or v is out of range", who);
+  p.k = static_cast<const char*>(k);
+  p.v = static_cast<const char*>(v);
+  p.k_token = k_token_stride * eb;
+  p.k_head = k_head_stride * eb;
+  p.v_token = v_token_stride * eb;
+  p.v_head = v_head_stride * eb;
+  if (((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | p.k_token | p.k_head |
+        p.v_token | p.v_head) & 15) != 0)
+    return mkv_fail(MKV_ERR_ALIGN, "%s: k or v is not 16-byte aligned", who);
+  p.tokens = tokens;
+  p.group = tokens <= 4096 ? 1 : 16;
+  const int waves = waves_of(p.c.bs_shift), parts = cache->block_size / 16;
+  const int heads_here = waves / parts;
+  const dim3 grid(static_cast<unsigned>((tokens + p.group - 1) / p.group),
+                  static_cast<unsigned>((cache->heads + heads_here - 1) / heads_here));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == MKV_BF16)
+    store_launch<MKV_BF16>(cache->head_size, grid, 64 * waves, p, s);
+  else if (dtype == MKV_F16)
+    store_launch<MKV_F16>(cache->head_size, grid, 64 * waves, p, s);
+  else
+    store_launch<MKV_F32>(cache->head_size, grid, 64 * waves, p, s);
+  return launched(who);
+}
+
+extern "C" int mkv_shift_scaled(const mkv_scaled_shift_desc_t* d, void* stream) {
+  const char* who = "mkv_shift_scaled";
+  if (d == nullptr) return mkv_fail(MKV_ERR_ARG, "%s: desc is NULL", who);
+  MoveParams p;
+  int rc = check_cache(who, d->src, false, &p.src);
+  if (rc == MKV_OK) rc = check_cache(who, d->dst, false, &p.dst);
+  if (rc != MKV_OK) return rc;
+  if (d->src.heads != d->dst.heads || d->src.head_size != d->dst.head_size)
+    return mkv_fail(MKV_ERR_ARG, "%s: source and destination differ in heads or head_size", who);
+  if (d->rotary < 0 || d->rotary > d->dst.head_size || d->rotary % 32 != 0)
+    return mkv_fail(MKV_ERR_UNSUPPORTED, "%s: rotary %d is not a multiple of 32 up to head_size",
+                    who, d->rotary);
+  if (d->n_spans < 0 || d->n_spans > MKV_MAX_SPANS)
+    return mkv_fail(MKV_ERR_ARG, "%s: n_spans %d outside [0, %d]", who, d->n_spans, MKV_MAX_SPANS);
+  if (d->layers < 0 || d->layers > 65535)
+    return mkv_fail(MKV_ERR_ARG, "%s: layers %d", who, d->layers);
+  if (d->units < 0 || d->units > INT32_MAX || d->src_table_len < 0 || d->dst_table_len < 0)
+    return mkv_fail(MKV_ERR_ARG, "%s: a size is negative or past 32 bits", who);
+  if (d->n_spans == 0 || d->layers == 0 || d->units == 0) return MKV_OK;
+  if (d->spans == nullptr || d->unit_starts == nullptr || d->src_layers == nullptr ||
+      d->dst_layers == nullptr || d->src_table == nullptr || d->dst_table == nullptr ||
+      (d->rotary > 0 && d->tables == nullptr))
+    return mkv_fail(MKV_ERR_ARG, "%s: a pointer is NULL", who);
+  if ((reinterpret_cast<uintptr_t>(d->tables) & 15) != 0)
+    return mkv_fail(MKV_ERR_ALIGN, "%s: tables are not 16-byte aligned", who);
+  p.src_layers = d->src_layers;
+  p.dst_layers = d->dst_layers;
+  p.spans = d->spans;
+  p.unit_starts = d->unit_starts;
+  p.tables = d->tables;
+  p.src_table = d->src_table;
+  p.dst_table = d->dst_table;
+  p.flags = d->error_flags;
+  p.src_table_len = d->src_table_len;
+  p.dst_table_len = d->dst_table_len;
+  p.n_spans = d->n_spans;
+  p.rotary = d->rotary;
+  const int waves = waves_of(p.dst.bs_shift), heads_here = waves / (d->dst.block_size / 16);
+  const dim3 grid(static_cast<unsigned>(d->units),
+                  static_cast<unsigned>((d->dst.heads + heads_here - 1) / heads_here),
+                  static_cast<unsigned>(d->layers));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (d->dst.head_size == 64)
+    move_kernel<64><<<grid, 64 * waves, 0, s>>>(p);
+  else if (d->dst.head_size == 128)
+    move_kernel<128><<<grid, 64 * waves, 0, s>>>(p);
+  else
+    move_kernel<256><<<grid, 64 * waves, 0, s>>>(p);
+  return launched(who);
+}

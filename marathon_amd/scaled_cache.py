@@ -1,0 +1,400 @@
+"""A paged KV cache held in 8 bits, with a scale for each block of tokens and KV head.
+
+The cache's rows are e4m3fn codes in the layouts of the other caches here (HND ``[blocks,
+heads, bs, 2D]``, NHD ``[blocks, bs, heads, 2D]``, or K and V planes apart); a value is ``code
+* 2 ** e`` with one ``e`` for the K rows and one for the V rows of each (block, head), held as
+``float8_e8m0fnu`` in ``scales`` ``[blocks, heads, 2]`` (``include/marathon_kvscaled.h`` has
+the format).  Four operators work on it, each one launch (attention over long histories two),
+asynchronous on the current stream:
+
+* :func:`step_slots`    -- an engine step's block tables, slot map and positions, built on
+  the GPU from the requests' lengths: :func:`marathon_amd.slots` for a whole batch, without
+  its host loop (shift_store.py:56-60);
+* :func:`store_scaled`  -- the step's new K and V rows into their blocks;
+* :func:`attend_scaled` -- the step's queries over the cache, causal, grouped heads;
+* :class:`ScaledShifts` -- reused spans into other blocks, K re-rotated by each span's delta,
+  every layer at once: :class:`marathon_amd.spans.SmallShifts` for this cache.
+
+A step's requests are described by ``block_tables`` (int32 ``[requests, width]``), ``starts``
+(int32 ``[requests + 1]``: request r's new tokens are rows ``starts[r]`` to ``starts[r + 1]``
+of the step's token arrays) and ``lens`` (int32 ``[requests]``: tokens held with the new ones),
+all on the GPU, so that a captured step replays with the lengths of its day.  Rows behind
+``starts[-1]`` (a padded batch) are neither read nor written.
+
+There is no CPU path and no gradient: tensors that are not on a HIP device raise, and so do
+queries that require one.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass, field
+
+import numpy as np
+import torch
+
+from . import _lib
+from .shift_kernels import current_stream, dtype_code
+from .spans import _on, _Staging, span_tables
+
+HEAD_SIZES = (64, 128, 256)
+BLOCK_SIZES = (16, 32, 64, 128)
+
+_ROW_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+_QUERY_DTYPES = (torch.bfloat16, torch.float16)
+
+
+def _current(device: torch.device) -> bool:
+    return device.index == torch.cuda.current_device()
+
+
+@dataclass
+class ScaledCache:
+    """One layer's cache: ``kv`` (``float8_e4m3fn``, fused rows ``[..., 2D]`` of K then V) and
+    ``scales`` (``float8_e8m0fnu`` ``[blocks, heads, 2]``, contiguous), of ``layout`` ``"hnd"``
+    or ``"nhd"``.  With ``v_cache``, ``kv`` holds K and ``v_cache`` V, rows ``[..., D]`` of the
+    same shape and strides.  The tensors are checked once, here, and kept."""
+
+    kv: torch.Tensor
+    scales: torch.Tensor
+    layout: str
+    block_size: int = 16
+    v_cache: torch.Tensor | None = None
+    desc: _lib.ScaledCacheDesc = field(init=False, repr=False)
+
+    def __post_init__(self):
+        kv, scales, v = self.kv, self.scales, self.v_cache
+        if self.layout not in ("hnd", "nhd"):
+            raise ValueError(f"layout {self.layout!r}: 'hnd' or 'nhd'")
+        if not kv.is_cuda:
+            raise RuntimeError("ScaledCache: kv is not on a HIP device; there is no CPU path")
+        if kv.dim() != 4:
+            raise ValueError(f"a {self.layout} cache is 4-D, got {tuple(kv.shape)}")
+        if kv.dtype != torch.float8_e4m3fn:
+            raise TypeError(f"cache dtype {kv.dtype}: float8_e4m3fn")
+        if kv.shape[2 if self.layout == "hnd" else 1] != self.block_size:
+            raise ValueError(f"{self.layout} cache {tuple(kv.shape)} has no blocks of "
+                             f"{self.block_size} tokens")
+        if v is not None and (v.shape != kv.shape or v.dtype != kv.dtype or v.device != kv.device
+                              or v.stride() != kv.stride()):
+            raise ValueError("v_cache differs from kv in shape, strides, dtype or device")
+        width = kv.shape[3]
+        if v is None and width % 2:
+            raise ValueError(f"fused rows of {width} values")
+        self.head_size = width if v is not None else width // 2
+        if self.head_size not in HEAD_SIZES:
+            raise ValueError(f"head_size {self.head_size}: one of {HEAD_SIZES}")
+        if self.block_size not in BLOCK_SIZES:
+            raise ValueError(f"block_size {self.block_size}: one of {BLOCK_SIZES}")
+        if kv.stride(3) != 1:
+            raise ValueError("rows must be contiguous in the last dimension")
+        self.heads = kv.shape[1 if self.layout == "hnd" else 2]
+        self.device = kv.device
+        if (scales.dtype != torch.float8_e8m0fnu or scales.device != kv.device
+                or tuple(scales.shape) != (kv.shape[0], self.heads, 2)
+                or not scales.is_contiguous()):
+            raise ValueError(f"scales: contiguous float8_e8m0fnu {(kv.shape[0], self.heads, 2)} "
+                             f"on {kv.device}, got {scales.dtype} {tuple(scales.shape)}")
+        # a dimension of one element never advances an address, and torch gives it any stride
+        strides = [s if n > 1 else 0 for s, n in zip(kv.stride(), kv.shape)]
+        block, head, token = (strides[:3] if self.layout == "hnd" else
+                              (strides[0], strides[2], strides[1]))
+        # the smallest steps between rows that do not overlap; a stride of 0 would have
+        # several tokens share one
+        if any(s == 0 and n > 1 for s, n in zip(kv.stride(), kv.shape)):
+            raise ValueError("an expanded cache (stride 0) cannot be written")
+        if any(s % 16 for s in strides[:3]) or kv.data_ptr() % 16 or (
+                v is not None and v.data_ptr() % 16) or scales.data_ptr() % 2:
+            raise ValueError("the cache's base and strides must be multiples of 16 bytes")
+        d = self.desc = _lib.ScaledCacheDesc()
+        if kv.numel():
+            d.k_base = kv.data_ptr()
+            d.v_base = kv.data_ptr() + self.head_size if v is None else v.data_ptr()
+            d.scales = scales.data_ptr()
+        d.num_blocks, d.block_stride, d.head_stride, d.token_stride = kv.shape[0], block, head, token
+        d.block_size, d.heads, d.head_size = self.block_size, self.heads, self.head_size
+
+
+def _flags(error_flags: torch.Tensor | None, device) -> int | None:
+    if error_flags is None:
+        return None
+    if error_flags.dtype != torch.int32 or error_flags.device != device or error_flags.numel() < 1:
+        raise ValueError(f"error_flags: int32 [1] on {device}")
+    return error_flags.data_ptr()
+
+
+def _int32(name: str, t: torch.Tensor, device, n: int | None) -> int:
+    """The address of a contiguous int32 vector (of ``n`` entries)."""
+    if t.dtype != torch.int32 or t.device != device or t.dim() != 1 or not t.is_contiguous():
+        raise ValueError(f"{name}: contiguous int32 vector on {device}, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
+    if n is not None and t.shape[0] != n:
+        raise ValueError(f"{name} has {t.shape[0]} entries, not {n}")
+    return t.data_ptr()
+
+
+def _table(t: torch.Tensor, device) -> tuple[int, int, int, int]:
+    """(address, row stride, requests, width) of a block table."""
+    if t.dtype != torch.int32 or t.device != device or t.dim() != 2:
+        raise ValueError(f"block_tables: int32 [requests, width] on {device}, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
+    n, width = t.shape
+    if width > 1 and t.stride(1) != 1:
+        raise ValueError("block_tables' rows must be contiguous")
+    return t.data_ptr(), t.stride(0) if n > 1 else width, n, width
+
+
+@dataclass
+class StepSlots:
+    """What :func:`step_slots` makes, all on the GPU: ``starts`` int32 ``[requests + 1]``,
+    ``lens`` int32 ``[requests]``, ``slots`` int64 ``[max_tokens]`` (-1 behind the last token),
+    ``positions`` int32 ``[max_tokens]`` (0 there) and ``free_at`` int32 ``[1]``."""
+
+    starts: torch.Tensor
+    lens: torch.Tensor
+    slots: torch.Tensor
+    positions: torch.Tensor
+    free_at: torch.Tensor
+
+
+def step_slots(held: torch.Tensor, new: torch.Tensor, block_tables: torch.Tensor,
+               free_blocks: torch.Tensor, free_at: torch.Tensor, block_size: int,
+               max_tokens: int, *, error_flags: torch.Tensor | None = None) -> StepSlots:
+    """Block tables and slot map of a step, from the requests' lengths on the GPU.
+
+    Request r holds ``held[r]`` tokens and gets ``new[r]`` more (int32).  The blocks that it
+    needs beyond ``ceil(held / block_size)`` are taken from ``free_blocks[free_at[0]:]``,
+    requests in order, and entered into ``block_tables`` in place; ``max_tokens`` bounds the
+    step's tokens (the length of the slot map).  ``slots`` is what :func:`scatter_shifted` and
+    a slot-addressed shift take, ``starts`` and ``lens`` what :func:`store_scaled` and
+    :func:`attend_scaled` take; the next step's ``held`` is ``lens`` and its ``free_at``
+    the one returned.
+
+    All or nothing: where the free list runs out, a request exceeds its table, the tokens
+    exceed ``max_tokens`` or a length is negative, bit ``MKV_FLAG_DST_RANGE`` is set in
+    ``error_flags``, the tables are left alone and the step is empty (``lens`` is ``held``,
+    every slot -1)."""
+    device = block_tables.device
+    if not block_tables.is_cuda:
+        raise RuntimeError("step_slots: block_tables is not on a HIP device; there is no CPU path")
+    at, stride, n, width = _table(block_tables, device)
+    if n > _lib.MKV_MAX_REQUESTS:
+        raise ValueError(f"{n} requests: at most {_lib.MKV_MAX_REQUESTS}")
+    if n > 1 and stride < width:
+        raise ValueError("block_tables' rows overlap")
+    block_size, max_tokens = int(block_size), int(max_tokens)
+    if block_size <= 0 or max_tokens < 0 or max_tokens >= 2**31:
+        raise ValueError(f"block_size {block_size}, max_tokens {max_tokens}")
+    held_at, new_at = _int32("held", held, device, n), _int32("new", new, device, n)
+    free_list = _int32("free_blocks", free_blocks, device, None)
+    free_from = _int32("free_at", free_at, device, 1)
+    flags = _flags(error_flags, device)
+
+    def out(size, dtype=torch.int32):
+        return torch.empty(size, dtype=dtype, device=device)
+
+    step = StepSlots(out(n + 1), out(n), out(max_tokens, torch.int64), out(max_tokens), out(1))
+    with _on(device, _current(device)):
+        _lib.check(_lib.lib().mkv_step_slots(
+            held_at, new_at, n, at, stride, width, free_list, free_blocks.shape[0], free_from,
+            block_size, step.starts.data_ptr(), step.lens.data_ptr(), step.slots.data_ptr(),
+            step.positions.data_ptr(), max_tokens, step.free_at.data_ptr(), flags,
+            current_stream(device)))
+    return step
+
+
+def store_scaled(cache: ScaledCache, k: torch.Tensor, v: torch.Tensor,
+                 block_tables: torch.Tensor, starts: torch.Tensor, lens: torch.Tensor, *,
+                 error_flags: torch.Tensor | None = None) -> None:
+    """Write the step's new rows ``k`` and ``v`` (``[tokens, heads, D]``, bf16, fp16 or fp32)
+    into their blocks.
+
+    A block that its request begins here gets the smallest scale that fits its new rows.  A
+    block begun in an earlier step keeps its rows and at least its scale; where the new rows
+    need a larger one, the old rows are encoded again under it, which keeps their values but
+    for codes that become subnormal.  Infinities saturate, NaNs stay NaN."""
+    device = cache.device
+    if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (cache.heads, cache.head_size):
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)}: [tokens, {cache.heads}, "
+                         f"{cache.head_size}]")
+    if k.dtype not in _ROW_DTYPES or v.dtype != k.dtype:
+        raise TypeError(f"k {k.dtype} and v {v.dtype}: one of {_ROW_DTYPES}")
+    if k.device != device or v.device != device:
+        raise ValueError(f"k on {k.device}, v on {v.device}, the cache on {device}")
+    if k.stride(2) != 1 or v.stride(2) != 1:
+        raise ValueError("rows must be contiguous in the last dimension")
+    at, stride, n, width = _table(block_tables, device)
+    args = (
+        ctypes.byref(cache.desc), k.data_ptr(), *_steps(k), v.data_ptr(), *_steps(v), k.shape[0],
+        dtype_code(k.dtype), at, stride, width, _int32("starts", starts, device, n + 1),
+        _int32("lens", lens, device, n), n, _flags(error_flags, device))
+    with _on(device, _current(device)):
+        _lib.check(_lib.lib().mkv_store_scaled(*args, current_stream(device)))
+
+
+def _steps(t: torch.Tensor) -> tuple[int, int]:
+    """Token and head strides; of a dimension of one element, 0 (torch gives it any)."""
+    return (t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0)
+
+
+def attend_scaled(cache: ScaledCache, q: torch.Tensor, block_tables: torch.Tensor,
+                  starts: torch.Tensor, lens: torch.Tensor, *, softmax_scale: float | None = None,
+                  max_new: int | None = None, max_len: int | None = None,
+                  out: torch.Tensor | None = None,
+                  error_flags: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of the step's queries ``q`` (``[tokens, query heads, D]``, bf16 or
+    fp16) over the cache; query head h reads KV head ``h // (query heads / heads)``.
+
+    Row i of request r stands at position ``lens[r] - new[r] + i`` and sees the positions up
+    to its own: store the step's rows first.  ``softmax_scale``: ``D ** -0.5`` unless given.
+    A row that sees nothing is zeros; rows of ``out`` behind ``starts[-1]`` are left as they
+    were (in a fresh ``out``, undefined).  Sums and softmax statistics are fp32.
+
+    ``max_new`` and ``max_len``: the largest number of new tokens and of tokens of a request,
+    where the host knows them (a captured step: the largest that will be replayed).  They
+    choose launch shapes only."""
+    device, d = cache.device, cache.head_size
+    if q.dim() != 3 or q.shape[2] != d or q.shape[1] == 0 or q.shape[1] % cache.heads:
+        raise ValueError(f"q {tuple(q.shape)}: [tokens, a multiple of {cache.heads}, {d}]")
+    if q.dtype not in _QUERY_DTYPES:
+        raise TypeError(f"q {q.dtype}: one of {_QUERY_DTYPES}")
+    if q.device != device:
+        raise ValueError(f"q on {q.device}, the cache on {device}")
+    if q.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("attend_scaled has no backward pass; detach q or use torch.no_grad()")
+    if q.stride(2) != 1:
+        raise ValueError("q's rows must be contiguous in the last dimension")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != device or out.stride(2) != 1:
+        raise ValueError(f"out {out.dtype} {tuple(out.shape)} on {out.device} does not fit q")
+    elif q.numel() and out.data_ptr() == q.data_ptr():
+        raise ValueError("out is q")
+    at, stride, n, width = _table(block_tables, device)
+    desc = _lib.AttendDesc()
+    ctypes.memmove(ctypes.byref(desc), ctypes.byref(cache.desc), ctypes.sizeof(cache.desc))
+    desc.q, (desc.q_token_stride, desc.q_head_stride) = q.data_ptr(), _steps(q)
+    desc.out, (desc.out_token_stride, desc.out_head_stride) = out.data_ptr(), _steps(out)
+    desc.block_tables, desc.table_stride, desc.table_width, desc.requests = at, stride, width, n
+    desc.starts = _int32("starts", starts, device, n + 1)
+    desc.lens = _int32("lens", lens, device, n)
+    desc.error_flags = _flags(error_flags, device)
+    desc.tokens, desc.q_heads, desc.dtype = q.shape[0], q.shape[1], dtype_code(q.dtype)
+    desc.max_new, desc.max_len = int(max_new or 0), int(max_len or 0)
+    desc.softmax_scale = d ** -0.5 if softmax_scale is None else float(softmax_scale)
+    L = _lib.lib()
+    need = L.mkv_attend_workspace_size(ctypes.byref(desc))
+    with _on(device, _current(device)):
+        if need > 0:  # the allocator hands it on in stream order
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+            desc.workspace, desc.workspace_bytes = workspace.data_ptr(), need
+        _lib.check(L.mkv_attend_scaled(ctypes.byref(desc), current_stream(device)))
+    return out
+
+
+class ScaledShifts:
+    """Shifts between block-scaled caches: ``src`` and ``dst`` are lists of one
+    :class:`ScaledCache` a layer, of one geometry each (block sizes and layouts may differ
+    between the two).  ``inv_freq``: fp32 ``[rotary / 2]``, ``rotary`` a multiple of 32; None
+    moves keys without turning them.
+
+    One runner serves every step over the same caches (:meth:`run`).  A graph that captured a
+    step reads the runner's buffers: the runner outlives it."""
+
+    def __init__(self, src: list, dst: list, inv_freq: torch.Tensor | None):
+        if len(src) != len(dst) or not src:
+            raise ValueError(f"src has {len(src)} layers, dst {len(dst)}")
+        for caches in (src, dst):
+            first = caches[0]
+            for c in caches[1:]:
+                if _geometry(c) != _geometry(first) or c.device != first.device:
+                    raise ValueError("the layers of one side differ in geometry or device")
+        a, b = src[0], dst[0]
+        if (a.heads, a.head_size) != (b.heads, b.head_size) or a.device != b.device:
+            raise ValueError("src and dst differ in heads, head_size or device")
+        self.src, self.dst, self.device, self.layers = list(src), list(dst), b.device, len(dst)
+        self.rotary = 0 if inv_freq is None else 2 * int(inv_freq.numel())
+        if self.rotary % 32 or self.rotary > b.head_size:
+            raise ValueError(f"rotary {self.rotary}: a multiple of 32, at most {b.head_size}")
+        self.inv_freq = None if inv_freq is None else inv_freq.detach().to(
+            "cpu", torch.float32).contiguous()
+        d = self.desc = _lib.ScaledShiftDesc()
+        d.src, d.dst = a.desc, b.desc
+        d.layers, d.rotary = self.layers, self.rotary
+        with _on(self.device, _current(self.device)):
+            # (a copy from pageable memory: it is there when the call returns)
+            self._bases = torch.tensor(
+                [[[c.desc.k_base or 0, c.desc.v_base or 0, c.desc.scales or 0] for c in caches]
+                 for caches in (src, dst)], dtype=torch.int64).to(self.device)
+            self._streams = {current_stream(self.device)}
+        d.src_layers = self._bases[0].data_ptr()
+        d.dst_layers = self._bases[1].data_ptr()
+        self._captured: list = []  # host buffers that captured graphs read
+
+    def run(self, rows: list, src_table, dst_table, *,
+            error_flags: torch.Tensor | None = None) -> None:
+        """Shift ``rows`` on the current stream: ``mkv_span_t`` field tuples (src_pos, dst_pos,
+        src_index, dst_index, n_tokens, delta, 0, 0), positions through the block tables
+        ``src_table`` and ``dst_table`` (int32, on the host; a span's tables begin at its
+        src_index and dst_index).  ``dst_pos`` is a multiple of the destination's block size:
+        a span writes whole blocks, each anew under the scale of its rows; rows behind a
+        span's last one stay.  The destination blocks of one call are distinct, and none is
+        one of its source blocks."""
+        bs = self.dst[0].block_size
+        spans = np.zeros(len(rows), dtype=_lib.SPAN_DTYPE)
+        for i, r in enumerate(rows):
+            spans[i] = tuple(r)
+        if len(rows) > _lib.MKV_MAX_SPANS:
+            raise ValueError(f"{len(rows)} spans: at most {_lib.MKV_MAX_SPANS}")
+        if (spans["dst_pos"] % bs != 0).any():
+            raise ValueError(f"a destination position is not a multiple of {bs}")
+        if (spans["n_tokens"] < 0).any() or (spans["src_pos"] < 0).any() or (
+                spans["dst_pos"] < 0).any():
+            raise ValueError("a span's position or length is negative")
+        tables = [_host_table(t) for t in (src_table, dst_table)]
+        starts = np.zeros(len(rows) + 1, dtype=np.int64)
+        np.cumsum(-(-spans["n_tokens"].astype(np.int64) // bs), out=starts[1:])
+        units = int(starts[-1])
+        if units == 0:
+            return
+        stage = _Staging()
+        parts = [spans.view(np.uint8).reshape(-1), starts, *tables]
+        if self.rotary:
+            parts.append(span_tables(spans["delta"], self.inv_freq, self.rotary))
+        at = [stage.add(p) for p in parts]
+        desc = _lib.ScaledShiftDesc()
+        ctypes.memmove(ctypes.byref(desc), ctypes.byref(self.desc), ctypes.sizeof(desc))
+        desc.error_flags = _flags(error_flags, self.device)
+        desc.n_spans, desc.units = len(rows), units
+        desc.src_table_len, desc.dst_table_len = tables[0].size, tables[1].size
+        with _on(self.device, _current(self.device)):
+            stream = current_stream(self.device)
+            if stream not in self._streams:
+                self._bases.record_stream(torch.cuda.current_stream(self.device))
+                self._streams.add(stream)
+            blob = stage.upload(self.device)
+            if stream and torch.cuda.is_current_stream_capturing():
+                self._captured.append(stage.host)
+            base = blob.data_ptr()
+            desc.spans, desc.unit_starts = base + at[0], base + at[1]
+            desc.src_table, desc.dst_table = base + at[2], base + at[3]
+            desc.tables = base + at[4] if self.rotary else None
+            _lib.check(_lib.lib().mkv_shift_scaled(ctypes.byref(desc), stream))
+
+
+def _geometry(c: ScaledCache) -> tuple:
+    d = c.desc
+    return (d.num_blocks, d.block_stride, d.head_stride, d.token_stride, d.block_size, d.heads,
+            d.head_size)
+
+
+def _host_table(t) -> np.ndarray:
+    if isinstance(t, torch.Tensor):
+        if t.is_cuda:
+            raise ValueError("a shift's block tables are on the host")
+        t = t.detach().numpy()
+    t = np.asarray(t).reshape(-1)
+    if t.dtype != np.int32:
+        if t.dtype.kind not in "iu" or (t.size and (t.min() < -2**31 or t.max() >= 2**31)):
+            raise ValueError("a shift's block tables hold int32 block ids")
+    return np.ascontiguousarray(t, dtype=np.int32)

@@ -1,0 +1,210 @@
+"""The block-scaled cache's host side without a GPU: the oracle that the GPU tests compare
+with, the descriptors' layout, and every refusal that needs no device memory."""
+
+from __future__ import annotations
+
+import ctypes
+import os
+import subprocess
+
+import numpy as np
+import pytest
+import torch
+
+from marathon_amd import ScaledCache, _lib, step_slots
+from tests import scaled_plain as plain
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def test_the_oracles_codec_is_e4m3fn():
+    codes = torch.arange(256, dtype=torch.uint8)
+    want = codes.view(torch.float8_e4m3fn).double().numpy()
+    assert np.array_equal(plain.VALUES, want, equal_nan=True)
+    x = np.concatenate((np.linspace(-448, 448, 40001), np.ldexp(np.linspace(-3, 3, 20001), -8)))
+    x = x.astype(np.float32)
+    got = torch.from_numpy(x).to(torch.float8_e4m3fn).view(torch.uint8).numpy()
+    assert np.array_equal(plain.encode(x.astype(np.float64)), got)
+    assert plain.encode(np.array([np.nan, np.inf, -1e9]))[:].tolist() == [0x7F, 0x7E, 0xFE]
+
+
+def test_the_oracles_scale_is_the_least_that_fits():
+    rng = np.random.default_rng(0)
+    for top in [448.0, 448.0001, 447.0, 1.75, 1.7500001, 3e-38, 5e35, *np.exp2(rng.uniform(-60, 60, 200))]:
+        e = plain.exponent_for(np.array([top, -top / 3, np.nan, np.inf]))
+        if plain.LOW < e < plain.HIGH:
+            assert top <= 448 * 2.0 ** e and top > 448 * 2.0 ** (e - 1)
+    assert plain.exponent_for(np.zeros(3)) == plain.LOW
+    assert plain.exponent_for(np.array([3e38])) == plain.HIGH
+
+
+PROBE = r"""
+#include <stddef.h>
+#include <stdio.h>
+#include "marathon_kvscaled.h"
+#define O(T, f) printf(#T "." #f " %zu\n", offsetof(T, f))
+int main(void) {
+  printf("%zu %zu %zu\n", sizeof(mkv_scaled_cache_t), sizeof(mkv_attend_desc_t),
+         sizeof(mkv_scaled_shift_desc_t));
+@
+  printf("limits %d %d %d\n", MKV_SCALE_MIN_EXP, MKV_SCALE_MAX_EXP, MKV_MAX_REQUESTS);
+  return 0;
+}
+"""
+STRUCTS = {"mkv_scaled_cache_t": _lib.ScaledCacheDesc, "mkv_attend_desc_t": _lib.AttendDesc,
+           "mkv_scaled_shift_desc_t": _lib.ScaledShiftDesc}
+
+
+def test_descriptors_match_the_header(tmp_path):
+    lines = "\n".join(f"  O({name}, {f[0]});" for name, s in STRUCTS.items() for f in s._fields_)
+    src = tmp_path / "probe.c"
+    src.write_text(PROBE.replace("@", lines))
+    exe = tmp_path / "probe"
+    subprocess.run(["gcc", "-std=c99", f"-I{os.path.join(ROOT, 'include')}", str(src), "-o",
+                    str(exe)], check=True)
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split("\n")
+    assert [int(x) for x in out[0].split()] == [ctypes.sizeof(s) for s in STRUCTS.values()]
+    for line in out[1:]:
+        if "." in line:
+            field, at = line.split()
+            name, f = field.split(".")
+            assert getattr(STRUCTS[name], f).offset == int(at), field
+    assert out[-2] == (f"limits {_lib.MKV_SCALE_MIN_EXP} {_lib.MKV_SCALE_MAX_EXP} "
+                       f"{_lib.MKV_MAX_REQUESTS}")
+
+
+def cache_desc(**kw):
+    d = _lib.ScaledCacheDesc()
+    d.k_base, d.v_base, d.scales = 1 << 20, (1 << 20) + 128, 1 << 24
+    d.num_blocks, d.block_stride, d.head_stride, d.token_stride = 10, 16 * 2 * 256, 16 * 256, 256
+    d.block_size, d.heads, d.head_size = 16, 2, 128
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+BAD_CACHES = [
+    (dict(head_size=96), _lib.MKV_ERR_UNSUPPORTED), (dict(block_size=8), _lib.MKV_ERR_UNSUPPORTED),
+    (dict(block_size=24), _lib.MKV_ERR_UNSUPPORTED), (dict(heads=0), _lib.MKV_ERR_ARG),
+    (dict(num_blocks=-1), _lib.MKV_ERR_ARG), (dict(token_stride=250), _lib.MKV_ERR_ALIGN),
+    (dict(head_stride=-16), _lib.MKV_ERR_ARG), (dict(k_base=None), _lib.MKV_ERR_ARG),
+    (dict(v_base=(1 << 20) + 8), _lib.MKV_ERR_ALIGN), (dict(scales=(1 << 24) + 1), _lib.MKV_ERR_ALIGN),
+    (dict(token_stride=1 << 32), _lib.MKV_ERR_UNSUPPORTED),
+    (dict(head_stride=1 << 62), _lib.MKV_ERR_UNSUPPORTED),
+    (dict(block_stride=1 << 62), _lib.MKV_ERR_UNSUPPORTED),
+]
+
+
+def attend_desc(**kw):
+    d = _lib.AttendDesc()
+    d.cache = cache_desc(**{k: kw.pop(k) for k in list(kw) if hasattr(_lib.ScaledCacheDesc, k)})
+    d.q = d.out = d.starts = d.lens = d.block_tables = 1 << 20
+    d.q_token_stride = d.out_token_stride = 512
+    d.q_head_stride = d.out_head_stride = 128
+    d.table_stride = d.table_width = 8
+    d.tokens, d.requests, d.q_heads, d.dtype, d.softmax_scale = 3, 2, 4, _lib.MKV_BF16, 0.1
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize("change,code", BAD_CACHES + [
+    (dict(dtype=_lib.MKV_F32), _lib.MKV_ERR_DTYPE), (dict(q_heads=3), _lib.MKV_ERR_ARG),
+    (dict(q_heads=0), _lib.MKV_ERR_ARG), (dict(tokens=-1), _lib.MKV_ERR_ARG),
+    (dict(tokens=1 << 31), _lib.MKV_ERR_ARG), (dict(requests=5000), _lib.MKV_ERR_ARG),
+    (dict(requests=-1), _lib.MKV_ERR_ARG), (dict(starts=None), _lib.MKV_ERR_ARG),
+    (dict(block_tables=None), _lib.MKV_ERR_ARG), (dict(table_width=-1), _lib.MKV_ERR_ARG),
+    (dict(softmax_scale=0.0), _lib.MKV_ERR_ARG), (dict(softmax_scale=float("nan")), _lib.MKV_ERR_ARG),
+    (dict(softmax_scale=1e6), _lib.MKV_ERR_ARG), (dict(max_new=-1), _lib.MKV_ERR_ARG),
+    (dict(q=None), _lib.MKV_ERR_ARG), (dict(q=(1 << 20) + 2), _lib.MKV_ERR_ALIGN),
+    (dict(out_head_stride=60), _lib.MKV_ERR_ALIGN), (dict(q_token_stride=-8), _lib.MKV_ERR_ARG),
+    (dict(q_token_stride=1 << 60), _lib.MKV_ERR_ARG),
+    (dict(max_len=100000, table_width=100000), _lib.MKV_ERR_ARG),  # no workspace
+])
+def test_attend_refuses(change, code):
+    desc = attend_desc(**change)
+    assert _lib.lib().mkv_attend_scaled(ctypes.byref(desc), None) == code
+    assert _lib.lib().mkv_last_error()
+
+
+def test_attend_of_nothing_and_its_workspace():
+    L = _lib.lib()
+    assert L.mkv_attend_scaled(ctypes.byref(attend_desc(tokens=0)), None) == _lib.MKV_OK
+    assert L.mkv_attend_scaled(ctypes.byref(attend_desc(requests=0)), None) == _lib.MKV_OK
+    assert L.mkv_attend_scaled(None, None) == _lib.MKV_ERR_ARG
+    assert L.mkv_attend_workspace_size(None) == -1
+    assert L.mkv_attend_workspace_size(ctypes.byref(attend_desc(head_size=96))) == -1
+    assert L.mkv_attend_workspace_size(ctypes.byref(attend_desc(max_len=10))) == 0
+    assert L.mkv_attend_workspace_size(
+        ctypes.byref(attend_desc(max_len=100000, table_width=100000))) > 0
+
+
+def store_args(cache=None, **kw):
+    a = dict(cache=cache or cache_desc(), k=1 << 20, kt=256, kh=128, v=1 << 20, vt=256, vh=128,
+             tokens=3, dtype=_lib.MKV_BF16, tables=1 << 20, stride=8, width=8, starts=1 << 20,
+             lens=1 << 20, requests=2)
+    a.update(kw)
+    return [ctypes.byref(a.pop("cache")), *a.values(), None, None]
+
+
+@pytest.mark.parametrize("change,code", BAD_CACHES)
+def test_store_refuses_caches(change, code):
+    assert _lib.lib().mkv_store_scaled(*store_args(cache_desc(**change))) == code
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(dtype=_lib.MKV_FP8_E4M3), _lib.MKV_ERR_DTYPE), (dict(tokens=-1), _lib.MKV_ERR_ARG),
+    (dict(k=None), _lib.MKV_ERR_ARG), (dict(v=(1 << 20) + 4), _lib.MKV_ERR_ALIGN),
+    (dict(kt=252), _lib.MKV_ERR_ALIGN), (dict(vh=-128), _lib.MKV_ERR_ARG),
+    (dict(lens=None), _lib.MKV_ERR_ARG), (dict(requests=4097), _lib.MKV_ERR_ARG),
+    (dict(tokens=0), _lib.MKV_OK), (dict(requests=0), _lib.MKV_OK)])
+def test_store_refuses(change, code):
+    assert _lib.lib().mkv_store_scaled(*store_args(**change)) == code
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(requests=4097), _lib.MKV_ERR_ARG), (dict(requests=-1), _lib.MKV_ERR_ARG),
+    (dict(bs=0), _lib.MKV_ERR_ARG), (dict(width=-1), _lib.MKV_ERR_ARG),
+    (dict(max_tokens=1 << 31), _lib.MKV_ERR_ARG), (dict(held=None), _lib.MKV_ERR_ARG),
+    (dict(slots=None), _lib.MKV_ERR_ARG), (dict(out=1 << 20), _lib.MKV_ERR_ARG)])
+def test_slots_refuse(change, code):
+    p = 1 << 20
+    a = dict(held=p, fresh=p, requests=2, tables=p, stride=4, width=4, free=p, free_len=9, at=p,
+             bs=16, starts=p, lens=p, slots=p, positions=p, max_tokens=5, out=p + 64)
+    a.update(change)
+    assert _lib.lib().mkv_step_slots(*a.values(), None, None) == code
+
+
+def shift_desc(src=None, dst=None, **kw):
+    d = _lib.ScaledShiftDesc()
+    d.src, d.dst = cache_desc(**(src or {})), cache_desc(**(dst or {}))
+    for f in ("src_layers", "dst_layers", "spans", "unit_starts", "tables", "src_table", "dst_table"):
+        setattr(d, f, 1 << 20)
+    d.src_table_len = d.dst_table_len = 9
+    d.units, d.n_spans, d.layers, d.rotary = 4, 2, 3, 128
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(src=dict(head_size=64)), _lib.MKV_ERR_ARG), (dict(dst=dict(heads=1)), _lib.MKV_ERR_ARG),
+    (dict(src=dict(block_size=20)), _lib.MKV_ERR_UNSUPPORTED),
+    (dict(rotary=16), _lib.MKV_ERR_UNSUPPORTED), (dict(rotary=160), _lib.MKV_ERR_UNSUPPORTED),
+    (dict(rotary=-32), _lib.MKV_ERR_UNSUPPORTED), (dict(n_spans=5000), _lib.MKV_ERR_ARG),
+    (dict(layers=70000), _lib.MKV_ERR_ARG), (dict(units=1 << 31), _lib.MKV_ERR_ARG),
+    (dict(spans=None), _lib.MKV_ERR_ARG), (dict(tables=None), _lib.MKV_ERR_ARG),
+    (dict(tables=(1 << 20) + 4), _lib.MKV_ERR_ALIGN), (dict(dst_table_len=-1), _lib.MKV_ERR_ARG),
+    (dict(units=0), _lib.MKV_OK), (dict(layers=0), _lib.MKV_OK)])
+def test_shift_refuses(change, code):
+    assert _lib.lib().mkv_shift_scaled(ctypes.byref(shift_desc(**change)), None) == code
+
+
+def test_there_is_no_cpu_path():
+    kv = torch.zeros((4, 2, 16, 256), dtype=torch.uint8).view(torch.float8_e4m3fn)
+    scales = torch.zeros((4, 2, 2), dtype=torch.uint8).view(torch.float8_e8m0fnu)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ScaledCache(kv, scales, "hnd")
+    t = torch.zeros((1, 2), dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        step_slots(t[:, 0], t[:, 0], t, t[0], t[0, :1], 16, 4)
