@@ -36,7 +36,8 @@
  *                 Rows at or behind starts[requests] belong to nobody.
  *   lens          int32 [requests]: tokens each request holds WITH its new ones, so row i
  *                 of request r is position lens[r] - (starts[r + 1] - starts[r]) + i.
- *   block_tables  int32 [requests, table_width], rows table_stride apart.
+ *   block_tables  int32 [requests, table_width], rows table_stride apart; at most 2^30 tokens
+ *                 a request.
  * A request whose starts leave the token arrays, or descend, is skipped (MKV_FLAG_SPAN).
  *
  * No counterpart in the reference, whose caches are bf16 and whose slots are made on the

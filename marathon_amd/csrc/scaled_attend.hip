@@ -36,6 +36,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 struct AttendParams {
   DevCache c;
@@ -48,12 +49,14 @@ struct AttendParams {
   int64_t tokens;
   int32_t group;   // query heads a KV head serves
   int32_t splits;  // most parts that a tile's tokens are cut into
+  int32_t per;     // tokens of a part, a multiple of 64 (more where `splits` would not reach)
   float scale;     // softmax_scale * log2(e)
 };
 
 constexpr float kInf = __builtin_inff();
 constexpr float kSlack = 8.0f;  // powers of two that a score may pass the running largest by
-constexpr int kMinSplit = 256;  // tokens a part has at least
+constexpr int kMinSplit = 512;  // tokens a part has at least
+constexpr int kMaxSplits = 256;
 
 // A tile: `BM` query rows (token, query head of the group) of one request, heads fastest.
 // Request r's tiles begin at starts[r] * group / BM + r: that leaves each at least as many as
@@ -61,13 +64,13 @@ constexpr int kMinSplit = 256;  // tokens a part has at least
 struct Tile {
   int64_t s0;     // the request's first token
   int64_t row0;   // the tile's first row in the request
+  int64_t first;  // position of the request's first new token
   int rows;       // rows of the tile, 1 to BM
   int request;
-  int64_t first;  // position of the request's first new token
-  int64_t full;   // tokens that every row sees
-  int64_t keys;   // tokens that some row sees
+  int full;       // tokens that every row sees
+  int keys;       // tokens that some row sees
   int parts;      // parts its tokens are cut into, and the tokens of each
-  int64_t per;
+  int per;
 };
 
 template <int BM>
@@ -102,14 +105,12 @@ __device__ __forceinline__ bool find_tile(const AttendParams& p, int64_t tile, T
   }
   const int64_t lo = t.first + t.row0 / group + 1;
   const int64_t hi = t.first + (t.row0 + t.rows - 1) / group + 1;
-  t.keys = hi < 0 ? 0 : (hi < most ? hi : most);
-  if (t.keys < 0) t.keys = 0;
-  t.full = lo < 0 ? 0 : (lo < t.keys ? lo : t.keys);
-  int64_t parts = (t.keys + kMinSplit - 1) / kMinSplit;
-  parts = parts < 1 ? 1 : (parts > p.splits ? p.splits : parts);
-  t.per = ((t.keys + parts - 1) / parts + 63) / 64 * 64;
-  t.parts = t.per > 0 ? static_cast<int>((t.keys + t.per - 1) / t.per) : 1;
-  if (t.parts < 1) t.parts = 1;
+  const int64_t keys = hi < most ? hi : most;
+  t.keys = keys < 0 ? 0 : static_cast<int>(keys);
+  t.full = lo < 0 ? 0 : static_cast<int>(lo < t.keys ? lo : t.keys);
+  const int per = (t.keys / p.splits + 64) & ~63;  // at least keys / splits
+  t.per = per > p.per ? per : p.per;
+  t.parts = t.keys > t.per ? (t.keys + t.per - 1) / t.per : 1;
   return true;
 }
 
@@ -134,6 +135,21 @@ __device__ __forceinline__ uint32_t round_pair(float a, float b) {
   return bits_as<uint32_t>(__builtin_convertvector(x, bf16x2));
 }
 
+// Two values of the output type.
+template <bool F16>
+__device__ __forceinline__ uint32_t out_pair(float a, float b) {
+  if constexpr (F16)
+    return bits_as<uint32_t>(f16x2{static_cast<_Float16>(a), static_cast<_Float16>(b)});
+  else
+    return round_pair(a, b);
+}
+
+// A load of what is read once: past the caches' ordinary replacement.
+template <typename T>
+__device__ __forceinline__ T once(const char* p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
+}
+
 // Whether a dword of codes holds a NaN, as a mask of its bytes (0x80 in each such byte).
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
   return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
@@ -153,12 +169,16 @@ template <int D>
 struct FewRaw {  // one step's codes, as loaded
   u32x4 k[2][D / 64];       // tile of 16 tokens; 16 bytes each
   uint32_t v[8][D / 64];    // token slot; D / 16 bytes
-  uint32_t scale[2];
-  bool ok[2];               // the tile's block id is one
 };
 
+// Waves a SIMD is to hold: what is in flight hides memory's latency.
+template <int D, int RT>
+constexpr int few_waves() {
+  return D == 64 ? (RT == 1 ? 4 : 3) : D == 128 ? (RT == 1 ? 4 : 2) : (RT == 1 ? 2 : 1);
+}
+
 template <bool F16, int D, int RT>
-__global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttendParams p) {
+__global__ __launch_bounds__(64 * kFewWaves, (few_waves<D, RT>())) void attend_few_kernel(AttendParams p) {
   constexpr int BM = 16 * RT, KS = D / 32, DT = D / 16, NQ = D / 64;
   __shared__ float s_o[2][D * 16];
   __shared__ float s_ml[kFewWaves][BM][2];
@@ -166,10 +186,37 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttendParams
   const int c = lane & 15, g = lane >> 4;
   const int head = blockIdx.y;
   Tile t;
-  if (!find_tile<BM>(p, blockIdx.x, t)) return;
+  // Workgroups go to the eight XCDs in turn: the tiles are turned by the part, so that a long
+  // request's parts do not all fall to one (32 ragged requests: 119 -> 112 us).
+  const unsigned tile = (blockIdx.x + blockIdx.z) % gridDim.x;
+  if (!find_tile<BM>(p, tile, t)) return;
   const int part = blockIdx.z;
   if (part >= t.parts) return;
-  const int64_t k0 = part * t.per, k1 = min(t.keys, k0 + t.per);
+  const int k0 = part * t.per, k1 = min(t.keys, k0 + t.per);
+
+  // Block ids and scales of this wave's next 64 steps, one step a lane: the loop then waits
+  // for no table, and its loads depend on nothing that it loads.
+  const int32_t* table = p.s.tables + t.request * p.s.table_stride;
+  int ids[2] = {-1, -1};
+  int scales[2] = {0, 0};
+  const auto look_up = [&](int at) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      // tokens behind the last one seen are read from its block and not used
+      const int tok = min(at + 32 * kFewWaves * lane + 16 * i, t.keys - 1);
+      ids[i] = table[tok >> p.c.bs_shift];
+      scales[i] = 127 | (127 << 8);
+      if (ids[i] < 0 || ids[i] >= p.c.num_blocks) {
+        raise(p.s.flags, MKV_FLAG_SRC_RANGE);
+        ids[i] = -1;
+      } else {
+        scales[i] = *reinterpret_cast<const uint16_t*>(
+            p.c.scales + (static_cast<int64_t>(ids[i]) * p.c.heads + head) * 2);
+      }
+    }
+  };
+  const int first = k0 + 32 * wave;
+  if (first < k1) look_up(first);
 
   // this lane's query rows: operand B of S^T = K Q^T
   u32x4 q[RT][KS];
@@ -204,38 +251,29 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttendParams
     for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4{0, 0, 0, 0};
   }
 
-  const int32_t* table = p.s.tables + t.request * p.s.table_stride;
   const int bs_mask = (1 << p.c.bs_shift) - 1;
-  const auto load = [&](int64_t at, FewRaw<D>& x) {
+  const int lane_k = c * p.c.tstride + 16 * g, lane_v = 4 * g * p.c.tstride + (D / 16) * c;
+  const auto load = [&](int at, int n, FewRaw<D>& x) {  // n: the step's lane in ids and scales
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      // rows behind the last token seen are read from its block and not used
-      const int64_t tok = at + 16 * i;
-      const int64_t last = t.keys - 1;
-      int64_t id = table[(tok < last ? tok : last) >> p.c.bs_shift];
-      x.ok[i] = id >= 0 && id < p.c.num_blocks;
-      if (!x.ok[i]) {
-        if (lane == 0) raise(p.s.flags, MKV_FLAG_SRC_RANGE);
-        id = 0;
-      }
-      const int row = static_cast<int>(tok) & bs_mask;
-      const int64_t block = id * p.c.bstride + head * static_cast<int64_t>(p.c.hstride);
-      x.scale[i] = *reinterpret_cast<const uint16_t*>(p.c.scales + (id * p.c.heads + head) * 2);
-      const char* kb = p.c.k + block + (row + c) * p.c.tstride + 16 * g;
+      const int id = max(__builtin_amdgcn_readlane(ids[i], n), 0);
+      const int64_t block = id * p.c.bstride + head * static_cast<int64_t>(p.c.hstride) +
+                            ((at + 16 * i) & bs_mask) * static_cast<int64_t>(p.c.tstride);
+      const char* kb = p.c.k + block;
+      const char* vb = p.c.v + block;
 #pragma unroll
-      for (int j = 0; j < NQ; ++j) x.k[i][j] = *reinterpret_cast<const u32x4*>(kb + 64 * j);
-      const char* vb = p.c.v + block + (row + 4 * g) * p.c.tstride + (D / 16) * c;
+      for (int j = 0; j < NQ; ++j) x.k[i][j] = once<u32x4>(kb + lane_k + 64 * j);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const char* a = vb + j * p.c.tstride;
+        const char* a = vb + lane_v + j * p.c.tstride;
         if constexpr (D == 64) {
-          x.v[4 * i + j][0] = *reinterpret_cast<const uint32_t*>(a);
+          x.v[4 * i + j][0] = once<uint32_t>(a);
         } else if constexpr (D == 128) {
-          const u32x2 w = *reinterpret_cast<const u32x2*>(a);
+          const u32x2 w = once<u32x2>(a);
           x.v[4 * i + j][0] = w[0];
           x.v[4 * i + j][1] = w[1];
         } else {
-          const u32x4 w = *reinterpret_cast<const u32x4*>(a);
+          const u32x4 w = once<u32x4>(a);
 #pragma unroll
           for (int u = 0; u < 4; ++u) x.v[4 * i + j][u] = w[u];
         }
@@ -243,10 +281,14 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttendParams
     }
   };
 
-  const auto step = [&](int64_t at, FewRaw<D>& x) {
-    const bool masked = at + 32 > t.full || !x.ok[0] || !x.ok[1];
-    const int ek[2] = {scale_exp(x.scale[0] & 0xFF), scale_exp(x.scale[1] & 0xFF)};
-    const float fv[2] = {pow2(scale_exp(x.scale[0] >> 8)), pow2(scale_exp(x.scale[1] >> 8))};
+  const auto step = [&](int at, int n, FewRaw<D>& x) {
+    const bool ok[2] = {__builtin_amdgcn_readlane(ids[0], n) >= 0,
+                        __builtin_amdgcn_readlane(ids[1], n) >= 0};
+    const bool masked = at + 32 > t.full || !ok[0] || !ok[1];
+    const int sc[2] = {__builtin_amdgcn_readlane(scales[0], n),
+                       __builtin_amdgcn_readlane(scales[1], n)};
+    const int ek[2] = {scale_exp(sc[0] & 0xFF), scale_exp(sc[1] & 0xFF)};
+    const float fv[2] = {pow2(scale_exp(sc[0] >> 8)), pow2(scale_exp(sc[1] >> 8))};
     // S^T: tile i's tokens by this lane's row, tokens 16 i + 4 g + r
     f32x4 s[RT][2];
 #pragma unroll
@@ -281,8 +323,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttendParams
       uint32_t any = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int64_t tok = at + 16 * (j >> 2) + 4 * g + (j & 3);
-        const bool seen = tok < t.keys && x.ok[j >> 2];
+        const int tok = at + 16 * (j >> 2) + 4 * g + (j & 3);
+        const bool seen = tok < t.keys && ok[j >> 2];
 #pragma unroll
         for (int u = 0; u < NQ; ++u) {
           x.v[j][u] = seen ? x.v[j][u] : 0u;
@@ -302,8 +344,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttendParams
         const int i = j >> 2;
         y[j] = s[rt][i][j & 3] * (F16 ? p.scale * pow2(ek[i]) : p.scale);
         if (masked) {
-          const int64_t tok = at + 16 * i + 4 * g + (j & 3);
-          const bool sees = tok < limit[rt] && x.ok[i];
+          const int tok = at + 16 * i + 4 * g + (j & 3);
+          const bool sees = tok < limit[rt] && ok[i];
           y[j] = sees ? y[j] : -kInf;
           see[rt] |= sees ? 1u << j : 0u;
         }
@@ -390,11 +432,16 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttendParams
     }
   };
 
-  {
-    FewRaw<D> x;
-    for (int64_t at = k0 + 32 * wave; at < k1; at += 32 * kFewWaves) {
-      load(at, x);
-      step(at, x);
+  // One step's codes in registers, and other waves to hide its loads: keeping the next step's
+  // as well takes the registers of one wave in three (119 us against 111, the same requests).
+  constexpr int kStride = 32 * kFewWaves;
+  for (int base = first; base < k1; base += 64 * kStride) {
+    if (base != first) look_up(base);
+    const int last = min(64, (k1 - base + kStride - 1) / kStride) - 1;
+    for (int n = 0; n <= last; ++n) {
+      FewRaw<D> x;
+      load(base + n * kStride, n, x);
+      step(base + n * kStride, n, x);
     }
   }
 
@@ -412,7 +459,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttendParams
   float* part_o = nullptr;
   float* part_ml = nullptr;
   if (t.parts > 1) {
-    const int64_t at = (static_cast<int64_t>(blockIdx.x) * p.c.heads + head) * p.splits + part;
+    const int64_t at = (static_cast<int64_t>(tile) * p.c.heads + head) * p.splits + part;
     part_o = p.part_o + at * BM * D;
     part_ml = p.part_ml + at * BM * 2;
   }
@@ -473,14 +520,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttendParams
           for (int r = 0; r < 4; ++r) {
 #pragma unroll
             for (int dt = 0; dt < DT; dt += 4) {
-              const float a = o[rt][dt][r] * by, b = o[rt][dt + 1][r] * by;
-              const float cc = o[rt][dt + 2][r] * by, d = o[rt][dt + 3][r] * by;
-              u32x2 w;
-              if constexpr (F16)
-                w = u32x2{bits_as<uint32_t>(f16x2{static_cast<_Float16>(a), static_cast<_Float16>(b)}),
-                          bits_as<uint32_t>(f16x2{static_cast<_Float16>(cc), static_cast<_Float16>(d)})};
-              else
-                w = u32x2{round_pair(a, b), round_pair(cc, d)};
+              const u32x2 w = {out_pair<F16>(o[rt][dt][r] * by, o[rt][dt + 1][r] * by),
+                               out_pair<F16>(o[rt][dt + 2][r] * by, o[rt][dt + 3][r] * by)};
               *reinterpret_cast<u32x2*>(at + ((D / 16) * (4 * g + r) + dt) * 2) = w;
             }
           }
@@ -490,38 +531,427 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttendParams
   }
 }
 
+// ------------------------------------------------------------- many rows: chunks, prefills
+//
+// Bound by the matrix products and the softmax's vector work, about even.  A workgroup's four
+// waves hold 32 rows each of a tile of 128 and one KV head and walk the tokens together, 64 a
+// step (32x32x16 products).  K's codes go to LDS as they are (half of bf16's LDS reads; each
+// wave decodes them, 64 conversions for 32 products); V is decoded and transposed once for all
+// waves on its way there, so that a lane reads 8 tokens of one dimension in 16 bytes.  Both
+// are read without bank conflicts: a row's 16-byte chunks are exchanged by its number, so that
+// 16 rows' chunks of one column cover the 64 banks.
+// The next step's codes are loaded into registers before a step is computed and written to
+// the other of two buffers behind it: one barrier a step.  Two workgroups fit a CU, and one
+// computes while the other waits.
+
+constexpr int kManyWaves = 4;
+constexpr int kManyRows = 32 * kManyWaves;
+
+// Where chunk `ch` of K's row r lies: rows of 64, 128 or 256 bytes.
+template <int D>
+__device__ __forceinline__ int k_place(int r, int ch) {
+  const int turn = D == 64 ? (r >> 2) & 3 : D == 128 ? (r >> 1) & 7 : r & 15;
+  return r * D + ((ch ^ turn) << 4);
+}
+
+template <bool F16, int D>
+__global__ __launch_bounds__(64 * kManyWaves, (D == 256 ? 1 : 2)) void attend_many_kernel(AttendParams p) {
+  constexpr int KS = D / 16, MT = D / 32, W = D / 16, KC = D / 16;
+  constexpr int kKBytes = 64 * D, kVBytes = 128 * D;  // of a step
+  constexpr int kKLoads = kKBytes / 16 / 256 > 0 ? kKBytes / 16 / 256 : 1;
+  __shared__ __attribute__((aligned(16))) char s_k[2][kKBytes];
+  __shared__ __attribute__((aligned(16))) char s_v[2][kVBytes];
+  __shared__ int s_odd[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
+  const int c = lane & 31, h = lane >> 5;
+  const int head = blockIdx.x;
+  Tile t;
+  // the last tiles first: of one request they see the most
+  const unsigned tile = gridDim.y - 1 - blockIdx.y;
+  if (!find_tile<kManyRows>(p, tile, t)) return;
+  const int part = blockIdx.z;
+  if (part >= t.parts) return;
+  const int k0 = part * t.per, k1 = min(t.keys, k0 + t.per);
+  if (tid < 2) s_odd[tid] = -1;
+
+  // ids and scales of the next 64 groups of 16 tokens, one a lane
+  const int32_t* table = p.s.tables + t.request * p.s.table_stride;
+  int id = -1, scale = 0;
+  const auto look_up = [&](int at) {
+    const int tok = min(at + 16 * lane, t.keys - 1);
+    id = -1;
+    scale = 127 | (127 << 8);
+    if (t.keys > 0) id = table[tok >> p.c.bs_shift];
+    if (id < 0 || id >= p.c.num_blocks) {
+      if (wave == 0 && t.keys > 0) raise(p.s.flags, MKV_FLAG_SRC_RANGE);
+      id = -1;
+    } else {
+      scale = *reinterpret_cast<const uint16_t*>(
+          p.c.scales + (static_cast<int64_t>(id) * p.c.heads + head) * 2);
+    }
+  };
+
+  // this wave's rows: operand B of S^T = K Q^T, dimensions 32 i + 16 h + 0..15
+  const int64_t row = t.row0 + wave * 32 + c;
+  const bool there = wave * 32 + c < t.rows;
+  u32x4 q[KS];
+  int limit = 0;
+  {
+    const int64_t token = row / p.group;
+    const int64_t sees = t.first + token + 1;
+    if (there) limit = static_cast<int>(sees < 0 ? 0 : (sees < t.keys ? sees : t.keys));
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) q[ks] = u32x4{0, 0, 0, 0};
+    if (there) {
+      const char* at = p.q + (t.s0 + token) * p.q_token +
+                       (static_cast<int64_t>(head) * p.group + row % p.group) * p.q_head;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        q[ks] = *reinterpret_cast<const u32x4*>(at + (32 * (ks / 2) + 16 * h + 8 * (ks & 1)) * 2);
+    }
+  }
+  int most = limit;  // tokens that some row of the wave sees
+  for (int x = 16; x > 0; x >>= 1) most = max(most, __shfl_xor(most, x));
+  most = uni(most);
+
+  f32x16 o[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[mt][i] = 0.0f;
+  float m = -kInf, l = 0.0f;
+
+  // A step's codes on their way to LDS.  K: this thread's 16 bytes of rows tid / KC + ...;
+  // V: W dimensions W * (tid % 16) + j of the 4 tokens 4 * (tid / 16) + i.
+  u32x4 rk[kKLoads];
+  uint32_t rv[4][D / 64];
+  const int bs_mask = (1 << p.c.bs_shift) - 1;
+  const auto block_of = [&](int n) {  // the block of group n of the looked-up ones
+    return max(__builtin_amdgcn_readlane(id, n), 0) * p.c.bstride +
+           head * static_cast<int64_t>(p.c.hstride);
+  };
+  constexpr int kRowsPass = 256 / KC;  // rows that one pass over the threads covers
+  const auto fetch = [&](int at, int n) {  // n: the step's first group
+#pragma unroll
+    for (int u = 0; u < kKLoads; ++u) {
+      const int r = u * kRowsPass + tid / KC;  // D = 64: 64 rows; 128: 32; 256: 16
+      // the wave's rows lie in one group: 16, 8 or 4 rows a wave
+      const int grp = uni((u * kRowsPass + wave * (64 / KC)) >> 4);
+      const char* kb = p.c.k + block_of(n + grp) + ((at + r) & bs_mask) * static_cast<int64_t>(p.c.tstride);
+      rk[u] = *reinterpret_cast<const u32x4*>(kb + 16 * (tid % KC));
+    }
+    const char* vb = p.c.v + block_of(n + wave) +
+                     ((at + 4 * (tid >> 4)) & bs_mask) * static_cast<int64_t>(p.c.tstride) +
+                     W * (tid & 15);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const char* a = vb + i * p.c.tstride;
+      if constexpr (D == 64) {
+        rv[i][0] = *reinterpret_cast<const uint32_t*>(a);
+      } else if constexpr (D == 128) {
+        const u32x2 w = *reinterpret_cast<const u32x2*>(a);
+        rv[i][0] = w[0];
+        rv[i][1] = w[1];
+      } else {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(a);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) rv[i][u] = w[u];
+      }
+    }
+  };
+  const auto stage = [&](int at, int n, int buf) {
+#pragma unroll
+    for (int u = 0; u < kKLoads; ++u) {
+      const int r = u * kRowsPass + tid / KC, ch = tid % KC;
+      *reinterpret_cast<u32x4*>(s_k[buf] + k_place<D>(r, ch)) = rk[u];
+    }
+    const bool good = __builtin_amdgcn_readlane(id, n + wave) >= 0;
+    if (at + 64 > t.full || !good) {
+      // what nobody sees must not reach the products, NaN codes times 0
+      uint32_t any = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool seen = good && at + 4 * (tid >> 4) + i < t.keys;
+#pragma unroll
+        for (int u = 0; u < D / 64; ++u) {
+          rv[i][u] = seen ? rv[i][u] : 0u;
+          any |= nan_bytes(rv[i][u]);
+        }
+      }
+      if (any != 0) s_odd[buf] = at;
+    }
+    const float f = pow2(scale_exp(__builtin_amdgcn_readlane(scale, n + wave) >> 8));
+    // tokens 16 t + 4 quad + i: chunk 2 t + (quad & 1), its half quad / 2
+    const int quad = (tid >> 4) & 3, chunk = 2 * wave + (quad & 1), half = quad >> 1;
+#pragma unroll
+    for (int u = 0; u < D / 64; ++u) {
+      const uint32_t a01 = __builtin_amdgcn_perm(rv[1][u], rv[0][u], 0x05010400u);
+      const uint32_t b01 = __builtin_amdgcn_perm(rv[3][u], rv[2][u], 0x05010400u);
+      const uint32_t a23 = __builtin_amdgcn_perm(rv[1][u], rv[0][u], 0x07030602u);
+      const uint32_t b23 = __builtin_amdgcn_perm(rv[3][u], rv[2][u], 0x07030602u);
+      const u32x2 w[4] = {{bf16_pair<false>(a01, f), bf16_pair<false>(b01, f)},
+                          {bf16_pair<true>(a01, f), bf16_pair<true>(b01, f)},
+                          {bf16_pair<false>(a23, f), bf16_pair<false>(b23, f)},
+                          {bf16_pair<true>(a23, f), bf16_pair<true>(b23, f)}};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = (4 * u + j) * 16 + (tid & 15);  // dimension W * (r % 16) + r / 16
+        *reinterpret_cast<u32x2*>(s_v[buf] + r * 128 + ((chunk ^ ((r >> 1) & 7)) << 4) + 8 * half) =
+            w[j];
+      }
+    }
+  };
+
+  const auto compute = [&](int at, int n, int buf) {
+    bool masked = at + 64 > t.full;
+    int ek[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      masked |= __builtin_amdgcn_readlane(id, n + i) < 0;
+      ek[i] = scale_exp(__builtin_amdgcn_readlane(scale, n + i) & 0xFF);
+    }
+    f32x16 s[2];
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[st][i] = 0.0f;
+      const float fk = pow2(c < 16 ? ek[2 * st] : ek[2 * st + 1]);
+      const int r = 32 * st + c;
+#pragma unroll
+      for (int i = 0; i < KS / 2; ++i) {
+        const int ch = 2 * i + h;
+        const u32x4 w = *reinterpret_cast<const u32x4*>(s_k[buf] + k_place<D>(r, ch));
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          const uint32_t w0 = w[2 * z], w1 = w[2 * z + 1];
+          if constexpr (F16) {
+            const u32x4 a = {f16_pair<false>(w0), f16_pair<true>(w0), f16_pair<false>(w1),
+                             f16_pair<true>(w1)};
+            s[st] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                bits_as<f16x8>(a), bits_as<f16x8>(q[2 * i + z]), s[st], 0, 0, 0);
+          } else {
+            const u32x4 a = {bf16_pair<false>(w0, fk), bf16_pair<true>(w0, fk),
+                             bf16_pair<false>(w1, fk), bf16_pair<true>(w1, fk)};
+            s[st] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                bits_as<bf16x8>(a), bits_as<bf16x8>(q[2 * i + z]), s[st], 0, 0, 0);
+          }
+        }
+      }
+    }
+    if constexpr (F16) {
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[st][i] *= pow2(ek[2 * st + (i >> 3)]);
+    }
+    // register i of tile st: token at + 32 st + 8 (i / 4) + 4 h + i % 4
+    uint32_t see = ~0u;
+    if (masked) {
+      see = 0;
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const bool sees = at + 32 * st + 8 * (i >> 2) + 4 * h + (i & 3) < limit &&
+                            __builtin_amdgcn_readlane(id, n + 2 * st + (i >> 3)) >= 0;
+          s[st][i] = sees ? s[st][i] : -kInf;
+          see |= sees ? 1u << (16 * st + i) : 0u;
+        }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int st = 0; st < 2; ++st)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[st][i]);
+    top *= p.scale;
+    if (__any(top > m + kSlack)) {
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float now = fmaxf(m, top);
+      const float f = now == -kInf ? 1.0f : fast_exp2(m - now);
+      m = now;
+      l *= f;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[mt][i] *= f;
+    }
+    const float base = m == -kInf ? 0.0f : m;
+    const bool odd = masked && uni(s_odd[buf]) == at;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {  // 16 tokens each
+      float y[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        y[j] = fast_exp2(__builtin_fmaf(s[g >> 1][8 * (g & 1) + j], p.scale, -base));
+        l += y[j];
+      }
+      u32x4 ph, pl;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        ph[j] = round_pair(y[2 * j], y[2 * j + 1]);
+        if constexpr (F16)
+          pl[j] = round_pair(y[2 * j] - __uint_as_float(ph[j] << 16),
+                             y[2 * j + 1] - __uint_as_float(ph[j] & 0xFFFF0000u));
+      }
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        const int r = 32 * mt + c;
+        u32x4 a = *reinterpret_cast<const u32x4*>(s_v[buf] + r * 128 +
+                                                  (((2 * g + h) ^ ((r >> 1) & 7)) << 4));
+        if (odd) {  // NaNs out of the product, and into exactly the rows that see them
+          u32x4 bad, ones;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const bool n0 = (a[j] & 0x7FFFu) > 0x7F80u, n1 = (a[j] & 0x7FFF0000u) > 0x7F800000u;
+            bad[j] = (n0 ? 0x3F80u : 0u) | (n1 ? 0x3F800000u : 0u);
+            a[j] &= (n0 ? 0u : 0xFFFFu) | (n1 ? 0u : 0xFFFF0000u);
+            ones[j] = ((see >> (8 * g + 2 * j)) & 1u ? 0x3F80u : 0u) |
+                      ((see >> (8 * g + 2 * j + 1)) & 1u ? 0x3F800000u : 0u);
+          }
+          f32x16 hit;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) hit[i] = 0.0f;
+          hit = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bits_as<bf16x8>(bad), bits_as<bf16x8>(ones),
+                                                        hit, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[mt][i] = hit[i] > 0.0f ? __builtin_nanf("") : o[mt][i];
+        }
+        o[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bits_as<bf16x8>(a), bits_as<bf16x8>(ph),
+                                                        o[mt], 0, 0, 0);
+        if constexpr (F16)
+          o[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bits_as<bf16x8>(a), bits_as<bf16x8>(pl),
+                                                          o[mt], 0, 0, 0);
+      }
+    }
+  };
+
+  if (k0 < k1) {
+    look_up(k0);
+    fetch(k0, 0);
+    __syncthreads();  // s_odd is set
+    stage(k0, 0, 0);
+    __syncthreads();
+    int n = 0, buf = 0;  // the step's first group among those looked up, and its buffer
+    for (int at = k0; at < k1; at += 64, buf ^= 1) {
+      // of the step's groups: kept for the computation where the next look-up replaces them
+      const bool more = at + 64 < k1;
+      if (n < 60) {
+        if (more) fetch(at + 64, n + 4);
+        if (at < most) compute(at, n, buf);
+        if (more) stage(at + 64, n + 4, buf ^ 1);
+        n += 4;
+      } else {
+        if (at < most) compute(at, n, buf);
+        if (more) {
+          look_up(at + 64);
+          fetch(at + 64, 0);
+          stage(at + 64, 0, buf ^ 1);
+        }
+        n = 0;
+      }
+      __syncthreads();
+    }
+  }
+
+  l += __shfl_xor(l, 32);
+  const int i = wave * 32 + c;
+  if (!there) return;
+  if (t.parts > 1) {
+    const int64_t at = (static_cast<int64_t>(tile) * p.c.heads + head) * p.splits + part;
+    if (h == 0) {
+      p.part_ml[(at * kManyRows + i) * 2] = m;
+      p.part_ml[(at * kManyRows + i) * 2 + 1] = l;
+    }
+    float* to = p.part_o + (at * kManyRows + i) * D;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {  // dimensions W * d + 0..W-1, two of each mt
+      const int d = 8 * (e >> 2) + 4 * h + (e & 3);
+#pragma unroll
+      for (int mt = 0; mt < MT; mt += 2)
+        *reinterpret_cast<f32x4*>(to + W * d + 2 * mt) =
+            f32x4{o[mt][e], o[mt][e + 8], o[mt + 1][e], o[mt + 1][e + 8]};
+    }
+  } else {
+    const float by = l == 0.0f ? 0.0f : 1.0f / l;
+    char* to = p.out + (t.s0 + row / p.group) * p.out_token +
+               (static_cast<int64_t>(head) * p.group + row % p.group) * p.out_head;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int d = 8 * (e >> 2) + 4 * h + (e & 3);
+#pragma unroll
+      for (int mt = 0; mt < MT; mt += 2)
+        *reinterpret_cast<u32x2*>(to + (W * d + 2 * mt) * 2) =
+            u32x2{out_pair<F16>(o[mt][e] * by, o[mt][e + 8] * by),
+                  out_pair<F16>(o[mt + 1][e] * by, o[mt + 1][e + 8] * by)};
+    }
+  }
+}
+
 // ------------------------------------------------------------------ the parts' results joined
 
-template <bool F16, int D, int BM>
+// A workgroup joins one row of a tile and KV head where there are many parts and few rows
+// (NG > 1: NG groups of D / 4 lanes take turns at the parts), or 256 / (D / 4) rows.
+
+template <bool F16, int D, int BM, bool MANY>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p) {
+  constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
+  __shared__ float s_f[kMaxSplits];
+  __shared__ float s_red[4];
+  __shared__ f32x4 s_o[kGroups][kLanes];
   Tile t;
   if (!find_tile<BM>(p, blockIdx.x, t) || t.parts <= 1) return;
-  const int head = blockIdx.y;
+  const int head = blockIdx.y, d = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
   const int64_t at = (static_cast<int64_t>(blockIdx.x) * p.c.heads + head) * p.splits;
-  for (int i = threadIdx.x; i < t.rows * (D / 4); i += 256) {
-    const int row = i / (D / 4), d = i % (D / 4) * 4;
-    float top = -kInf;
-    for (int s = 0; s < t.parts; ++s) top = fmaxf(top, p.part_ml[((at + s) * BM + row) * 2]);
-    const float base = top == -kInf ? 0.0f : top;
-    float sum = 0.0f;
+  const int step = MANY ? gridDim.z : gridDim.z * kGroups;
+  for (int row = MANY ? blockIdx.z : blockIdx.z * kGroups + grp; row < t.rows; row += step) {
     f32x4 o = {0, 0, 0, 0};
-    for (int s = 0; s < t.parts; ++s) {
-      const float* ml = p.part_ml + ((at + s) * BM + row) * 2;
-      const float f = fast_exp2(ml[0] - base);
-      sum += ml[1] * f;
-      o += *reinterpret_cast<const f32x4*>(p.part_o + ((at + s) * BM + row) * D + d) * f;
+    float sum = 0.0f;
+    if constexpr (MANY) {
+      const int tid = threadIdx.x;
+      float m = -kInf, l = 0.0f;
+      if (tid < t.parts) {
+        const float* ml = p.part_ml + ((at + tid) * BM + row) * 2;
+        m = ml[0];
+        l = ml[1];
+      }
+      float top = m;
+      for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+      __syncthreads();  // the last row's reads are done
+      if ((tid & 63) == 0) s_red[tid >> 6] = top;
+      __syncthreads();
+      top = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+      const float f = fast_exp2(m - (top == -kInf ? 0.0f : top));
+      s_f[tid] = f;
+      float part = l * f;
+      for (int x = 32; x > 0; x >>= 1) part += __shfl_xor(part, x);
+      __syncthreads();
+      if ((tid & 63) == 0) s_red[tid >> 6] = part;
+#pragma unroll 4
+      for (int s = grp; s < t.parts; s += kGroups)
+        o += *reinterpret_cast<const f32x4*>(p.part_o + ((at + s) * BM + row) * D + 4 * d) * s_f[s];
+      s_o[grp][d] = o;
+      __syncthreads();
+      sum = s_red[0] + s_red[1] + s_red[2] + s_red[3];
+      if (grp != 0) continue;
+#pragma unroll
+      for (int i = 1; i < kGroups; ++i) o += s_o[i][d];
+    } else {
+      float top = -kInf;
+      for (int s = 0; s < t.parts; ++s) top = fmaxf(top, p.part_ml[((at + s) * BM + row) * 2]);
+      const float base = top == -kInf ? 0.0f : top;
+      for (int s = 0; s < t.parts; ++s) {
+        const float* ml = p.part_ml + ((at + s) * BM + row) * 2;
+        const float f = fast_exp2(ml[0] - base);
+        sum += ml[1] * f;
+        o += *reinterpret_cast<const f32x4*>(p.part_o + ((at + s) * BM + row) * D + 4 * d) * f;
+      }
     }
     o *= sum == 0.0f ? 0.0f : 1.0f / sum;
     const int64_t r = t.row0 + row;
     char* to = p.out + (t.s0 + r / p.group) * p.out_token +
                (static_cast<int64_t>(head) * p.group + r % p.group) * p.out_head;
-    u32x2 w;
-    if constexpr (F16)
-      w = u32x2{bits_as<uint32_t>(f16x2{static_cast<_Float16>(o[0]), static_cast<_Float16>(o[1])}),
-                bits_as<uint32_t>(f16x2{static_cast<_Float16>(o[2]), static_cast<_Float16>(o[3])})};
-    else
-      w = u32x2{round_pair(o[0], o[1]), round_pair(o[2], o[3])};
-    *reinterpret_cast<u32x2*>(to + d * 2) = w;
+    *reinterpret_cast<u32x2*>(to + d * 8) =
+        u32x2{out_pair<F16>(o[0], o[1]), out_pair<F16>(o[2], o[3])};
   }
 }
 
@@ -530,15 +960,22 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p) {
 // How a call runs: rows a tile has, tiles, and the parts that a tile's tokens may be cut into.
 struct Shape {
   int rows;
+  int64_t each;  // rows of the largest request
   int64_t tiles;
   int splits;
 };
+
+constexpr int64_t kWantFew = 4096;
+#ifndef MKV_WM
+#define MKV_WM 1024
+#endif
+constexpr int64_t kWantMany = MKV_WM;
 
 int check(const mkv_attend_desc_t& d, AttendParams* p, Shape* shape) {
   const char* who = "mkv_attend_scaled";
   int rc = check_cache(who, d.cache, true, &p->c);
   if (rc == MKV_OK)
-    rc = check_step(who, d.block_tables, d.table_stride, d.table_width, d.starts, d.lens,
+    rc = check_step(who, d.cache.block_size, d.block_tables, d.table_stride, d.table_width, d.starts, d.lens,
                     d.requests, d.error_flags, &p->s);
   if (rc != MKV_OK) return rc;
   if (d.dtype != MKV_BF16 && d.dtype != MKV_F16)
@@ -569,18 +1006,23 @@ int check(const mkv_attend_desc_t& d, AttendParams* p, Shape* shape) {
 
   const int64_t rows = d.tokens * p->group;
   const int64_t each = static_cast<int64_t>(d.max_new > 0 ? d.max_new : d.tokens) * p->group;
-  shape->rows = each <= 16 ? 16 : 32;
+  shape->each = each;
+  shape->rows = each <= 16 ? 16 : each <= 32 ? 32 : kManyRows;
   shape->tiles = rows / shape->rows + d.requests;
-  // parts: enough workgroups for three on each of 256 CUs, none under kMinSplit tokens
+  // Parts of one size for all requests, so that long and short histories fill the chip alike:
+  // about `want` workgroups if every request were the longest.
   const int64_t room = static_cast<int64_t>(d.table_width) * d.cache.block_size;
   const int64_t longest = d.max_len > 0 && d.max_len < room ? d.max_len : room;
-  const int64_t groups = shape->tiles * d.cache.heads;
-  int64_t splits = groups > 0 ? (768 + groups - 1) / groups : 1;
-  const int64_t most_parts = (longest + kMinSplit - 1) / kMinSplit;
-  splits = splits > most_parts ? most_parts : splits;
-  splits = splits < 1 ? 1 : splits > 256 ? 256 : splits;
-  shape->splits = static_cast<int>(splits);
+  const int64_t largest = (each + shape->rows - 1) / shape->rows;  // tiles of one request
+  const int64_t busy = rows / shape->rows + d.requests;
+  const int64_t groups = (busy < largest * d.requests ? busy : largest * d.requests) * d.cache.heads;
+  const int64_t want = shape->rows == kManyRows ? kWantMany : kWantFew;
+  int64_t per = longest * (groups > 0 ? groups : 1) / want;
+  if (per < longest / kMaxSplits + 64) per = longest / kMaxSplits + 64;
+  per = ((per < kMinSplit ? kMinSplit : per) + 63) / 64 * 64;
+  shape->splits = static_cast<int>(longest > per ? (longest + per - 1) / per : 1);
   p->splits = shape->splits;
+  p->per = static_cast<int>(per);
   if (shape->tiles > INT32_MAX)
     return mkv_fail(MKV_ERR_UNSUPPORTED, "%s: %lld tiles", who, (long long)shape->tiles);
   return MKV_OK;
@@ -594,17 +1036,22 @@ template <bool F16, int D, int RT>
 void launch_few(const AttendParams& p, const Shape& s, int heads, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(s.tiles), heads, s.splits);
   attend_few_kernel<F16, D, RT><<<grid, 64 * kFewWaves, 0, stream>>>(p);
-  if (s.splits > 1)
-    attend_join_kernel<F16, D, 16 * RT>
-        <<<dim3(static_cast<unsigned>(s.tiles), heads), 256, 0, stream>>>(p);
+  if (s.splits > 1) {
+    const unsigned rows = static_cast<unsigned>(s.each < 16 * RT ? (s.each > 0 ? s.each : 1) : 16 * RT);
+    attend_join_kernel<F16, D, 16 * RT, true>
+        <<<dim3(static_cast<unsigned>(s.tiles), heads, rows), 256, 0, stream>>>(p);
+  }
 }
 
 template <bool F16, int D>
 void launch(const AttendParams& p, const Shape& s, int heads, hipStream_t stream) {
-  if (s.rows == 16)
-    launch_few<F16, D, 1>(p, s, heads, stream);
-  else
-    launch_few<F16, D, 2>(p, s, heads, stream);
+  if (s.rows == 16) return launch_few<F16, D, 1>(p, s, heads, stream);
+  if (s.rows == 32) return launch_few<F16, D, 2>(p, s, heads, stream);
+  const unsigned tiles = static_cast<unsigned>(s.tiles);
+  attend_many_kernel<F16, D><<<dim3(heads, tiles, s.splits), 64 * kManyWaves, 0, stream>>>(p);
+  if (s.splits > 1)
+    attend_join_kernel<F16, D, kManyRows, false>
+        <<<dim3(tiles, heads, kManyRows * D / 1024), 256, 0, stream>>>(p);
 }
 
 template <bool F16>

@@ -117,8 +117,8 @@ inline int check_cache(const char* who, const mkv_scaled_cache_t& c, bool bases,
 }
 
 // Host: the step's arrays.
-inline int check_step(const char* who, const int32_t* tables, int64_t table_stride,
-                      int32_t table_width, const int32_t* starts, const int32_t* lens,
+inline int check_step(const char* who, int32_t block_size, const int32_t* tables,
+                      int64_t table_stride, int32_t table_width, const int32_t* starts, const int32_t* lens,
                       int32_t requests, int32_t* flags, DevStep* out) {
   if (requests < 0 || requests > MKV_MAX_REQUESTS)
     return mkv_fail(MKV_ERR_ARG, "%s: requests %d outside [0, %d]", who, requests,
@@ -126,6 +126,8 @@ inline int check_step(const char* who, const int32_t* tables, int64_t table_stri
   if (table_width < 0 || table_stride < 0)
     return mkv_fail(MKV_ERR_ARG, "%s: block table of width %d, stride %lld", who, table_width,
                     (long long)table_stride);
+  if (static_cast<int64_t>(table_width) * block_size > (1 << 30))
+    return mkv_fail(MKV_ERR_UNSUPPORTED, "%s: block tables of more than 2^30 tokens", who);
   if (requests > 0 &&
       (starts == nullptr || lens == nullptr || (tables == nullptr && table_width > 0)))
     return mkv_fail(MKV_ERR_ARG, "%s: starts, lens or block_tables is NULL", who);

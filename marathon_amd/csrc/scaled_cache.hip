@@ -617,7 +617,7 @@ extern "C" int mkv_store_scaled(const mkv_scaled_cache_t* cache, const void* k,
   StoreParams p;
   int rc = check_cache(who, *cache, true, &p.c);
   if (rc == MKV_OK)
-    rc = check_step(who, block_tables, table_stride, table_width, starts, lens, requests,
+    rc = check_step(who, cache->block_size, block_tables, table_stride, table_width, starts, lens, requests,
                     error_flags, &p.s);
   if (rc != MKV_OK) return rc;
   if (dtype != MKV_BF16 && dtype != MKV_F16 && dtype != MKV_F32)
