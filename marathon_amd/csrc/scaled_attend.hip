@@ -317,8 +317,9 @@ __global__ __launch_bounds__(64 * kFewWaves, (few_waves<D, RT>())) void attend_f
         }
       }
     }
-    // what lies in rows that nobody sees must not reach the products: NaN codes times 0
-    bool odd = false;  // a NaN in V where some rows see a token and others do not
+    // What lies in rows that nobody sees must not reach the products, NaN codes times 0; nor
+    // NaNs in V that only some rows see: those are noted, and marked behind the products.
+    bool odd = false;
     if (masked) {
       uint32_t any = 0;
 #pragma unroll
@@ -328,13 +329,15 @@ __global__ __launch_bounds__(64 * kFewWaves, (few_waves<D, RT>())) void attend_f
 #pragma unroll
         for (int u = 0; u < NQ; ++u) {
           x.v[j][u] = seen ? x.v[j][u] : 0u;
-          any |= nan_bytes(x.v[j][u]);
+          const uint32_t bad = nan_bytes(x.v[j][u]);
+          any |= bad;
+          x.v[j][u] &= ~((bad >> 7) * 255u);
         }
       }
       odd = __any(any != 0);
     }
     uint32_t ph[RT][4], pl[RT][4];  // P^T: pairs of tokens; and what bf16 leaves (F16)
-    uint32_t see[RT];               // odd: which of the lane's 8 tokens its row sees
+    uint32_t see[RT];               // masked: which of the lane's 8 tokens its row sees
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       float y[8];
@@ -396,15 +399,6 @@ __global__ __launch_bounds__(64 * kFewWaves, (few_waves<D, RT>())) void attend_f
           const uint32_t src = w < 2 ? even[j] : high[j];
           a[j] = (w & 1) ? bf16_pair<true>(src, fv[j >> 1]) : bf16_pair<false>(src, fv[j >> 1]);
         }
-        u32x4 bad;
-        if (odd) {  // NaNs out of the product, and into exactly the rows that see them
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const bool n0 = (a[j] & 0x7FFFu) > 0x7F80u, n1 = (a[j] & 0x7FFF0000u) > 0x7F800000u;
-            bad[j] = (n0 ? 0x3F80u : 0u) | (n1 ? 0x3F800000u : 0u);
-            a[j] &= (n0 ? 0u : 0xFFFFu) | (n1 ? 0u : 0xFFFF0000u);
-          }
-        }
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
           const u32x4 b = {ph[rt][0], ph[rt][1], ph[rt][2], ph[rt][3]};
@@ -415,18 +409,35 @@ __global__ __launch_bounds__(64 * kFewWaves, (few_waves<D, RT>())) void attend_f
             o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
                 bits_as<bf16x8>(a), bits_as<bf16x8>(b2), o[rt][dt], 0, 0, 0);
           }
-          if (odd) {
-            u32x4 ones;
+        }
+      }
+    }
+    if (odd) {  // counted into exactly the rows that see them
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              ones[j] = ((see[rt] >> (2 * j)) & 1u ? 0x3F80u : 0u) |
-                        ((see[rt] >> (2 * j + 1)) & 1u ? 0x3F800000u : 0u);
-            const f32x4 hit = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                bits_as<bf16x8>(bad), bits_as<bf16x8>(ones), f32x4{0, 0, 0, 0}, 0, 0, 0);
+      for (int dt = 0; dt < DT; ++dt) {
+        u32x4 bad = {0, 0, 0, 0};
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              o[rt][dt][r] = hit[r] > 0.0f ? __builtin_nanf("") : o[rt][dt][r];
-          }
+        for (int j = 0; j < 8; ++j) {
+          const int i = j >> 2, row = at + 16 * i + 4 * g + (j & 3);
+          bool nan = row < t.keys && ok[i];
+          if (nan)
+            nan = (p.c.v[max(__builtin_amdgcn_readlane(ids[i], n), 0) * p.c.bstride +
+                         head * static_cast<int64_t>(p.c.hstride) +
+                         (row & bs_mask) * static_cast<int64_t>(p.c.tstride) + DT * c + dt] &
+                   0x7F) == 0x7F;
+          bad[j >> 1] |= nan ? 0x3F80u << (16 * (j & 1)) : 0u;
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          u32x4 ones = {0, 0, 0, 0};
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            ones[j >> 1] |= (see[rt] >> j) & 1u ? 0x3F80u << (16 * (j & 1)) : 0u;
+          const f32x4 hit = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              bits_as<bf16x8>(bad), bits_as<bf16x8>(ones), f32x4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            o[rt][dt][r] = hit[r] > 0.0f ? __builtin_nanf("") : o[rt][dt][r];
         }
       }
     }
@@ -574,21 +585,24 @@ __global__ __launch_bounds__(64 * kManyWaves, (D == 256 ? 1 : 2)) void attend_ma
   const int k0 = part * t.per, k1 = min(t.keys, k0 + t.per);
   if (tid < 2) s_odd[tid] = -1;
 
-  // ids and scales of the next 64 groups of 16 tokens, one a lane
+  // ids and scales of 64 groups of 16 tokens, one a lane; and those of the 64 behind them
   const int32_t* table = p.s.tables + t.request * p.s.table_stride;
-  int id = -1, scale = 0;
+  struct Groups {
+    int id, scale;
+  };
   const auto look_up = [&](int at) {
-    const int tok = min(at + 16 * lane, t.keys - 1);
-    id = -1;
-    scale = 127 | (127 << 8);
-    if (t.keys > 0) id = table[tok >> p.c.bs_shift];
-    if (id < 0 || id >= p.c.num_blocks) {
-      if (wave == 0 && t.keys > 0) raise(p.s.flags, MKV_FLAG_SRC_RANGE);
-      id = -1;
-    } else {
-      scale = *reinterpret_cast<const uint16_t*>(
-          p.c.scales + (static_cast<int64_t>(id) * p.c.heads + head) * 2);
+    Groups x = {-1, 127 | (127 << 8)};
+    if (at < k1) {
+      x.id = table[min(at + 16 * lane, t.keys - 1) >> p.c.bs_shift];
+      if (x.id < 0 || x.id >= p.c.num_blocks) {
+        if (wave == 0) raise(p.s.flags, MKV_FLAG_SRC_RANGE);
+        x.id = -1;
+      } else {
+        x.scale = *reinterpret_cast<const uint16_t*>(
+            p.c.scales + (static_cast<int64_t>(x.id) * p.c.heads + head) * 2);
+      }
     }
+    return x;
   };
 
   // this wave's rows: operand B of S^T = K Q^T, dimensions 32 i + 16 h + 0..15
@@ -626,21 +640,21 @@ __global__ __launch_bounds__(64 * kManyWaves, (D == 256 ? 1 : 2)) void attend_ma
   u32x4 rk[kKLoads];
   uint32_t rv[4][D / 64];
   const int bs_mask = (1 << p.c.bs_shift) - 1;
-  const auto block_of = [&](int n) {  // the block of group n of the looked-up ones
-    return max(__builtin_amdgcn_readlane(id, n), 0) * p.c.bstride +
+  const auto block_of = [&](const Groups& x, int n) {
+    return max(__builtin_amdgcn_readlane(x.id, n), 0) * p.c.bstride +
            head * static_cast<int64_t>(p.c.hstride);
   };
   constexpr int kRowsPass = 256 / KC;  // rows that one pass over the threads covers
-  const auto fetch = [&](int at, int n) {  // n: the step's first group
+  const auto fetch = [&](int at, const Groups& x, int n) {  // n: the step's first group in x
 #pragma unroll
     for (int u = 0; u < kKLoads; ++u) {
       const int r = u * kRowsPass + tid / KC;  // D = 64: 64 rows; 128: 32; 256: 16
       // the wave's rows lie in one group: 16, 8 or 4 rows a wave
       const int grp = uni((u * kRowsPass + wave * (64 / KC)) >> 4);
-      const char* kb = p.c.k + block_of(n + grp) + ((at + r) & bs_mask) * static_cast<int64_t>(p.c.tstride);
+      const char* kb = p.c.k + block_of(x, n + grp) + ((at + r) & bs_mask) * static_cast<int64_t>(p.c.tstride);
       rk[u] = *reinterpret_cast<const u32x4*>(kb + 16 * (tid % KC));
     }
-    const char* vb = p.c.v + block_of(n + wave) +
+    const char* vb = p.c.v + block_of(x, n + wave) +
                      ((at + 4 * (tid >> 4)) & bs_mask) * static_cast<int64_t>(p.c.tstride) +
                      W * (tid & 15);
 #pragma unroll
@@ -659,15 +673,16 @@ __global__ __launch_bounds__(64 * kManyWaves, (D == 256 ? 1 : 2)) void attend_ma
       }
     }
   };
-  const auto stage = [&](int at, int n, int buf) {
+  const auto stage = [&](int at, const Groups& x, int n, int buf) {
 #pragma unroll
     for (int u = 0; u < kKLoads; ++u) {
       const int r = u * kRowsPass + tid / KC, ch = tid % KC;
       *reinterpret_cast<u32x4*>(s_k[buf] + k_place<D>(r, ch)) = rk[u];
     }
-    const bool good = __builtin_amdgcn_readlane(id, n + wave) >= 0;
+    const bool good = __builtin_amdgcn_readlane(x.id, n + wave) >= 0;
     if (at + 64 > t.full || !good) {
-      // what nobody sees must not reach the products, NaN codes times 0
+      // what nobody sees must not reach the products, NaN codes times 0; nor NaNs that only
+      // some rows see: those are noted, and marked behind the products
       uint32_t any = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -675,12 +690,14 @@ __global__ __launch_bounds__(64 * kManyWaves, (D == 256 ? 1 : 2)) void attend_ma
 #pragma unroll
         for (int u = 0; u < D / 64; ++u) {
           rv[i][u] = seen ? rv[i][u] : 0u;
-          any |= nan_bytes(rv[i][u]);
+          const uint32_t bad = nan_bytes(rv[i][u]);
+          any |= bad;
+          rv[i][u] &= ~((bad >> 7) * 255u);
         }
       }
       if (any != 0) s_odd[buf] = at;
     }
-    const float f = pow2(scale_exp(__builtin_amdgcn_readlane(scale, n + wave) >> 8));
+    const float f = pow2(scale_exp(__builtin_amdgcn_readlane(x.scale, n + wave) >> 8));
     // tokens 16 t + 4 quad + i: chunk 2 t + (quad & 1), its half quad / 2
     const int quad = (tid >> 4) & 3, chunk = 2 * wave + (quad & 1), half = quad >> 1;
 #pragma unroll
@@ -702,13 +719,13 @@ __global__ __launch_bounds__(64 * kManyWaves, (D == 256 ? 1 : 2)) void attend_ma
     }
   };
 
-  const auto compute = [&](int at, int n, int buf) {
+  const auto compute = [&](int at, const Groups& x, int n, int buf) {
     bool masked = at + 64 > t.full;
     int ek[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      masked |= __builtin_amdgcn_readlane(id, n + i) < 0;
-      ek[i] = scale_exp(__builtin_amdgcn_readlane(scale, n + i) & 0xFF);
+      masked |= __builtin_amdgcn_readlane(x.id, n + i) < 0;
+      ek[i] = scale_exp(__builtin_amdgcn_readlane(x.scale, n + i) & 0xFF);
     }
     f32x16 s[2];
 #pragma unroll
@@ -753,7 +770,7 @@ __global__ __launch_bounds__(64 * kManyWaves, (D == 256 ? 1 : 2)) void attend_ma
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const bool sees = at + 32 * st + 8 * (i >> 2) + 4 * h + (i & 3) < limit &&
-                            __builtin_amdgcn_readlane(id, n + 2 * st + (i >> 3)) >= 0;
+                            __builtin_amdgcn_readlane(x.id, n + 2 * st + (i >> 3)) >= 0;
           s[st][i] = sees ? s[st][i] : -kInf;
           see |= sees ? 1u << (16 * st + i) : 0u;
         }
@@ -776,79 +793,87 @@ __global__ __launch_bounds__(64 * kManyWaves, (D == 256 ? 1 : 2)) void attend_ma
         for (int i = 0; i < 16; ++i) o[mt][i] *= f;
     }
     const float base = m == -kInf ? 0.0f : m;
-    const bool odd = masked && uni(s_odd[buf]) == at;
+    u32x4 ph[4], pl[4];  // P^T: 16 tokens each; and what bf16 leaves of it (F16)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {  // 16 tokens each
+    for (int g = 0; g < 4; ++g) {
       float y[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         y[j] = fast_exp2(__builtin_fmaf(s[g >> 1][8 * (g & 1) + j], p.scale, -base));
         l += y[j];
       }
-      u32x4 ph, pl;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        ph[j] = round_pair(y[2 * j], y[2 * j + 1]);
+        ph[g][j] = round_pair(y[2 * j], y[2 * j + 1]);
         if constexpr (F16)
-          pl[j] = round_pair(y[2 * j] - __uint_as_float(ph[j] << 16),
-                             y[2 * j + 1] - __uint_as_float(ph[j] & 0xFFFF0000u));
+          pl[g][j] = round_pair(y[2 * j] - __uint_as_float(ph[g][j] << 16),
+                                y[2 * j + 1] - __uint_as_float(ph[g][j] & 0xFFFF0000u));
       }
+    }
+    asm volatile("" : "+v"(l));  // summed here: sunk below the products, 32 terms stay live
+    const auto v_of = [&](int g, int mt) {
+      const int r = 32 * mt + c;
+      return *reinterpret_cast<const u32x4*>(s_v[buf] + r * 128 + (((2 * g + h) ^ ((r >> 1) & 7)) << 4));
+    };
+    const auto times = [&](u32x4 a, u32x4 b, f32x16 z) {
+      return __builtin_amdgcn_mfma_f32_32x32x16_bf16(bits_as<bf16x8>(a), bits_as<bf16x8>(b), z, 0, 0, 0);
+    };
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        const int r = 32 * mt + c;
-        u32x4 a = *reinterpret_cast<const u32x4*>(s_v[buf] + r * 128 +
-                                                  (((2 * g + h) ^ ((r >> 1) & 7)) << 4));
-        if (odd) {  // NaNs out of the product, and into exactly the rows that see them
-          u32x4 bad, ones;
+        const u32x4 a = v_of(g, mt);
+        o[mt] = times(a, ph[g], o[mt]);
+        if constexpr (F16) o[mt] = times(a, pl[g], o[mt]);
+      }
+    }
+    if (masked && uni(s_odd[buf]) == at) {
+      // NaNs in V that some rows see and others do not: counted into exactly the rows that do
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const bool n0 = (a[j] & 0x7FFFu) > 0x7F80u, n1 = (a[j] & 0x7FFF0000u) > 0x7F800000u;
-            bad[j] = (n0 ? 0x3F80u : 0u) | (n1 ? 0x3F800000u : 0u);
-            a[j] &= (n0 ? 0u : 0xFFFFu) | (n1 ? 0u : 0xFFFF0000u);
-            ones[j] = ((see >> (8 * g + 2 * j)) & 1u ? 0x3F80u : 0u) |
-                      ((see >> (8 * g + 2 * j + 1)) & 1u ? 0x3F800000u : 0u);
+      for (int mt = 0; mt < MT; ++mt) {
+        const int r = 32 * mt + c, d = W * (r & 15) + (r >> 4);
+        f32x16 hit;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) hit[i] = 0.0f;
+#pragma unroll 1
+        for (int g = 0; g < 4; ++g) {
+          const char* vb = p.c.v + block_of(x, n + g) + d;
+          u32x4 bad = {0, 0, 0, 0}, ones = {0, 0, 0, 0};
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int tok = at + 16 * g + 8 * (j >> 2) + 4 * h + (j & 3);
+            bool nan = tok < t.keys && __builtin_amdgcn_readlane(x.id, n + g) >= 0;
+            if (nan) nan = (vb[(tok & bs_mask) * static_cast<int64_t>(p.c.tstride)] & 0x7F) == 0x7F;
+            bad[j >> 1] |= nan ? 0x3F80u << (16 * (j & 1)) : 0u;
+            ones[j >> 1] |= (see >> (8 * g + j)) & 1u ? 0x3F80u << (16 * (j & 1)) : 0u;
           }
-          f32x16 hit;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) hit[i] = 0.0f;
-          hit = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bits_as<bf16x8>(bad), bits_as<bf16x8>(ones),
-                                                        hit, 0, 0, 0);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[mt][i] = hit[i] > 0.0f ? __builtin_nanf("") : o[mt][i];
+          hit = times(bad, ones, hit);
         }
-        o[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bits_as<bf16x8>(a), bits_as<bf16x8>(ph),
-                                                        o[mt], 0, 0, 0);
-        if constexpr (F16)
-          o[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bits_as<bf16x8>(a), bits_as<bf16x8>(pl),
-                                                          o[mt], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[mt][i] = hit[i] > 0.0f ? __builtin_nanf("") : o[mt][i];
       }
     }
   };
 
   if (k0 < k1) {
-    look_up(k0);
-    fetch(k0, 0);
+    Groups now = look_up(k0), next = look_up(k0 + 1024);
+    fetch(k0, now, 0);
     __syncthreads();  // s_odd is set
-    stage(k0, 0, 0);
+    stage(k0, now, 0, 0);
     __syncthreads();
-    int n = 0, buf = 0;  // the step's first group among those looked up, and its buffer
+    int n = 0, buf = 0;  // the step's first group in `now`, and its buffer
     for (int at = k0; at < k1; at += 64, buf ^= 1) {
-      // of the step's groups: kept for the computation where the next look-up replaces them
       const bool more = at + 64 < k1;
-      if (n < 60) {
-        if (more) fetch(at + 64, n + 4);
-        if (at < most) compute(at, n, buf);
-        if (more) stage(at + 64, n + 4, buf ^ 1);
-        n += 4;
-      } else {
-        if (at < most) compute(at, n, buf);
-        if (more) {
-          look_up(at + 64);
-          fetch(at + 64, 0);
-          stage(at + 64, 0, buf ^ 1);
-        }
-        n = 0;
+      const int n1 = (n + 4) & 63;
+      const Groups then = n1 == 0 ? next : now;
+      if (more) fetch(at + 64, then, n1);
+      if (at < most) compute(at, now, n, buf);
+      if (more) stage(at + 64, then, n1, buf ^ 1);
+      if (n1 == 0) {
+        now = next;
+        next = look_up(at + 64 + 1024);
       }
+      n = n1;
       __syncthreads();
     }
   }
