@@ -546,10 +546,11 @@ __global__ __launch_bounds__(64 * kFewWaves, (few_waves<D, RT>())) void attend_f
 //
 // Bound by the matrix products and the softmax's vector work, about even.  A workgroup's four
 // waves hold 32 rows each of a tile of 128 and one KV head and walk the tokens together, 64 a
-// step (32x32x16 products).  K's codes go to LDS as they are (half of bf16's LDS reads; each
-// wave decodes them, 64 conversions for 32 products); V is decoded and transposed once for all
-// waves on its way there, so that a lane reads 8 tokens of one dimension in 16 bytes.  Both
-// are read without bank conflicts: a row's 16-byte chunks are exchanged by its number, so that
+// step (32x32x16 products).  Codes are decoded once for all waves on their way to LDS, V
+// transposed besides, so that a lane reads 8 dimensions of a token of K, and 8 tokens of a
+// dimension of V, in 16 bytes.  (K kept as codes there halves its reads, but each wave then
+// decodes it again, 64 conversions for 32 products: 1,168 us against 1,060 for a chunk of 2,048
+// over 22,141 tokens.)  Both are read without bank conflicts: a row's 16-byte chunks are exchanged by its number, so that
 // 16 rows' chunks of one column cover the 64 banks.
 // The next step's codes are loaded into registers before a step is computed and written to
 // the other of two buffers behind it: one barrier a step.  Two workgroups fit a CU, and one
@@ -558,20 +559,18 @@ __global__ __launch_bounds__(64 * kFewWaves, (few_waves<D, RT>())) void attend_f
 constexpr int kManyWaves = 4;
 constexpr int kManyRows = 32 * kManyWaves;
 
-// Where chunk `ch` of K's row r lies: rows of 64, 128 or 256 bytes.
+// Where chunk `ch` (8 values) of K's row r lies: rows of 128, 256 or 512 bytes.
 template <int D>
 __device__ __forceinline__ int k_place(int r, int ch) {
-  const int turn = D == 64 ? (r >> 2) & 3 : D == 128 ? (r >> 1) & 7 : r & 15;
-  return r * D + ((ch ^ turn) << 4);
+  return r * (2 * D) + ((ch ^ (D == 64 ? (r >> 1) & 7 : r & 15)) << 4);
 }
 
 template <bool F16, int D>
 __global__ __launch_bounds__(64 * kManyWaves, (D == 256 ? 1 : 2)) void attend_many_kernel(AttendParams p) {
   constexpr int KS = D / 16, MT = D / 32, W = D / 16, KC = D / 16;
-  constexpr int kKBytes = 64 * D, kVBytes = 128 * D;  // of a step
-  constexpr int kKLoads = kKBytes / 16 / 256 > 0 ? kKBytes / 16 / 256 : 1;
-  __shared__ __attribute__((aligned(16))) char s_k[2][kKBytes];
-  __shared__ __attribute__((aligned(16))) char s_v[2][kVBytes];
+  constexpr int kKLoads = 64 * D / 16 / 256;
+  __shared__ __attribute__((aligned(16))) char s_k[2][128 * D];
+  __shared__ __attribute__((aligned(16))) char s_v[2][128 * D];
   __shared__ int s_odd[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
   const int c = lane & 31, h = lane >> 5;
@@ -605,7 +604,7 @@ __global__ __launch_bounds__(64 * kManyWaves, (D == 256 ? 1 : 2)) void attend_ma
     return x;
   };
 
-  // this wave's rows: operand B of S^T = K Q^T, dimensions 32 i + 16 h + 0..15
+  // this wave's rows: operand B of S^T = K Q^T
   const int64_t row = t.row0 + wave * 32 + c;
   const bool there = wave * 32 + c < t.rows;
   u32x4 q[KS];
@@ -621,7 +620,7 @@ __global__ __launch_bounds__(64 * kManyWaves, (D == 256 ? 1 : 2)) void attend_ma
                        (static_cast<int64_t>(head) * p.group + row % p.group) * p.q_head;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
-        q[ks] = *reinterpret_cast<const u32x4*>(at + (32 * (ks / 2) + 16 * h + 8 * (ks & 1)) * 2);
+        q[ks] = *reinterpret_cast<const u32x4*>(at + (16 * ks + 8 * h) * 2);
     }
   }
   int most = limit;  // tokens that some row of the wave sees
@@ -644,22 +643,28 @@ __global__ __launch_bounds__(64 * kManyWaves, (D == 256 ? 1 : 2)) void attend_ma
     return max(__builtin_amdgcn_readlane(x.id, n), 0) * p.c.bstride +
            head * static_cast<int64_t>(p.c.hstride);
   };
-  constexpr int kRowsPass = 256 / KC;  // rows that one pass over the threads covers
+  // A wave's rows of a load lie in one group of 16 tokens: a scalar base, and offsets that
+  // never change.  K: 16, 8 or 4 rows a load; V: 16 tokens.
+  constexpr int kRowsPass = 256 / KC;  // rows that one load of all threads covers
+  const uint32_t k_off = (tid / KC % 16) * p.c.tstride + 16 * (tid % KC);
+  const uint32_t v_off = 4 * (tid >> 4 & 3) * p.c.tstride + W * (tid & 15);
+  const auto k_group = [&](int u) { return (u * kRowsPass + wave * (64 / KC)) >> 4; };
+  const auto k_row = [&](int u) { return u * kRowsPass + tid / KC; };
   const auto fetch = [&](int at, const Groups& x, int n) {  // n: the step's first group in x
 #pragma unroll
     for (int u = 0; u < kKLoads; ++u) {
-      const int r = u * kRowsPass + tid / KC;  // D = 64: 64 rows; 128: 32; 256: 16
-      // the wave's rows lie in one group: 16, 8 or 4 rows a wave
-      const int grp = uni((u * kRowsPass + wave * (64 / KC)) >> 4);
-      const char* kb = p.c.k + block_of(x, n + grp) + ((at + r) & bs_mask) * static_cast<int64_t>(p.c.tstride);
-      rk[u] = *reinterpret_cast<const u32x4*>(kb + 16 * (tid % KC));
+      const int g = k_group(u);
+      const char* kb = p.c.k + block_of(x, n + g) +
+                       ((at + 16 * g) & bs_mask) * static_cast<int64_t>(p.c.tstride);
+      // rows of one load past the 16th of the block's group (D = 256: four loads a group)
+      const int down = (u * kRowsPass + wave * (64 / KC)) % 16 - wave * (64 / KC) % 16;
+      rk[u] = *reinterpret_cast<const u32x4*>(kb + down * static_cast<int64_t>(p.c.tstride) + k_off);
     }
     const char* vb = p.c.v + block_of(x, n + wave) +
-                     ((at + 4 * (tid >> 4)) & bs_mask) * static_cast<int64_t>(p.c.tstride) +
-                     W * (tid & 15);
+                     ((at + 16 * wave) & bs_mask) * static_cast<int64_t>(p.c.tstride);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const char* a = vb + i * p.c.tstride;
+      const char* a = vb + i * static_cast<int64_t>(p.c.tstride) + v_off;
       if constexpr (D == 64) {
         rv[i][0] = *reinterpret_cast<const uint32_t*>(a);
       } else if constexpr (D == 128) {
@@ -676,8 +681,19 @@ __global__ __launch_bounds__(64 * kManyWaves, (D == 256 ? 1 : 2)) void attend_ma
   const auto stage = [&](int at, const Groups& x, int n, int buf) {
 #pragma unroll
     for (int u = 0; u < kKLoads; ++u) {
-      const int r = u * kRowsPass + tid / KC, ch = tid % KC;
-      *reinterpret_cast<u32x4*>(s_k[buf] + k_place<D>(r, ch)) = rk[u];
+      const float f = pow2(scale_exp(__builtin_amdgcn_readlane(x.scale, n + k_group(u)) & 0xFF));
+      const int r = k_row(u), ch = 2 * (tid % KC);
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {
+        const uint32_t w0 = rk[u][2 * z], w1 = rk[u][2 * z + 1];
+        u32x4 w;
+        if constexpr (F16)
+          w = u32x4{f16_pair<false>(w0), f16_pair<true>(w0), f16_pair<false>(w1), f16_pair<true>(w1)};
+        else
+          w = u32x4{bf16_pair<false>(w0, f), bf16_pair<true>(w0, f), bf16_pair<false>(w1, f),
+                    bf16_pair<true>(w1, f)};
+        *reinterpret_cast<u32x4*>(s_k[buf] + k_place<D>(r, ch + z)) = w;
+      }
     }
     const bool good = __builtin_amdgcn_readlane(x.id, n + wave) >= 0;
     if (at + 64 > t.full || !good) {
@@ -732,27 +748,16 @@ __global__ __launch_bounds__(64 * kManyWaves, (D == 256 ? 1 : 2)) void attend_ma
     for (int st = 0; st < 2; ++st) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[st][i] = 0.0f;
-      const float fk = pow2(c < 16 ? ek[2 * st] : ek[2 * st + 1]);
-      const int r = 32 * st + c;
 #pragma unroll
-      for (int i = 0; i < KS / 2; ++i) {
-        const int ch = 2 * i + h;
-        const u32x4 w = *reinterpret_cast<const u32x4*>(s_k[buf] + k_place<D>(r, ch));
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          const uint32_t w0 = w[2 * z], w1 = w[2 * z + 1];
-          if constexpr (F16) {
-            const u32x4 a = {f16_pair<false>(w0), f16_pair<true>(w0), f16_pair<false>(w1),
-                             f16_pair<true>(w1)};
-            s[st] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                bits_as<f16x8>(a), bits_as<f16x8>(q[2 * i + z]), s[st], 0, 0, 0);
-          } else {
-            const u32x4 a = {bf16_pair<false>(w0, fk), bf16_pair<true>(w0, fk),
-                             bf16_pair<false>(w1, fk), bf16_pair<true>(w1, fk)};
-            s[st] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                bits_as<bf16x8>(a), bits_as<bf16x8>(q[2 * i + z]), s[st], 0, 0, 0);
-          }
-        }
+      for (int ks = 0; ks < KS; ++ks) {
+        const u32x4 a =
+            *reinterpret_cast<const u32x4*>(s_k[buf] + k_place<D>(32 * st + c, 2 * ks + h));
+        if constexpr (F16)
+          s[st] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bits_as<f16x8>(a), bits_as<f16x8>(q[ks]),
+                                                         s[st], 0, 0, 0);
+        else
+          s[st] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              bits_as<bf16x8>(a), bits_as<bf16x8>(q[ks]), s[st], 0, 0, 0);
       }
     }
     if constexpr (F16) {
