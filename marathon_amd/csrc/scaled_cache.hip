@@ -163,45 +163,66 @@ __device__ __forceinline__ int exponent_for(uint32_t bits) {
   return min(max(e, MKV_SCALE_MIN_EXP), MKV_SCALE_MAX_EXP);
 }
 
-__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
-
-// The larger of a lane's bits and every other lane's.
+// The largest of a wave's values, in every lane: neighbours exchanged by the vector unit
+// itself (quads, halves and whole rows of 16 mirrored, rows broadcast), where __shfl goes
+// through LDS six times.
 __device__ __forceinline__ uint32_t wave_max(uint32_t m) {
-  for (int d = 32; d > 0; d >>= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), d)));
-  return m;
+  const auto with = [](uint32_t x, uint32_t y) { return max(x, y); };
+#define MKV_DPP(ctrl, rows) \
+  with(m, static_cast<uint32_t>(__builtin_amdgcn_update_dpp( \
+              static_cast<int>(m), static_cast<int>(m), ctrl, rows, 0xF, false)))
+  m = MKV_DPP(0xB1, 0xF);   // quad_perm 1 0 3 2
+  m = MKV_DPP(0x4E, 0xF);   // quad_perm 2 3 0 1
+  m = MKV_DPP(0x141, 0xF);  // row_half_mirror
+  m = MKV_DPP(0x140, 0xF);  // row_mirror
+  m = MKV_DPP(0x142, 0xA);  // row_bcast 15, into rows 1 and 3
+  m = MKV_DPP(0x143, 0xC);  // row_bcast 31, into rows 2 and 3
+#undef MKV_DPP
+  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(m), 63));
 }
 
-// 16 values to 16 codes under 2^e.  Values fit 448 * 2^e unless `wild`: then infinities and
-// what is larger saturate, and NaNs become 0x7F.
-__device__ __forceinline__ u32x4 encode16(const float* x, int e, bool wild) {
-  const float s = pow2(-e);
-  u32x4 w;
+// Four values to four codes under 2^e (the conversion divides by it, exactly, and rounds to
+// nearest even).  Values fit 448 * 2^e unless `wild`: then infinities and what is larger
+// saturate, and NaNs become 0x7F.
+__device__ __forceinline__ uint32_t encode4(const float* x, float scale, bool wild) {
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  float q[4] = {x[0], x[1], x[2], x[3]};
+  if (wild) {
+    const float top = 448.0f * scale;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float q[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) q[j] = x[4 * i + j] * s;
-    if (wild) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) q[j] = mkv_fp8::clamp448(q[j]);
-    }
-    w[i] = mkv_fp8::encode4(q);
-    if (wild) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (x[4 * i + j] != x[4 * i + j]) w[i] = mkv_fp8::with_nan(w[i], j);
-    }
+    for (int j = 0; j < 4; ++j) q[j] = __builtin_amdgcn_fmed3f(q[j], -top, top);
   }
-  return w;
+  s16x2 w = {0, 0};
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, q[0], q[1], scale, false);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, q[2], q[3], scale, true);
+  uint32_t c = __builtin_bit_cast(uint32_t, w);
+  if (wild) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (x[j] != x[j]) c = mkv_fp8::with_nan(c, j);
+  }
+  return c;
+}
+
+__device__ __forceinline__ u32x4 encode16(const float* x, int e, bool wild) {
+  const float s = pow2(e);
+  return u32x4{encode4(x, s, wild), encode4(x + 4, s, wild), encode4(x + 8, s, wild),
+               encode4(x + 12, s, wild)};
+}
+
+// Four codes times the power of two s: the conversion multiplies.
+__device__ __forceinline__ void decode4(uint32_t w, float s, float* x) {
+  const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, s, false);
+  const f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, s, true);
+  x[0] = a[0];
+  x[1] = a[1];
+  x[2] = b[0];
+  x[3] = b[1];
 }
 
 __device__ __forceinline__ void decode16(u32x4 w, float s, float* x) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    mkv_fp8::decode4(w[i], x + 4 * i);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x[4 * i + j] *= s;
-  }
+  for (int i = 0; i < 4; ++i) decode4(w[i], s, x + 4 * i);
 }
 
 // Where a lane stands in its wave's 16 rows of one (block, head): rows of D values in chunks
@@ -213,63 +234,56 @@ struct Rows {
   static constexpr int kPasses = 16 / kPerPass;
 };
 
-// The largest finite |x| (bits) of K and of V over the rows of a (block, head), which `parts`
-// waves share, and whether any value there needs care: an infinity, a NaN, or one that
-// saturates under the largest scale.
+// The largest finite |x| (bits) of the K or V rows of a (block, head), which `parts` waves
+// share, and whether any value there needs care: an infinity, a NaN, or one that saturates
+// under the largest scale.
 struct Largest {
-  uint32_t k, v, wild;
+  uint32_t bits, wild;
 };
 
-__device__ __forceinline__ uint32_t finite_bits(float x) {
-  const uint32_t b = abs_bits(x);
-  return b >= kInfBits ? 0u : b;
+// The largest |x| of a lane's values; a NaN where there is one.
+template <int N>
+__device__ __forceinline__ uint32_t lane_max(const float* x) {
+  float m = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; i += 2)  // one v_maximum3 for two values
+    m = __builtin_elementwise_maximum(
+        __builtin_elementwise_maximum(__builtin_fabsf(x[i]), __builtin_fabsf(x[i + 1])), m);
+  return __float_as_uint(m) & 0x7FFFFFFFu;
 }
 
-// Over a wave's values, N times 16 a lane of each.
 template <int N>
-__device__ __forceinline__ Largest largest(const float (*k)[16], const float (*v)[16]) {
-  Largest m = {0, 0, 0};
+__device__ __forceinline__ uint32_t finite_max(const float* x) {
+  uint32_t m = 0;
 #pragma unroll
-  for (int u = 0; u < N; ++u) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      m.k = max(m.k, abs_bits(k[u][i]));
-      m.v = max(m.v, abs_bits(v[u][i]));
-    }
-  }
-  m.k = wave_max(m.k);
-  m.v = wave_max(m.v);
-  if (max(m.k, m.v) > kTopBits) {
-    m = {0, 0, 1};
-#pragma unroll
-    for (int u = 0; u < N; ++u) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        m.k = max(m.k, finite_bits(k[u][i]));
-        m.v = max(m.v, finite_bits(v[u][i]));
-      }
-    }
-    m.k = wave_max(m.k);
-    m.v = wave_max(m.v);
+  for (int i = 0; i < N; ++i) {
+    const uint32_t b = __float_as_uint(x[i]) & 0x7FFFFFFFu;
+    m = max(m, b >= kInfBits ? 0u : b);
   }
   return m;
 }
 
+// Over a wave's values, N a lane.
+template <int N>
+__device__ __forceinline__ Largest largest(const float* x) {
+  Largest m = {wave_max(lane_max<N>(x)), 0};
+  if (m.bits > kTopBits) m = {wave_max(finite_max<N>(x)), 1};
+  return m;
+}
+
 // Exchange between the waves of one (block, head); every wave of the workgroup calls it.
-__device__ __forceinline__ Largest across(Largest m, int parts, uint32_t (*lds)[3], int wave) {
+__device__ __forceinline__ Largest across(Largest m, int parts, uint32_t (*lds)[2], int wave) {
   if (parts == 1) return m;
   __syncthreads();  // the last exchange has been read
   if ((threadIdx.x & 63) == 0) {
-    lds[wave][0] = m.k;
-    lds[wave][1] = m.v;
-    lds[wave][2] = m.wild;
+    lds[wave][0] = m.bits;
+    lds[wave][1] = m.wild;
   }
   __syncthreads();
   const int first = wave - wave % parts;
   for (int i = 0; i < parts; ++i) {
-    m.k = max(m.k, lds[first + i][0]);
-    m.v = max(m.v, lds[first + i][1]);
-    m.wild |= lds[first + i][2];
+    m.bits = max(m.bits, lds[first + i][0]);
+    m.wild |= lds[first + i][1];
   }
   return m;
 }
@@ -328,7 +342,7 @@ template <int ET, int D>
 __global__ __launch_bounds__(64 * kMaxWaves) void store_kernel(StoreParams p) {
   using R = Rows<D>;
   constexpr int kBytes = ET == MKV_F32 ? 4 : 2;
-  __shared__ uint32_t s_max[kMaxWaves][3];
+  __shared__ uint32_t s_max[kMaxWaves][2];
   const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);
   const int bs = 1 << p.c.bs_shift, parts = bs >> 4;
   const int heads_here = (blockDim.x >> 6) / parts;
@@ -382,9 +396,9 @@ __global__ __launch_bounds__(64 * kMaxWaves) void store_kernel(StoreParams p) {
         load16<ET>(p.v + at * p.v_token + head * p.v_head + chunk * 16 * kBytes, v[u]);
       }
     }
-    const Largest most = across(largest<R::kPasses>(k, v), parts, s_max, wave);
-    const bool wild = most.wild != 0;
-    int ek = exponent_for(most.k), ev = exponent_for(most.v);
+    const Largest most_k = across(largest<16 * R::kPasses>(k[0]), parts, s_max, wave);
+    const Largest most_v = across(largest<16 * R::kPasses>(v[0]), parts, s_max, wave);
+    int ek = exponent_for(most_k.bits), ev = exponent_for(most_v.bits);
     if (active) {
       uint8_t* scale = p.c.scales + (id * p.c.heads + head) * 2;
       char* kb = p.c.k + id * p.c.bstride + head * p.c.hstride + chunk * 16;
@@ -400,12 +414,12 @@ __global__ __launch_bounds__(64 * kMaxWaves) void store_kernel(StoreParams p) {
           if (nk > ok) {
             u32x4* w = reinterpret_cast<u32x4*>(kb + row * p.c.tstride);
             decode16(*w, 1.0f, x);
-            *w = encode16(x, nk - ok > 126 ? 126 : nk - ok, true);
+            *w = encode16(x, min(nk - ok, 100), true);
           }
           if (nv > ov) {
             u32x4* w = reinterpret_cast<u32x4*>(vb + row * p.c.tstride);
             decode16(*w, 1.0f, x);
-            *w = encode16(x, nv - ov > 126 ? 126 : nv - ov, true);
+            *w = encode16(x, min(nv - ov, 100), true);
           }
         }
         ek = nk;
@@ -415,8 +429,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) void store_kernel(StoreParams p) {
       for (int u = 0; u < R::kPasses; ++u) {
         const int row = part * 16 + u * R::kPerPass + sub;
         if (row < off || row >= off + n) continue;
-        *reinterpret_cast<u32x4*>(kb + row * p.c.tstride) = encode16(k[u], ek, wild);
-        *reinterpret_cast<u32x4*>(vb + row * p.c.tstride) = encode16(v[u], ev, wild);
+        *reinterpret_cast<u32x4*>(kb + row * p.c.tstride) = encode16(k[u], ek, most_k.wild);
+        *reinterpret_cast<u32x4*>(vb + row * p.c.tstride) = encode16(v[u], ev, most_v.wild);
       }
     }
     if (parts > 1) __syncthreads();  // every wave has read the old scale
@@ -428,6 +442,14 @@ __global__ __launch_bounds__(64 * kMaxWaves) void store_kernel(StoreParams p) {
 }
 
 // ------------------------------------------------------------------------------- shift
+
+#ifndef MKV_MOVE_PER
+#define MKV_MOVE_PER 8
+#endif
+#ifndef MKV_MOVE_GROUPS
+#define MKV_MOVE_GROUPS 2048
+#endif
+constexpr int64_t kMoveGroups = MKV_MOVE_GROUPS;
 
 struct MoveParams {
   DevCache src;  // geometry; the layers' bases come from the arrays below
@@ -444,19 +466,25 @@ struct MoveParams {
   int64_t dst_table_len;
   int32_t n_spans;
   int32_t rotary;
+  int32_t layers;
+  int32_t per;  // layers of a workgroup
 };
 
-// A workgroup makes one destination block of `heads_here` heads and one layer.
+// A workgroup makes one destination block of `heads_here` heads, in `per` layers one after
+// the other: the block's span, ids and rotation are found once, and a layer's codes are on
+// their way while the last one's are turned.  A lane holds the two halves of 8 pairs that the
+// rotation mixes (or 16 values that it leaves alone), so that no value moves between lanes.
 template <int D>
 __global__ __launch_bounds__(64 * kMaxWaves) void move_kernel(MoveParams p) {
   using R = Rows<D>;
-  __shared__ uint32_t s_max[kMaxWaves][3];
+  constexpr int P = R::kPasses;
+  __shared__ uint32_t s_max[kMaxWaves][2];
   const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);
   const int dbs = 1 << p.dst.bs_shift, parts = dbs >> 4;
   const int heads_here = (blockDim.x >> 6) / parts;
   const int head = blockIdx.y * heads_here + wave / parts, part = wave % parts;
   const bool active = head < p.dst.heads;
-  const int chunk = lane % R::kChunks, sub = lane / R::kChunks;
+  const int piece = lane % R::kChunks, sub = lane / R::kChunks;
   const int64_t unit = blockIdx.x;
   const int64_t* us = p.unit_starts;
   const int s = last_at_most(p.n_spans, unit, [us](int i) { return us[i]; });
@@ -476,21 +504,26 @@ __global__ __launch_bounds__(64 * kMaxWaves) void move_kernel(MoveParams p) {
     if (threadIdx.x == 0) raise(p.flags, MKV_FLAG_DST_RANGE);
     return;
   }
-  const uint64_t* sl = p.src_layers + 3 * static_cast<int64_t>(blockIdx.z);
-  const uint64_t* dl = p.dst_layers + 3 * static_cast<int64_t>(blockIdx.z);
-  const char* sk = reinterpret_cast<const char*>(sl[0]);
-  const char* sv = reinterpret_cast<const char*>(sl[1]);
-  const uint8_t* ss = reinterpret_cast<const uint8_t*>(sl[2]);
 
-  u32x4 kw[R::kPasses], vw[R::kPasses];
-  int scale[R::kPasses];
-  bool there[R::kPasses];
+  if (p.src.num_blocks == 0) {  // nothing to read
+    if (threadIdx.x == 0) raise(p.flags, MKV_FLAG_SRC_RANGE);
+    return;
+  }
+
+  // K's two pieces of 8: dimensions 8 i and 8 i + rotary / 2, or 16 neighbours behind rotary
+  const bool turn = sp.delta != 0 && p.rotary > 0;
+  const bool turned = turn && piece < p.rotary / 16;
+  const int lo = turned ? 8 * piece : 16 * piece;
+  const int hi = turned ? 8 * piece + p.rotary / 2 : 16 * piece + 8;
+
+  // where each pass's row comes from (the same in every layer)
+  int64_t from_row[P], from_scale[P];
+  bool there[P];
 #pragma unroll
-  for (int u = 0; u < R::kPasses; ++u) {
+  for (int u = 0; u < P; ++u) {
     const int row = part * 16 + u * R::kPerPass + sub;
     there[u] = false;
-    kw[u] = vw[u] = u32x4{0, 0, 0, 0};
-    scale[u] = 127 | (127 << 8);
+    from_row[u] = from_scale[u] = 0;
     if (active && row < n) {
       const int64_t pos = sp.src_pos + first + row;
       const int64_t col = sp.src_index + (pos >> p.src.bs_shift);
@@ -498,65 +531,125 @@ __global__ __launch_bounds__(64 * kMaxWaves) void move_kernel(MoveParams p) {
       if (pos >= 0 && col >= 0 && col < p.src_table_len) from = p.src_table[col];
       if (from >= 0 && from < p.src.num_blocks) {
         there[u] = true;
-        const int64_t at = from * p.src.bstride + head * p.src.hstride +
-                           (pos & ((1 << p.src.bs_shift) - 1)) * p.src.tstride + chunk * 16;
-        kw[u] = *reinterpret_cast<const u32x4*>(sk + at);
-        vw[u] = *reinterpret_cast<const u32x4*>(sv + at);
-        scale[u] = *reinterpret_cast<const uint16_t*>(ss + (from * p.src.heads + head) * 2);
-      } else if (chunk == 0) {
+        from_row[u] = from * p.src.bstride + head * static_cast<int64_t>(p.src.hstride) +
+                      (pos & ((1 << p.src.bs_shift) - 1)) * p.src.tstride;
+        from_scale[u] = (from * p.src.heads + head) * 2;
+      } else if (piece == 0 && blockIdx.z == 0) {
         raise(p.flags, MKV_FLAG_SRC_RANGE);
       }
     }
   }
-  const bool turn = sp.delta != 0 && p.rotary > 0;
-  const int half = p.rotary >> 5;  // chunks to a lane's partner
-  const bool turned = turn && chunk < 2 * half;
-  const int partner = chunk < half ? lane + half : lane - half;
-  float cs[16], sn[16];
-  if (turned) {
-    const float* t = p.tables + static_cast<int64_t>(s) * 2 * p.rotary + chunk * 16;
+  // every row of the wave has a source: nothing to blank out
+  bool whole = active;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      cs[i] = t[i];
-      sn[i] = t[p.rotary + i];
+  for (int u = 0; u < P; ++u) whole = whole && __all(there[u]);
+
+  struct Raw {
+    u32x2 lo[P], hi[P];
+    u32x4 v[P];
+    uint32_t scale[P];
+  };
+  const auto load = [&](int layer, Raw& x) {  // rows without a source read the cache's first
+    const uint64_t* b = p.src_layers + 3 * static_cast<int64_t>(layer);
+    const char* k = reinterpret_cast<const char*>(b[0]);
+    const char* v = reinterpret_cast<const char*>(b[1]);
+    const char* sc = reinterpret_cast<const char*>(b[2]);
+#pragma unroll
+    for (int u = 0; u < P; ++u) {
+      x.scale[u] = *reinterpret_cast<const uint16_t*>(sc + from_scale[u]);
+      x.lo[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(k + from_row[u] + lo));
+      x.hi[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(k + from_row[u] + hi));
+      x.v[u] = __builtin_nontemporal_load(
+          reinterpret_cast<const u32x4*>(v + from_row[u] + 16 * piece));
     }
-  }
-  float k[R::kPasses][16], v[R::kPasses][16];
+  };
+  float cs[8], sn[8];
 #pragma unroll
-  for (int u = 0; u < R::kPasses; ++u) {
-    const float fk = pow2(scale_exp(scale[u] & 0xFF)), fv = pow2(scale_exp(scale[u] >> 8));
-    decode16(kw[u], fk, k[u]);
-    decode16(vw[u], fv, v[u]);
-    if (turn) {
-      u32x4 w;
+  for (int i = 0; i < 8; ++i) cs[i] = 1.0f, sn[i] = 0.0f;
+  const int64_t to = id * p.dst.bstride + head * static_cast<int64_t>(p.dst.hstride);
+  const auto make = [&](int layer, Raw& x) {
+    const uint64_t* b = p.dst_layers + 3 * static_cast<int64_t>(layer);
+    char* kb = reinterpret_cast<char*>(b[0]) + to;
+    char* vb = reinterpret_cast<char*>(b[1]) + to;
+    if (!whole) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = __shfl(static_cast<int>(kw[u][i]), turned ? partner : lane);
-      float y[16];
-      decode16(w, fk, y);
-      if (turned) {
+      for (int u = 0; u < P; ++u) {
+        if (there[u]) continue;
+        x.lo[u] = x.hi[u] = u32x2{0, 0};
+        x.v[u] = u32x4{0, 0, 0, 0};
+      }
+    }
+    float y[P][16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float a = k[u][i] * cs[i], b = y[i] * sn[i];
-          k[u][i] = a + b;
+    for (int u = 0; u < P; ++u) {
+      const float f = pow2(scale_exp(x.scale[u] & 0xFF));
+      float c[8], d[8];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        decode4(x.lo[u][i], f, c + 4 * i);
+        decode4(x.hi[u][i], f, d + 4 * i);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        y[u][i] = c[i];
+        y[u][8 + i] = d[i];
+        if (turned) {
+          const float c0 = c[i] * cs[i], c1 = d[i] * sn[i];
+          const float d0 = d[i] * cs[i], d1 = c[i] * -sn[i];
+          y[u][i] = c0 + c1;
+          y[u][8 + i] = d0 + d1;
         }
       }
     }
-  }
-  const Largest most = across(largest<R::kPasses>(k, v), parts, s_max, wave);
-  const bool wild = most.wild != 0;
-  if (!active) return;
-  const int ek = exponent_for(most.k), ev = exponent_for(most.v);
-  const int64_t to = id * p.dst.bstride + head * p.dst.hstride + chunk * 16;
+    const Largest mk = across(largest<16 * P>(y[0]), parts, s_max, wave);
+    const int ek = exponent_for(mk.bits);
+    const float sk = pow2(ek);
 #pragma unroll
-  for (int u = 0; u < R::kPasses; ++u) {
-    if (!there[u]) continue;
-    const int64_t at = to + (part * 16 + u * R::kPerPass + sub) * p.dst.tstride;
-    *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(dl[0]) + at) = encode16(k[u], ek, wild);
-    *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(dl[1]) + at) = encode16(v[u], ev, wild);
+    for (int u = 0; u < P; ++u) {
+      const int row = (part * 16 + u * R::kPerPass + sub) * p.dst.tstride;
+      const u32x2 c = {encode4(y[u], sk, mk.wild), encode4(y[u] + 4, sk, mk.wild)};
+      const u32x2 d = {encode4(y[u] + 8, sk, mk.wild), encode4(y[u] + 12, sk, mk.wild)};
+      if (there[u]) {
+        __builtin_nontemporal_store(c, reinterpret_cast<u32x2*>(kb + row + lo));
+        __builtin_nontemporal_store(d, reinterpret_cast<u32x2*>(kb + row + hi));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < P; ++u) decode16(x.v[u], pow2(scale_exp(x.scale[u] >> 8)), y[u]);
+    const Largest mv = across(largest<16 * P>(y[0]), parts, s_max, wave);
+    const int ev = exponent_for(mv.bits);
+#pragma unroll
+    for (int u = 0; u < P; ++u) {
+      const int row = (part * 16 + u * R::kPerPass + sub) * p.dst.tstride;
+      const u32x4 c = encode16(y[u], ev, mv.wild);
+      if (there[u]) __builtin_nontemporal_store(c, reinterpret_cast<u32x4*>(vb + row + 16 * piece));
+    }
+    if (active && part == 0 && lane == 0)
+      *reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(b[2]) +
+                                   (id * p.dst.heads + head) * 2) =
+          static_cast<uint16_t>((ek + 127) | ((ev + 127) << 8));
+  };
+
+  // (loads on every path, the last layer's again behind it: see the attention kernels)
+  const int layer0 = blockIdx.z * p.per, last = min(layer0 + p.per, p.layers) - 1;
+  Raw x, z;
+  load(layer0, x);
+  if (turned) {
+    const float* t = p.tables + static_cast<int64_t>(s) * 2 * p.rotary + 8 * piece;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      cs[i] = t[i];
+      sn[i] = t[p.rotary + i];  // -sin for the first half of a pair, +sin for the second
+    }
   }
-  if (part == 0 && lane == 0)
-    *reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(dl[2]) + (id * p.dst.heads + head) * 2) =
-        static_cast<uint16_t>((ek + 127) | ((ev + 127) << 8));
+  for (int layer = layer0;; layer += 2) {
+    load(min(layer + 1, last), z);
+    make(layer, x);
+    if (layer >= last) break;
+    load(min(layer + 2, last), x);
+    make(layer + 1, z);
+    if (layer + 1 >= last) break;
+  }
 }
 
 template <int ET>
@@ -695,9 +788,13 @@ extern "C" int mkv_shift_scaled(const mkv_scaled_shift_desc_t* d, void* stream) 
   p.n_spans = d->n_spans;
   p.rotary = d->rotary;
   const int waves = waves_of(p.dst.bs_shift), heads_here = waves / (d->dst.block_size / 16);
-  const dim3 grid(static_cast<unsigned>(d->units),
-                  static_cast<unsigned>((d->dst.heads + heads_here - 1) / heads_here),
-                  static_cast<unsigned>(d->layers));
+  const int64_t head_groups = (d->dst.heads + heads_here - 1) / heads_here;
+  // layers a workgroup: as many as leave the chip workgroups enough
+  const int64_t all = d->units * head_groups * d->layers;
+  p.layers = d->layers;
+  p.per = static_cast<int>(all / kMoveGroups < 1 ? 1 : all / kMoveGroups > MKV_MOVE_PER ? MKV_MOVE_PER : all / kMoveGroups);
+  const dim3 grid(static_cast<unsigned>(d->units), static_cast<unsigned>(head_groups),
+                  static_cast<unsigned>((d->layers + p.per - 1) / p.per));
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (d->dst.head_size == 64)
     move_kernel<64><<<grid, 64 * waves, 0, s>>>(p);
