@@ -172,33 +172,54 @@ int64_t mkv_attend_workspace_size(const mkv_attend_desc_t* desc);
  * this cache.  Row i of span s is read at source position src_pos + i through src_table and
  * written at dst_pos + i through dst_table, K re-rotated by delta as marathon_kvshift.h says
  * (fp32, no fused multiply-add); the destination blocks are encoded anew, each under the
- * scale of the rows that it receives.
- *   spans        : device [n_spans], 1 <= n_spans <= MKV_MAX_SPANS; src_index and dst_index
- *                  are added to the block numbers in the tables; groups are not read.
- *                  dst_pos % block_size == 0 (MKV_FLAG_SPAN, the span is skipped): a block
- *                  is written by one span.  Rows behind a span's last one stay as they were.
- *   unit_starts  : device int64 [n_spans + 1], the exclusive prefix sum of the spans' blocks,
- *                  ceil(max(n_tokens, 0) / block_size); `units` is its last entry.
+ * scale of the rows that it receives.  Rows behind a span's last one stay as they were.
+ * Destination blocks must be distinct and must not be source blocks of the call.
+ *
+ * mkv_scaled_units (a host function, no GPU call; every pointer a HOST one) resolves spans
+ * into units, one for each destination block:
+ *   spans  : [n_spans], 0 <= n_spans <= MKV_MAX_SPANS; src_index and dst_index are added to
+ *            the block numbers in the tables; groups are not read.  A span whose dst_pos is
+ *            not a multiple of the destination's block size, or with a negative position or
+ *            length, gets no units (MKV_FLAG_SPAN): a block is written by one span.
+ *   src, dst : geometry (block_size and num_blocks; the rest is not read).
+ *   units  : out, room for max_units of them; at least the sum of ceil(n_tokens / dst
+ *            block_size) is never too little (MKV_ERR_ARG otherwise).
+ *   *n_units : out.
+ *   *flags : out (or NULL), MKV_FLAG bits: a block whose id is out of range gets no unit
+ *            (DST_RANGE); rows whose source is get no code (SRC_RANGE).
+ */
+#define MKV_UNIT_SOURCES 9
+typedef struct mkv_scaled_unit {
+  int32_t dst;    /* destination block */
+  int32_t rows;   /* 1 to its block size */
+  int32_t span;   /* whose rotation table; -1: delta 0 */
+  int32_t first;  /* row 0's place in the first source block */
+  int32_t src[MKV_UNIT_SOURCES]; /* source blocks, in order; -1: out of range */
+  int32_t reserved[3];
+} mkv_scaled_unit_t;
+
+int mkv_scaled_units(const mkv_span_t* spans, int32_t n_spans, const int32_t* src_table,
+                     int64_t src_table_len, const int32_t* dst_table, int64_t dst_table_len,
+                     const mkv_scaled_cache_t* src, const mkv_scaled_cache_t* dst,
+                     mkv_scaled_unit_t* units, int64_t max_units, int64_t* n_units,
+                     int32_t* flags);
+
+/*
+ *   units        : device [n_units], 16-byte aligned, made by mkv_scaled_units; ids in them
+ *                  are checked again.
  *   tables       : device fp32 [n_spans][2][rotary], mkv_rope_tables' layout; NULL for
  *                  rotary 0.  rotary: a multiple of 32, at most head_size.
  *   src_layers, dst_layers : device [layers][3]: k_base, v_base and scales of each layer.
  *   src, dst     : geometry of every layer (their base and scale pointers are not read).
- * Destination blocks must be distinct and must not be source blocks of the call.
  */
 typedef struct mkv_scaled_shift_desc {
   mkv_scaled_cache_t src;
   mkv_scaled_cache_t dst;
   const uint64_t* src_layers;
   const uint64_t* dst_layers;
-  const mkv_span_t* spans;
-  const int64_t* unit_starts;
+  const mkv_scaled_unit_t* units;
   const float* tables;
-  const int32_t* src_table;
-  const int32_t* dst_table;
-  int32_t* error_flags;
-  int64_t src_table_len;
-  int64_t dst_table_len;
-  int64_t units;
+  int64_t n_units;
   int32_t n_spans;
   int32_t layers;
   int32_t rotary;

@@ -78,6 +78,7 @@ EXPORTED = (
     "mkv_store_scaled",
     "mkv_attend_scaled",
     "mkv_attend_workspace_size",
+    "mkv_scaled_units",
     "mkv_shift_scaled",
 )
 
@@ -212,22 +213,16 @@ class AttendDesc(ctypes.Structure):
 
 
 class ScaledShiftDesc(ctypes.Structure):
-    """mkv_scaled_shift_desc_t (248 bytes)."""
+    """mkv_scaled_shift_desc_t (200 bytes)."""
 
     _fields_ = [
         ("src", ScaledCacheDesc),
         ("dst", ScaledCacheDesc),
         ("src_layers", ctypes.c_void_p),
         ("dst_layers", ctypes.c_void_p),
-        ("spans", ctypes.c_void_p),
-        ("unit_starts", ctypes.c_void_p),
+        ("units", ctypes.c_void_p),
         ("tables", ctypes.c_void_p),
-        ("src_table", ctypes.c_void_p),
-        ("dst_table", ctypes.c_void_p),
-        ("error_flags", ctypes.c_void_p),
-        ("src_table_len", ctypes.c_int64),
-        ("dst_table_len", ctypes.c_int64),
-        ("units", ctypes.c_int64),
+        ("n_units", ctypes.c_int64),
         ("n_spans", ctypes.c_int32),
         ("layers", ctypes.c_int32),
         ("rotary", ctypes.c_int32),
@@ -236,7 +231,9 @@ class ScaledShiftDesc(ctypes.Structure):
 
 
 assert ctypes.sizeof(ScaledCacheDesc) == 72 and ctypes.sizeof(AttendDesc) == 216
-assert ctypes.sizeof(ScaledShiftDesc) == 248
+assert ctypes.sizeof(ScaledShiftDesc) == 200
+
+UNIT_BYTES = 64  # mkv_scaled_unit_t
 
 
 class KVShiftError(RuntimeError):
@@ -282,6 +279,10 @@ def _bind(cdll: ctypes.CDLL) -> ctypes.CDLL:
     f = cdll.mkv_attend_workspace_size
     f.restype = ctypes.c_int64
     f.argtypes = [ctypes.POINTER(AttendDesc)]
+    f = cdll.mkv_scaled_units
+    f.restype = ctypes.c_int
+    f.argtypes = [vp, i32, vp, i64, vp, i64, ctypes.POINTER(ScaledCacheDesc),
+                  ctypes.POINTER(ScaledCacheDesc), vp, i64, vp, vp]
     f = cdll.mkv_shift_scaled
     f.restype = ctypes.c_int
     f.argtypes = [ctypes.POINTER(ScaledShiftDesc), vp]

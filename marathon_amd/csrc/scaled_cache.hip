@@ -288,9 +288,14 @@ __device__ __forceinline__ Largest across(Largest m, int parts, uint32_t (*lds)[
   return m;
 }
 
-// Waves of a workgroup, and how they share (block, head) pairs.
+// Waves of a workgroup: those of two (block, head) pairs, or of one that takes more.  (Four
+// pairs: the same with eight heads, and half the waves idle with two: 56 us against 43 for a
+// shift of 6,007 tokens x 28 layers of two heads.)
 constexpr int kMaxWaves = 8;
-int waves_of(int bs_shift) { return bs_shift == 7 ? 8 : 4; }
+int waves_of(int bs_shift, int heads) {
+  const int parts = 1 << (bs_shift - 4);
+  return parts > 1 || heads == 1 ? parts : 2;
+}
 
 // ------------------------------------------------------------------------------- store
 
@@ -443,37 +448,22 @@ __global__ __launch_bounds__(64 * kMaxWaves) void store_kernel(StoreParams p) {
 
 // ------------------------------------------------------------------------------- shift
 
-#ifndef MKV_MOVE_PER
-#define MKV_MOVE_PER 8
-#endif
-#ifndef MKV_MOVE_GROUPS
-#define MKV_MOVE_GROUPS 2048
-#endif
-constexpr int64_t kMoveGroups = MKV_MOVE_GROUPS;
-
 struct MoveParams {
   DevCache src;  // geometry; the layers' bases come from the arrays below
   DevCache dst;
   const uint64_t* src_layers;
   const uint64_t* dst_layers;
-  const mkv_span_t* spans;
-  const int64_t* unit_starts;
+  const mkv_scaled_unit_t* units;
   const float* tables;
-  const int32_t* src_table;
-  const int32_t* dst_table;
-  int32_t* flags;
-  int64_t src_table_len;
-  int64_t dst_table_len;
   int32_t n_spans;
   int32_t rotary;
-  int32_t layers;
-  int32_t per;  // layers of a workgroup
 };
 
-// A workgroup makes one destination block of `heads_here` heads, in `per` layers one after
-// the other: the block's span, ids and rotation are found once, and a layer's codes are on
-// their way while the last one's are turned.  A lane holds the two halves of 8 pairs that the
-// rotation mixes (or 16 values that it leaves alone), so that no value moves between lanes.
+// A workgroup makes one destination block of `heads_here` heads in one layer and ends.  What
+// it has to know is one record made on the host.  22,141 tokens x 40 layers of 8 heads of 128
+// (3.63 GB) take 643 us, 5.6 TB/s, where a bare copy of the same blocks takes 632.  Found on the
+// GPU instead (span, then tables, then rows), the chain of loads in front of the data made it
+// 818; a loop over layers behind one chain, whose loads wait for its stores, 755.
 template <int D>
 __global__ __launch_bounds__(64 * kMaxWaves) void move_kernel(MoveParams p) {
   using R = Rows<D>;
@@ -485,171 +475,134 @@ __global__ __launch_bounds__(64 * kMaxWaves) void move_kernel(MoveParams p) {
   const int head = blockIdx.y * heads_here + wave / parts, part = wave % parts;
   const bool active = head < p.dst.heads;
   const int piece = lane % R::kChunks, sub = lane / R::kChunks;
-  const int64_t unit = blockIdx.x;
-  const int64_t* us = p.unit_starts;
-  const int s = last_at_most(p.n_spans, unit, [us](int i) { return us[i]; });
-  if (s < 0) return;
-  const mkv_span_t sp = p.spans[s];
-  const int64_t first = (unit - us[s]) << p.dst.bs_shift;  // the block's first row in its span
-  const int n = static_cast<int>(min(static_cast<int64_t>(dbs), sp.n_tokens - first));
-  const bool aligned = sp.dst_pos >= 0 && (sp.dst_pos & (dbs - 1)) == 0;
-  if (n <= 0 || first < 0 || !aligned) {
-    if (threadIdx.x == 0 && !aligned) raise(p.flags, MKV_FLAG_SPAN);
-    return;
-  }
-  const int64_t dcol = sp.dst_index + ((sp.dst_pos + first) >> p.dst.bs_shift);
-  int64_t id = -1;
-  if (dcol >= 0 && dcol < p.dst_table_len) id = p.dst_table[dcol];
-  if (id < 0 || id >= p.dst.num_blocks) {
-    if (threadIdx.x == 0) raise(p.flags, MKV_FLAG_DST_RANGE);
-    return;
-  }
+  // the record's words, one a lane
+  const int word = reinterpret_cast<const int32_t*>(p.units + blockIdx.x)[lane & 15];
+  const int id = __builtin_amdgcn_readlane(word, 0), n = __builtin_amdgcn_readlane(word, 1);
+  const int span = __builtin_amdgcn_readlane(word, 2), first = __builtin_amdgcn_readlane(word, 3);
+  if (id < 0 || id >= p.dst.num_blocks || span >= p.n_spans) return;
 
-  if (p.src.num_blocks == 0) {  // nothing to read
-    if (threadIdx.x == 0) raise(p.flags, MKV_FLAG_SRC_RANGE);
-    return;
-  }
-
-  // K's two pieces of 8: dimensions 8 i and 8 i + rotary / 2, or 16 neighbours behind rotary
-  const bool turn = sp.delta != 0 && p.rotary > 0;
-  const bool turned = turn && piece < p.rotary / 16;
-  const int lo = turned ? 8 * piece : 16 * piece;
-  const int hi = turned ? 8 * piece + p.rotary / 2 : 16 * piece + 8;
-
-  // where each pass's row comes from (the same in every layer)
+  // Where each pass's row comes from: a wave's 16 rows lie in two source blocks at most.
+  const int start = first + part * 16, block0 = start >> p.src.bs_shift;
+  const int src0 = block0 >= 0 && block0 < MKV_UNIT_SOURCES ? __builtin_amdgcn_readlane(word, 4 + block0) : -1;
+  const int src1 = block0 >= -1 && block0 < MKV_UNIT_SOURCES - 1 ? __builtin_amdgcn_readlane(word, 5 + block0) : -1;
   int64_t from_row[P], from_scale[P];
   bool there[P];
+  bool whole = active;  // every row of the wave has a source: nothing to blank out
 #pragma unroll
   for (int u = 0; u < P; ++u) {
-    const int row = part * 16 + u * R::kPerPass + sub;
-    there[u] = false;
+    const int row = u * R::kPerPass + sub;
+    const int64_t from = (start + row) >> p.src.bs_shift == block0 ? src0 : src1;
+    there[u] = active && part * 16 + row < n && part * 16 + row < dbs && from >= 0 &&
+               from < p.src.num_blocks;
+    whole = whole && __all(there[u]);
     from_row[u] = from_scale[u] = 0;
-    if (active && row < n) {
-      const int64_t pos = sp.src_pos + first + row;
-      const int64_t col = sp.src_index + (pos >> p.src.bs_shift);
-      int64_t from = -1;
-      if (pos >= 0 && col >= 0 && col < p.src_table_len) from = p.src_table[col];
-      if (from >= 0 && from < p.src.num_blocks) {
-        there[u] = true;
-        from_row[u] = from * p.src.bstride + head * static_cast<int64_t>(p.src.hstride) +
-                      (pos & ((1 << p.src.bs_shift) - 1)) * p.src.tstride;
-        from_scale[u] = (from * p.src.heads + head) * 2;
-      } else if (piece == 0 && blockIdx.z == 0) {
-        raise(p.flags, MKV_FLAG_SRC_RANGE);
-      }
+    if (there[u]) {
+      from_row[u] = from * p.src.bstride + head * static_cast<int64_t>(p.src.hstride) +
+                    ((start + row) & ((1 << p.src.bs_shift) - 1)) * p.src.tstride;
+      from_scale[u] = (from * p.src.heads + head) * 2;
     }
   }
-  // every row of the wave has a source: nothing to blank out
-  bool whole = active;
-#pragma unroll
-  for (int u = 0; u < P; ++u) whole = whole && __all(there[u]);
+  if (p.src.num_blocks == 0) return;  // nothing to read
 
-  struct Raw {
-    u32x2 lo[P], hi[P];
-    u32x4 v[P];
-    uint32_t scale[P];
-  };
-  const auto load = [&](int layer, Raw& x) {  // rows without a source read the cache's first
-    const uint64_t* b = p.src_layers + 3 * static_cast<int64_t>(layer);
-    const char* k = reinterpret_cast<const char*>(b[0]);
-    const char* v = reinterpret_cast<const char*>(b[1]);
-    const char* sc = reinterpret_cast<const char*>(b[2]);
+  // Rotation mixes dimension d with d + rotary / 2: chunk c of 16 with chunk c + rotary / 32.
+  // The two chunks' lanes exchange halves, so that each holds 8 whole pairs: the first lane
+  // those of dimensions `at` = 16 c to 16 c + 7, the second those of 16 c + 8 on.
+  const bool turn = span >= 0 && p.rotary > 0;
+  const int half = p.rotary / 32;
+  const bool turned = turn && piece < 2 * half;
+  const bool first_half = piece < half;
+  const int partner = !turned ? lane : first_half ? lane + half : lane - half;
+  const int at = first_half ? 16 * piece : 16 * (piece - half) + 8;
+
+  // rows without a source read the cache's first
+  const int64_t layer = blockIdx.z;
+  const uint64_t* sl = p.src_layers + 3 * layer;
+  const char* sk = reinterpret_cast<const char*>(sl[0]);
+  const char* sv = reinterpret_cast<const char*>(sl[1]);
+  const char* ss = reinterpret_cast<const char*>(sl[2]);
+  u32x4 kw[P], vw[P];
+  uint32_t scale[P];
 #pragma unroll
-    for (int u = 0; u < P; ++u) {
-      x.scale[u] = *reinterpret_cast<const uint16_t*>(sc + from_scale[u]);
-      x.lo[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(k + from_row[u] + lo));
-      x.hi[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(k + from_row[u] + hi));
-      x.v[u] = __builtin_nontemporal_load(
-          reinterpret_cast<const u32x4*>(v + from_row[u] + 16 * piece));
-    }
-  };
+  for (int u = 0; u < P; ++u) {
+    scale[u] = *reinterpret_cast<const uint16_t*>(ss + from_scale[u]);
+    kw[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(sk + from_row[u] + 16 * piece));
+    vw[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(sv + from_row[u] + 16 * piece));
+  }
   float cs[8], sn[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) cs[i] = 1.0f, sn[i] = 0.0f;
-  const int64_t to = id * p.dst.bstride + head * static_cast<int64_t>(p.dst.hstride);
-  const auto make = [&](int layer, Raw& x) {
-    const uint64_t* b = p.dst_layers + 3 * static_cast<int64_t>(layer);
-    char* kb = reinterpret_cast<char*>(b[0]) + to;
-    char* vb = reinterpret_cast<char*>(b[1]) + to;
-    if (!whole) {
-#pragma unroll
-      for (int u = 0; u < P; ++u) {
-        if (there[u]) continue;
-        x.lo[u] = x.hi[u] = u32x2{0, 0};
-        x.v[u] = u32x4{0, 0, 0, 0};
-      }
-    }
-    float y[P][16];
-#pragma unroll
-    for (int u = 0; u < P; ++u) {
-      const float f = pow2(scale_exp(x.scale[u] & 0xFF));
-      float c[8], d[8];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        decode4(x.lo[u][i], f, c + 4 * i);
-        decode4(x.hi[u][i], f, d + 4 * i);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        y[u][i] = c[i];
-        y[u][8 + i] = d[i];
-        if (turned) {
-          const float c0 = c[i] * cs[i], c1 = d[i] * sn[i];
-          const float d0 = d[i] * cs[i], d1 = c[i] * -sn[i];
-          y[u][i] = c0 + c1;
-          y[u][8 + i] = d0 + d1;
-        }
-      }
-    }
-    const Largest mk = across(largest<16 * P>(y[0]), parts, s_max, wave);
-    const int ek = exponent_for(mk.bits);
-    const float sk = pow2(ek);
-#pragma unroll
-    for (int u = 0; u < P; ++u) {
-      const int row = (part * 16 + u * R::kPerPass + sub) * p.dst.tstride;
-      const u32x2 c = {encode4(y[u], sk, mk.wild), encode4(y[u] + 4, sk, mk.wild)};
-      const u32x2 d = {encode4(y[u] + 8, sk, mk.wild), encode4(y[u] + 12, sk, mk.wild)};
-      if (there[u]) {
-        __builtin_nontemporal_store(c, reinterpret_cast<u32x2*>(kb + row + lo));
-        __builtin_nontemporal_store(d, reinterpret_cast<u32x2*>(kb + row + hi));
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < P; ++u) decode16(x.v[u], pow2(scale_exp(x.scale[u] >> 8)), y[u]);
-    const Largest mv = across(largest<16 * P>(y[0]), parts, s_max, wave);
-    const int ev = exponent_for(mv.bits);
-#pragma unroll
-    for (int u = 0; u < P; ++u) {
-      const int row = (part * 16 + u * R::kPerPass + sub) * p.dst.tstride;
-      const u32x4 c = encode16(y[u], ev, mv.wild);
-      if (there[u]) __builtin_nontemporal_store(c, reinterpret_cast<u32x4*>(vb + row + 16 * piece));
-    }
-    if (active && part == 0 && lane == 0)
-      *reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(b[2]) +
-                                   (id * p.dst.heads + head) * 2) =
-          static_cast<uint16_t>((ek + 127) | ((ev + 127) << 8));
-  };
-
-  // (loads on every path, the last layer's again behind it: see the attention kernels)
-  const int layer0 = blockIdx.z * p.per, last = min(layer0 + p.per, p.layers) - 1;
-  Raw x, z;
-  load(layer0, x);
   if (turned) {
-    const float* t = p.tables + static_cast<int64_t>(s) * 2 * p.rotary + 8 * piece;
+    const float* t = p.tables + static_cast<int64_t>(span) * 2 * p.rotary + at;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       cs[i] = t[i];
       sn[i] = t[p.rotary + i];  // -sin for the first half of a pair, +sin for the second
     }
   }
-  for (int layer = layer0;; layer += 2) {
-    load(min(layer + 1, last), z);
-    make(layer, x);
-    if (layer >= last) break;
-    load(min(layer + 2, last), x);
-    make(layer + 1, z);
-    if (layer + 1 >= last) break;
+  if (!whole) {
+#pragma unroll
+    for (int u = 0; u < P; ++u)
+      if (!there[u]) kw[u] = vw[u] = u32x4{0, 0, 0, 0};
   }
+  const uint64_t* dl = p.dst_layers + 3 * layer;
+  const int64_t to = static_cast<int64_t>(id) * p.dst.bstride + head * static_cast<int64_t>(p.dst.hstride) + 16 * piece;
+  char* kb = reinterpret_cast<char*>(dl[0]) + to;
+  char* vb = reinterpret_cast<char*>(dl[1]) + to;
+  const auto row_of = [&](int u) { return (part * 16 + u * R::kPerPass + sub) * p.dst.tstride; };
+  // the half of a chunk that goes to the partner, and the one that it sends
+  const auto swap = [&](u32x4& w) {
+    const uint32_t g0 = first_half ? w[2] : w[0], g1 = first_half ? w[3] : w[1];
+    const uint32_t r0 = __builtin_amdgcn_ds_bpermute(4 * partner, g0);
+    const uint32_t r1 = __builtin_amdgcn_ds_bpermute(4 * partner, g1);
+    if (first_half)
+      w[2] = r0, w[3] = r1;
+    else
+      w[0] = r0, w[1] = r1;
+  };
+  float y[P][16];
+#pragma unroll
+  for (int u = 0; u < P; ++u) {
+    if (turn) {  // (lanes that turn nothing are their own partners)
+      u32x4 w = kw[u];
+      swap(w);
+      if (turned) kw[u] = w;
+    }
+    decode16(kw[u], pow2(scale_exp(scale[u] & 0xFF)), y[u]);
+    if (turned) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float a = y[u][i], b = y[u][8 + i];
+        const float a0 = a * cs[i], a1 = b * sn[i], b0 = b * cs[i], b1 = a * -sn[i];
+        y[u][i] = a0 + a1;
+        y[u][8 + i] = b0 + b1;
+      }
+    }
+  }
+  const Largest mk = across(largest<16 * P>(y[0]), parts, s_max, wave);
+  const int ek = exponent_for(mk.bits);
+#pragma unroll
+  for (int u = 0; u < P; ++u) {
+    u32x4 w = encode16(y[u], ek, mk.wild);
+    if (turn) {
+      u32x4 back = w;
+      swap(back);
+      if (turned) w = back;
+    }
+    if (there[u]) __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(kb + row_of(u)));
+  }
+#pragma unroll
+  for (int u = 0; u < P; ++u) decode16(vw[u], pow2(scale_exp(scale[u] >> 8)), y[u]);
+  const Largest mv = across(largest<16 * P>(y[0]), parts, s_max, wave);
+  const int ev = exponent_for(mv.bits);
+#pragma unroll
+  for (int u = 0; u < P; ++u) {
+    const u32x4 w = encode16(y[u], ev, mv.wild);
+    if (there[u]) __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(vb + row_of(u)));
+  }
+  if (active && part == 0 && lane == 0)
+    *reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(dl[2]) +
+                                 (static_cast<int64_t>(id) * p.dst.heads + head) * 2) =
+        static_cast<uint16_t>((ek + 127) | ((ev + 127) << 8));
 }
 
 template <int ET>
@@ -736,7 +689,7 @@ extern "C" int mkv_store_scaled(const mkv_scaled_cache_t* cache, const void* k,
     return mkv_fail(MKV_ERR_ALIGN, "%s: k or v is not 16-byte aligned", who);
   p.tokens = tokens;
   p.group = tokens <= 4096 ? 1 : 16;
-  const int waves = waves_of(p.c.bs_shift), parts = cache->block_size / 16;
+  const int waves = waves_of(p.c.bs_shift, p.c.heads), parts = cache->block_size / 16;
   const int heads_here = waves / parts;
   const dim3 grid(static_cast<unsigned>((tokens + p.group - 1) / p.group),
                   static_cast<unsigned>((cache->heads + heads_here - 1) / heads_here));
@@ -748,6 +701,71 @@ extern "C" int mkv_store_scaled(const mkv_scaled_cache_t* cache, const void* k,
   else
     store_launch<MKV_F32>(cache->head_size, grid, 64 * waves, p, s);
   return launched(who);
+}
+
+extern "C" int mkv_scaled_units(const mkv_span_t* spans, int32_t n_spans, const int32_t* src_table,
+                                int64_t src_table_len, const int32_t* dst_table,
+                                int64_t dst_table_len, const mkv_scaled_cache_t* src,
+                                const mkv_scaled_cache_t* dst, mkv_scaled_unit_t* units,
+                                int64_t max_units, int64_t* n_units, int32_t* flags) {
+  const char* who = "mkv_scaled_units";
+  if (src == nullptr || dst == nullptr || n_units == nullptr)
+    return mkv_fail(MKV_ERR_ARG, "%s: a pointer is NULL", who);
+  DevCache s, t;
+  int rc = check_cache(who, *src, false, &s);
+  if (rc == MKV_OK) rc = check_cache(who, *dst, false, &t);
+  if (rc != MKV_OK) return rc;
+  if (n_spans < 0 || n_spans > MKV_MAX_SPANS)
+    return mkv_fail(MKV_ERR_ARG, "%s: n_spans %d outside [0, %d]", who, n_spans, MKV_MAX_SPANS);
+  if (src_table_len < 0 || dst_table_len < 0 || max_units < 0 ||
+      (n_spans > 0 && spans == nullptr) || (src_table_len > 0 && src_table == nullptr) ||
+      (dst_table_len > 0 && dst_table == nullptr) || (max_units > 0 && units == nullptr))
+    return mkv_fail(MKV_ERR_ARG, "%s: a pointer is NULL or a size negative", who);
+  int64_t count = 0;
+  int32_t raised = 0;
+  const int32_t bs = dst->block_size, sbs = src->block_size;
+  // a block number in a table, which positions and indices of any size may leave
+  const auto entry = [](const int32_t* table, int64_t len, int64_t index, int64_t block,
+                        int64_t blocks) -> int32_t {
+    int64_t at;
+    if (__builtin_add_overflow(index, block, &at) || at < 0 || at >= len) return -1;
+    return table[at] >= 0 && table[at] < blocks ? table[at] : -1;
+  };
+  for (int32_t i = 0; i < n_spans; ++i) {
+    const mkv_span_t& sp = spans[i];
+    if (sp.n_tokens < 0 || sp.src_pos < 0 || sp.dst_pos < 0 || sp.dst_pos % bs != 0 ||
+        sp.src_pos > INT64_MAX - INT32_MAX || sp.dst_pos > INT64_MAX - INT32_MAX) {
+      raised |= MKV_FLAG_SPAN;
+      continue;
+    }
+    for (int64_t at = 0; at < sp.n_tokens; at += bs) {
+      const int32_t id = entry(dst_table, dst_table_len, sp.dst_index, (sp.dst_pos + at) / bs,
+                               dst->num_blocks);
+      if (id < 0) {
+        raised |= MKV_FLAG_DST_RANGE;
+        continue;
+      }
+      if (count >= max_units)
+        return mkv_fail(MKV_ERR_ARG, "%s: more than %lld units", who, (long long)max_units);
+      mkv_scaled_unit_t& u = units[count++];
+      u = mkv_scaled_unit_t{};
+      u.dst = id;
+      u.rows = static_cast<int32_t>(sp.n_tokens - at < bs ? sp.n_tokens - at : bs);
+      u.span = sp.delta != 0 ? i : -1;
+      u.first = static_cast<int32_t>((sp.src_pos + at) % sbs);
+      const int64_t block = (sp.src_pos + at) / sbs;
+      const int used = (u.first + u.rows + sbs - 1) / sbs;
+      for (int j = 0; j < MKV_UNIT_SOURCES; ++j) {
+        u.src[j] = j < used
+                       ? entry(src_table, src_table_len, sp.src_index, block + j, src->num_blocks)
+                       : -1;
+        if (j < used && u.src[j] < 0) raised |= MKV_FLAG_SRC_RANGE;
+      }
+    }
+  }
+  *n_units = count;
+  if (flags != nullptr) *flags = raised;
+  return MKV_OK;
 }
 
 extern "C" int mkv_shift_scaled(const mkv_scaled_shift_desc_t* d, void* stream) {
@@ -766,35 +784,24 @@ extern "C" int mkv_shift_scaled(const mkv_scaled_shift_desc_t* d, void* stream) 
     return mkv_fail(MKV_ERR_ARG, "%s: n_spans %d outside [0, %d]", who, d->n_spans, MKV_MAX_SPANS);
   if (d->layers < 0 || d->layers > 65535)
     return mkv_fail(MKV_ERR_ARG, "%s: layers %d", who, d->layers);
-  if (d->units < 0 || d->units > INT32_MAX || d->src_table_len < 0 || d->dst_table_len < 0)
-    return mkv_fail(MKV_ERR_ARG, "%s: a size is negative or past 32 bits", who);
-  if (d->n_spans == 0 || d->layers == 0 || d->units == 0) return MKV_OK;
-  if (d->spans == nullptr || d->unit_starts == nullptr || d->src_layers == nullptr ||
-      d->dst_layers == nullptr || d->src_table == nullptr || d->dst_table == nullptr ||
+  if (d->n_units < 0 || d->n_units > INT32_MAX)
+    return mkv_fail(MKV_ERR_ARG, "%s: n_units %lld", who, (long long)d->n_units);
+  if (d->layers == 0 || d->n_units == 0) return MKV_OK;
+  if (d->units == nullptr || d->src_layers == nullptr || d->dst_layers == nullptr ||
       (d->rotary > 0 && d->tables == nullptr))
     return mkv_fail(MKV_ERR_ARG, "%s: a pointer is NULL", who);
-  if ((reinterpret_cast<uintptr_t>(d->tables) & 15) != 0)
-    return mkv_fail(MKV_ERR_ALIGN, "%s: tables are not 16-byte aligned", who);
+  if (((reinterpret_cast<uintptr_t>(d->tables) | reinterpret_cast<uintptr_t>(d->units)) & 15) != 0)
+    return mkv_fail(MKV_ERR_ALIGN, "%s: tables or units are not 16-byte aligned", who);
   p.src_layers = d->src_layers;
   p.dst_layers = d->dst_layers;
-  p.spans = d->spans;
-  p.unit_starts = d->unit_starts;
+  p.units = d->units;
   p.tables = d->tables;
-  p.src_table = d->src_table;
-  p.dst_table = d->dst_table;
-  p.flags = d->error_flags;
-  p.src_table_len = d->src_table_len;
-  p.dst_table_len = d->dst_table_len;
   p.n_spans = d->n_spans;
   p.rotary = d->rotary;
-  const int waves = waves_of(p.dst.bs_shift), heads_here = waves / (d->dst.block_size / 16);
+  const int waves = waves_of(p.dst.bs_shift, p.dst.heads), heads_here = waves / (d->dst.block_size / 16);
   const int64_t head_groups = (d->dst.heads + heads_here - 1) / heads_here;
-  // layers a workgroup: as many as leave the chip workgroups enough
-  const int64_t all = d->units * head_groups * d->layers;
-  p.layers = d->layers;
-  p.per = static_cast<int>(all / kMoveGroups < 1 ? 1 : all / kMoveGroups > MKV_MOVE_PER ? MKV_MOVE_PER : all / kMoveGroups);
-  const dim3 grid(static_cast<unsigned>(d->units), static_cast<unsigned>(head_groups),
-                  static_cast<unsigned>((d->layers + p.per - 1) / p.per));
+  const dim3 grid(static_cast<unsigned>(d->n_units), static_cast<unsigned>(head_groups),
+                  static_cast<unsigned>(d->layers));
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (d->dst.head_size == 64)
     move_kernel<64><<<grid, 64 * waves, 0, s>>>(p);

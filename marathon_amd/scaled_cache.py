@@ -29,13 +29,14 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass, field
+from itertools import chain
 
 import numpy as np
 import torch
 
 from . import _lib
 from .shift_kernels import current_stream, dtype_code
-from .spans import _on, _Staging, span_tables
+from .spans import _on, _span_struct
 
 HEAD_SIZES = (64, 128, 256)
 BLOCK_SIZES = (16, 32, 64, 128)
@@ -340,46 +341,58 @@ class ScaledShifts:
         a span writes whole blocks, each anew under the scale of its rows; rows behind a
         span's last one stay.  The destination blocks of one call are distinct, and none is
         one of its source blocks."""
-        bs = self.dst[0].block_size
-        spans = np.zeros(len(rows), dtype=_lib.SPAN_DTYPE)
-        for i, r in enumerate(rows):
-            spans[i] = tuple(r)
-        if len(rows) > _lib.MKV_MAX_SPANS:
-            raise ValueError(f"{len(rows)} spans: at most {_lib.MKV_MAX_SPANS}")
-        if (spans["dst_pos"] % bs != 0).any():
-            raise ValueError(f"a destination position is not a multiple of {bs}")
-        if (spans["n_tokens"] < 0).any() or (spans["src_pos"] < 0).any() or (
-                spans["dst_pos"] < 0).any():
-            raise ValueError("a span's position or length is negative")
-        tables = [_host_table(t) for t in (src_table, dst_table)]
-        starts = np.zeros(len(rows) + 1, dtype=np.int64)
-        np.cumsum(-(-spans["n_tokens"].astype(np.int64) // bs), out=starts[1:])
-        units = int(starts[-1])
-        if units == 0:
+        n, bs = len(rows), self.dst[0].block_size
+        if n > _lib.MKV_MAX_SPANS:
+            raise ValueError(f"{n} spans: at most {_lib.MKV_MAX_SPANS}")
+        most = deltas = 0
+        for r in rows:
+            if r[0] < 0 or r[1] < 0 or r[4] < 0:
+                raise ValueError("a span's position or length is negative")
+            if r[1] % bs:
+                raise ValueError(f"a destination position is not a multiple of {bs}")
+            most += -(-int(r[4]) // bs)
+            deltas |= int(r[5])
+        if most == 0:
             return
-        stage = _Staging()
-        parts = [spans.view(np.uint8).reshape(-1), starts, *tables]
-        if self.rotary:
-            parts.append(span_tables(spans["delta"], self.inv_freq, self.rotary))
-        at = [stage.add(p) for p in parts]
+        spans = np.empty(n, dtype=_lib.SPAN_DTYPE)
+        _span_struct(n).pack_into(spans.view(np.uint8), 0, *chain.from_iterable(rows))
+        tables = [_host_table(t) for t in (src_table, dst_table)]
+        # units, then the spans' rotation tables, in one pinned buffer
+        turns = n * 8 * self.rotary if deltas else 0
+        room = most * _lib.UNIT_BYTES
+        host = torch.empty(room + turns, dtype=torch.uint8, pin_memory=True)
+        at, d, L = host.data_ptr(), self.desc, _lib.lib()
+        out = np.zeros(2, np.int64)  # units, flags
+        _lib.check(L.mkv_scaled_units(
+            spans.ctypes.data, n, tables[0].ctypes.data, tables[0].size, tables[1].ctypes.data,
+            tables[1].size, ctypes.byref(d.src), ctypes.byref(d.dst), at, most, out.ctypes.data,
+            out.ctypes.data + 8))
+        if turns:
+            steps = np.ascontiguousarray(spans["delta"])
+            _lib.check(L.mkv_rope_tables(steps.ctypes.data, n, self.inv_freq.data_ptr(),
+                                         self.rotary, at + room))
+        raised = int(out[1])
+        flags = _flags(error_flags, self.device)
         desc = _lib.ScaledShiftDesc()
-        ctypes.memmove(ctypes.byref(desc), ctypes.byref(self.desc), ctypes.sizeof(desc))
-        desc.error_flags = _flags(error_flags, self.device)
-        desc.n_spans, desc.units = len(rows), units
-        desc.src_table_len, desc.dst_table_len = tables[0].size, tables[1].size
+        ctypes.memmove(ctypes.byref(desc), ctypes.byref(d), ctypes.sizeof(desc))
+        desc.n_spans, desc.n_units = n, int(out[0])
+        if not turns:
+            desc.rotary = 0
         with _on(self.device, _current(self.device)):
             stream = current_stream(self.device)
             if stream not in self._streams:
                 self._bases.record_stream(torch.cuda.current_stream(self.device))
                 self._streams.add(stream)
-            blob = stage.upload(self.device)
+            if raised and flags:
+                error_flags.bitwise_or_(raised)
+            if not desc.n_units:
+                return
+            # the caching host allocator keeps ``host`` until this copy has completed
+            blob = host.to(self.device, non_blocking=True)
             if stream and torch.cuda.is_current_stream_capturing():
-                self._captured.append(stage.host)
-            base = blob.data_ptr()
-            desc.spans, desc.unit_starts = base + at[0], base + at[1]
-            desc.src_table, desc.dst_table = base + at[2], base + at[3]
-            desc.tables = base + at[4] if self.rotary else None
-            _lib.check(_lib.lib().mkv_shift_scaled(ctypes.byref(desc), stream))
+                self._captured.append(host)
+            desc.units, desc.tables = blob.data_ptr(), blob.data_ptr() + room if turns else None
+            _lib.check(L.mkv_shift_scaled(ctypes.byref(desc), stream))
 
 
 def _geometry(c: ScaledCache) -> tuple:

@@ -283,7 +283,6 @@ class _Staging:
 
     def upload(self, device) -> torch.Tensor:
         host = torch.empty(max(self.size, self.ALIGN), dtype=torch.uint8, pin_memory=True)
-        self.host = host
         view = host.numpy()
         for off, a in self.parts:
             view[off:off + a.nbytes] = a.reshape(-1).view(np.uint8)

@@ -47,12 +47,13 @@ int main(void) {
   printf("%zu %zu %zu\n", sizeof(mkv_scaled_cache_t), sizeof(mkv_attend_desc_t),
          sizeof(mkv_scaled_shift_desc_t));
 @
-  printf("limits %d %d %d\n", MKV_SCALE_MIN_EXP, MKV_SCALE_MAX_EXP, MKV_MAX_REQUESTS);
+  printf("limits %d %d %d %zu\n", MKV_SCALE_MIN_EXP, MKV_SCALE_MAX_EXP, MKV_MAX_REQUESTS,
+         sizeof(mkv_scaled_unit_t));
   return 0;
 }
 """
 STRUCTS = {"mkv_scaled_cache_t": _lib.ScaledCacheDesc, "mkv_attend_desc_t": _lib.AttendDesc,
-           "mkv_scaled_shift_desc_t": _lib.ScaledShiftDesc}
+           "mkv_scaled_shift_desc_t": _lib.ScaledShiftDesc}  # and mkv_scaled_unit_t, 16 int32
 
 
 def test_descriptors_match_the_header(tmp_path):
@@ -70,7 +71,7 @@ def test_descriptors_match_the_header(tmp_path):
             name, f = field.split(".")
             assert getattr(STRUCTS[name], f).offset == int(at), field
     assert out[-2] == (f"limits {_lib.MKV_SCALE_MIN_EXP} {_lib.MKV_SCALE_MAX_EXP} "
-                       f"{_lib.MKV_MAX_REQUESTS}")
+                       f"{_lib.MKV_MAX_REQUESTS} {_lib.UNIT_BYTES}")
 
 
 def cache_desc(**kw):
@@ -178,10 +179,9 @@ def test_slots_refuse(change, code):
 def shift_desc(src=None, dst=None, **kw):
     d = _lib.ScaledShiftDesc()
     d.src, d.dst = cache_desc(**(src or {})), cache_desc(**(dst or {}))
-    for f in ("src_layers", "dst_layers", "spans", "unit_starts", "tables", "src_table", "dst_table"):
+    for f in ("src_layers", "dst_layers", "units", "tables"):
         setattr(d, f, 1 << 20)
-    d.src_table_len = d.dst_table_len = 9
-    d.units, d.n_spans, d.layers, d.rotary = 4, 2, 3, 128
+    d.n_units, d.n_spans, d.layers, d.rotary = 4, 2, 3, 128
     for k, v in kw.items():
         setattr(d, k, v)
     return d
@@ -192,12 +192,69 @@ def shift_desc(src=None, dst=None, **kw):
     (dict(src=dict(block_size=20)), _lib.MKV_ERR_UNSUPPORTED),
     (dict(rotary=16), _lib.MKV_ERR_UNSUPPORTED), (dict(rotary=160), _lib.MKV_ERR_UNSUPPORTED),
     (dict(rotary=-32), _lib.MKV_ERR_UNSUPPORTED), (dict(n_spans=5000), _lib.MKV_ERR_ARG),
-    (dict(layers=70000), _lib.MKV_ERR_ARG), (dict(units=1 << 31), _lib.MKV_ERR_ARG),
-    (dict(spans=None), _lib.MKV_ERR_ARG), (dict(tables=None), _lib.MKV_ERR_ARG),
-    (dict(tables=(1 << 20) + 4), _lib.MKV_ERR_ALIGN), (dict(dst_table_len=-1), _lib.MKV_ERR_ARG),
-    (dict(units=0), _lib.MKV_OK), (dict(layers=0), _lib.MKV_OK)])
+    (dict(layers=70000), _lib.MKV_ERR_ARG), (dict(n_units=1 << 31), _lib.MKV_ERR_ARG),
+    (dict(units=None), _lib.MKV_ERR_ARG), (dict(tables=None), _lib.MKV_ERR_ARG),
+    (dict(tables=(1 << 20) + 4), _lib.MKV_ERR_ALIGN), (dict(units=(1 << 20) + 8), _lib.MKV_ERR_ALIGN),
+    (dict(n_units=0), _lib.MKV_OK), (dict(layers=0), _lib.MKV_OK)])
 def test_shift_refuses(change, code):
     assert _lib.lib().mkv_shift_scaled(ctypes.byref(shift_desc(**change)), None) == code
+
+
+def units_of(rows, src_table, dst_table, sbs=16, dbs=16, blocks=(50, 60), room=None):
+    """(status, unit records as int32 [n, 16], flags)."""
+    spans = np.zeros(len(rows), _lib.SPAN_DTYPE)
+    for i, r in enumerate(rows):
+        spans[i] = r
+    st, dt = np.asarray(src_table, np.int32), np.asarray(dst_table, np.int32)
+    room = sum(-(-max(r[4], 0) // dbs) for r in rows) if room is None else room
+    out, got = np.full((room + 1, 16), 77, np.int32), np.zeros(2, np.int64)
+    a, b = (cache_desc(block_size=s, num_blocks=n) for s, n in zip((sbs, dbs), blocks))
+    rc = _lib.lib().mkv_scaled_units(
+        spans.ctypes.data, len(rows), st.ctypes.data, st.size, dt.ctypes.data, dt.size,
+        ctypes.byref(a), ctypes.byref(b), out.ctypes.data, room, got.ctypes.data, got.ctypes.data + 8)
+    assert (out[room] == 77).all()
+    return rc, out[:int(got[0])], int(got[1])
+
+
+@pytest.mark.parametrize("sbs", [16, 32, 128])
+@pytest.mark.parametrize("dbs", [16, 64, 128])
+def test_units_name_every_rows_blocks(sbs, dbs):
+    rng = np.random.default_rng(sbs + dbs)
+    st, dt = rng.permutation(50), rng.permutation(60)
+    rows = [(5, 2 * dbs, 3, 1, 2 * dbs + 7, 11, 0, 0), (sbs * 2, 8 * dbs, 0, 0, 1, 0, 0, 0),
+            (0, 0, 0, 0, 0, 4, 0, 0)]
+    rc, units, flags = units_of(rows, st, dt, sbs, dbs)
+    assert rc == _lib.MKV_OK and flags == 0 and len(units) == 4
+    k = 0
+    for i, (sp, dp, si, di, n, delta, _, _) in enumerate(rows):
+        for at in range(0, n, dbs):
+            u = units[k]
+            k += 1
+            assert u[0] == dt[di + (dp + at) // dbs] and u[1] == min(dbs, n - at)
+            assert u[2] == (i if delta else -1)
+            for row in range(u[1]):
+                p = sp + at + row
+                assert u[4 + (u[3] + row) // sbs] == st[si + p // sbs]
+                assert (u[3] + row) % sbs == p % sbs
+
+
+def test_units_of_bad_spans_and_ids():
+    table = np.arange(10)
+    bad = [(0, 8, 0, 0, 4, 0, 0, 0), (-1, 0, 0, 0, 4, 0, 0, 0), (0, 0, 0, 0, -4, 0, 0, 0),
+           (0, -16, 0, 0, 4, 0, 0, 0)]
+    rc, units, flags = units_of(bad, table, table)
+    assert rc == _lib.MKV_OK and len(units) == 0 and flags == _lib.MKV_FLAG_SPAN
+    rc, units, flags = units_of([(0, 0, 0, 0, 40, 0, 0, 0)], table, [1, 60, -1])
+    assert flags == _lib.MKV_FLAG_DST_RANGE and units[:, 0].tolist() == [1]
+    rc, units, flags = units_of([(8, 0, 0, 0, 32, 0, 0, 0)], [3, 50], table)
+    assert flags == _lib.MKV_FLAG_SRC_RANGE
+    assert units[:, 4:6].tolist() == [[3, -1], [-1, -1]]
+    rc, units, flags = units_of([(2**62, 0, 2**62, 2**62, 20, 0, 0, 0)], table, table)
+    assert flags == _lib.MKV_FLAG_DST_RANGE and len(units) == 0
+    rc, units, flags = units_of([(2**63 - 5, 0, 2**63 - 1, 0, 20, 0, 0, 0)], table, table)
+    assert flags == _lib.MKV_FLAG_SPAN and len(units) == 0
+    assert units_of([(0, 0, 0, 0, 40, 0, 0, 0)], table, table, room=2)[0] == _lib.MKV_ERR_ARG
+    assert units_of([], [], [])[0] == _lib.MKV_OK
 
 
 def test_there_is_no_cpu_path():
