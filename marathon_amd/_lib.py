@@ -346,6 +346,10 @@ def binding():
                         f"{path} was built for (ABI, torch) {built}, not "
                         f"{(MKV_ABI_VERSION, torch.__version__)}; rebuild")
                 module.bind(ctypes.cast(cdll.mkv_scatter_shifted, ctypes.c_void_p).value)
+                module.bind_scaled(*(
+                    ctypes.cast(getattr(cdll, name), ctypes.c_void_p).value
+                    for name in ("mkv_step_slots", "mkv_store_scaled", "mkv_attend_scaled",
+                                 "mkv_attend_workspace_size")))
                 _BINDING = module
     return _BINDING
 

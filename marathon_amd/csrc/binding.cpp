@@ -1,4 +1,4 @@
-// binding.cpp -- the per-layer call's launch path from torch tensors, for CPython.
+// binding.cpp -- the small calls' launch paths from torch tensors, for CPython.
 //
 // scatter(src, kv, slots, block_size, hnd, shift, k_scale, error_flags) is
 // shift_kernels.scatter_shifted's usual call: it reads the tensors through torch's C++
@@ -12,16 +12,26 @@
 // that need a copy or a conversion, subclasses and wrapped tensors, another current device,
 // anything the general path refuses): nothing has been launched then, and the caller takes
 // the general path, which also raises the errors.
+//
+// slots, store and attend are scaled_cache.py's step_slots, store_scaled and attend_scaled in
+// the same way: a decode step's kernels run 4 to 20 us, and through Python methods and ctypes
+// the calls took 10 to 15 on the host.  They return their tensors (store: None on success
+// becomes True), the library's status as an int, or None for the general path.
 
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <cmath>
+
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+#include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include "marathon_kvscaled.h"
 #include "marathon_kvshift.h"
 
 namespace {
@@ -174,6 +184,288 @@ PyObject* scatter(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   }
 }
 
+// ------------------------------------------------------- the block-scaled cache's calls
+
+typedef decltype(&mkv_step_slots) slots_fn;
+typedef decltype(&mkv_store_scaled) store_fn;
+typedef decltype(&mkv_attend_scaled) attend_fn;
+typedef decltype(&mkv_attend_workspace_size) attend_size_fn;
+slots_fn g_slots = nullptr;
+store_fn g_store = nullptr;
+attend_fn g_attend = nullptr;
+attend_size_fn g_attend_size = nullptr;
+
+// A contiguous int32 vector on `dev` (of n entries, unless n < 0), or null.
+const int32_t* vector_of(PyObject* o, const at::Device& dev, int64_t n) {
+  const at::Tensor* t = plain(o);
+  if (t == nullptr || t->device() != dev || t->scalar_type() != at::kInt || t->dim() != 1 ||
+      !t->is_contiguous() || (n >= 0 && t->size(0) != n))
+    return nullptr;
+  // (an empty vector has no address; any other will do)
+  return t->numel() > 0 ? static_cast<const int32_t*>(t->data_ptr()) : reinterpret_cast<int32_t*>(64);
+}
+
+struct Table {
+  int32_t* at = nullptr;
+  int64_t stride = 0, n = 0, width = 0;
+};
+
+bool table_of(PyObject* o, const at::Device* dev, Table& out) {
+  const at::Tensor* t = plain(o);
+  if (t == nullptr || !t->is_cuda() || (dev != nullptr && t->device() != *dev) ||
+      t->scalar_type() != at::kInt || t->dim() != 2 || (t->size(1) > 1 && t->stride(1) != 1) ||
+      t->size(0) > MKV_MAX_REQUESTS || t->size(1) > INT32_MAX)
+    return false;
+  out.at = static_cast<int32_t*>(t->data_ptr());
+  out.n = t->size(0);
+  out.width = t->size(1);
+  out.stride = out.n > 1 ? t->stride(0) : out.width;
+  return true;
+}
+
+// error_flags: kUsual with null for None; kOther for anything but an int32 tensor on `dev`.
+int flags_of(PyObject* o, const at::Device& dev, int32_t*& out) {
+  out = nullptr;
+  if (o == Py_None) return kUsual;
+  const at::Tensor* t = plain(o);
+  if (t == nullptr || t->device() != dev || t->scalar_type() != at::kInt || t->numel() < 1)
+    return kOther;
+  out = static_cast<int32_t*>(t->data_ptr());
+  return kUsual;
+}
+
+bool whole(PyObject* o, int64_t lo, int64_t hi, int64_t& out) {
+  if (!PyLong_CheckExact(o)) return false;
+  int over = 0;
+  out = PyLong_AsLongLongAndOverflow(o, &over);
+  return over == 0 && out >= lo && out <= hi;
+}
+
+// A contiguous tensor over a part of `base`'s storage (one allocation serves a call's outputs).
+at::Tensor part_of(const at::Tensor& base, at::ScalarType type, int64_t byte, int64_t n) {
+  const caffe2::TypeMeta meta = c10::scalarTypeToTypeMeta(type);
+  auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(), meta);
+  impl->set_storage_offset(byte / static_cast<int64_t>(meta.itemsize()));
+  impl->set_sizes_contiguous({n});
+  return at::Tensor(std::move(impl));
+}
+
+// slots(held, new, block_tables, free_blocks, free_at, block_size, max_tokens, error_flags)
+PyObject* slots(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 8 || g_slots == nullptr) {
+    PyErr_SetString(PyExc_TypeError, "slots takes 8 arguments, after bind_scaled()");
+    return nullptr;
+  }
+  try {
+    if (at::impl::PythonTorchFunctionTLS::stack_len() != 0) Py_RETURN_NONE;
+    Table tab;
+    if (!table_of(args[2], nullptr, tab) || (tab.n > 1 && tab.stride < tab.width)) Py_RETURN_NONE;
+    const at::Device dev = THPVariable_Unpack(args[2]).device();
+    const int32_t* held = vector_of(args[0], dev, tab.n);
+    const int32_t* fresh = vector_of(args[1], dev, tab.n);
+    const int32_t* free_blocks = vector_of(args[3], dev, -1);
+    const int32_t* free_at = vector_of(args[4], dev, 1);
+    int64_t bs, most;
+    int32_t* flags;
+    if (held == nullptr || fresh == nullptr || free_blocks == nullptr || free_at == nullptr ||
+        !whole(args[5], 1, INT32_MAX, bs) || !whole(args[6], 0, INT32_MAX, most) ||
+        flags_of(args[7], dev, flags) != kUsual || c10::hip::current_device() != dev.index())
+      Py_RETURN_NONE;
+    const int64_t free_len = THPVariable_Unpack(args[3]).numel(), n = tab.n;
+    // slots, positions, starts, lens, free_at: each at a multiple of 16 bytes
+    const auto up = [](int64_t x) { return (x + 15) / 16 * 16; };
+    const int64_t at1 = up(8 * most), at2 = at1 + up(4 * most), at3 = at2 + up(4 * (n + 1)),
+                  at4 = at3 + up(4 * n);
+    const at::Tensor base = at::empty({(at4 + 16) / 8}, at::TensorOptions().dtype(at::kLong).device(dev));
+    char* b = static_cast<char*>(base.data_ptr());
+    void* stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_slots(held, fresh, static_cast<int32_t>(n), tab.at, tab.stride,
+                 static_cast<int32_t>(tab.width), free_blocks, free_len, free_at,
+                 static_cast<int32_t>(bs), reinterpret_cast<int32_t*>(b + at2),
+                 reinterpret_cast<int32_t*>(b + at3), reinterpret_cast<int64_t*>(b),
+                 reinterpret_cast<int32_t*>(b + at1), most, reinterpret_cast<int32_t*>(b + at4), flags,
+                 stream);
+    Py_END_ALLOW_THREADS
+    if (rc != MKV_OK) return PyLong_FromLong(rc);
+    const at::Tensor out[5] = {part_of(base, at::kInt, at2, n + 1), part_of(base, at::kInt, at3, n),
+                               part_of(base, at::kLong, 0, most), part_of(base, at::kInt, at1, most),
+                               part_of(base, at::kInt, at4, 1)};
+    PyObject* made = PyTuple_New(5);
+    if (made == nullptr) return nullptr;
+    for (int i = 0; i < 5; ++i) {
+      PyObject* o = THPVariable_Wrap(out[i]);
+      if (o == nullptr) {
+        Py_DECREF(made);
+        return nullptr;
+      }
+      PyTuple_SET_ITEM(made, i, o);
+    }
+    return made;
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
+// store(cache descriptor's address, device index, k, v, block_tables, starts, lens, error_flags)
+PyObject* store(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 8 || g_store == nullptr) {
+    PyErr_SetString(PyExc_TypeError, "store takes 8 arguments, after bind_scaled()");
+    return nullptr;
+  }
+  try {
+    if (at::impl::PythonTorchFunctionTLS::stack_len() != 0) Py_RETURN_NONE;
+    const auto* cache = static_cast<const mkv_scaled_cache_t*>(PyLong_AsVoidPtr(args[0]));
+    if (cache == nullptr) return nullptr;
+    int64_t index;
+    const at::Tensor* k = plain(args[2]);
+    const at::Tensor* v = plain(args[3]);
+    if (!whole(args[1], 0, 127, index) || k == nullptr || v == nullptr || !k->is_cuda()) Py_RETURN_NONE;
+    const at::Device dev(at::kCUDA, static_cast<c10::DeviceIndex>(index));
+    Table tab;
+    int32_t* flags;
+    const int code = dtype_code(k->scalar_type());
+    if (k->dim() != 3 || k->device() != dev || v->device() != dev || k->sizes() != v->sizes() ||
+        k->scalar_type() != v->scalar_type() || (code != MKV_BF16 && code != MKV_F16 && code != MKV_F32) ||
+        k->size(1) != cache->heads || k->size(2) != cache->head_size || k->stride(2) != 1 ||
+        v->stride(2) != 1 || !table_of(args[4], &dev, tab) || flags_of(args[7], dev, flags) != kUsual ||
+        c10::hip::current_device() != dev.index())
+      Py_RETURN_NONE;
+    const int32_t* starts = vector_of(args[5], dev, tab.n + 1);
+    const int32_t* lens = vector_of(args[6], dev, tab.n);
+    if (starts == nullptr || lens == nullptr) Py_RETURN_NONE;
+    const int64_t n = k->size(0), many = n > 1, heads = k->size(1) > 1;
+    void* stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+    const void* kp = k->data_ptr();
+    const void* vp = v->data_ptr();
+    const int64_t kt = many ? k->stride(0) : 0, kh = heads ? k->stride(1) : 0,
+                  vt = many ? v->stride(0) : 0, vh = heads ? v->stride(1) : 0;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_store(cache, kp, kt, kh, vp, vt, vh, n, code, tab.at, tab.stride,
+                 static_cast<int32_t>(tab.width), starts, lens, static_cast<int32_t>(tab.n), flags, stream);
+    Py_END_ALLOW_THREADS
+    if (rc != MKV_OK) return PyLong_FromLong(rc);
+    Py_RETURN_TRUE;
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
+// attend(cache descriptor's address, device index, q, block_tables, starts, lens, scale,
+//        max_new, max_len, out, error_flags)
+PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 11 || g_attend == nullptr || g_attend_size == nullptr) {
+    PyErr_SetString(PyExc_TypeError, "attend takes 11 arguments, after bind_scaled()");
+    return nullptr;
+  }
+  try {
+    if (at::impl::PythonTorchFunctionTLS::stack_len() != 0) Py_RETURN_NONE;
+    const auto* cache = static_cast<const mkv_scaled_cache_t*>(PyLong_AsVoidPtr(args[0]));
+    if (cache == nullptr) return nullptr;
+    int64_t index, most_new = 0, most_len = 0;
+    const at::Tensor* q = plain(args[2]);
+    if (!whole(args[1], 0, 127, index) || q == nullptr || !q->is_cuda()) Py_RETURN_NONE;
+    const at::Device dev(at::kCUDA, static_cast<c10::DeviceIndex>(index));
+    Table tab;
+    int32_t* flags;
+    const int code = dtype_code(q->scalar_type());
+    if (q->dim() != 3 || q->device() != dev || (code != MKV_BF16 && code != MKV_F16) ||
+        q->size(2) != cache->head_size || q->size(1) == 0 || q->size(1) % cache->heads != 0 ||
+        q->size(1) > INT32_MAX || q->stride(2) != 1 ||
+        (q->requires_grad() && c10::GradMode::is_enabled()) || !table_of(args[3], &dev, tab) ||
+        flags_of(args[10], dev, flags) != kUsual || c10::hip::current_device() != dev.index())
+      Py_RETURN_NONE;
+    const int32_t* starts = vector_of(args[4], dev, tab.n + 1);
+    const int32_t* lens = vector_of(args[5], dev, tab.n);
+    if (starts == nullptr || lens == nullptr ||
+        (args[7] != Py_None && !whole(args[7], 0, INT32_MAX, most_new)) ||
+        (args[8] != Py_None && !whole(args[8], 0, INT32_MAX, most_len)))
+      Py_RETURN_NONE;
+    mkv_attend_desc_t d{};
+    if (args[6] == Py_None) {
+      d.softmax_scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(cache->head_size)));
+    } else {
+      if (!PyFloat_CheckExact(args[6])) Py_RETURN_NONE;
+      d.softmax_scale = static_cast<float>(PyFloat_AS_DOUBLE(args[6]));
+    }
+    at::Tensor out;
+    if (args[9] == Py_None) {
+      out = at::empty(q->sizes(), at::TensorOptions().dtype(q->dtype()).device(dev));
+    } else {
+      const at::Tensor* o = plain(args[9]);
+      if (o == nullptr || o->device() != dev || o->scalar_type() != q->scalar_type() ||
+          o->sizes() != q->sizes() || o->stride(2) != 1 ||
+          (q->numel() > 0 && o->data_ptr() == q->data_ptr()))
+        Py_RETURN_NONE;
+      out = *o;
+    }
+    const bool many = q->size(0) > 1, heads = q->size(1) > 1;
+    d.cache = *cache;
+    d.q = q->data_ptr();
+    d.out = out.data_ptr();
+    d.block_tables = tab.at;
+    d.starts = starts;
+    d.lens = lens;
+    d.error_flags = flags;
+    d.q_token_stride = many ? q->stride(0) : 0;
+    d.q_head_stride = heads ? q->stride(1) : 0;
+    d.out_token_stride = many ? out.stride(0) : 0;
+    d.out_head_stride = heads ? out.stride(1) : 0;
+    d.table_stride = tab.stride;
+    d.tokens = q->size(0);
+    d.table_width = static_cast<int32_t>(tab.width);
+    d.requests = static_cast<int32_t>(tab.n);
+    d.q_heads = static_cast<int32_t>(q->size(1));
+    d.dtype = code;
+    d.max_new = static_cast<int32_t>(most_new);
+    d.max_len = static_cast<int32_t>(most_len);
+    const int64_t need = g_attend_size(&d);
+    at::Tensor workspace;  // (its memory goes back in stream order)
+    if (need > 0) {
+      workspace = at::empty({need}, at::TensorOptions().dtype(at::kByte).device(dev));
+      d.workspace = workspace.data_ptr();
+      d.workspace_bytes = need;
+    }
+    void* stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_attend(&d, stream);
+    Py_END_ALLOW_THREADS
+    if (rc != MKV_OK) return PyLong_FromLong(rc);
+    if (args[9] != Py_None) return (Py_INCREF(args[9]), args[9]);
+    return THPVariable_Wrap(out);
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
+// The addresses of mkv_step_slots, mkv_store_scaled, mkv_attend_scaled and
+// mkv_attend_workspace_size.
+PyObject* bind_scaled(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  void* p[4];
+  if (nargs != 4) {
+    PyErr_SetString(PyExc_TypeError, "bind_scaled takes 4 addresses");
+    return nullptr;
+  }
+  for (int i = 0; i < 4; ++i) {
+    p[i] = PyLong_AsVoidPtr(args[i]);
+    if (p[i] == nullptr) {
+      if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "NULL function");
+      return nullptr;
+    }
+  }
+  g_slots = reinterpret_cast<slots_fn>(p[0]);
+  g_store = reinterpret_cast<store_fn>(p[1]);
+  g_attend = reinterpret_cast<attend_fn>(p[2]);
+  g_attend_size = reinterpret_cast<attend_size_fn>(p[3]);
+  Py_RETURN_NONE;
+}
+
 PyObject* bind(PyObject*, PyObject* address) {
   void* p = PyLong_AsVoidPtr(address);
   if (p == nullptr) {
@@ -188,6 +480,14 @@ PyMethodDef methods[] = {
     {"scatter", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(scatter)), METH_FASTCALL,
      "mkv_scatter_shifted on torch tensors; None: take the general path"},
     {"bind", bind, METH_O, "the address of mkv_scatter_shifted"},
+    {"slots", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(slots)), METH_FASTCALL,
+     "mkv_step_slots on torch tensors; None: take the general path"},
+    {"store", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(store)), METH_FASTCALL,
+     "mkv_store_scaled on torch tensors; None: take the general path"},
+    {"attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attend)), METH_FASTCALL,
+     "mkv_attend_scaled on torch tensors; None: take the general path"},
+    {"bind_scaled", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind_scaled)),
+     METH_FASTCALL, "the addresses that slots, store and attend call"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "marathon_binding", nullptr, -1, methods,

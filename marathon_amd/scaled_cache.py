@@ -21,6 +21,10 @@ of the step's token arrays) and ``lens`` (int32 ``[requests]``: tokens held with
 all on the GPU, so that a captured step replays with the lengths of its day.  Rows behind
 ``starts[-1]`` (a padded batch) are neither read nor written.
 
+The calls on tensors that need no conversion go through the CPython binding, which makes these
+functions' checks on the tensors themselves; it answers None, with nothing launched, for any
+other call, which the code here takes (and refuses, where it must).
+
 There is no CPU path and no gradient: tensors that are not on a HIP device raise, and so do
 queries that require one.
 """
@@ -28,6 +32,7 @@ queries that require one.
 from __future__ import annotations
 
 import ctypes
+import warnings
 from dataclasses import dataclass, field
 from itertools import chain
 
@@ -43,6 +48,26 @@ BLOCK_SIZES = (16, 32, 64, 128)
 
 _ROW_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 _QUERY_DTYPES = (torch.bfloat16, torch.float16)
+
+
+class _Usual:
+    """The binding's calls, loaded at the first use; where the module cannot be loaded, calls
+    that always answer None (the general path launches the same kernels)."""
+
+    def __getattr__(self, name):
+        try:
+            call = getattr(_lib.binding(), name)
+        except (RuntimeError, ImportError, OSError) as e:
+            warnings.warn(f"{name}: the general path is taken, slower on the host: {e}",
+                          RuntimeWarning, stacklevel=3)
+
+            def call(*args):
+                return None
+        setattr(self, name, call)
+        return call
+
+
+_usual = _Usual()
 
 
 def _current(device: torch.device) -> bool:
@@ -114,6 +139,7 @@ class ScaledCache:
             d.scales = scales.data_ptr()
         d.num_blocks, d.block_stride, d.head_stride, d.token_stride = kv.shape[0], block, head, token
         d.block_size, d.heads, d.head_size = self.block_size, self.heads, self.head_size
+        self.handle = (ctypes.addressof(d), kv.get_device())  # for the binding; `desc` is kept
 
 
 def _flags(error_flags: torch.Tensor | None, device) -> int | None:
@@ -175,6 +201,12 @@ def step_slots(held: torch.Tensor, new: torch.Tensor, block_tables: torch.Tensor
     exceed ``max_tokens`` or a length is negative, bit ``MKV_FLAG_DST_RANGE`` is set in
     ``error_flags``, the tables are left alone and the step is empty (``lens`` is ``held``,
     every slot -1)."""
+    made = _usual.slots(held, new, block_tables, free_blocks, free_at, block_size, max_tokens,
+                        error_flags)
+    if made is not None:
+        if type(made) is int:
+            _lib.check(made)
+        return StepSlots(*made)
     device = block_tables.device
     if not block_tables.is_cuda:
         raise RuntimeError("step_slots: block_tables is not on a HIP device; there is no CPU path")
@@ -214,6 +246,11 @@ def store_scaled(cache: ScaledCache, k: torch.Tensor, v: torch.Tensor,
     block begun in an earlier step keeps its rows and at least its scale; where the new rows
     need a larger one, the old rows are encoded again under it, which keeps their values but
     for codes that become subnormal.  Infinities saturate, NaNs stay NaN."""
+    done = _usual.store(*cache.handle, k, v, block_tables, starts, lens, error_flags)
+    if done is not None:
+        if done is not True:
+            _lib.check(done)
+        return
     device = cache.device
     if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (cache.heads, cache.head_size):
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)}: [tokens, {cache.heads}, "
@@ -254,6 +291,12 @@ def attend_scaled(cache: ScaledCache, q: torch.Tensor, block_tables: torch.Tenso
     ``max_new`` and ``max_len``: the largest number of new tokens and of tokens of a request,
     where the host knows them (a captured step: the largest that will be replayed).  They
     choose launch shapes only."""
+    got = _usual.attend(*cache.handle, q, block_tables, starts, lens, softmax_scale, max_new,
+                        max_len, out, error_flags)
+    if got is not None:
+        if type(got) is int:
+            _lib.check(got)
+        return got
     device, d = cache.device, cache.head_size
     if q.dim() != 3 or q.shape[2] != d or q.shape[1] == 0 or q.shape[1] % cache.heads:
         raise ValueError(f"q {tuple(q.shape)}: [tokens, a multiple of {cache.heads}, {d}]")
