@@ -183,26 +183,23 @@ int64_t mkv_attend_workspace_size(const mkv_attend_desc_t* desc);
  *            length, gets no units (MKV_FLAG_SPAN): a block is written by one span.
  *   src, dst : geometry (block_size and num_blocks; the rest is not read).
  *   units  : out, room for max_units of them; at least the sum of ceil(n_tokens / dst
- *            block_size) is never too little (MKV_ERR_ARG otherwise).
+ *            block_size) is never too little (MKV_ERR_ARG otherwise).  A unit is
+ *            MKV_UNIT_WORDS(src block_size, dst block_size) words, int32:
+ *              0  destination block         1  rows, 1 to its block size
+ *              2  span, whose rotation table it takes; -1: delta 0
+ *              3  row 0's place in the first source block
+ *              4..  source blocks, in order; -1: out of range; then zeros
  *   *n_units : out.
  *   *flags : out (or NULL), MKV_FLAG bits: a block whose id is out of range gets no unit
  *            (DST_RANGE); rows whose source is get no code (SRC_RANGE).
  */
-#define MKV_UNIT_SOURCES 9
-typedef struct mkv_scaled_unit {
-  int32_t dst;    /* destination block */
-  int32_t rows;   /* 1 to its block size */
-  int32_t span;   /* whose rotation table; -1: delta 0 */
-  int32_t first;  /* row 0's place in the first source block */
-  int32_t src[MKV_UNIT_SOURCES]; /* source blocks, in order; -1: out of range */
-  int32_t reserved[3];
-} mkv_scaled_unit_t;
+#define MKV_UNIT_SOURCES(src_bs, dst_bs) ((dst_bs) > (src_bs) ? (dst_bs) / (src_bs) + 1 : 2)
+#define MKV_UNIT_WORDS(src_bs, dst_bs) ((4 + MKV_UNIT_SOURCES(src_bs, dst_bs) + 3) / 4 * 4)
 
 int mkv_scaled_units(const mkv_span_t* spans, int32_t n_spans, const int32_t* src_table,
                      int64_t src_table_len, const int32_t* dst_table, int64_t dst_table_len,
                      const mkv_scaled_cache_t* src, const mkv_scaled_cache_t* dst,
-                     mkv_scaled_unit_t* units, int64_t max_units, int64_t* n_units,
-                     int32_t* flags);
+                     int32_t* units, int64_t max_units, int64_t* n_units, int32_t* flags);
 
 /*
  *   units        : device [n_units], 16-byte aligned, made by mkv_scaled_units; ids in them
@@ -217,7 +214,7 @@ typedef struct mkv_scaled_shift_desc {
   mkv_scaled_cache_t dst;
   const uint64_t* src_layers;
   const uint64_t* dst_layers;
-  const mkv_scaled_unit_t* units;
+  const int32_t* units;
   const float* tables;
   int64_t n_units;
   int32_t n_spans;

@@ -233,7 +233,12 @@ class ScaledShiftDesc(ctypes.Structure):
 assert ctypes.sizeof(ScaledCacheDesc) == 72 and ctypes.sizeof(AttendDesc) == 216
 assert ctypes.sizeof(ScaledShiftDesc) == 200
 
-UNIT_BYTES = 64  # mkv_scaled_unit_t
+
+def unit_words(src_bs: int, dst_bs: int) -> int:
+    """MKV_UNIT_WORDS: int32 words of a unit of a block-scaled shift."""
+    sources = dst_bs // src_bs + 1 if dst_bs > src_bs else 2
+    return (4 + sources + 3) // 4 * 4
+
 
 
 class KVShiftError(RuntimeError):

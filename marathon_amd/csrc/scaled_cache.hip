@@ -453,10 +453,12 @@ struct MoveParams {
   DevCache dst;
   const uint64_t* src_layers;
   const uint64_t* dst_layers;
-  const mkv_scaled_unit_t* units;
+  const int32_t* units;
   const float* tables;
   int32_t n_spans;
   int32_t rotary;
+  int32_t words;    // of a unit, 16 at most
+  int32_t sources;  // source blocks in it
 };
 
 // A workgroup makes one destination block of `heads_here` heads in one layer and ends.  What
@@ -476,15 +478,17 @@ __global__ __launch_bounds__(64 * kMaxWaves) void move_kernel(MoveParams p) {
   const bool active = head < p.dst.heads;
   const int piece = lane % R::kChunks, sub = lane / R::kChunks;
   // the record's words, one a lane
-  const int word = reinterpret_cast<const int32_t*>(p.units + blockIdx.x)[lane & 15];
+  const int word = p.units[static_cast<int64_t>(blockIdx.x) * p.words + min(lane, p.words - 1)];
   const int id = __builtin_amdgcn_readlane(word, 0), n = __builtin_amdgcn_readlane(word, 1);
   const int span = __builtin_amdgcn_readlane(word, 2), first = __builtin_amdgcn_readlane(word, 3);
   if (id < 0 || id >= p.dst.num_blocks || span >= p.n_spans) return;
 
   // Where each pass's row comes from: a wave's 16 rows lie in two source blocks at most.
   const int start = first + part * 16, block0 = start >> p.src.bs_shift;
-  const int src0 = block0 >= 0 && block0 < MKV_UNIT_SOURCES ? __builtin_amdgcn_readlane(word, 4 + block0) : -1;
-  const int src1 = block0 >= -1 && block0 < MKV_UNIT_SOURCES - 1 ? __builtin_amdgcn_readlane(word, 5 + block0) : -1;
+  const auto source = [&](int b) {
+    return b >= 0 && b < p.sources ? __builtin_amdgcn_readlane(word, 4 + b) : -1;
+  };
+  const int src0 = source(block0), src1 = source(block0 + 1);
   int64_t from_row[P], from_scale[P];
   bool there[P];
   bool whole = active;  // every row of the wave has a source: nothing to blank out
@@ -706,8 +710,8 @@ extern "C" int mkv_store_scaled(const mkv_scaled_cache_t* cache, const void* k,
 extern "C" int mkv_scaled_units(const mkv_span_t* spans, int32_t n_spans, const int32_t* src_table,
                                 int64_t src_table_len, const int32_t* dst_table,
                                 int64_t dst_table_len, const mkv_scaled_cache_t* src,
-                                const mkv_scaled_cache_t* dst, mkv_scaled_unit_t* units,
-                                int64_t max_units, int64_t* n_units, int32_t* flags) {
+                                const mkv_scaled_cache_t* dst, int32_t* units, int64_t max_units,
+                                int64_t* n_units, int32_t* flags) {
   const char* who = "mkv_scaled_units";
   if (src == nullptr || dst == nullptr || n_units == nullptr)
     return mkv_fail(MKV_ERR_ARG, "%s: a pointer is NULL", who);
@@ -724,6 +728,7 @@ extern "C" int mkv_scaled_units(const mkv_span_t* spans, int32_t n_spans, const 
   int64_t count = 0;
   int32_t raised = 0;
   const int32_t bs = dst->block_size, sbs = src->block_size;
+  const int32_t sources = MKV_UNIT_SOURCES(sbs, bs), words = MKV_UNIT_WORDS(sbs, bs);
   // a block number in a table, which positions and indices of any size may leave
   const auto entry = [](const int32_t* table, int64_t len, int64_t index, int64_t block,
                         int64_t blocks) -> int32_t {
@@ -747,19 +752,21 @@ extern "C" int mkv_scaled_units(const mkv_span_t* spans, int32_t n_spans, const 
       }
       if (count >= max_units)
         return mkv_fail(MKV_ERR_ARG, "%s: more than %lld units", who, (long long)max_units);
-      mkv_scaled_unit_t& u = units[count++];
-      u = mkv_scaled_unit_t{};
-      u.dst = id;
-      u.rows = static_cast<int32_t>(sp.n_tokens - at < bs ? sp.n_tokens - at : bs);
-      u.span = sp.delta != 0 ? i : -1;
-      u.first = static_cast<int32_t>((sp.src_pos + at) % sbs);
+      int32_t* u = units + words * count++;
+      const int32_t rows = static_cast<int32_t>(sp.n_tokens - at < bs ? sp.n_tokens - at : bs);
+      const int32_t first = static_cast<int32_t>((sp.src_pos + at) % sbs);
       const int64_t block = (sp.src_pos + at) / sbs;
-      const int used = (u.first + u.rows + sbs - 1) / sbs;
-      for (int j = 0; j < MKV_UNIT_SOURCES; ++j) {
-        u.src[j] = j < used
-                       ? entry(src_table, src_table_len, sp.src_index, block + j, src->num_blocks)
-                       : -1;
-        if (j < used && u.src[j] < 0) raised |= MKV_FLAG_SRC_RANGE;
+      const int32_t used = (first + rows + sbs - 1) / sbs;
+      u[0] = id;
+      u[1] = rows;
+      u[2] = sp.delta != 0 ? i : -1;
+      u[3] = first;
+      for (int32_t j = 0; j < words - 4; ++j) {
+        u[4 + j] = j >= sources ? 0 : -1;
+        if (j < used) {
+          u[4 + j] = entry(src_table, src_table_len, sp.src_index, block + j, src->num_blocks);
+          if (u[4 + j] < 0) raised |= MKV_FLAG_SRC_RANGE;
+        }
       }
     }
   }
@@ -798,6 +805,8 @@ extern "C" int mkv_shift_scaled(const mkv_scaled_shift_desc_t* d, void* stream) 
   p.tables = d->tables;
   p.n_spans = d->n_spans;
   p.rotary = d->rotary;
+  p.words = MKV_UNIT_WORDS(d->src.block_size, d->dst.block_size);
+  p.sources = MKV_UNIT_SOURCES(d->src.block_size, d->dst.block_size);
   const int waves = waves_of(p.dst.bs_shift, p.dst.heads), heads_here = waves / (d->dst.block_size / 16);
   const int64_t head_groups = (d->dst.heads + heads_here - 1) / heads_here;
   const dim3 grid(static_cast<unsigned>(d->n_units), static_cast<unsigned>(head_groups),

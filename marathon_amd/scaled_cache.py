@@ -365,6 +365,7 @@ class ScaledShifts:
         d = self.desc = _lib.ScaledShiftDesc()
         d.src, d.dst = a.desc, b.desc
         d.layers, d.rotary = self.layers, self.rotary
+        self._unit_bytes = 4 * _lib.unit_words(a.block_size, b.block_size)
         with _on(self.device, _current(self.device)):
             # (a copy from pageable memory: it is there when the call returns)
             self._bases = torch.tensor(
@@ -402,7 +403,7 @@ class ScaledShifts:
         tables = [_host_table(t) for t in (src_table, dst_table)]
         # units, then the spans' rotation tables, in one pinned buffer
         turns = n * 8 * self.rotary if deltas else 0
-        room = most * _lib.UNIT_BYTES
+        room = most * self._unit_bytes
         host = torch.empty(room + turns, dtype=torch.uint8, pin_memory=True)
         at, d, L = host.data_ptr(), self.desc, _lib.lib()
         out = np.zeros(2, np.int64)  # units, flags

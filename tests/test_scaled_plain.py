@@ -47,13 +47,15 @@ int main(void) {
   printf("%zu %zu %zu\n", sizeof(mkv_scaled_cache_t), sizeof(mkv_attend_desc_t),
          sizeof(mkv_scaled_shift_desc_t));
 @
-  printf("limits %d %d %d %zu\n", MKV_SCALE_MIN_EXP, MKV_SCALE_MAX_EXP, MKV_MAX_REQUESTS,
-         sizeof(mkv_scaled_unit_t));
+  printf("limits %d %d %d\n", MKV_SCALE_MIN_EXP, MKV_SCALE_MAX_EXP, MKV_MAX_REQUESTS);
+  for (int s = 16; s <= 128; s *= 2)
+    for (int d = 16; d <= 128; d *= 2) printf("%d ", MKV_UNIT_WORDS(s, d));
+  printf("\n");
   return 0;
 }
 """
 STRUCTS = {"mkv_scaled_cache_t": _lib.ScaledCacheDesc, "mkv_attend_desc_t": _lib.AttendDesc,
-           "mkv_scaled_shift_desc_t": _lib.ScaledShiftDesc}  # and mkv_scaled_unit_t, 16 int32
+           "mkv_scaled_shift_desc_t": _lib.ScaledShiftDesc}
 
 
 def test_descriptors_match_the_header(tmp_path):
@@ -70,8 +72,10 @@ def test_descriptors_match_the_header(tmp_path):
             field, at = line.split()
             name, f = field.split(".")
             assert getattr(STRUCTS[name], f).offset == int(at), field
-    assert out[-2] == (f"limits {_lib.MKV_SCALE_MIN_EXP} {_lib.MKV_SCALE_MAX_EXP} "
-                       f"{_lib.MKV_MAX_REQUESTS} {_lib.UNIT_BYTES}")
+    assert out[-3] == (f"limits {_lib.MKV_SCALE_MIN_EXP} {_lib.MKV_SCALE_MAX_EXP} "
+                       f"{_lib.MKV_MAX_REQUESTS}")
+    sizes = (16, 32, 64, 128)
+    assert out[-2].split() == [str(_lib.unit_words(s, d)) for s in sizes for d in sizes]
 
 
 def cache_desc(**kw):
@@ -201,13 +205,14 @@ def test_shift_refuses(change, code):
 
 
 def units_of(rows, src_table, dst_table, sbs=16, dbs=16, blocks=(50, 60), room=None):
-    """(status, unit records as int32 [n, 16], flags)."""
+    """(status, units as int32 [n, words], flags)."""
     spans = np.zeros(len(rows), _lib.SPAN_DTYPE)
     for i, r in enumerate(rows):
         spans[i] = r
     st, dt = np.asarray(src_table, np.int32), np.asarray(dst_table, np.int32)
     room = sum(-(-max(r[4], 0) // dbs) for r in rows) if room is None else room
-    out, got = np.full((room + 1, 16), 77, np.int32), np.zeros(2, np.int64)
+    words = _lib.unit_words(sbs, dbs)
+    out, got = np.full((room + 1, words), 77, np.int32), np.zeros(2, np.int64)
     a, b = (cache_desc(block_size=s, num_blocks=n) for s, n in zip((sbs, dbs), blocks))
     rc = _lib.lib().mkv_scaled_units(
         spans.ctypes.data, len(rows), st.ctypes.data, st.size, dt.ctypes.data, dt.size,
