@@ -23,7 +23,7 @@ using namespace mkv_scaled;
 
 // ------------------------------------------------------------------------- step slots
 
-constexpr int kSlotThreads = 1024;
+constexpr int kSlotThreads = 256;  // (1,024: 5.1 / 6.6 us against 3.9 / 5.2, 32 and 256 requests)
 
 struct SlotParams {
   const int32_t* held;
@@ -43,9 +43,17 @@ struct SlotParams {
   int32_t requests;
   int32_t table_width;
   int32_t block_size;
+  int32_t bs_shift;  // -1 where block_size is no power of two
 };
 
-__device__ __forceinline__ int64_t blocks_of(int64_t tokens, int bs) { return (tokens + bs - 1) / bs; }
+// Sizes of at most 2^31 - 1 tokens: 32 bits, unsigned, hold them and what is added.
+__device__ __forceinline__ uint32_t block_of(uint32_t pos, const SlotParams& p) {
+  return p.bs_shift >= 0 ? pos >> p.bs_shift : pos / static_cast<uint32_t>(p.block_size);
+}
+
+__device__ __forceinline__ uint32_t blocks_of(uint32_t tokens, const SlotParams& p) {
+  return tokens == 0 ? 0u : block_of(tokens - 1, p) + 1;
+}
 
 // The last r in [0, n) with a[r] <= at, by halves in LDS; a[0] = 0 <= at.
 __device__ __forceinline__ int owner(const int32_t* a, int n, int at) {
@@ -63,7 +71,7 @@ __global__ __launch_bounds__(kSlotThreads) void step_slots_kernel(SlotParams p) 
   __shared__ int64_t s_wave[2][kSlotThreads / 64];
   __shared__ int32_t s_bad;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int n = p.requests, bs = p.block_size;
+  const int n = p.requests;
   if (tid == 0) s_bad = 0;
   __syncthreads();
   // prefix sums over the requests, a stretch of kSlotThreads at a time
@@ -75,11 +83,11 @@ __global__ __launch_bounds__(kSlotThreads) void step_slots_kernel(SlotParams p) 
       held = p.held[r];
       add = p.fresh[r];
       if (held < 0 || add < 0 || held + add > INT32_MAX ||
-          blocks_of(held + add, bs) > p.table_width) {
+          blocks_of(static_cast<uint32_t>(held + add), p) > static_cast<uint32_t>(p.table_width)) {
         s_bad = 1;
         held = add = 0;
       }
-      need = blocks_of(held + add, bs) - blocks_of(held, bs);
+      need = blocks_of(static_cast<uint32_t>(held + add), p) - blocks_of(static_cast<uint32_t>(held), p);
     }
     int64_t a = add, b = need;  // inclusive within the wave
     for (int d = 1; d < 64; d <<= 1) {
@@ -128,7 +136,7 @@ __global__ __launch_bounds__(kSlotThreads) void step_slots_kernel(SlotParams p) 
   if (!bad) {  // table entries of the fresh blocks
     for (int64_t j = gtid; j < blocks; j += step) {
       const int r = owner(s_block, n, static_cast<int>(j));
-      const int64_t col = blocks_of(p.held[r], bs) + (j - s_block[r]);
+      const int64_t col = blocks_of(static_cast<uint32_t>(p.held[r]), p) + (j - s_block[r]);
       p.tables[r * p.table_stride + col] = p.free_blocks[at + j];
     }
   }
@@ -139,11 +147,12 @@ __global__ __launch_bounds__(kSlotThreads) void step_slots_kernel(SlotParams p) 
       const int r = owner(s_start, n, static_cast<int>(t));
       const int held = p.held[r];
       pos = held + static_cast<int>(t) - s_start[r];
-      const int64_t b = pos / bs, before = blocks_of(held, bs);
+      const uint32_t b = block_of(static_cast<uint32_t>(pos), p);
+      const uint32_t before = blocks_of(static_cast<uint32_t>(held), p);
       // a fresh block's id comes from the free list: other workgroups may be writing its entry
       const int64_t id = b < before ? p.tables[r * p.table_stride + b]
                                     : p.free_blocks[at + s_block[r] + (b - before)];
-      slot = id < 0 ? -1 : id * bs + pos % bs;
+      slot = id < 0 ? -1 : id * p.block_size + (static_cast<uint32_t>(pos) - b * p.block_size);
     }
     p.slots[t] = slot;
     p.positions[t] = pos;
@@ -650,9 +659,10 @@ extern "C" int mkv_step_slots(const int32_t* held, const int32_t* fresh, int32_t
     return mkv_fail(MKV_ERR_ARG, "%s: free_at_out is free_at itself", who);
   const SlotParams p = {held,   fresh,    block_tables, table_stride, free_blocks, free_at,
                         starts, lens,     slots,        positions,    free_at_out, error_flags,
-                        free_len, max_tokens, requests, table_width,  block_size};
+                        free_len, max_tokens, requests, table_width,  block_size,
+                        (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1};
   const int64_t want = (max_tokens + kSlotThreads - 1) / kSlotThreads;
-  const int grid = static_cast<int>(want < 1 ? 1 : want > 256 ? 256 : want);
+  const int grid = static_cast<int>(want < 1 ? 1 : want > 512 ? 512 : want);
   step_slots_kernel<<<grid, kSlotThreads, 0, static_cast<hipStream_t>(stream)>>>(p);
   return launched(who);
 }
