@@ -656,9 +656,7 @@ __global__ __launch_bounds__(64 * kManyWaves, (D == 256 ? 1 : 2)) void attend_ma
       const int g = k_group(u);
       const char* kb = p.c.k + block_of(x, n + g) +
                        ((at + 16 * g) & bs_mask) * static_cast<int64_t>(p.c.tstride);
-      // rows of one load past the 16th of the block's group (D = 256: four loads a group)
-      const int down = (u * kRowsPass + wave * (64 / KC)) % 16 - wave * (64 / KC) % 16;
-      rk[u] = *reinterpret_cast<const u32x4*>(kb + down * static_cast<int64_t>(p.c.tstride) + k_off);
+      rk[u] = *reinterpret_cast<const u32x4*>(kb + k_off);
     }
     const char* vb = p.c.v + block_of(x, n + wave) +
                      ((at + 16 * wave) & bs_mask) * static_cast<int64_t>(p.c.tstride);
@@ -702,7 +700,7 @@ __global__ __launch_bounds__(64 * kManyWaves, (D == 256 ? 1 : 2)) void attend_ma
       uint32_t any = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const bool seen = good && at + 4 * (tid >> 4) + i < t.keys;
+        const bool seen = good && i < t.keys - at - 4 * (tid >> 4);
 #pragma unroll
         for (int u = 0; u < D / 64; ++u) {
           rv[i][u] = seen ? rv[i][u] : 0u;
@@ -767,17 +765,16 @@ __global__ __launch_bounds__(64 * kManyWaves, (D == 256 ? 1 : 2)) void attend_ma
         for (int i = 0; i < 16; ++i) s[st][i] *= pow2(ek[2 * st + (i >> 3)]);
     }
     // register i of tile st: token at + 32 st + 8 (i / 4) + 4 h + i % 4
-    uint32_t see = ~0u;
+    // (compared with what is left, the places are constants: none is kept in a register)
     if (masked) {
-      see = 0;
+      const int left = limit - at - 4 * h;
 #pragma unroll
       for (int st = 0; st < 2; ++st)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const bool sees = at + 32 * st + 8 * (i >> 2) + 4 * h + (i & 3) < limit &&
+          const bool sees = 32 * st + 8 * (i >> 2) + (i & 3) < left &&
                             __builtin_amdgcn_readlane(x.id, n + 2 * st + (i >> 3)) >= 0;
           s[st][i] = sees ? s[st][i] : -kInf;
-          see |= sees ? 1u << (16 * st + i) : 0u;
         }
     }
     float top = s[0][0];
@@ -850,7 +847,7 @@ __global__ __launch_bounds__(64 * kManyWaves, (D == 256 ? 1 : 2)) void attend_ma
             bool nan = tok < t.keys && __builtin_amdgcn_readlane(x.id, n + g) >= 0;
             if (nan) nan = (vb[(tok & bs_mask) * static_cast<int64_t>(p.c.tstride)] & 0x7F) == 0x7F;
             bad[j >> 1] |= nan ? 0x3F80u << (16 * (j & 1)) : 0u;
-            ones[j >> 1] |= (see >> (8 * g + j)) & 1u ? 0x3F80u << (16 * (j & 1)) : 0u;
+            ones[j >> 1] |= tok < limit ? 0x3F80u << (16 * (j & 1)) : 0u;
           }
           hit = times(bad, ones, hit);
         }
@@ -996,10 +993,7 @@ struct Shape {
 };
 
 constexpr int64_t kWantFew = 4096;
-#ifndef MKV_WM
-#define MKV_WM 1024
-#endif
-constexpr int64_t kWantMany = MKV_WM;
+constexpr int64_t kWantMany = 1024;
 
 int check(const mkv_attend_desc_t& d, AttendParams* p, Shape* shape) {
   const char* who = "mkv_attend_scaled";
