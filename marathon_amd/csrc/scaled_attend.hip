@@ -49,6 +49,7 @@ struct AttendParams {
   int64_t tokens;
   int32_t group;   // query heads a KV head serves
   int32_t splits;  // most parts that a tile's tokens are cut into
+  int32_t rows_from, rows_to;  // the requests that this launch is for, by their rows
   int32_t per;     // tokens of a part, a multiple of 64 (more where `splits` would not reach)
   float scale;     // softmax_scale * log2(e)
 };
@@ -80,18 +81,21 @@ __device__ __forceinline__ bool find_tile(const AttendParams& p, int64_t tile, T
   const auto begin = [starts, group](int i) {
     return static_cast<int64_t>(starts[i]) * group / BM + i;
   };
-  const int r = last_at_most(p.s.requests, tile, begin);
+  const bool single = p.rows_to <= BM;  // a request has one tile: the grid has one for each
+  const int r = single ? static_cast<int>(tile) : last_at_most(p.s.requests, tile, begin);
   if (r < 0) return false;
   t.request = r;
   t.s0 = starts[r];
   const int64_t s1 = starts[r + 1];
-  const int64_t first_tile = t.s0 * group / BM + r;
+  const int64_t first_tile = single ? tile : begin(r);
   if (t.s0 < 0 || s1 < t.s0 || s1 > p.tokens) {
     if (threadIdx.x == 0 && tile == first_tile) raise(p.s.flags, MKV_FLAG_SPAN);
     return false;
   }
   t.row0 = (tile - first_tile) * BM;
-  const int64_t rows = (s1 - t.s0) * group - t.row0;
+  const int64_t all = (s1 - t.s0) * group;
+  if (all < p.rows_from || all > p.rows_to) return false;  // another launch's
+  const int64_t rows = all - t.row0;
   if (rows <= 0) return false;
   t.rows = static_cast<int>(rows < BM ? rows : BM);
   const int64_t len = p.s.lens[r];
@@ -984,23 +988,61 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p) {
 
 // ------------------------------------------------------------------------------- host
 
-// How a call runs: rows a tile has, tiles, and the parts that a tile's tokens may be cut into.
+// How a call's requests run: rows a tile has, tiles, the parts that a tile's tokens may be cut
+// into and the tokens of one, and the requests (by their rows) that it is for.
 struct Shape {
   int rows;
   int64_t each;  // rows of the largest request
   int64_t tiles;
   int splits;
+  int per;
+  int32_t from, to;
+
+  int64_t parts(int heads) const { return splits > 1 ? tiles * heads * splits : 0; }
+  int64_t bytes(int heads, int head_size) const {
+    return parts(heads) * rows * (head_size + 2) * 4;
+  }
+};
+
+// One launch for all requests, or one for the few rows of most and one for the many of others.
+struct Plan {
+  Shape shape[2];
+  int count;
 };
 
 constexpr int64_t kWantFew = 4096;
 constexpr int64_t kWantMany = 1024;
 
-int check(const mkv_attend_desc_t& d, AttendParams* p, Shape* shape) {
+// A tile's rows by those of the largest request, and the parts: of one size for all requests,
+// so that long and short histories fill the chip alike, about `want` workgroups if every
+// request were the longest.
+Shape shape_for(const mkv_attend_desc_t& d, int64_t each, int32_t from, int32_t to) {
+  Shape s;
+  const int64_t rows = d.tokens * (d.q_heads / d.cache.heads);
+  s.each = each;
+  s.rows = each <= 16 ? 16 : each <= 32 ? 32 : kManyRows;
+  s.tiles = to <= s.rows ? d.requests : rows / s.rows + d.requests;
+  s.from = from;
+  s.to = to;
+  const int64_t room = static_cast<int64_t>(d.table_width) * d.cache.block_size;
+  const int64_t longest = d.max_len > 0 && d.max_len < room ? d.max_len : room;
+  const int64_t largest = (each + s.rows - 1) / s.rows * d.requests;  // if all were the largest
+  const int64_t groups = (s.tiles < largest ? s.tiles : largest) * d.cache.heads;
+  const int64_t want = s.rows == kManyRows ? kWantMany : kWantFew;
+  int64_t per = longest * (groups > 0 ? groups : 1) / want;
+  if (per < longest / kMaxSplits + 64) per = longest / kMaxSplits + 64;
+  per = ((per < kMinSplit ? kMinSplit : per) + 63) / 64 * 64;
+  s.splits = static_cast<int>(longest > per ? (longest + per - 1) / per : 1);
+  s.per = static_cast<int>(per);
+  return s;
+}
+
+int check(const mkv_attend_desc_t& d, AttendParams* p, Plan* plan) {
   const char* who = "mkv_attend_scaled";
   int rc = check_cache(who, d.cache, true, &p->c);
   if (rc == MKV_OK)
-    rc = check_step(who, d.cache.block_size, d.block_tables, d.table_stride, d.table_width, d.starts, d.lens,
-                    d.requests, d.error_flags, &p->s);
+    rc = check_step(who, d.cache.block_size, d.block_tables, d.table_stride, d.table_width,
+                    d.starts, d.lens, d.requests, d.error_flags, &p->s);
   if (rc != MKV_OK) return rc;
   if (d.dtype != MKV_BF16 && d.dtype != MKV_F16)
     return mkv_fail(MKV_ERR_DTYPE, "%s: dtype %d is not bf16 or fp16", who, d.dtype);
@@ -1028,32 +1070,30 @@ int check(const mkv_attend_desc_t& d, AttendParams* p, Shape* shape) {
   p->group = d.q_heads / d.cache.heads;
   p->scale = d.softmax_scale * 1.4426950408889634f;
 
-  const int64_t rows = d.tokens * p->group;
-  const int64_t each = static_cast<int64_t>(d.max_new > 0 ? d.max_new : d.tokens) * p->group;
-  shape->each = each;
-  shape->rows = each <= 16 ? 16 : each <= 32 ? 32 : kManyRows;
-  shape->tiles = rows / shape->rows + d.requests;
-  // Parts of one size for all requests, so that long and short histories fill the chip alike:
-  // about `want` workgroups if every request were the longest.
-  const int64_t room = static_cast<int64_t>(d.table_width) * d.cache.block_size;
-  const int64_t longest = d.max_len > 0 && d.max_len < room ? d.max_len : room;
-  const int64_t largest = (each + shape->rows - 1) / shape->rows;  // tiles of one request
-  const int64_t busy = rows / shape->rows + d.requests;
-  const int64_t groups = (busy < largest * d.requests ? busy : largest * d.requests) * d.cache.heads;
-  const int64_t want = shape->rows == kManyRows ? kWantMany : kWantFew;
-  int64_t per = longest * (groups > 0 ? groups : 1) / want;
-  if (per < longest / kMaxSplits + 64) per = longest / kMaxSplits + 64;
-  per = ((per < kMinSplit ? kMinSplit : per) + 63) / 64 * 64;
-  shape->splits = static_cast<int>(longest > per ? (longest + per - 1) / per : 1);
-  p->splits = shape->splits;
-  p->per = static_cast<int>(per);
-  if (shape->tiles > INT32_MAX)
-    return mkv_fail(MKV_ERR_UNSUPPORTED, "%s: %lld tiles", who, (long long)shape->tiles);
+  const int64_t new_most = d.max_new > 0 && d.max_new < d.tokens ? d.max_new : d.tokens;
+  const int64_t each = new_most * p->group;
+  // A long chunk beside decoding requests: where those behind the largest have 16 rows or
+  // fewer on average, the requests of up to 16 rows get a launch of their own, of 16 rows a
+  // tile in place of 128. Measured as one launch / two, 4 query heads a KV head: a chunk of
+  // 1,024 tokens beside 31 requests at 16,000 tokens 535 / 440 us, 1,000 beside 255 at 4,000
+  // 400 / 348, 1,000 beside one at 16,000 314 / 306, 512 beside 3 143 / 145; with a chunk of
+  // 129 beside 31 149 / 173, of 13 beside one 41 / 59: there the one launch has room for both.
+  const int64_t rest = (d.tokens - new_most) * p->group;
+  if (each >= 2048 && d.requests > 1 && rest <= 16 * static_cast<int64_t>(d.requests - 1)) {
+    plan->shape[0] = shape_for(d, 16, 0, 16);
+    plan->shape[1] = shape_for(d, each, 17, INT32_MAX);
+    plan->count = 2;
+  } else {
+    plan->shape[0] = shape_for(d, each, 0, INT32_MAX);
+    plan->count = 1;
+  }
+  for (int i = 0; i < plan->count; ++i) {  // the grid's limits
+    const Shape& s = plan->shape[i];
+    if (s.tiles > (s.rows == kManyRows ? 65535 : UINT32_MAX / (64 * kFewWaves)))
+      return mkv_fail(MKV_ERR_UNSUPPORTED, "%s: %lld query rows", who,
+                      (long long)(d.tokens * p->group));
+  }
   return MKV_OK;
-}
-
-int64_t parts_of(const mkv_attend_desc_t& d, const Shape& s) {
-  return s.splits > 1 ? s.tiles * d.cache.heads * s.splits : 0;
 }
 
 template <bool F16, int D, int RT>
@@ -1093,17 +1133,20 @@ void launch(int d, const AttendParams& p, const Shape& s, int heads, hipStream_t
 extern "C" int64_t mkv_attend_workspace_size(const mkv_attend_desc_t* d) {
   if (d == nullptr) return -1;
   AttendParams p;
-  Shape s;
-  if (check(*d, &p, &s) != MKV_OK) return -1;
-  return parts_of(*d, s) * s.rows * (d->cache.head_size + 2) * 4;
+  Plan plan;
+  if (check(*d, &p, &plan) != MKV_OK) return -1;
+  int64_t bytes = 0;
+  for (int i = 0; i < plan.count; ++i)
+    bytes += plan.shape[i].bytes(d->cache.heads, d->cache.head_size);
+  return bytes;
 }
 
 extern "C" int mkv_attend_scaled(const mkv_attend_desc_t* d, void* stream) {
   const char* who = "mkv_attend_scaled";
   if (d == nullptr) return mkv_fail(MKV_ERR_ARG, "%s: desc is NULL", who);
   AttendParams p;
-  Shape s;
-  const int rc = check(*d, &p, &s);
+  Plan plan;
+  const int rc = check(*d, &p, &plan);
   if (rc != MKV_OK) return rc;
   if (d->tokens == 0 || d->requests == 0) return MKV_OK;
   if (d->q == nullptr || d->out == nullptr)
@@ -1111,19 +1154,27 @@ extern "C" int mkv_attend_scaled(const mkv_attend_desc_t* d, void* stream) {
   if (((reinterpret_cast<uintptr_t>(d->q) | reinterpret_cast<uintptr_t>(d->out) | p.q_token |
         p.q_head | p.out_token | p.out_head) & 15) != 0)
     return mkv_fail(MKV_ERR_ALIGN, "%s: q or out is not 16-byte aligned", who);
-  const int64_t parts = parts_of(*d, s);
-  const int64_t need = parts * s.rows * (d->cache.head_size + 2) * 4;
+  const int64_t need = mkv_attend_workspace_size(d);
   if (need > 0 && (d->workspace == nullptr || d->workspace_bytes < need))
     return mkv_fail(MKV_ERR_ARG, "%s: workspace of %lld bytes, %lld needed", who,
                     (long long)d->workspace_bytes, (long long)need);
   if ((reinterpret_cast<uintptr_t>(d->workspace) & 15) != 0)
     return mkv_fail(MKV_ERR_ALIGN, "%s: workspace is not 16-byte aligned", who);
-  p.part_o = static_cast<float*>(d->workspace);
-  p.part_ml = need > 0 ? p.part_o + parts * s.rows * d->cache.head_size : nullptr;
-  hipStream_t hs = static_cast<hipStream_t>(stream);
-  if (d->dtype == MKV_F16)
-    launch<true>(d->cache.head_size, p, s, d->cache.heads, hs);
-  else
-    launch<false>(d->cache.head_size, p, s, d->cache.heads, hs);
+  char* room = static_cast<char*>(d->workspace);
+  for (int i = 0; i < plan.count; ++i) {
+    const Shape& s = plan.shape[i];
+    p.splits = s.splits;
+    p.per = s.per;
+    p.rows_from = s.from;
+    p.rows_to = s.to;
+    p.part_o = reinterpret_cast<float*>(room);
+    p.part_ml = p.part_o + s.parts(d->cache.heads) * s.rows * d->cache.head_size;
+    room += s.bytes(d->cache.heads, d->cache.head_size);
+    hipStream_t hs = static_cast<hipStream_t>(stream);
+    if (d->dtype == MKV_F16)
+      launch<true>(d->cache.head_size, p, s, d->cache.heads, hs);
+    else
+      launch<false>(d->cache.head_size, p, s, d->cache.heads, hs);
+  }
   return launched(who);
 }

@@ -711,6 +711,8 @@ extern "C" int mkv_store_scaled(const mkv_scaled_cache_t* cache, const void* k,
   // workgroup, 22,141 of 8 heads 112 / 73 / 29.
   const int64_t each = tokens * ((cache->heads + heads_here - 1) / heads_here);
   p.group = each <= 4096 ? 1 : each <= 32768 ? 4 : 16;
+  if ((tokens + p.group - 1) / p.group > UINT32_MAX / (64 * waves))
+    return mkv_fail(MKV_ERR_UNSUPPORTED, "%s: %lld tokens", who, (long long)tokens);
   const dim3 grid(static_cast<unsigned>((tokens + p.group - 1) / p.group),
                   static_cast<unsigned>((cache->heads + heads_here - 1) / heads_here));
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -824,6 +826,8 @@ extern "C" int mkv_shift_scaled(const mkv_scaled_shift_desc_t* d, void* stream) 
   p.words = MKV_UNIT_WORDS(d->src.block_size, d->dst.block_size);
   p.sources = MKV_UNIT_SOURCES(d->src.block_size, d->dst.block_size);
   const int waves = waves_of(p.dst.bs_shift, p.dst.heads), heads_here = waves / (d->dst.block_size / 16);
+  if (d->n_units > UINT32_MAX / (64 * waves))
+    return mkv_fail(MKV_ERR_UNSUPPORTED, "%s: %lld units", who, (long long)d->n_units);
   const int64_t head_groups = (d->dst.heads + heads_here - 1) / heads_here;
   const dim3 grid(static_cast<unsigned>(d->n_units), static_cast<unsigned>(head_groups),
                   static_cast<unsigned>(d->layers));

@@ -377,6 +377,9 @@ ATTENDS = [  # new, held, heads, group, D, bs, layout, dtype
     ([70], [530], 2, 1, 256, 16, "nhd", "fp16"),
     ([33, 150], [0, 90], 2, 5, 64, 32, "hnd", "bf16"),
     ([1], [3], 1, 40, 128, 16, "hnd", "bf16"),
+    # a chunk beside decoding requests, which get a launch of their own
+    ([1, 1, 260, 3, 1, 0, 2], [700, 3, 40, 75, 15, 8, 90], 2, 8, 128, 16, "hnd", "bf16"),
+    ([300, 1, 1], [600, 1400, 0], 1, 8, 64, 16, "nhd", "fp16"),
 ]
 
 

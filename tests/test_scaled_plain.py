@@ -125,6 +125,8 @@ def attend_desc(**kw):
     (dict(out_head_stride=60), _lib.MKV_ERR_ALIGN), (dict(q_token_stride=-8), _lib.MKV_ERR_ARG),
     (dict(q_token_stride=1 << 60), _lib.MKV_ERR_ARG),
     (dict(max_len=100000, table_width=100000), _lib.MKV_ERR_ARG),  # no workspace
+    (dict(table_width=1 << 27), _lib.MKV_ERR_UNSUPPORTED),
+    (dict(tokens=1 << 23, q_heads=4), _lib.MKV_ERR_UNSUPPORTED),  # more tiles than a grid has
 ])
 def test_attend_refuses(change, code):
     desc = attend_desc(**change)
