@@ -208,7 +208,12 @@ int mkv_scaled_units(const mkv_span_t* spans, int32_t n_spans, const int32_t* sr
  *                  rotary 0.  rotary: a multiple of 32, at most head_size.
  *   src_layers, dst_layers : device [layers][3]: k_base, v_base and scales of each layer.
  *   src, dst     : geometry of every layer (their base and scale pointers are not read).
+ *   on_host      : 1 if units and tables are host memory.  They are read before the call
+ *                  returns and passed on in the arguments of launches that each take
+ *                  MKV_SHIFT_HOST_BYTES of both (MKV_ERR_ARG for a unit of no span).
  */
+#define MKV_SHIFT_HOST_BYTES 3584
+
 typedef struct mkv_scaled_shift_desc {
   mkv_scaled_cache_t src;
   mkv_scaled_cache_t dst;
@@ -220,7 +225,7 @@ typedef struct mkv_scaled_shift_desc {
   int32_t n_spans;
   int32_t layers;
   int32_t rotary;
-  int32_t reserved;
+  int32_t on_host;
 } mkv_scaled_shift_desc_t;
 
 int mkv_shift_scaled(const mkv_scaled_shift_desc_t* desc, void* stream);

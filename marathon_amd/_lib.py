@@ -226,7 +226,7 @@ class ScaledShiftDesc(ctypes.Structure):
         ("n_spans", ctypes.c_int32),
         ("layers", ctypes.c_int32),
         ("rotary", ctypes.c_int32),
-        ("reserved", ctypes.c_int32),
+        ("on_host", ctypes.c_int32),
     ]
 
 
@@ -239,6 +239,9 @@ def unit_words(src_bs: int, dst_bs: int) -> int:
     sources = dst_bs // src_bs + 1 if dst_bs > src_bs else 2
     return (4 + sources + 3) // 4 * 4
 
+
+#: MKV_SHIFT_HOST_BYTES: what a launch of a block-scaled shift takes from host memory.
+SHIFT_HOST_BYTES = 3584
 
 
 class KVShiftError(RuntimeError):

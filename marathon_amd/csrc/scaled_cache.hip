@@ -15,6 +15,9 @@
 
 #include "fp8_e4m3.h"
 
+#include <cstring>
+#include <type_traits>
+
 #pragma clang fp contract(off)
 
 namespace {
@@ -472,13 +475,25 @@ struct MoveParams {
   int32_t sources;  // source blocks in it
 };
 
+// Units, and the spans' tables from word `tables_at` on, in the launch's own arguments.  A
+// small shift is bound by its latency: 512 tokens x 40 layers of 8 heads take 18.8 us a call,
+// where a copy of 2 KB in front of the kernel makes it 28.
+constexpr int kHostWords = MKV_SHIFT_HOST_BYTES / 4;
+struct MoveWords {
+  int32_t tables_at;
+  int32_t word[kHostWords];
+};
+struct NoWords {};
+static_assert(sizeof(MoveParams) + sizeof(MoveWords) <= 4096, "a launch's arguments");
+
 // A workgroup makes one destination block of `heads_here` heads in one layer and ends.  What
 // it has to know is one record made on the host.  22,141 tokens x 40 layers of 8 heads of 128
 // (3.63 GB) take 643 us, 5.6 TB/s, where a bare copy of the same blocks takes 632.  Found on the
 // GPU instead (span, then tables, then rows), the chain of loads in front of the data made it
 // 818; a loop over layers behind one chain, whose loads wait for its stores, 755.
-template <int D>
-__global__ __launch_bounds__(64 * kMaxWaves) void move_kernel(MoveParams p) {
+template <int D, typename Words>
+__global__ __launch_bounds__(64 * kMaxWaves) void move_kernel(MoveParams p, Words w) {
+  constexpr bool kHere = std::is_same_v<Words, MoveWords>;
   using R = Rows<D>;
   constexpr int P = R::kPasses;
   __shared__ uint32_t s_max[kMaxWaves][2];
@@ -489,7 +504,12 @@ __global__ __launch_bounds__(64 * kMaxWaves) void move_kernel(MoveParams p) {
   const bool active = head < p.dst.heads;
   const int piece = lane % R::kChunks, sub = lane / R::kChunks;
   // the record's words, one a lane
-  const int word = p.units[static_cast<int64_t>(blockIdx.x) * p.words + min(lane, p.words - 1)];
+  const int64_t word_at = static_cast<int64_t>(blockIdx.x) * p.words + min(lane, p.words - 1);
+  int word;
+  if constexpr (kHere)
+    word = w.word[word_at];
+  else
+    word = p.units[word_at];
   const int id = __builtin_amdgcn_readlane(word, 0), n = __builtin_amdgcn_readlane(word, 1);
   const int span = __builtin_amdgcn_readlane(word, 2), first = __builtin_amdgcn_readlane(word, 3);
   if (id < 0 || id >= p.dst.num_blocks || span >= p.n_spans) return;
@@ -547,11 +567,21 @@ __global__ __launch_bounds__(64 * kMaxWaves) void move_kernel(MoveParams p) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) cs[i] = 1.0f, sn[i] = 0.0f;
   if (turned) {
-    const float* t = p.tables + static_cast<int64_t>(span) * 2 * p.rotary + at;
+    // (-sin for the first half of a pair, +sin for the second)
+    if constexpr (kHere) {
+      const int t = w.tables_at + span * 2 * p.rotary + at;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      cs[i] = t[i];
-      sn[i] = t[p.rotary + i];  // -sin for the first half of a pair, +sin for the second
+      for (int i = 0; i < 8; ++i) {
+        cs[i] = __builtin_bit_cast(float, w.word[t + i]);
+        sn[i] = __builtin_bit_cast(float, w.word[t + p.rotary + i]);
+      }
+    } else {
+      const float* t = p.tables + static_cast<int64_t>(span) * 2 * p.rotary + at;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        cs[i] = t[i];
+        sn[i] = t[p.rotary + i];
+      }
     }
   }
   if (!whole) {
@@ -815,7 +845,8 @@ extern "C" int mkv_shift_scaled(const mkv_scaled_shift_desc_t* d, void* stream) 
   if (d->units == nullptr || d->src_layers == nullptr || d->dst_layers == nullptr ||
       (d->rotary > 0 && d->tables == nullptr))
     return mkv_fail(MKV_ERR_ARG, "%s: a pointer is NULL", who);
-  if (((reinterpret_cast<uintptr_t>(d->tables) | reinterpret_cast<uintptr_t>(d->units)) & 15) != 0)
+  if (!d->on_host &&
+      ((reinterpret_cast<uintptr_t>(d->tables) | reinterpret_cast<uintptr_t>(d->units)) & 15) != 0)
     return mkv_fail(MKV_ERR_ALIGN, "%s: tables or units are not 16-byte aligned", who);
   p.src_layers = d->src_layers;
   p.dst_layers = d->dst_layers;
@@ -829,14 +860,61 @@ extern "C" int mkv_shift_scaled(const mkv_scaled_shift_desc_t* d, void* stream) 
   if (d->n_units > UINT32_MAX / (64 * waves))
     return mkv_fail(MKV_ERR_UNSUPPORTED, "%s: %lld units", who, (long long)d->n_units);
   const int64_t head_groups = (d->dst.heads + heads_here - 1) / heads_here;
-  const dim3 grid(static_cast<unsigned>(d->n_units), static_cast<unsigned>(head_groups),
-                  static_cast<unsigned>(d->layers));
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (d->dst.head_size == 64)
-    move_kernel<64><<<grid, 64 * waves, 0, s>>>(p);
-  else if (d->dst.head_size == 128)
-    move_kernel<128><<<grid, 64 * waves, 0, s>>>(p);
-  else
-    move_kernel<256><<<grid, 64 * waves, 0, s>>>(p);
+  const auto launch = [&](int64_t units, auto words) {
+    using W = decltype(words);
+    const dim3 grid(static_cast<unsigned>(units), static_cast<unsigned>(head_groups),
+                    static_cast<unsigned>(d->layers));
+    if (d->dst.head_size == 64)
+      move_kernel<64, W><<<grid, 64 * waves, 0, s>>>(p, words);
+    else if (d->dst.head_size == 128)
+      move_kernel<128, W><<<grid, 64 * waves, 0, s>>>(p, words);
+    else
+      move_kernel<256, W><<<grid, 64 * waves, 0, s>>>(p, words);
+  };
+  if (!d->on_host) {
+    launch(d->n_units, NoWords{});
+    return launched(who);
+  }
+  // As many units to a launch as fit with the tables from their lowest span to their highest
+  // (one unit and one table always do: 16 words and 512).
+  static_assert(16 + 2 * 256 <= kHostWords);
+  for (int64_t u = 0; u < d->n_units; ++u) {
+    const int32_t span = d->units[u * p.words + 2];
+    if (span < -1 || span >= d->n_spans)
+      return mkv_fail(MKV_ERR_ARG, "%s: unit %lld is of span %d of %d", who, (long long)u, span,
+                      d->n_spans);
+  }
+  for (int64_t u = 0; u < d->n_units;) {
+    MoveWords w;
+    memset(&w, 0, sizeof w);
+    int32_t lo = 0, hi = -1;
+    int n = 0;
+    for (; u + n < d->n_units; ++n) {
+      const int32_t span = d->units[(u + n) * p.words + 2];
+      int32_t l = lo, h = hi;
+      if (span >= 0 && d->rotary > 0) {
+        l = hi < lo || span < lo ? span : lo;
+        h = hi < lo || span > hi ? span : hi;
+      }
+      const int64_t words = (n + 1) * static_cast<int64_t>(p.words) +
+                            (static_cast<int64_t>(h) - l + 1) * 2 * d->rotary;
+      if (words > kHostWords) break;
+      lo = l;
+      hi = h;
+    }
+    p.n_spans = hi - lo + 1;
+    w.tables_at = n * p.words;
+    for (int i = 0; i < n; ++i) {
+      int32_t* to = w.word + i * p.words;
+      memcpy(to, d->units + (u + i) * p.words, 4 * p.words);
+      to[2] = to[2] < 0 || d->rotary == 0 ? -1 : to[2] - lo;
+    }
+    if (p.n_spans > 0)
+      memcpy(w.word + w.tables_at, d->tables + static_cast<int64_t>(lo) * 2 * d->rotary,
+             static_cast<size_t>(p.n_spans) * 2 * d->rotary * 4);
+    launch(n, w);
+    u += n;
+  }
   return launched(who);
 }

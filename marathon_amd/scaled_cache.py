@@ -374,7 +374,6 @@ class ScaledShifts:
             self._streams = {current_stream(self.device)}
         d.src_layers = self._bases[0].data_ptr()
         d.dst_layers = self._bases[1].data_ptr()
-        self._captured: list = []  # host buffers that captured graphs read
 
     def run(self, rows: list, src_table, dst_table, *,
             error_flags: torch.Tensor | None = None) -> None:
@@ -398,28 +397,29 @@ class ScaledShifts:
             deltas |= int(r[5])
         if most == 0:
             return
-        spans = np.empty(n, dtype=_lib.SPAN_DTYPE)
-        _span_struct(n).pack_into(spans.view(np.uint8), 0, *chain.from_iterable(rows))
-        tables = [_host_table(t) for t in (src_table, dst_table)]
-        # units, then the spans' rotation tables, in one pinned buffer
+        spans = _span_struct(n).pack(*chain.from_iterable(rows))
+        (src, src_at, src_len), (dst, dst_at, dst_len) = map(_host_table, (src_table, dst_table))
+        # Units, then the spans' rotation tables, in one buffer.  What fits into one launch's
+        # arguments goes along in them, more through pinned memory and a copy (377 units: 41 us
+        # against 49 for the launches it would take, 1,388 units: 634 against 786).  A capture
+        # takes all of it in arguments: it may not allocate pinned memory, and its replays
+        # then read nothing on the host.
         turns = n * 8 * self.rotary if deltas else 0
         room = most * self._unit_bytes
-        host = torch.empty(room + turns, dtype=torch.uint8, pin_memory=True)
+        small = room + turns <= _lib.SHIFT_HOST_BYTES or self._capturing()
+        host = torch.empty(room + turns, dtype=torch.uint8, pin_memory=not small)
         at, d, L = host.data_ptr(), self.desc, _lib.lib()
-        out = np.zeros(2, np.int64)  # units, flags
+        made, flag = ctypes.c_int64(), ctypes.c_int32()
         _lib.check(L.mkv_scaled_units(
-            spans.ctypes.data, n, tables[0].ctypes.data, tables[0].size, tables[1].ctypes.data,
-            tables[1].size, ctypes.byref(d.src), ctypes.byref(d.dst), at, most, out.ctypes.data,
-            out.ctypes.data + 8))
+            spans, n, src_at, src_len, dst_at, dst_len, ctypes.byref(d.src), ctypes.byref(d.dst),
+            at, most, ctypes.byref(made), ctypes.byref(flag)))
         if turns:
-            steps = np.ascontiguousarray(spans["delta"])
+            steps = np.ascontiguousarray(np.frombuffer(spans, _lib.SPAN_DTYPE)["delta"])
             _lib.check(L.mkv_rope_tables(steps.ctypes.data, n, self.inv_freq.data_ptr(),
                                          self.rotary, at + room))
-        raised = int(out[1])
         flags = _flags(error_flags, self.device)
-        desc = _lib.ScaledShiftDesc()
-        ctypes.memmove(ctypes.byref(desc), ctypes.byref(d), ctypes.sizeof(desc))
-        desc.n_spans, desc.n_units = n, int(out[0])
+        desc = _lib.ScaledShiftDesc.from_buffer_copy(d)
+        desc.n_spans, desc.n_units = n, made.value
         if not turns:
             desc.rotary = 0
         with _on(self.device, _current(self.device)):
@@ -427,16 +427,23 @@ class ScaledShifts:
             if stream not in self._streams:
                 self._bases.record_stream(torch.cuda.current_stream(self.device))
                 self._streams.add(stream)
-            if raised and flags:
-                error_flags.bitwise_or_(raised)
+            if flag.value and flags:
+                error_flags.bitwise_or_(flag.value)
             if not desc.n_units:
                 return
-            # the caching host allocator keeps ``host`` until this copy has completed
-            blob = host.to(self.device, non_blocking=True)
-            if stream and torch.cuda.is_current_stream_capturing():
-                self._captured.append(host)
-            desc.units, desc.tables = blob.data_ptr(), blob.data_ptr() + room if turns else None
+            blob = host
+            if small:
+                desc.on_host = 1
+            else:
+                # the caching host allocator keeps ``host`` until this copy has completed
+                blob = host.to(self.device, non_blocking=True)
+            at = blob.data_ptr()
+            desc.units, desc.tables = at, at + room if turns else None
             _lib.check(L.mkv_shift_scaled(ctypes.byref(desc), stream))
+
+    def _capturing(self) -> bool:
+        with _on(self.device, _current(self.device)):
+            return torch.cuda.is_current_stream_capturing()
 
 
 def _geometry(c: ScaledCache) -> tuple:
@@ -445,13 +452,17 @@ def _geometry(c: ScaledCache) -> tuple:
             d.head_size)
 
 
-def _host_table(t) -> np.ndarray:
+def _host_table(t) -> tuple:
+    """A block table on the host: what keeps it alive, its address and its length."""
     if isinstance(t, torch.Tensor):
         if t.is_cuda:
             raise ValueError("a shift's block tables are on the host")
+        if t.dtype == torch.int32 and t.is_contiguous():
+            return t, t.data_ptr(), t.numel()
         t = t.detach().numpy()
     t = np.asarray(t).reshape(-1)
     if t.dtype != np.int32:
         if t.dtype.kind not in "iu" or (t.size and (t.min() < -2**31 or t.max() >= 2**31)):
             raise ValueError("a shift's block tables hold int32 block ids")
-    return np.ascontiguousarray(t, dtype=np.int32)
+    t = np.ascontiguousarray(t, dtype=np.int32)
+    return t, t.ctypes.data, t.size

@@ -537,6 +537,8 @@ SHIFTS = [  # spans (src_pos, dst_pos, n, delta), heads, D, rotary, sbs, dbs, la
     ([(17, 0, 40, -17), (70, 64, 64, 0), (150, 128, 3, 9)], 2, 256, 128, 32, 64, "nhd", "nhd"),
     ([(1, 128, 200, 127)], 2, 64, 64, 64, 128, "hnd", "hnd"),
     ([(9, 16, 50, -100000)], 5, 128, 0, 128, 16, "nhd", "hnd"),
+    # more units than a launch's arguments hold
+    ([(7, 0, 1500, 21), (2100, 1504, 501, -9)], 1, 64, 64, 16, 16, "hnd", "nhd"),
 ]
 
 
@@ -728,6 +730,29 @@ def test_a_captured_shift_keeps_its_spans(gpu):
     plain.shift(src.codes, src.scales, dst.codes, dst.scales, [(0, 0, 0, 0, 16, 0, 0, 0)], table,
                 table, 16, 16, inv.numpy())
     dst.check()
+
+
+@pytest.mark.parametrize("spans", [1, 60])  # one launch's arguments, and more
+def test_a_captured_shift_next_to_eager_ones(gpu, spans):
+    rng = np.random.default_rng(52)
+    src, dst = Cache(gpu, rng, 61, 2, 64, 16), Cache(gpu, rng, 130, 2, 64, 16)
+    inv = inv_freq_for(64, 1e4)
+    runner = ScaledShifts([src.dev], [dst.dev], inv)
+    table = np.arange(130, dtype=np.int32)
+    rows = [(3 + i, 32 * i, 0, 0, 17, i - 7, 0, 0) for i in range(spans)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        runner.run(rows, table, table)
+    for i in range(4):
+        other = [(5 * i + j, 32 * j, 0, 0, 32, i + j, 0, 0) for j in range(spans)]
+        runner.run(other, table, table)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for r in (other, rows):
+            plain.shift(src.codes, src.scales, dst.codes, dst.scales, r, table, table, 16, 16,
+                        inv.numpy())
+        dst.check()
 
 
 def test_on_another_stream(gpu):

@@ -201,9 +201,18 @@ def shift_desc(src=None, dst=None, **kw):
     (dict(layers=70000), _lib.MKV_ERR_ARG), (dict(n_units=1 << 31), _lib.MKV_ERR_ARG),
     (dict(units=None), _lib.MKV_ERR_ARG), (dict(tables=None), _lib.MKV_ERR_ARG),
     (dict(tables=(1 << 20) + 4), _lib.MKV_ERR_ALIGN), (dict(units=(1 << 20) + 8), _lib.MKV_ERR_ALIGN),
+    (dict(on_host=1, units=None), _lib.MKV_ERR_ARG),
     (dict(n_units=0), _lib.MKV_OK), (dict(layers=0), _lib.MKV_OK)])
 def test_shift_refuses(change, code):
     assert _lib.lib().mkv_shift_scaled(ctypes.byref(shift_desc(**change)), None) == code
+
+
+@pytest.mark.parametrize("span", [-2, 2, 1 << 30])
+def test_shift_refuses_units_of_no_span(span):
+    units, tables = np.zeros((3, 8), np.int32), np.zeros((2, 2, 128), np.float32)
+    units[2, 2] = span
+    desc = shift_desc(on_host=1, n_units=3, units=units.ctypes.data, tables=tables.ctypes.data)
+    assert _lib.lib().mkv_shift_scaled(ctypes.byref(desc), None) == _lib.MKV_ERR_ARG
 
 
 def units_of(rows, src_table, dst_table, sbs=16, dbs=16, blocks=(50, 60), room=None):
