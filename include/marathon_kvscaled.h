@@ -122,7 +122,8 @@ int mkv_store_scaled(const mkv_scaled_cache_t* cache, const void* k, int64_t k_t
  * Causal grouped-query attention over the cache.
  *   q, out : [tokens, q_heads, head_size] of dtype MKV_BF16 or MKV_F16, contiguous in the
  *            last dimension, aligned to 16 bytes; q_heads a multiple of the cache's heads,
- *            query head h reads KV head h / (q_heads / heads).
+ *            query head h reads KV head h / (q_heads / heads).  out's rows do not overlap
+ *            each other, q or the cache.
  *   out[i] = sum_j p_j V[j],  p = softmax over j <= position(i), j < lens[r], of
  *            softmax_scale * q[i] . K[j]
  * computed with fp32 sums and softmax statistics.  A row that sees no key is zeros; rows
@@ -173,7 +174,7 @@ int64_t mkv_attend_workspace_size(const mkv_attend_desc_t* desc);
  * written at dst_pos + i through dst_table, K re-rotated by delta as marathon_kvshift.h says
  * (fp32, no fused multiply-add); the destination blocks are encoded anew, each under the
  * scale of the rows that it receives.  Rows behind a span's last one stay as they were.
- * Destination blocks must be distinct and must not be source blocks of the call.
+ * Destination blocks are distinct and no source blocks of the call.
  *
  * mkv_scaled_units (a host function, no GPU call; every pointer a HOST one) resolves spans
  * into units, one for each destination block:
@@ -181,7 +182,9 @@ int64_t mkv_attend_workspace_size(const mkv_attend_desc_t* desc);
  *            the block numbers in the tables; groups are not read.  A span whose dst_pos is
  *            not a multiple of the destination's block size, or with a negative position or
  *            length, gets no units (MKV_FLAG_SPAN): a block is written by one span.
- *   src, dst : geometry (block_size and num_blocks; the rest is not read).
+ *   src, dst : geometry (block_size and num_blocks; the rest is not read).  A block that is a
+ *            destination twice is refused (MKV_ERR_ARG); within one cache, which is said by
+ *            one pointer for both, so is a source block that is a destination too.
  *   units  : out, room for max_units of them; at least the sum of ceil(n_tokens / dst
  *            block_size) is never too little (MKV_ERR_ARG otherwise).  A unit is
  *            MKV_UNIT_WORDS(src block_size, dst block_size) words, int32:

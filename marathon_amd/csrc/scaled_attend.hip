@@ -1049,7 +1049,7 @@ int check(const mkv_attend_desc_t& d, AttendParams* p, Plan* plan) {
   if (d.q_heads <= 0 || d.q_heads % d.cache.heads != 0)
     return mkv_fail(MKV_ERR_ARG, "%s: %d query heads for %d KV heads", who, d.q_heads,
                     d.cache.heads);
-  if (d.tokens < 0 || d.tokens * d.q_heads > INT32_MAX || d.tokens > INT32_MAX)
+  if (d.tokens < 0 || d.tokens > INT32_MAX || d.tokens * d.q_heads > INT32_MAX)
     return mkv_fail(MKV_ERR_ARG, "%s: tokens %lld", who, (long long)d.tokens);
   if (d.max_new < 0 || d.max_len < 0)
     return mkv_fail(MKV_ERR_ARG, "%s: max_new %d, max_len %d", who, d.max_new, d.max_len);
@@ -1154,6 +1154,9 @@ extern "C" int mkv_attend_scaled(const mkv_attend_desc_t* d, void* stream) {
   if (((reinterpret_cast<uintptr_t>(d->q) | reinterpret_cast<uintptr_t>(d->out) | p.q_token |
         p.q_head | p.out_token | p.out_head) & 15) != 0)
     return mkv_fail(MKV_ERR_ALIGN, "%s: q or out is not 16-byte aligned", who);
+  if ((d->tokens > 1 && d->out_token_stride < d->cache.head_size) ||
+      (d->q_heads > 1 && d->out_head_stride < d->cache.head_size))
+    return mkv_fail(MKV_ERR_ARG, "%s: out's rows overlap", who);
   const int64_t need = mkv_attend_workspace_size(d);
   if (need > 0 && (d->workspace == nullptr || d->workspace_bytes < need))
     return mkv_fail(MKV_ERR_ARG, "%s: workspace of %lld bytes, %lld needed", who,

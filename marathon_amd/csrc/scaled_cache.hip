@@ -15,6 +15,7 @@
 
 #include "fp8_e4m3.h"
 
+#include <cstdlib>
 #include <cstring>
 #include <type_traits>
 
@@ -818,6 +819,28 @@ extern "C" int mkv_scaled_units(const mkv_span_t* spans, int32_t n_spans, const 
       }
     }
   }
+  // A block written twice, or read by one unit and written by another, would hold whichever
+  // came last: a bit for each destination block says whether one is.
+  auto* taken = static_cast<uint8_t*>(count > 0 ? calloc((dst->num_blocks + 7) / 8, 1) : nullptr);
+  if (count > 0 && taken == nullptr)
+    return mkv_fail(MKV_ERR_ARG, "%s: no memory for %lld blocks", who, (long long)dst->num_blocks);
+  int32_t twice = -1, read = -1;
+  for (int64_t n = 0; n < count; ++n) {
+    const int32_t id = units[words * n];
+    if (taken[id >> 3] >> (id & 7) & 1) twice = id;
+    taken[id >> 3] |= static_cast<uint8_t>(1 << (id & 7));
+  }
+  for (int64_t n = 0; src == dst && n < count; ++n)
+    for (int32_t j = 0; j < sources; ++j) {
+      const int32_t* u = units + words * n;
+      const int32_t id = j < (u[3] + u[1] + sbs - 1) / sbs ? u[4 + j] : -1;
+      if (id >= 0 && id < dst->num_blocks && taken[id >> 3] >> (id & 7) & 1) read = id;
+    }
+  free(taken);
+  if (twice >= 0)
+    return mkv_fail(MKV_ERR_ARG, "%s: block %d is a destination twice", who, twice);
+  if (read >= 0)
+    return mkv_fail(MKV_ERR_ARG, "%s: block %d is a source and a destination", who, read);
   *n_units = count;
   if (flags != nullptr) *flags = raised;
   return MKV_OK;

@@ -286,7 +286,8 @@ def attend_scaled(cache: ScaledCache, q: torch.Tensor, block_tables: torch.Tenso
     Row i of request r stands at position ``lens[r] - new[r] + i`` and sees the positions up
     to its own: store the step's rows first.  ``softmax_scale``: ``D ** -0.5`` unless given.
     A row that sees nothing is zeros; rows of ``out`` behind ``starts[-1]`` are left as they
-    were (in a fresh ``out``, undefined).  Sums and softmax statistics are fp32.
+    were (in a fresh ``out``, undefined).  ``out`` shares no memory with ``q`` or the cache.
+    Sums and softmax statistics are fp32.
 
     ``max_new`` and ``max_len``: the largest number of new tokens and of tokens of a request,
     where the host knows them (a captured step: the largest that will be replayed).  They
@@ -365,6 +366,7 @@ class ScaledShifts:
         d = self.desc = _lib.ScaledShiftDesc()
         d.src, d.dst = a.desc, b.desc
         d.layers, d.rotary = self.layers, self.rotary
+        self._one_cache = a.desc.k_base == b.desc.k_base and _geometry(a) == _geometry(b)
         self._unit_bytes = 4 * _lib.unit_words(a.block_size, b.block_size)
         with _on(self.device, _current(self.device)):
             # (a copy from pageable memory: it is there when the call returns)
@@ -383,22 +385,24 @@ class ScaledShifts:
         src_index and dst_index).  ``dst_pos`` is a multiple of the destination's block size:
         a span writes whole blocks, each anew under the scale of its rows; rows behind a
         span's last one stay.  The destination blocks of one call are distinct, and none is
-        one of its source blocks."""
+        one of its source blocks (in one cache; both are refused)."""
         n, bs = len(rows), self.dst[0].block_size
         if n > _lib.MKV_MAX_SPANS:
             raise ValueError(f"{n} spans: at most {_lib.MKV_MAX_SPANS}")
-        most = deltas = 0
+        src, src_at, src_len = _host_table(src_table)
+        dst, dst_at, dst_len = _host_table(dst_table)
+        most = deltas = tokens = 0
         for r in rows:
             if r[0] < 0 or r[1] < 0 or r[4] < 0:
                 raise ValueError("a span's position or length is negative")
             if r[1] % bs:
                 raise ValueError(f"a destination position is not a multiple of {bs}")
-            most += -(-int(r[4]) // bs)
+            tokens |= int(r[4])
+            most += min(-(-int(r[4]) // bs), dst_len)  # units: blocks beyond the table get none
             deltas |= int(r[5])
-        if most == 0:
+        if tokens == 0:
             return
         spans = _span_struct(n).pack(*chain.from_iterable(rows))
-        (src, src_at, src_len), (dst, dst_at, dst_len) = map(_host_table, (src_table, dst_table))
         # Units, then the spans' rotation tables, in one buffer.  What fits into one launch's
         # arguments goes along in them, more through pinned memory and a copy (377 units: 41 us
         # against 49 for the launches it would take, 1,388 units: 634 against 786).  A capture
@@ -411,8 +415,9 @@ class ScaledShifts:
         at, d, L = host.data_ptr(), self.desc, _lib.lib()
         made, flag = ctypes.c_int64(), ctypes.c_int32()
         _lib.check(L.mkv_scaled_units(
-            spans, n, src_at, src_len, dst_at, dst_len, ctypes.byref(d.src), ctypes.byref(d.dst),
-            at, most, ctypes.byref(made), ctypes.byref(flag)))
+            spans, n, src_at, src_len, dst_at, dst_len,
+            ctypes.byref(d.dst if self._one_cache else d.src), ctypes.byref(d.dst), at, most,
+            ctypes.byref(made), ctypes.byref(flag)))
         if turns:
             steps = np.ascontiguousarray(np.frombuffer(spans, _lib.SPAN_DTYPE)["delta"])
             _lib.check(L.mkv_rope_tables(steps.ctypes.data, n, self.inv_freq.data_ptr(),
@@ -428,7 +433,7 @@ class ScaledShifts:
                 self._bases.record_stream(torch.cuda.current_stream(self.device))
                 self._streams.add(stream)
             if flag.value and flags:
-                error_flags.bitwise_or_(flag.value)
+                error_flags[(0,) * error_flags.dim()].bitwise_or_(flag.value)
             if not desc.n_units:
                 return
             blob = host

@@ -881,4 +881,13 @@ def test_python_refusals(gpu):
             runner.run(rows, tab, [2, 3])
     runner.run([], [0], [1])
     runner.run([(0, 0, 0, 0, 0, 5, 0, 0)], [0], [1])
+    for tab, to in ([[0, 1], [2, 2]], [[0, 1], [3, 1]]):  # a block written twice, or read too
+        with pytest.raises(_lib.KVShiftError):
+            runner.run([(0, 0, 0, 0, 32, 0, 0, 0)], tab, to)
+    flags = i32([0, 0, 0], gpu)  # a span far longer than its tables
+    runner.run([(0, 0, 0, 0, 2**31 - 1, 0, 0, 0)], [0], [-1], error_flags=flags)
+    assert flags.tolist() == [_lib.MKV_FLAG_DST_RANGE, 0, 0]
     cache.check()
+    q = torch.zeros(3, 2, cache.dev.head_size, dtype=torch.bfloat16, device=gpu)
+    with pytest.raises(_lib.KVShiftError, match="overlap"):
+        attend_scaled(cache.dev, q, tables, starts, lens, out=q[:1].clone().expand(3, -1, -1))

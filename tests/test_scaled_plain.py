@@ -273,6 +273,31 @@ def test_units_of_bad_spans_and_ids():
     assert units_of([], [], [])[0] == _lib.MKV_OK
 
 
+def test_units_refuse_a_block_twice():
+    table = np.arange(10)
+    rows = [(0, 0, 0, 0, 40, 0, 0, 0), (50, 64, 0, 0, 16, 0, 0, 0)]
+    assert units_of(rows, table, [9, 8, 7, 5, 6])[0] == _lib.MKV_OK
+    assert units_of(rows, table, [9, 8, 7, 5, 8])[0] == _lib.MKV_ERR_ARG
+    assert units_of([rows[0], rows[0]], table, table)[0] == _lib.MKV_ERR_ARG
+
+
+def test_units_of_one_cache_refuse_a_source_that_is_written():
+    cache, out = cache_desc(num_blocks=12), np.zeros((8, 8), np.int32)
+    spans, got = np.zeros(1, _lib.SPAN_DTYPE), np.zeros(2, np.int64)
+    spans[0] = (9, 0, 0, 0, 31, 5, 0, 0)  # of blocks 0, 1 and 2 of its table
+
+    def rc(dst, src_desc):
+        st, dt = np.asarray([3, 4, 5, 6], np.int32), np.asarray(dst, np.int32)
+        return _lib.lib().mkv_scaled_units(
+            spans.ctypes.data, 1, st.ctypes.data, 4, dt.ctypes.data, 2, ctypes.byref(src_desc),
+            ctypes.byref(cache), out.ctypes.data, 8, got.ctypes.data, got.ctypes.data + 8)
+
+    for dst, code in (([0, 11], _lib.MKV_OK), ([6, 2], _lib.MKV_OK), ([0, 3], _lib.MKV_ERR_ARG),
+                      ([5, 11], _lib.MKV_ERR_ARG), ([4, 0], _lib.MKV_ERR_ARG)):
+        assert rc(dst, cache) == code
+        assert rc(dst, cache_desc(num_blocks=12)) == _lib.MKV_OK
+
+
 def test_there_is_no_cpu_path():
     kv = torch.zeros((4, 2, 16, 256), dtype=torch.uint8).view(torch.float8_e4m3fn)
     scales = torch.zeros((4, 2, 2), dtype=torch.uint8).view(torch.float8_e8m0fnu)
