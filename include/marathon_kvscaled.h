@@ -38,7 +38,8 @@
  *                 of request r is position lens[r] - (starts[r + 1] - starts[r]) + i.
  *   block_tables  int32 [requests, table_width], rows table_stride apart; at most 2^30 tokens
  *                 a request.
- * A request whose starts leave the token arrays, or descend, is skipped (MKV_FLAG_SPAN).
+ * A request whose starts leave the token arrays is skipped (MKV_FLAG_SPAN); where starts
+ * descend, rows stay untouched or go to a neighbouring request, with the flag or without.
  *
  * No counterpart in the reference, whose caches are bf16 and whose slots are made on the
  * host (src/marathon/shift_store.py:56-60).
@@ -169,7 +170,7 @@ int mkv_attend_scaled(const mkv_attend_desc_t* desc, void* stream);
 int64_t mkv_attend_workspace_size(const mkv_attend_desc_t* desc);
 
 /*
- * Spans moved between block-scaled caches, every layer in one launch: mkv_shift_spans for
+ * Spans moved between block-scaled caches, every layer at once: mkv_shift_spans for
  * this cache.  Row i of span s is read at source position src_pos + i through src_table and
  * written at dst_pos + i through dst_table, K re-rotated by delta as marathon_kvshift.h says
  * (fp32, no fused multiply-add); the destination blocks are encoded anew, each under the
