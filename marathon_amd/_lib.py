@@ -274,6 +274,17 @@ def _bind(cdll: ctypes.CDLL) -> ctypes.CDLL:
     f = cdll.mkv_rope_tables
     f.restype = ctypes.c_int
     f.argtypes = [vp, i32, vp, i32, vp]
+    cdll.mkv_last_error.restype = ctypes.c_char_p
+    cdll.mkv_last_error.argtypes = []
+    cdll.mkv_abi_version.restype = ctypes.c_int32
+    cdll.mkv_abi_version.argtypes = []
+    return cdll
+
+
+def _bind_scaled(cdll: ctypes.CDLL) -> ctypes.CDLL:
+    """The block-scaled cache's entry points: the library has them, a build of the shift path
+    alone does not."""
+    i32, i64, vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p
     f = cdll.mkv_step_slots
     f.restype = ctypes.c_int
     f.argtypes = [vp, vp, i32, vp, i64, i32, vp, i64, vp, i32, vp, vp, vp, vp, i64, vp, vp, vp]
@@ -294,10 +305,6 @@ def _bind(cdll: ctypes.CDLL) -> ctypes.CDLL:
     f = cdll.mkv_shift_scaled
     f.restype = ctypes.c_int
     f.argtypes = [ctypes.POINTER(ScaledShiftDesc), vp]
-    cdll.mkv_last_error.restype = ctypes.c_char_p
-    cdll.mkv_last_error.argtypes = []
-    cdll.mkv_abi_version.restype = ctypes.c_int32
-    cdll.mkv_abi_version.argtypes = []
     return cdll
 
 
@@ -320,7 +327,7 @@ def lib() -> ctypes.CDLL:
                 )
             import torch  # noqa: F401  (bind to torch's HIP runtime)
 
-            cdll = _bind(ctypes.CDLL(LIB_PATH, mode=ctypes.RTLD_LOCAL))
+            cdll = _bind_scaled(_bind(ctypes.CDLL(LIB_PATH, mode=ctypes.RTLD_LOCAL)))
             if cdll.mkv_abi_version() != MKV_ABI_VERSION:
                 raise RuntimeError("libmarathon_kvshift ABI version mismatch; rebuild")
             _LIB = cdll
