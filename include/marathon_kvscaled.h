@@ -91,7 +91,8 @@ typedef struct mkv_scaled_cache {
  *   starts, lens  : out, as above.
  *   slots         : out int64 [max_tokens]: block * block_size + row of every new token, -1
  *                   behind the last one.  positions: out int32 [max_tokens], 0 there.
- *   free_at_out   : out int32 [1]: where the free list begins now.  Not free_at itself.
+ *   free_at_out   : out int32 [1]: where the free list begins now.  Not free_at itself; nor
+ *                   does another output share memory with an input.
  * All or nothing: where a length is negative, the new tokens exceed max_tokens, a request
  * exceeds its table or the free list runs out, MKV_FLAG_DST_RANGE is raised, no table entry
  * changes, lens = held, starts and positions are 0, slots are -1 and free_at_out = free_at.

@@ -27,7 +27,7 @@ using namespace mkv_scaled;
 
 // ------------------------------------------------------------------------- step slots
 
-constexpr int kSlotThreads = 256;  // (1,024: 5.1 / 6.6 us against 3.9 / 5.2, 32 and 256 requests)
+constexpr int kSlotThreads = 256;  // (1,024 took 5.1 / 6.6 us where 256 took 3.9 / 5.2)
 
 struct SlotParams {
   const int32_t* held;
@@ -69,13 +69,17 @@ __device__ __forceinline__ int owner(const int32_t* a, int n, int at) {
   return lo;
 }
 
+// 32 requests of a token each take 3.6 us, 256 requests and 50,021 tokens 5.0: the lengths, the
+// scan's exchanges, a table entry, a slot, each waiting for the one before.
 __global__ __launch_bounds__(kSlotThreads) void step_slots_kernel(SlotParams p) {
   __shared__ int32_t s_start[MKV_MAX_REQUESTS + 1];  // new tokens before request r
   __shared__ int32_t s_block[MKV_MAX_REQUESTS + 1];  // fresh blocks before request r
+  __shared__ int32_t s_held[MKV_MAX_REQUESTS];
   __shared__ int64_t s_wave[2][kSlotThreads / 64];
   __shared__ int32_t s_bad;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int n = p.requests;
+  const int64_t at = p.free_at[0];  // (here, beside the lengths' loads)
   if (tid == 0) s_bad = 0;
   __syncthreads();
   // prefix sums over the requests, a stretch of kSlotThreads at a time
@@ -86,6 +90,7 @@ __global__ __launch_bounds__(kSlotThreads) void step_slots_kernel(SlotParams p) 
     if (r < n) {
       held = p.held[r];
       add = p.fresh[r];
+      s_held[r] = static_cast<int32_t>(held);
       if (held < 0 || add < 0 || held + add > INT32_MAX ||
           blocks_of(static_cast<uint32_t>(held + add), p) > static_cast<uint32_t>(p.table_width)) {
         s_bad = 1;
@@ -121,7 +126,6 @@ __global__ __launch_bounds__(kSlotThreads) void step_slots_kernel(SlotParams p) 
     }
     __syncthreads();
   }
-  const int64_t at = p.free_at[0];
   const bool bad = s_bad != 0 || tokens > p.max_tokens || at < 0 ||
                    at + blocks > p.free_len;
   const int64_t gtid = static_cast<int64_t>(blockIdx.x) * kSlotThreads + tid;
@@ -134,13 +138,14 @@ __global__ __launch_bounds__(kSlotThreads) void step_slots_kernel(SlotParams p) 
     }
     for (int r = tid; r < n; r += kSlotThreads) {
       p.starts[r] = bad ? 0 : s_start[r];
-      p.lens[r] = p.held[r] + (bad ? 0 : p.fresh[r]);
+      const int32_t end = r + 1 < n ? s_start[r + 1] : static_cast<int32_t>(tokens);
+      p.lens[r] = s_held[r] + (bad ? 0 : end - s_start[r]);
     }
   }
   if (!bad) {  // table entries of the fresh blocks
     for (int64_t j = gtid; j < blocks; j += step) {
       const int r = owner(s_block, n, static_cast<int>(j));
-      const int64_t col = blocks_of(static_cast<uint32_t>(p.held[r]), p) + (j - s_block[r]);
+      const int64_t col = blocks_of(static_cast<uint32_t>(s_held[r]), p) + (j - s_block[r]);
       p.tables[r * p.table_stride + col] = p.free_blocks[at + j];
     }
   }
@@ -149,7 +154,7 @@ __global__ __launch_bounds__(kSlotThreads) void step_slots_kernel(SlotParams p) 
     int32_t pos = 0;
     if (!bad && t < tokens) {
       const int r = owner(s_start, n, static_cast<int>(t));
-      const int held = p.held[r];
+      const int held = s_held[r];
       pos = held + static_cast<int>(t) - s_start[r];
       const uint32_t b = block_of(static_cast<uint32_t>(pos), p);
       const uint32_t before = blocks_of(static_cast<uint32_t>(held), p);
