@@ -765,12 +765,12 @@ __global__ __launch_bounds__(64 * kManyWaves, (D == 256 ? 1 : 2)) void attend_ma
               bits_as<bf16x8>(a), bits_as<bf16x8>(q[ks]), s[st], 0, 0, 0);
       }
     }
-    if constexpr (F16) {
+    // What the scores of each 16 tokens are multiplied by (fp16: bare codes), as they are
+    // used; no less than fp32's smallest, so that masked ones stay -inf.
+    float by[4];
 #pragma unroll
-      for (int st = 0; st < 2; ++st)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[st][i] *= pow2(ek[2 * st + (i >> 3)]);
-    }
+    for (int g = 0; g < 4; ++g)
+      by[g] = F16 ? fmaxf(p.scale * pow2(ek[g]), 0x1p-126f) : p.scale;
     // register i of tile st: token at + 32 st + 8 (i / 4) + 4 h + i % 4
     // (compared with what is left, the places are constants: none is kept in a register)
     if (masked) {
@@ -784,12 +784,22 @@ __global__ __launch_bounds__(64 * kManyWaves, (D == 256 ? 1 : 2)) void attend_ma
           s[st][i] = sees ? s[st][i] : -kInf;
         }
     }
-    float top = s[0][0];
+    float top = -kInf;
+    if constexpr (F16) {
 #pragma unroll
-    for (int st = 0; st < 2; ++st)
+      for (int g = 0; g < 4; ++g) {
+        float most = s[g >> 1][8 * (g & 1)];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[st][i]);
-    top *= p.scale;
+        for (int j = 1; j < 8; ++j) most = fmaxf(most, s[g >> 1][8 * (g & 1) + j]);
+        top = fmaxf(top, most * by[g]);
+      }
+    } else {
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[st][i]);
+      top *= p.scale;
+    }
     if (__any(top > m + kSlack)) {
       top = fmaxf(top, __shfl_xor(top, 32));
       const float now = fmaxf(m, top);
@@ -808,7 +818,7 @@ __global__ __launch_bounds__(64 * kManyWaves, (D == 256 ? 1 : 2)) void attend_ma
       float y[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        y[j] = fast_exp2(__builtin_fmaf(s[g >> 1][8 * (g & 1) + j], p.scale, -base));
+        y[j] = fast_exp2(__builtin_fmaf(s[g >> 1][8 * (g & 1) + j], by[g], -base));
         l += y[j];
       }
 #pragma unroll
@@ -971,13 +981,28 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p) {
       for (int i = 1; i < kGroups; ++i) o += s_o[i][d];
     } else {
       float top = -kInf;
-      for (int s = 0; s < t.parts; ++s) top = fmaxf(top, p.part_ml[((at + s) * BM + row) * 2]);
-      const float base = top == -kInf ? 0.0f : top;
-      for (int s = 0; s < t.parts; ++s) {
-        const float* ml = p.part_ml + ((at + s) * BM + row) * 2;
-        const float f = fast_exp2(ml[0] - base);
-        sum += ml[1] * f;
-        o += *reinterpret_cast<const f32x4*>(p.part_o + ((at + s) * BM + row) * D + 4 * d) * f;
+      for (int s = 0; s < t.parts; s += 4) {  // four parts' loads at once
+        float m[4], l[4];
+        f32x4 x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int64_t from = (at + min(s + j, t.parts - 1)) * BM + row;
+          m[j] = s + j < t.parts ? p.part_ml[from * 2] : -kInf;
+          l[j] = p.part_ml[from * 2 + 1];
+          x[j] = *reinterpret_cast<const f32x4*>(p.part_o + from * D + 4 * d);
+        }
+        const float now = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), top);
+        const float base = now == -kInf ? 0.0f : now;
+        const float old = fast_exp2(top - base);
+        sum *= old;
+        o *= old;
+        top = now;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float f = fast_exp2(m[j] - base);
+          sum += l[j] * f;
+          o += x[j] * f;
+        }
       }
     }
     o *= sum == 0.0f ? 0.0f : 1.0f / sum;
