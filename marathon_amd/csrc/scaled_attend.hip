@@ -561,7 +561,8 @@ __global__ __launch_bounds__(64 * kFewWaves, (few_waves<D, RT>())) void attend_f
 // The next step's codes are loaded into registers before a step is computed and written to
 // the other of two buffers behind it: one barrier a step.  Two workgroups fit a CU, and one
 // computes while the other waits.  A chunk of 2,048 tokens over 22,141, 40 query heads of 128
-// (0.97 TFLOP), takes 1,110 us: 0.87 PFLOP/s, where a library product of 8,192^3 reaches 1.22.
+// (0.97 TFLOP), takes 1,040 to 1,070 us: 0.92 PFLOP/s, where a library product of 8,192^3
+// reaches 1.22.
 
 constexpr int kManyWaves = 4;
 constexpr int kManyRows = 32 * kManyWaves;
@@ -1056,7 +1057,14 @@ Shape shape_for(const mkv_attend_desc_t& d, int64_t each, int32_t from, int32_t 
   const int64_t longest = d.max_len > 0 && d.max_len < room ? d.max_len : room;
   const int64_t largest = (each + s.rows - 1) / s.rows * d.requests;  // if all were the largest
   const int64_t groups = (s.tiles < largest ? s.tiles : largest) * d.cache.heads;
-  const int64_t want = s.rows == kManyRows ? kWantMany : kWantFew;
+  // 512 workgroups of the many kernel run at once: of one to two times as many tiles, or where
+  // requests differ in length, more and shorter parts leave less of the chip idle at the end.
+  // Measured with 1,024 / 1,536 wanted, heads of 128 but one: 648 tiles over 22,141 tokens 1,166 /
+  // 1,129 us, 540 over 12,000 577 / 541, 632 over 12,000 644 / 621, 520 over 22,000 (heads of
+  // 64) 526 / 503, 520 over 8,000 364 / 372; 1,064 of eight requests 282 / 258; but one
+  // request's 1,032 over 16,000 1,285 / 1,319 and over 2,000 309 / 339.
+  const bool more = groups >= 512 && (groups < 1024 || d.requests > 1);
+  const int64_t want = s.rows != kManyRows ? kWantFew : more ? kWantMany * 3 / 2 : kWantMany;
   int64_t per = longest * (groups > 0 ? groups : 1) / want;
   if (per < longest / kMaxSplits + 64) per = longest / kMaxSplits + 64;
   per = ((per < kMinSplit ? kMinSplit : per) + 63) / 64 * 64;
