@@ -175,7 +175,10 @@ int64_t mkv_attend_workspace_size(const mkv_attend_desc_t* desc);
  * this cache.  Row i of span s is read at source position src_pos + i through src_table and
  * written at dst_pos + i through dst_table, K re-rotated by delta as marathon_kvshift.h says
  * (fp32, no fused multiply-add); the destination blocks are encoded anew, each under the
- * scale of the rows that it receives.  Rows behind a span's last one stay as they were.
+ * scale of the rows that it receives.  Of rows behind a span's last one the codes stay, but
+ * the block's scale is the new rows': their values are undefined until they are written.
+ * A block is written with all of its rows or, where a source block of one is out of range,
+ * left as it was, its scales among it.
  * Destination blocks are distinct and no source blocks of the call.
  *
  * mkv_scaled_units (a host function, no GPU call; every pointer a HOST one) resolves spans
@@ -196,7 +199,8 @@ int64_t mkv_attend_workspace_size(const mkv_attend_desc_t* desc);
  *              4..  source blocks, in order; -1: out of range; then zeros
  *   *n_units : out.
  *   *flags : out (or NULL), MKV_FLAG bits: a block whose id is out of range gets no unit
- *            (DST_RANGE); rows whose source is get no code (SRC_RANGE).
+ *            (DST_RANGE); a unit one of whose source blocks is leaves its block as it was
+ *            (SRC_RANGE).
  */
 #define MKV_UNIT_SOURCES(src_bs, dst_bs) ((dst_bs) > (src_bs) ? (dst_bs) / (src_bs) + 1 : 2)
 #define MKV_UNIT_WORDS(src_bs, dst_bs) ((4 + MKV_UNIT_SOURCES(src_bs, dst_bs) + 3) / 4 * 4)

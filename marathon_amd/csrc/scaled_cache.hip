@@ -518,7 +518,13 @@ __global__ __launch_bounds__(64 * kMaxWaves) void move_kernel(MoveParams p, Word
     word = p.units[word_at];
   const int id = __builtin_amdgcn_readlane(word, 0), n = __builtin_amdgcn_readlane(word, 1);
   const int span = __builtin_amdgcn_readlane(word, 2), first = __builtin_amdgcn_readlane(word, 3);
-  if (id < 0 || id >= p.dst.num_blocks || span >= p.n_spans) return;
+  if (id < 0 || id >= p.dst.num_blocks || span >= p.n_spans || n < 1 || first < 0) return;
+  // A block is written with all of its rows or not at all: under the scale of some of them, what
+  // the block held in place of the others would be other values.  (Every wave of the workgroup
+  // decides alike.)
+  const int64_t used = ((static_cast<int64_t>(first) + n - 1) >> p.src.bs_shift) + 1;
+  if (used > p.sources || __any(lane >= 4 && lane < 4 + used && (word < 0 || word >= p.src.num_blocks)))
+    return;
 
   // Where each pass's row comes from: a wave's 16 rows lie in two source blocks at most.
   const int start = first + part * 16, block0 = start >> p.src.bs_shift;
@@ -528,13 +534,12 @@ __global__ __launch_bounds__(64 * kMaxWaves) void move_kernel(MoveParams p, Word
   const int src0 = source(block0), src1 = source(block0 + 1);
   int64_t from_row[P], from_scale[P];
   bool there[P];
-  bool whole = active;  // every row of the wave has a source: nothing to blank out
+  bool whole = active;  // every row of the wave is the span's: nothing to blank out
 #pragma unroll
   for (int u = 0; u < P; ++u) {
     const int row = u * R::kPerPass + sub;
     const int64_t from = (start + row) >> p.src.bs_shift == block0 ? src0 : src1;
-    there[u] = active && part * 16 + row < n && part * 16 + row < dbs && from >= 0 &&
-               from < p.src.num_blocks;
+    there[u] = active && part * 16 + row < n;
     whole = whole && __all(there[u]);
     from_row[u] = from_scale[u] = 0;
     if (there[u]) {
@@ -543,7 +548,6 @@ __global__ __launch_bounds__(64 * kMaxWaves) void move_kernel(MoveParams p, Word
       from_scale[u] = (from * p.src.heads + head) * 2;
     }
   }
-  if (p.src.num_blocks == 0) return;  // nothing to read
 
   // Rotation mixes dimension d with d + rotary / 2: chunk c of 16 with chunk c + rotary / 32.
   // The two chunks' lanes exchange halves, so that each holds 8 whole pairs: the first lane
@@ -555,7 +559,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void move_kernel(MoveParams p, Word
   const int partner = !turned ? lane : first_half ? lane + half : lane - half;
   const int at = first_half ? 16 * piece : 16 * (piece - half) + 8;
 
-  // rows without a source read the cache's first
+  // the other rows read the cache's first
   const int64_t layer = blockIdx.z;
   const uint64_t* sl = p.src_layers + 3 * layer;
   const char* sk = reinterpret_cast<const char*>(sl[0]);

@@ -383,9 +383,11 @@ class ScaledShifts:
         src_index, dst_index, n_tokens, delta, 0, 0), positions through the block tables
         ``src_table`` and ``dst_table`` (int32, on the host; a span's tables begin at its
         src_index and dst_index).  ``dst_pos`` is a multiple of the destination's block size:
-        a span writes whole blocks, each anew under the scale of its rows; rows behind a
-        span's last one stay.  The destination blocks of one call are distinct, and none is
-        one of its source blocks (in one cache; both are refused)."""
+        a span writes whole blocks, each anew under the scale of its rows; behind a span's
+        last row the codes stay, but not the values, whose scale was another.  A block one of
+        whose rows has no source (a table too short, an id out of range) is left as it was,
+        with ``MKV_FLAG_SRC_RANGE`` in ``error_flags``.  The destination blocks of one call are
+        distinct, and none is one of its source blocks (in one cache; both are refused)."""
         n, bs = len(rows), self.dst[0].block_size
         if n > _lib.MKV_MAX_SPANS:
             raise ValueError(f"{n} spans: at most {_lib.MKV_MAX_SPANS}")
