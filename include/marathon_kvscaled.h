@@ -38,8 +38,9 @@
  *                 of request r is position lens[r] - (starts[r + 1] - starts[r]) + i.
  *   block_tables  int32 [requests, table_width], rows table_stride apart; at most 2^30 tokens
  *                 a request.
- * A request whose starts leave the token arrays is skipped (MKV_FLAG_SPAN); where starts
- * descend, rows stay untouched or go to a neighbouring request, with the flag or without.
+ * A request whose starts leave the token arrays is skipped; where starts descend, rows stay
+ * untouched or go to a neighbouring request.  Both raise MKV_FLAG_SPAN, as does, in a store, a
+ * request with more new tokens than tokens, which is skipped.
  *
  * No counterpart in the reference, whose caches are bf16 and whose slots are made on the
  * host (src/marathon/shift_store.py:56-60).

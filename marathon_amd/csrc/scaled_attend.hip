@@ -88,10 +88,7 @@ __device__ __forceinline__ bool find_tile(const AttendParams& p, int64_t tile, T
   t.s0 = starts[r];
   const int64_t s1 = starts[r + 1];
   const int64_t first_tile = single ? tile : begin(r);
-  if (t.s0 < 0 || s1 < t.s0 || s1 > p.tokens) {
-    if (threadIdx.x == 0 && tile == first_tile) raise(p.s.flags, MKV_FLAG_SPAN);
-    return false;
-  }
+  if (t.s0 < 0 || s1 < t.s0 || s1 > p.tokens) return false;  // flagged by the first workgroup
   t.row0 = (tile - first_tile) * BM;
   const int64_t all = (s1 - t.s0) * group;
   if (all < p.rows_from || all > p.rows_to) return false;  // another launch's
@@ -195,6 +192,10 @@ __global__ __launch_bounds__(64 * kFewWaves, (few_waves<D, RT>())) void attend_f
   // Workgroups go to the eight XCDs in turn: the tiles are turned by the part, so that a long
   // request's parts do not all fall to one (32 ragged requests: 119 -> 112 us).
   const unsigned tile = (blockIdx.x + blockIdx.z) % gridDim.x;
+  if (static_cast<int>(blockIdx.z) == p.splits) {  // (a part of its own: no register is held for it)
+    if (blockIdx.x + blockIdx.y == 0) check_starts(p.s, p.tokens, false);
+    return;
+  }
   if (!find_tile<BM>(p, tile, t)) return;
   const int part = blockIdx.z;
   if (part >= t.parts) return;
@@ -586,6 +587,7 @@ __global__ __launch_bounds__(64 * kManyWaves, (D == 256 ? 1 : 2)) void attend_ma
   Tile t;
   // the last tiles first: of one request they see the most
   const unsigned tile = gridDim.y - 1 - blockIdx.y;
+  if (blockIdx.x + blockIdx.y + blockIdx.z == 0) check_starts(p.s, p.tokens, false);
   if (!find_tile<kManyRows>(p, tile, t)) return;
   const int part = blockIdx.z;
   if (part >= t.parts) return;
@@ -1134,7 +1136,8 @@ int check(const mkv_attend_desc_t& d, AttendParams* p, Plan* plan) {
 
 template <bool F16, int D, int RT>
 void launch_few(const AttendParams& p, const Shape& s, int heads, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(s.tiles), heads, s.splits);
+  // one part more, which looks through the starts
+  const dim3 grid(static_cast<unsigned>(s.tiles), heads, s.splits + (p.s.flags != nullptr ? 1 : 0));
   attend_few_kernel<F16, D, RT><<<grid, 64 * kFewWaves, 0, stream>>>(p);
   if (s.splits > 1) {
     const unsigned rows = static_cast<unsigned>(s.each < 16 * RT ? (s.each > 0 ? s.each : 1) : 16 * RT);

@@ -74,6 +74,19 @@ __device__ __forceinline__ int last_at_most(int n, int64_t at, F value) {
   return hit == 0 ? -1 : base + 63 - __builtin_clzll(hit);
 }
 
+// Flags requests whose starts leave the token arrays or descend, whether or not a workgroup
+// would come across them (with `rows_held`, also those with more new tokens than tokens).  One
+// workgroup of a launch calls it, in front of its own work: what it loads is looked up next.
+__device__ __forceinline__ void check_starts(const DevStep& s, int64_t tokens, bool rows_held) {
+  if (s.flags == nullptr) return;
+  bool bad = false;
+  for (int r = threadIdx.x; r < s.requests; r += blockDim.x) {
+    const int64_t s0 = s.starts[r], s1 = s.starts[r + 1];
+    bad = bad || s0 < 0 || s1 < s0 || s1 > tokens || (rows_held && s.lens[r] < s1 - s0);
+  }
+  if (bad) raise(s.flags, MKV_FLAG_SPAN);
+}
+
 // Host: an entry point's cache, checked and translated.
 inline int check_cache(const char* who, const mkv_scaled_cache_t& c, bool bases, DevCache* out) {
   if (c.head_size != 64 && c.head_size != 128 && c.head_size != 256)

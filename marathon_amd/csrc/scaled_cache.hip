@@ -372,6 +372,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void store_kernel(StoreParams p) {
   const int head = blockIdx.y * heads_here + wave / parts, part = wave % parts;
   const bool active = head < p.c.heads;
   const int chunk = lane % R::kChunks, sub = lane / R::kChunks;
+  if (blockIdx.x == 0 && blockIdx.y == 0) check_starts(p.s, p.tokens, true);
   int64_t t = static_cast<int64_t>(blockIdx.x) * p.group;
   const int64_t end = min(t + p.group, p.tokens);
   while (t < end) {  // the same steps in every wave of the workgroup
@@ -386,8 +387,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void store_kernel(StoreParams p) {
     if (t < s0 || t >= s1) break;  // behind the last request, or starts that descend
     const int64_t first_pos = p.s.lens[r] - (s1 - s0);
     const int64_t pos = first_pos + (t - s0);
-    if (s0 < 0 || s1 > p.tokens || first_pos < 0) {
-      if (t == s0 && lane == 0 && wave == 0) raise(p.s.flags, MKV_FLAG_SPAN);
+    if (s0 < 0 || s1 > p.tokens || first_pos < 0) {  // flagged by the first workgroup
       t = s1;
       continue;
     }
