@@ -250,6 +250,11 @@ at::Tensor part_of(const at::Tensor& base, at::ScalarType type, int64_t byte, in
   return at::Tensor(std::move(impl));
 }
 
+// Whether a call on `t` would lose a gradient, backward or forward (the general path refuses).
+bool needs_grad(const at::Tensor& t) {
+  return (t.requires_grad() && c10::GradMode::is_enabled()) || t._fw_grad(0).defined();
+}
+
 // slots(held, new, block_tables, free_blocks, free_at, block_size, max_tokens, error_flags)
 PyObject* slots(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != 8 || g_slots == nullptr) {
@@ -330,7 +335,7 @@ PyObject* store(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (k->dim() != 3 || k->device() != dev || v->device() != dev || k->sizes() != v->sizes() ||
         k->scalar_type() != v->scalar_type() || (code != MKV_BF16 && code != MKV_F16 && code != MKV_F32) ||
         k->size(1) != cache->heads || k->size(2) != cache->head_size || k->stride(2) != 1 ||
-        v->stride(2) != 1 || !table_of(args[4], &dev, tab) || flags_of(args[7], dev, flags) != kUsual ||
+        v->stride(2) != 1 || needs_grad(*k) || needs_grad(*v) || !table_of(args[4], &dev, tab) || flags_of(args[7], dev, flags) != kUsual ||
         c10::hip::current_device() != dev.index())
       Py_RETURN_NONE;
     const int32_t* starts = vector_of(args[5], dev, tab.n + 1);
@@ -376,7 +381,7 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (q->dim() != 3 || q->device() != dev || (code != MKV_BF16 && code != MKV_F16) ||
         q->size(2) != cache->head_size || q->size(1) == 0 || q->size(1) % cache->heads != 0 ||
         q->size(1) > INT32_MAX || q->stride(2) != 1 ||
-        (q->requires_grad() && c10::GradMode::is_enabled()) || !table_of(args[3], &dev, tab) ||
+        needs_grad(*q) || !table_of(args[3], &dev, tab) ||
         flags_of(args[10], dev, flags) != kUsual || c10::hip::current_device() != dev.index())
       Py_RETURN_NONE;
     const int32_t* starts = vector_of(args[4], dev, tab.n + 1);
@@ -398,7 +403,7 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     } else {
       const at::Tensor* o = plain(args[9]);
       if (o == nullptr || o->device() != dev || o->scalar_type() != q->scalar_type() ||
-          o->sizes() != q->sizes() || o->stride(2) != 1 ||
+          o->sizes() != q->sizes() || o->stride(2) != 1 || needs_grad(*o) ||
           (q->numel() > 0 && o->data_ptr() == q->data_ptr()))
         Py_RETURN_NONE;
       out = *o;

@@ -26,7 +26,7 @@ functions' checks on the tensors themselves; it answers None, with nothing launc
 other call, which the code here takes (and refuses, where it must).
 
 There is no CPU path and no gradient: tensors that are not on a HIP device raise, and so do
-queries that require one.
+rows, queries and outputs that require a gradient or carry a tangent.
 """
 
 from __future__ import annotations
@@ -38,6 +38,7 @@ from itertools import chain
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .shift_kernels import current_stream, dtype_code
@@ -140,6 +141,16 @@ class ScaledCache:
         d.num_blocks, d.block_stride, d.head_stride, d.token_stride = kv.shape[0], block, head, token
         d.block_size, d.heads, d.head_size = self.block_size, self.heads, self.head_size
         self.handle = (ctypes.addressof(d), kv.get_device())  # for the binding; `desc` is kept
+
+
+def _no_gradient(who: str, **tensors: torch.Tensor | None) -> None:
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{who} has no backward pass; detach {name} or use torch.no_grad()")
+        if forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{who} has no derivative for the tangent of {name}")
 
 
 def _flags(error_flags: torch.Tensor | None, device) -> int | None:
@@ -259,6 +270,7 @@ def store_scaled(cache: ScaledCache, k: torch.Tensor, v: torch.Tensor,
         raise TypeError(f"k {k.dtype} and v {v.dtype}: one of {_ROW_DTYPES}")
     if k.device != device or v.device != device:
         raise ValueError(f"k on {k.device}, v on {v.device}, the cache on {device}")
+    _no_gradient("store_scaled", k=k, v=v)
     if k.stride(2) != 1 or v.stride(2) != 1:
         raise ValueError("rows must be contiguous in the last dimension")
     at, stride, n, width = _table(block_tables, device)
@@ -305,8 +317,7 @@ def attend_scaled(cache: ScaledCache, q: torch.Tensor, block_tables: torch.Tenso
         raise TypeError(f"q {q.dtype}: one of {_QUERY_DTYPES}")
     if q.device != device:
         raise ValueError(f"q on {q.device}, the cache on {device}")
-    if q.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("attend_scaled has no backward pass; detach q or use torch.no_grad()")
+    _no_gradient("attend_scaled", q=q, out=out)
     if q.stride(2) != 1:
         raise ValueError("q's rows must be contiguous in the last dimension")
     if out is None:
