@@ -379,8 +379,8 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     int32_t* flags;
     const int code = dtype_code(q->scalar_type());
     if (q->dim() != 3 || q->device() != dev || (code != MKV_BF16 && code != MKV_F16) ||
-        q->size(2) != cache->head_size || q->size(1) == 0 || q->size(1) % cache->heads != 0 ||
-        q->size(1) > INT32_MAX || q->stride(2) != 1 ||
+        cache->heads <= 0 || q->size(2) != cache->head_size || q->size(1) == 0 ||
+        q->size(1) % cache->heads != 0 || q->size(1) > INT32_MAX || q->stride(2) != 1 ||
         needs_grad(*q) || !table_of(args[3], &dev, tab) ||
         flags_of(args[10], dev, flags) != kUsual || c10::hip::current_device() != dev.index())
       Py_RETURN_NONE;

@@ -116,6 +116,8 @@ class ScaledCache:
         if kv.stride(3) != 1:
             raise ValueError("rows must be contiguous in the last dimension")
         self.heads = kv.shape[1 if self.layout == "hnd" else 2]
+        if self.heads == 0:
+            raise ValueError(f"a cache of no heads: {tuple(kv.shape)}")
         self.device = kv.device
         if (scales.dtype != torch.float8_e8m0fnu or scales.device != kv.device
                 or tuple(scales.shape) != (kv.shape[0], self.heads, 2)
