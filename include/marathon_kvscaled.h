@@ -65,6 +65,7 @@ extern "C" {
  *   k_base, v_base : element 0 of K and V; fused rows have v_base = k_base + head_size.
  *   scales         : device [num_blocks, heads, 2] e8m0 bytes, contiguous: K's, then V's.
  *   block_stride, head_stride, token_stride : bytes (= elements), multiples of 16.
+ *                    No row of K or V lies in another.
  *   block_size     : 16, 32, 64 or 128.   head_size : 64, 128 or 256.
  */
 typedef struct mkv_scaled_cache {

@@ -41,6 +41,7 @@ import torch
 from torch.autograd import forward_ad
 
 from . import _lib
+from .row_memory import Rows, share
 from .shift_kernels import current_stream, dtype_code
 from .spans import _on, _span_struct
 
@@ -80,7 +81,8 @@ class ScaledCache:
     """One layer's cache: ``kv`` (``float8_e4m3fn``, fused rows ``[..., 2D]`` of K then V) and
     ``scales`` (``float8_e8m0fnu`` ``[blocks, heads, 2]``, contiguous), of ``layout`` ``"hnd"``
     or ``"nhd"``.  With ``v_cache``, ``kv`` holds K and ``v_cache`` V, rows ``[..., D]`` of the
-    same shape and strides.  The tensors are checked once, here, and kept."""
+    same shape and strides.  No row lies in another.  The tensors are checked once, here, and
+    kept."""
 
     kv: torch.Tensor
     scales: torch.Tensor
@@ -128,10 +130,17 @@ class ScaledCache:
         strides = [s if n > 1 else 0 for s, n in zip(kv.stride(), kv.shape)]
         block, head, token = (strides[:3] if self.layout == "hnd" else
                               (strides[0], strides[2], strides[1]))
-        # the smallest steps between rows that do not overlap; a stride of 0 would have
-        # several tokens share one
-        if any(s == 0 and n > 1 for s, n in zip(kv.stride(), kv.shape)):
-            raise ValueError("an expanded cache (stride 0) cannot be written")
+        steps = ((block, kv.shape[0]), (head, self.heads), (token, self.block_size))
+        self.rows = [Rows(kv.data_ptr(), width, steps)]
+        if v is not None:
+            self.rows.append(Rows(v.data_ptr(), width, steps))
+        self.scale_rows = Rows(scales.data_ptr(), 2 * self.heads, ((2 * self.heads, kv.shape[0]),))
+        # (an expanded cache, of stride 0, is one whose rows lie in one another)
+        if not self.rows[0].apart():
+            raise ValueError(f"a cache of shape {tuple(kv.shape)} and strides {kv.stride()} has rows "
+                             "that overlap")
+        if v is not None and share(*self.rows):
+            raise ValueError("kv and v_cache share memory")
         if any(s % 16 for s in strides[:3]) or kv.data_ptr() % 16 or (
                 v is not None and v.data_ptr() % 16) or scales.data_ptr() % 2:
             raise ValueError("the cache's base and strides must be multiples of 16 bytes")
