@@ -365,6 +365,10 @@ class ScaledShifts:
     between the two).  ``inv_freq``: fp32 ``[rotary / 2]``, ``rotary`` a multiple of 32; None
     moves keys without turning them.
 
+    Layers may share memory, of one list or of both, where they are one cache or views of whole
+    blocks of one: :meth:`run` then refuses to read a block that it writes, in any layer.  A layer
+    that stands in both lists twice is moved once.  No two of ``dst`` share memory otherwise.
+
     One runner serves every step over the same caches (:meth:`run`).  A graph that captured a
     step reads the runner's buffers: the runner outlives it."""
 
@@ -379,7 +383,15 @@ class ScaledShifts:
         a, b = src[0], dst[0]
         if (a.heads, a.head_size) != (b.heads, b.head_size) or a.device != b.device:
             raise ValueError("src and dst differ in heads, head_size or device")
-        self.src, self.dst, self.device, self.layers = list(src), list(dst), b.device, len(dst)
+        # a pair of caches that is there before writes the same bytes to the same place
+        pairs = list({(bytes(s.desc), bytes(d.desc)): (s, d) for s, d in zip(src, dst)}.values())
+        src, dst = [s for s, _ in pairs], [d for _, d in pairs]
+        self.src, self.dst, self.device, self.layers = src, dst, b.device, len(dst)
+        for i, c in enumerate(dst):
+            if any(_offset(c, other) is not None for other in dst[:i]):
+                raise ValueError("two layers of dst share memory")
+        # where a source block n is the destination's block n + offset of some layer
+        offsets = {_offset(s, d) for s in src for d in dst} - {None}
         self.rotary = 0 if inv_freq is None else 2 * int(inv_freq.numel())
         if self.rotary % 32 or self.rotary > b.head_size:
             raise ValueError(f"rotary {self.rotary}: a multiple of 32, at most {b.head_size}")
@@ -388,7 +400,8 @@ class ScaledShifts:
         d = self.desc = _lib.ScaledShiftDesc()
         d.src, d.dst = a.desc, b.desc
         d.layers, d.rotary = self.layers, self.rotary
-        self._one_cache = a.desc.k_base == b.desc.k_base and _geometry(a) == _geometry(b)
+        self._one_cache = 0 in offsets and _geometry(a) == _geometry(b)
+        self._offsets = sorted(offsets - {0} if self._one_cache else offsets)
         self._unit_bytes = 4 * _lib.unit_words(a.block_size, b.block_size)
         with _on(self.device, _current(self.device)):
             # (a copy from pageable memory: it is there when the call returns)
@@ -442,6 +455,8 @@ class ScaledShifts:
             spans, n, src_at, src_len, dst_at, dst_len,
             ctypes.byref(d.dst if self._one_cache else d.src), ctypes.byref(d.dst), at, most,
             ctypes.byref(made), ctypes.byref(flag)))
+        if self._offsets:
+            self._refuse_shared(host.numpy()[:made.value * self._unit_bytes].view(np.int32))
         if turns:
             steps = np.ascontiguousarray(np.frombuffer(spans, _lib.SPAN_DTYPE)["delta"])
             _lib.check(L.mkv_rope_tables(steps.ctypes.data, n, self.inv_freq.data_ptr(),
@@ -470,9 +485,38 @@ class ScaledShifts:
             desc.units, desc.tables = at, at + room if turns else None
             _lib.check(L.mkv_shift_scaled(ctypes.byref(desc), stream))
 
+    def _refuse_shared(self, units: np.ndarray) -> None:
+        """Raise where a unit's source block is another's destination, in views of one cache."""
+        u = units.reshape(-1, self._unit_bytes // 4)
+        bs = self.src[0].block_size
+        used = (u[:, 3] + u[:, 1] + bs - 1) // bs
+        ids = u[:, 4:]
+        ids = ids[(np.arange(ids.shape[1]) < used[:, None]) & (ids >= 0)]
+        for offset in self._offsets:
+            both = np.intersect1d(ids.astype(np.int64) + offset, u[:, 0])
+            if both.size:
+                raise _lib.KVShiftError(
+                    _lib.MKV_ERR_ARG, f"block {both[0]} is a destination and, {offset} blocks "
+                    "behind, a source")
+
     def _capturing(self) -> bool:
         with _on(self.device, _current(self.device)):
             return torch.cuda.is_current_stream_capturing()
+
+
+def _offset(a: ScaledCache, b: ScaledCache) -> int | None:
+    """The n by which block i of ``a`` is block i + n of ``b``; None where they share nothing."""
+    if not (share(a.scale_rows, b.scale_rows)
+            or any(share(x, y) for x in a.rows for y in b.rows)):
+        return None
+    x, y = a.desc, b.desc
+    step = max(x.block_stride, y.block_stride)  # (0 in a cache of one block)
+    n, rest = divmod((x.k_base or 0) - (y.k_base or 0), step) if step else (0, x.k_base != y.k_base)
+    if (rest or x.v_base - y.v_base != n * step or x.scales - y.scales != 2 * a.heads * n
+            or _geometry(a)[2:] != _geometry(b)[2:] or len(a.rows) != len(b.rows)
+            or (x.block_stride != y.block_stride and min(x.num_blocks, y.num_blocks) > 1)):
+        raise ValueError("two caches share memory, but not as views of one cache's blocks")
+    return n
 
 
 def _geometry(c: ScaledCache) -> tuple:
