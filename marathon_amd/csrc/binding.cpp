@@ -255,6 +255,30 @@ bool needs_grad(const at::Tensor& t) {
   return (t.requires_grad() && c10::GradMode::is_enabled()) || t._fw_grad(0).defined();
 }
 
+// The addresses of a [tokens, heads, D] tensor's rows, from its first byte to behind its last.
+struct Range {
+  uintptr_t from, to;
+  bool meets(uintptr_t a, uintptr_t b) const { return from < b && a < to; }
+};
+
+Range range_of(const at::Tensor& t) {
+  const uintptr_t from = reinterpret_cast<uintptr_t>(t.data_ptr());
+  if (t.numel() == 0) return {from, from};
+  const int64_t last = (t.size(0) - 1) * t.stride(0) + (t.size(1) - 1) * t.stride(1) + t.size(2);
+  return {from, from + static_cast<uintptr_t>(last) * t.element_size()};
+}
+
+// Whether rows in `r` may lie in the cache.
+bool meets_cache(const Range& r, const mkv_scaled_cache_t& c) {
+  if (c.num_blocks <= 0) return false;
+  const uintptr_t size = (c.num_blocks - 1) * c.block_stride + (c.heads - 1) * c.head_stride +
+                         (c.block_size - 1) * c.token_stride + c.head_size;
+  for (const void* p : {static_cast<const void*>(c.k_base), static_cast<const void*>(c.v_base)})
+    if (r.meets(reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + size)) return true;
+  const uintptr_t s = reinterpret_cast<uintptr_t>(c.scales);
+  return r.meets(s, s + 2 * c.num_blocks * c.heads);
+}
+
 // slots(held, new, block_tables, free_blocks, free_at, block_size, max_tokens, error_flags)
 PyObject* slots(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != 8 || g_slots == nullptr) {
@@ -403,9 +427,11 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     } else {
       const at::Tensor* o = plain(args[9]);
       if (o == nullptr || o->device() != dev || o->scalar_type() != q->scalar_type() ||
-          o->sizes() != q->sizes() || o->stride(2) != 1 || needs_grad(*o) ||
-          (q->numel() > 0 && o->data_ptr() == q->data_ptr()))
+          o->sizes() != q->sizes() || o->stride(2) != 1 || needs_grad(*o))
         Py_RETURN_NONE;
+      // the general path tells rows that interleave from rows that share memory
+      const Range rows = range_of(*q), written = range_of(*o);
+      if (written.meets(rows.from, rows.to) || meets_cache(written, *cache)) Py_RETURN_NONE;
       out = *o;
     }
     const bool many = q->size(0) > 1, heads = q->size(1) > 1;

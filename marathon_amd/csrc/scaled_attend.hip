@@ -1193,9 +1193,15 @@ extern "C" int mkv_attend_scaled(const mkv_attend_desc_t* d, void* stream) {
   if (((reinterpret_cast<uintptr_t>(d->q) | reinterpret_cast<uintptr_t>(d->out) | p.q_token |
         p.q_head | p.out_token | p.out_head) & 15) != 0)
     return mkv_fail(MKV_ERR_ALIGN, "%s: q or out is not 16-byte aligned", who);
-  if ((d->tokens > 1 && d->out_token_stride < d->cache.head_size) ||
-      (d->q_heads > 1 && d->out_head_stride < d->cache.head_size))
-    return mkv_fail(MKV_ERR_ARG, "%s: out's rows overlap", who);
+  // out's rows: the smaller stride passes a row, the larger one all that the smaller reaches
+  const bool heads_first = d->out_head_stride <= d->out_token_stride;
+  int64_t reach = d->cache.head_size;
+  for (const bool heads : {heads_first, !heads_first}) {
+    const int64_t n = heads ? d->q_heads : d->tokens;
+    const int64_t step = heads ? d->out_head_stride : d->out_token_stride;
+    if (n > 1 && step < reach) return mkv_fail(MKV_ERR_ARG, "%s: out's rows overlap", who);
+    reach += step * (n - 1);
+  }
   const int64_t need = mkv_attend_workspace_size(d);
   if (need > 0 && (d->workspace == nullptr || d->workspace_bytes < need))
     return mkv_fail(MKV_ERR_ARG, "%s: workspace of %lld bytes, %lld needed", who,

@@ -298,6 +298,12 @@ def _steps(t: torch.Tensor) -> tuple[int, int]:
     return (t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0)
 
 
+def _rows_of(t: torch.Tensor) -> Rows:
+    size = t.element_size()
+    steps = ((size * s, n) for s, n in zip(_steps(t), t.shape))
+    return Rows(t.data_ptr(), size * t.shape[2], tuple(steps))
+
+
 def attend_scaled(cache: ScaledCache, q: torch.Tensor, block_tables: torch.Tensor,
                   starts: torch.Tensor, lens: torch.Tensor, *, softmax_scale: float | None = None,
                   max_new: int | None = None, max_len: int | None = None,
@@ -309,7 +315,8 @@ def attend_scaled(cache: ScaledCache, q: torch.Tensor, block_tables: torch.Tenso
     Row i of request r stands at position ``lens[r] - new[r] + i`` and sees the positions up
     to its own: store the step's rows first.  ``softmax_scale``: ``D ** -0.5`` unless given.
     A row that sees nothing is zeros; rows of ``out`` behind ``starts[-1]`` are left as they
-    were (in a fresh ``out``, undefined).  ``out`` shares no memory with ``q`` or the cache.
+    were (in a fresh ``out``, undefined).  ``out``'s rows share no memory with each other, ``q`` or
+    the cache (ranges that interleave in strides that differ are taken to); it is refused.
     Sums and softmax statistics are fp32.
 
     ``max_new`` and ``max_len``: the largest number of new tokens and of tokens of a request,
@@ -335,8 +342,12 @@ def attend_scaled(cache: ScaledCache, q: torch.Tensor, block_tables: torch.Tenso
         out = torch.empty(q.shape, dtype=q.dtype, device=device)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != device or out.stride(2) != 1:
         raise ValueError(f"out {out.dtype} {tuple(out.shape)} on {out.device} does not fit q")
-    elif q.numel() and out.data_ptr() == q.data_ptr():
-        raise ValueError("out is q")
+    else:
+        written = _rows_of(out)
+        if share(written, _rows_of(q)):
+            raise ValueError("out shares memory with q")
+        if any(share(written, r) for r in (*cache.rows, cache.scale_rows)):
+            raise ValueError("out shares memory with the cache")
     at, stride, n, width = _table(block_tables, device)
     desc = _lib.AttendDesc()
     ctypes.memmove(ctypes.byref(desc), ctypes.byref(cache.desc), ctypes.sizeof(cache.desc))

@@ -7,10 +7,10 @@ import numpy as np
 import pytest
 import torch
 
-from marathon_amd import ScaledCache, ScaledShifts, _lib
+from marathon_amd import ScaledCache, ScaledShifts, _lib, attend_scaled
 from marathon_amd.shift_kernels import inv_freq_for
 from tests import scaled_plain as plain
-from tests.test_gpu_scaled import Cache
+from tests.test_gpu_scaled import Cache, i32
 
 pytestmark = pytest.mark.gpu
 
@@ -153,3 +153,62 @@ def test_layers_that_interleave_share_nothing(gpu):
         e = torch.exp2(scales[i + 2].double() - 127)
         y = y.reshape(6, 2, 16, 2, 64) * e[:, :, None, :, None]
         assert torch.equal(x.reshape(6, 2, 16, 2, 64)[:3] * 0.25, y[[0, 2, 1]])
+
+
+# ------------------------------------------------------------------------- attention's output
+
+
+def attend_args(gpu):
+    cache, = caches(gpu, 1)
+    return cache, (i32([[0, 1], [2, 3]], gpu), i32([0, 2, 3], gpu), i32([20, 30], gpu))
+
+
+def test_outputs_that_overlap_are_refused(gpu):
+    cache, step = attend_args(gpu)
+    flat = torch.zeros(8192, dtype=torch.bfloat16, device=gpu)
+    q = torch.randn(3, 4, 64, dtype=torch.bfloat16, device=gpu)
+    for strides in [(64, 64, 1),      # (token 1, head 0) is (token 0, head 1)
+                    (128, 64, 1),     # token 1 begins among token 0's heads
+                    (64, 128, 1), (0, 64, 1), (256, 0, 1), (256, 32, 1), (32, 256, 1)]:
+        with pytest.raises(_lib.KVShiftError, match="overlap"):
+            attend_scaled(cache.dev, q, *step, out=flat.as_strided((3, 4, 64), strides))
+    assert not flat.any()
+    want = attend_scaled(cache.dev, q, *step)
+    for strides in [(256, 64, 1), (64, 192, 1), (320, 72, 1), (64, 256, 1)]:
+        out = flat.as_strided((3, 4, 64), strides)
+        assert torch.equal(attend_scaled(cache.dev, q, *step, out=out), want)
+        flat.zero_()
+    one = i32([[0, 1]], gpu), i32([0, 1], gpu), i32([20], gpu)
+    out = flat.as_strided((1, 4, 64), (0, 64, 1))  # of one token, whose stride is nobody's
+    assert torch.equal(attend_scaled(cache.dev, q[:1], *one, out=out),
+                       attend_scaled(cache.dev, q[:1], *one))
+
+
+def test_an_output_in_the_queries_or_the_cache_is_refused(gpu):
+    cache, step = attend_args(gpu)
+    flat = torch.randn(8192, device=gpu).to(torch.bfloat16)
+    q = flat.as_strided((3, 4, 64), (256, 64, 1))
+    before = flat.clone()
+    for at, strides in [(0, (256, 64, 1)), (64, (256, 64, 1)), (512, (256, 64, 1)),
+                        (8, (256, 64, 1)), (0, (512, 64, 1)), (256, (1024, 256, 1))]:
+        with pytest.raises(ValueError, match="memory with q"):
+            attend_scaled(cache.dev, q, *step, out=flat.as_strided((3, 4, 64), strides, at))
+    assert torch.equal(flat, before)
+    inside = cache.planes[0].view(torch.bfloat16).view(-1)[:768].view(3, 4, 64)
+    with pytest.raises(ValueError, match="memory with the cache"):
+        attend_scaled(cache.dev, q, *step, out=inside)
+    cache.check()
+
+
+def test_an_output_between_the_queries_is_taken(gpu):
+    """Queries and outputs in one buffer, a token's beside each other."""
+    cache, step = attend_args(gpu)
+    both = torch.randn(3, 12, 64, device=gpu).to(torch.bfloat16)
+    q, out = both[:, :4], both[:, 4:8]
+    rest = both[:, 8:].clone()
+    want = attend_scaled(cache.dev, q.clone(), *step)
+    assert attend_scaled(cache.dev, q, *step, out=out) is out
+    assert torch.equal(out, want) and torch.equal(both[:, 8:], rest)
+    wide = torch.randn(3, 4, 128, device=gpu).to(torch.bfloat16)
+    want = attend_scaled(cache.dev, wide[..., :64].clone(), *step)
+    assert torch.equal(attend_scaled(cache.dev, wide[..., :64], *step, out=wide[..., 64:]), want)
