@@ -46,7 +46,7 @@ MKV_MAX_HEAD_SIZE = 512
 MKV_DIRECT_MAX_SPANS = 63
 MKV_SMALL_MAX_SPANS = 8
 MKV_SMALL_MAX_INDEX = 64
-MKV_ABI_VERSION = (3 << 16) | 5
+MKV_ABI_VERSION = (3 << 16) | 6
 MKV_ORDER_NONE = 0
 MKV_ORDER_DST_PAGE = 1
 MKV_NOALLOC_SCRATCH_BYTES = 16 << 20
@@ -327,10 +327,13 @@ def lib() -> ctypes.CDLL:
                 )
             import torch  # noqa: F401  (bind to torch's HIP runtime)
 
-            cdll = _bind_scaled(_bind(ctypes.CDLL(LIB_PATH, mode=ctypes.RTLD_LOCAL)))
-            if cdll.mkv_abi_version() != MKV_ABI_VERSION:
-                raise RuntimeError("libmarathon_kvshift ABI version mismatch; rebuild")
-            _LIB = cdll
+            cdll = ctypes.CDLL(LIB_PATH, mode=ctypes.RTLD_LOCAL)
+            cdll.mkv_abi_version.restype = ctypes.c_int32
+            built = cdll.mkv_abi_version()  # first: another version may lack entry points
+            if built != MKV_ABI_VERSION:
+                raise RuntimeError(f"libmarathon_kvshift ABI version mismatch ({built}, not "
+                                   f"{MKV_ABI_VERSION}); rebuild")
+            _LIB = _bind_scaled(_bind(cdll))
     return _LIB
 
 
