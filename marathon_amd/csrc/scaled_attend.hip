@@ -1043,6 +1043,7 @@ struct Plan {
 
 constexpr int64_t kWantFew = 4096;
 constexpr int64_t kWantMany = 1024;
+constexpr int64_t kMostParts = 8;  // times as many parts as wanted that a workspace has room for
 
 // A tile's rows by those of the largest request, and the parts: of one size for all requests,
 // so that long and short histories fill the chip alike, about `want` workgroups if every
@@ -1071,6 +1072,12 @@ Shape shape_for(const mkv_attend_desc_t& d, int64_t each, int32_t from, int32_t 
   if (per < longest / kMaxSplits + 64) per = longest / kMaxSplits + 64;
   per = ((per < kMinSplit ? kMinSplit : per) + 63) / 64 * 64;
   s.splits = static_cast<int>(longest > per ? (longest + per - 1) / per : 1);
+  // Every tile has room for its parts' results, also where the hints promise fewer tiles than the
+  // token array has room for (a padded batch, a wrong hint): a token for one request of an array
+  // of 8,192 would ask for 31 GB.  Parts of such a call are fewer and longer.
+  const int64_t all = s.tiles * d.cache.heads;
+  if (all * s.splits > kMostParts * want)
+    s.splits = static_cast<int>(all < kMostParts * want ? kMostParts * want / all : 1);
   s.per = static_cast<int>(per);
   return s;
 }

@@ -120,3 +120,20 @@ def test_a_row_that_sees_one_token_is_its_value(gpu):
     want = plain.rows(cache.codes, cache.scales, [1], 1, 16)[0, :, 1]
     assert (out[0] == 0).all()
     assert np.array_equal(out[1].double().cpu().numpy(), np.repeat(want, 2, 0))
+
+
+@pytest.mark.parametrize("tokens,new,lengths,most", [
+    (6000, [1], [20000], 1),             # a padded array
+    (6000, [1, 2], [9000, 40], 1),       # and a hint that is too small
+    (3000, [2900, 1], [2900, 4000], 1),  # a wrong hint
+])
+def test_a_small_hint_for_a_large_array(gpu, tokens, new, lengths, most):
+    rng = np.random.default_rng(tokens + len(new))
+    cache, tables, rows = random_cache(gpu, rng, lengths, 4, 64, 16, "hnd")
+    tables = torch.nn.functional.pad(tables, (0, 3000), value=-1)
+    q = torch.randn(tokens, 16, 64, device=gpu, dtype=torch.bfloat16)
+    out = torch.full_like(q, 3.0)
+    attend_scaled(cache, q, tables, i32(np.cumsum([0] + new), gpu), i32(lengths, gpu), out=out,
+                  max_new=most)
+    check(out, q, rows, new, q.dtype)
+    assert (out[sum(new):] == 3.0).all()

@@ -60,3 +60,17 @@ def test_without_its_module_of_this_version_scatter_goes_the_general_way(monkeyp
     t = torch.zeros((1, 2), dtype=torch.int32)
     with pytest.warns(RuntimeWarning, match="general path"):
         assert scaled_cache._Usual().slots(t) is None
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("tokens,requests,group", [(8192, 1, 4), (8192, 1, 64), (60000, 2, 1),
+                                                   (2048, 32, 16), (20000, 4096, 8)])
+def test_a_small_hint_for_a_large_array_asks_for_a_bounded_workspace(tokens, requests, group, d):
+    """A row of D sums and its two statistics, 32 bits each; 8 * 4,096 parts of 32 rows, or
+    8 * 1,536 of 128, at most, for each of two launches."""
+    heads = 8
+    desc = attend_desc(heads=heads, head_size=d, num_blocks=1 << 20, tokens=tokens,
+                       requests=requests, q_heads=heads * group, table_width=1 << 16, max_new=1)
+    most = 2 * 8 * max(4096 * 32, 1536 * 128) * (d + 2) * 4
+    size = _lib.lib().mkv_attend_workspace_size(ctypes.byref(desc))
+    assert 0 <= size <= most
