@@ -358,7 +358,8 @@ def attend_scaled(cache: ScaledCache, q: torch.Tensor, block_tables: torch.Tenso
     desc.lens = _int32("lens", lens, device, n)
     desc.error_flags = _flags(error_flags, device)
     desc.tokens, desc.q_heads, desc.dtype = q.shape[0], q.shape[1], dtype_code(q.dtype)
-    desc.max_new, desc.max_len = int(max_new or 0), int(max_len or 0)
+    # (no request has more than 2^31 - 1 tokens, whatever the hints say)
+    desc.max_new, desc.max_len = (max(-1, min(int(m or 0), 2**31 - 1)) for m in (max_new, max_len))
     desc.softmax_scale = d ** -0.5 if softmax_scale is None else float(softmax_scale)
     L = _lib.lib()
     need = L.mkv_attend_workspace_size(ctypes.byref(desc))

@@ -137,3 +137,14 @@ def test_a_small_hint_for_a_large_array(gpu, tokens, new, lengths, most):
                   max_new=most)
     check(out, q, rows, new, q.dtype)
     assert (out[sum(new):] == 3.0).all()
+
+
+@pytest.mark.parametrize("most", [2**31 - 1, 2**31, 2**32 + 1, 2**40])
+def test_hints_of_any_size(gpu, most):
+    rng = np.random.default_rng(5)
+    cache, tables, rows = random_cache(gpu, rng, [300], 2, 64, 16, "hnd")
+    q = torch.randn(2, 8, 64, device=gpu, dtype=torch.bfloat16)
+    step = tables, i32([0, 2], gpu), i32([300], gpu)
+    check(attend_scaled(cache, q, *step, max_new=most, max_len=most), q, rows, [2], q.dtype)
+    with pytest.raises(Exception, match="max_len"):
+        attend_scaled(cache, q, *step, max_len=-most)
