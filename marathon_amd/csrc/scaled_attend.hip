@@ -1042,7 +1042,6 @@ struct Plan {
 };
 
 constexpr int64_t kWantFew = 4096;
-constexpr int64_t kWantMany = 1024;
 constexpr int64_t kMostParts = 8;  // times as many parts as wanted that a workspace has room for
 
 // A tile's rows by those of the largest request, and the parts: of one size for all requests,
@@ -1060,18 +1059,41 @@ Shape shape_for(const mkv_attend_desc_t& d, int64_t each, int32_t from, int32_t 
   const int64_t longest = d.max_len > 0 && d.max_len < room ? d.max_len : room;
   const int64_t largest = (each + s.rows - 1) / s.rows * d.requests;  // if all were the largest
   const int64_t groups = (s.tiles < largest ? s.tiles : largest) * d.cache.heads;
-  // 512 workgroups of the many kernel run at once: of one to two times as many tiles, or where
-  // requests differ in length, more and shorter parts leave less of the chip idle at the end.
-  // Measured with 1,024 / 1,536 wanted, heads of 128 but one: 648 tiles over 22,141 tokens 1,166 /
-  // 1,129 us, 540 over 12,000 577 / 541, 632 over 12,000 644 / 621, 520 over 22,000 (heads of
-  // 64) 526 / 503, 520 over 8,000 364 / 372; 1,064 of eight requests 282 / 258; but one
-  // request's 1,032 over 16,000 1,285 / 1,319 and over 2,000 309 / 339.
-  const bool more = groups >= 512 && (groups < 1024 || d.requests > 1);
-  const int64_t want = s.rows != kManyRows ? kWantFew : more ? kWantMany * 3 / 2 : kWantMany;
-  int64_t per = longest * (groups > 0 ? groups : 1) / want;
-  if (per < longest / kMaxSplits + 64) per = longest / kMaxSplits + 64;
-  per = ((per < kMinSplit ? kMinSplit : per) + 63) / 64 * 64;
-  s.splits = static_cast<int>(longest > per ? (longest + per - 1) / per : 1);
+  const auto per_of = [&](int64_t want) {  // tokens of a part
+    int64_t per = longest * (groups > 0 ? groups : 1) / want;
+    if (per < longest / kMaxSplits + 64) per = longest / kMaxSplits + 64;
+    return ((per < kMinSplit ? kMinSplit : per) + 63) / 64 * 64;
+  };
+  const auto parts_of = [&](int64_t per) { return longest > per ? (longest + per - 1) / per : 1; };
+  int64_t want = kWantFew, per = per_of(want);
+  if (s.rows == kManyRows && (d.requests > 1 || d.cache.head_size == 64)) {
+    // Requests differ in length: short parts fill the chip alike.  Eight requests with 1,024 / 1,536
+    // wanted, heads of 128: 576 tiles 114.7 / 114.1 us, 808 301 / 287, 1,064 280 / 256; of 64: 808
+    // 183 / 187, 1,064 166 / 148; of 256: 1,064 823 / 764.  Fewer tiles want fewer: 200 of seven
+    // requests (heads of 64) 47.8 / 50.7.  One request, heads of 64: 512 over 22,000 tokens
+    // 539 / 506, 976 over 8,000 462 / 416; 348 over 1,835 73.7 / 80.9, 1,080 over 2,000 204 / 215.
+    want = groups >= 512 && (groups < 1024 || d.requests > 1) ? 1536 : 1024;
+    per = per_of(want);
+  } else if (s.rows == kManyRows) {
+    // One request: twice as many parts as run at once, by the kernel's registers and LDS; but half
+    // as many again where those would leave a tenth of the slots that they take in turns empty,
+    // if there are as many tiles as slots or the parts are long.  Twice / three times as many,
+    // heads of 128: 376 tiles over 22,000 tokens 705 / 653 us, over 2,000 113 / 125; 512 over
+    // 8,000 366 / 373; 572 over 556 183 / 162; 640 over 22,141 1,124 / 1,073; 856 over 8,000
+    // 666 / 635; 976 over 8,000 724 / 734; 1,080 over 8,000 879 / 840.  Of 256: 176 over 8,000
+    // 491 / 433, 512 over 8,000 1,109 / 1,243, 640 over 22,000 4,269 / 3,947; the exception
+    // 320 over 8,000, 747 / 784.
+    const int64_t resident = d.cache.head_size == 256 ? 256 : 512;
+    want = 2 * resident;
+    per = per_of(want);
+    const int64_t n = groups * parts_of(per), slots = (n + resident - 1) / resident * resident;
+    const int64_t shorter = per_of(3 * resident);
+    if (10 * n < 9 * slots && (groups >= resident || shorter >= 2048)) {
+      want = 3 * resident;
+      per = shorter;
+    }
+  }
+  s.splits = static_cast<int>(parts_of(per));
   // Every tile has room for its parts' results, also where the hints promise fewer tiles than the
   // token array has room for (a padded batch, a wrong hint): a token for one request of an array
   // of 8,192 would ask for 31 GB.  Parts of such a call are fewer and longer.

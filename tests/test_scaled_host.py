@@ -74,3 +74,21 @@ def test_a_small_hint_for_a_large_array_asks_for_a_bounded_workspace(tokens, req
     most = 2 * 8 * max(4096 * 32, 1536 * 128) * (d + 2) * 4
     size = _lib.lib().mkv_attend_workspace_size(ctypes.byref(desc))
     assert 0 <= size <= most
+
+
+@pytest.mark.parametrize("d,tokens,parts", [
+    (256, 2048, 1),   # 512 tiles, 256 at once: two rounds
+    (256, 1024, 2), (256, 512, 4),
+    (256, 704, 5),    # 176 tiles: three parts each would leave a third of three rounds empty
+    (128, 4096, 1),   # 1,024 tiles, 512 at once
+    (128, 2048, 2), (128, 1024, 4),
+    (128, 2560, 3),   # 640
+])
+def test_the_parts_of_a_chunk_fill_the_chip(d, tokens, parts):
+    """One request, 8 heads of 4 query heads, 8,192 tokens held: tiles of 128 rows, of which as
+    many run at once as the kernel's registers and LDS let."""
+    desc = attend_desc(heads=8, head_size=d, num_blocks=4096, tokens=tokens, requests=1, q_heads=32,
+                       table_width=1024, max_new=tokens, max_len=8192 + tokens)
+    rows = tokens * 4 // 128 + 1  # and a tile to spare
+    want = rows * 8 * parts * 128 * (d + 2) * 4 if parts > 1 else 0
+    assert _lib.lib().mkv_attend_workspace_size(ctypes.byref(desc)) == want
