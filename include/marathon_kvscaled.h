@@ -130,13 +130,15 @@ int mkv_store_scaled(const mkv_scaled_cache_t* cache, const void* k, int64_t k_t
  *            each other, q or the cache.
  *   out[i] = sum_j p_j V[j],  p = softmax over j <= position(i), j < lens[r], of
  *            softmax_scale * q[i] . K[j]
- * computed with fp32 sums and softmax statistics.  A row that sees no key is zeros; rows
- * that belong to no request are left as they were.  Tokens of a block whose id is out of
- * range are not seen (MKV_FLAG_SRC_RANGE), nor are those behind the block table.  What lies
- * in rows that a query does not see has no effect, NaNs included.
+ * computed with fp32 sums and softmax statistics.  Where it meets V, p is held in two bf16 terms,
+ * off by at most 2^-17 of itself; in one, off by 2^-8, in the kernel of more than 32 rows for bf16
+ * queries (rows: max_new, or without it the tokens, times the query heads of a KV head).
+ * A row that sees no key is zeros; rows that belong to no request are left as they were.  Tokens
+ * of a block whose id is out of range are not seen (MKV_FLAG_SRC_RANGE), nor are those behind
+ * the block table.  What lies in rows that a query does not see has no effect, NaNs included.
  *   max_new, max_len : the largest number of new tokens and of tokens of a request, where the
  *            caller knows them (0: not known).  They choose launch shapes; wrong ones cost
- *            time and change no result but for the order of its sums.
+ *            time, and change a result by the order of its sums and by p's roundings alone.
  *   workspace : device, mkv_attend_workspace_size() bytes for the same arguments, 16-byte
  *            aligned; overwritten, so calls that overlap on one workspace race.  May be NULL
  *            where that size is 0.

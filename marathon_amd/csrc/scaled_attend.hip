@@ -11,8 +11,11 @@
 // its power of two is exact in bf16, so K and V lose nothing.  (The 8-bit matrix instructions
 // would take the codes as they are, at the same cost for bf16 queries cut into two e4m3 terms,
 // but they align a step's products to about 13 bits below the largest: measured 2^-12.5 of
-// it.)  The one rounding is p's: to bf16 for bf16 queries (half a step is 2^-9 of it, below
-// the output's own); for fp16 queries p is cut into two bf16 terms, which leaves 2^-17.
+// it.)  The one rounding is p's.  The kernel of few rows cuts it into two bf16 terms, which leaves
+// 2^-17: the second product hides behind memory (a batch's next tokens 110.7 -> 111.2 us, one
+// request's 19.8 -> 19.9; of 17 to 32 rows 27.4 -> 30.9).  The kernel of many rows does so for
+// fp16 queries; for bf16 ones it rounds p to bf16, by half a step of it, 2^-8, as the output
+// itself is: a second product would take 2,048 tokens over 22,141 from 1,072 to 1,380 us.
 // fp16 queries multiply the bare codes (exact in fp16, where a scaled value may not be) and
 // the scale is applied to s_j.
 //
@@ -343,7 +346,7 @@ __global__ __launch_bounds__(64 * kFewWaves, (few_waves<D, RT>())) void attend_f
       }
       odd = __any(any != 0);
     }
-    uint32_t ph[RT][4], pl[RT][4];  // P^T: pairs of tokens; and what bf16 leaves (F16)
+    uint32_t ph[RT][4], pl[RT][4];  // P^T: pairs of tokens; and what bf16 leaves of them
     uint32_t see[RT];               // masked: which of the lane's 8 tokens its row sees
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -382,9 +385,8 @@ __global__ __launch_bounds__(64 * kFewWaves, (few_waves<D, RT>())) void attend_f
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         ph[rt][j] = round_pair(y[2 * j], y[2 * j + 1]);
-        if constexpr (F16)
-          pl[rt][j] = round_pair(y[2 * j] - __uint_as_float(ph[rt][j] << 16),
-                                 y[2 * j + 1] - __uint_as_float(ph[rt][j] & 0xFFFF0000u));
+        pl[rt][j] = round_pair(y[2 * j] - __uint_as_float(ph[rt][j] << 16),
+                               y[2 * j + 1] - __uint_as_float(ph[rt][j] & 0xFFFF0000u));
       }
     }
     // O^T += V^T P^T: dimension tile dt holds dimensions (D / 16) * c + dt
@@ -411,11 +413,9 @@ __global__ __launch_bounds__(64 * kFewWaves, (few_waves<D, RT>())) void attend_f
           const u32x4 b = {ph[rt][0], ph[rt][1], ph[rt][2], ph[rt][3]};
           o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bits_as<bf16x8>(a),
                                                               bits_as<bf16x8>(b), o[rt][dt], 0, 0, 0);
-          if constexpr (F16) {
-            const u32x4 b2 = {pl[rt][0], pl[rt][1], pl[rt][2], pl[rt][3]};
-            o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                bits_as<bf16x8>(a), bits_as<bf16x8>(b2), o[rt][dt], 0, 0, 0);
-          }
+          const u32x4 b2 = {pl[rt][0], pl[rt][1], pl[rt][2], pl[rt][3]};
+          o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bits_as<bf16x8>(a),
+                                                              bits_as<bf16x8>(b2), o[rt][dt], 0, 0, 0);
         }
       }
     }

@@ -317,11 +317,14 @@ def attend_scaled(cache: ScaledCache, q: torch.Tensor, block_tables: torch.Tenso
     A row that sees nothing is zeros; rows of ``out`` behind ``starts[-1]`` are left as they
     were (in a fresh ``out``, undefined).  ``out``'s rows share no memory with each other, ``q`` or
     the cache (ranges that interleave in strides that differ are taken to); it is refused.
-    Sums and softmax statistics are fp32.
+    Sums and softmax statistics are fp32.  Where a probability meets V it is off by at most 2^-17
+    of itself, or by 2^-8, as a bf16 output itself is, for bf16 queries in the kernel of more than
+    32 rows (``max_new``, or without it the tokens, times the query heads of a KV head).
 
     ``max_new`` and ``max_len``: the largest number of new tokens and of tokens of a request,
-    where the host knows them (a captured step: the largest that will be replayed).  They
-    choose launch shapes only."""
+    where the host knows them (a captured step: the largest that will be replayed).  They choose
+    launch shapes, and a result only by the order of its sums and the roundings above.  Without
+    ``max_new`` a batch's decode step is taken for one request's chunk."""
     got = _usual.attend(*cache.handle, q, block_tables, starts, lens, softmax_scale, max_new,
                         max_len, out, error_flags)
     if got is not None:

@@ -38,11 +38,12 @@ def random_cache(gpu, rng, lengths, heads, d, bs, layout):
     return cache, i32(tables, gpu), rows
 
 
-def check(got, q, rows, new, dtype):
+def check(got, q, rows, new, dtype, whole_p=False):
     """Each entry within the roundings that the definition of the operator allows: of the output
-    half a step; of p 2^-9 of each term (2^-17 for fp16) and 2^-20 for exponential, sums and
-    quotient; of a score (D + 4) * 2^-24 of the sizes of its products.  p's share moves the
-    output by at most twice itself of sum(p |v|)."""
+    half a step; of p, in the sum over V alone, half a step of bf16, 2^-8 of each term (2^-17
+    where two terms hold it: for fp16, or ``whole_p``); of exponential, sums and quotient 2^-20;
+    of a score (D + 4) * 2^-24 of the sizes of its products, a share of p in the sums above and
+    below."""
     d, at = q.shape[2], 0
     eps = torch.finfo(dtype).eps / 2
     for x, n in zip(rows, new):
@@ -56,8 +57,9 @@ def check(got, q, rows, new, dtype):
             p = torch.softmax((qh @ k.T * d ** -0.5).masked_fill(mask, -torch.inf), 1)
             size = (qh.abs() @ k.T.abs() * d ** -0.5).masked_fill(mask, 0.0).amax(1, keepdim=True)
             want = p @ v
-            share = (2.0 ** -9 if dtype == torch.bfloat16 else 2.0 ** -17) + 2.0 ** -20
-            tol = 2 * (share + (d + 4) * 2.0 ** -24 * size) * (p @ v.abs())
+            rounded = 2.0 ** -8 if dtype == torch.bfloat16 and not whole_p else 2.0 ** -17
+            share = 2 * (2.0 ** -20 + (d + 4) * 2.0 ** -24 * size) + rounded
+            tol = share * (p @ v.abs())
             tol = tol + eps * (want.abs() + tol) + 1e-30
             off = (got[at:at + n, h].double() - want).abs()
             assert (off <= tol).all(), (h, float((off / tol).max()))
@@ -148,3 +150,16 @@ def test_hints_of_any_size(gpu, most):
     check(attend_scaled(cache, q, *step, max_new=most, max_len=most), q, rows, [2], q.dtype)
     with pytest.raises(Exception, match="max_len"):
         attend_scaled(cache, q, *step, max_len=-most)
+
+
+@pytest.mark.parametrize("lengths,new,heads,group,d", [
+    ([5000, 700, 17], [1, 1, 1], 2, 4, 128), ([3000, 90], [2, 1], 1, 8, 64), ([2000], [1], 2, 16, 256),
+    ([4000, 33], [4, 1], 2, 8, 128), ([1500], [8], 1, 4, 256)])
+def test_few_rows_keep_their_probabilities(gpu, lengths, new, heads, group, d):
+    """Up to 32 rows: p in two bf16 terms for bf16 queries too."""
+    rng = np.random.default_rng(sum(lengths) + d)
+    cache, tables, rows = random_cache(gpu, rng, lengths, heads, d, 16, "hnd")
+    q = torch.randn(sum(new), heads * group, d, device=gpu).to(torch.bfloat16)
+    got = attend_scaled(cache, q, tables, i32(np.cumsum([0] + new), gpu), i32(lengths, gpu),
+                        max_new=max(new))
+    check(got, q, rows, new, q.dtype, whole_p=True)
