@@ -746,11 +746,26 @@ extern "C" int mkv_store_scaled(const mkv_scaled_cache_t* cache, const void* k,
   p.tokens = tokens;
   const int waves = waves_of(p.c.bs_shift, p.c.heads), parts = cache->block_size / 16;
   const int heads_here = waves / parts;
-  // Small stores want every block a workgroup of its own, large ones few workgroups that lead
-  // nothing: 5,003 ragged tokens of 4 heads take 12 / 6.9 / 7.8 us with 1 / 4 / 16 tokens a
-  // workgroup, 22,141 of 8 heads 112 / 73 / 29.
+  // Decode steps want every token, and small stores every block, a workgroup of its own; large
+  // stores few workgroups that lead nothing, up to one a block.  In us with 1 / 4 / 8 / 16 tokens a
+  // workgroup, blocks of 16, 8 heads of 128 but where said:
+  //   1,000 requests of one token 11.8 / 15.7 / 26 / 44, 4,096 39 / 39 / 36 / 52
+  //   8 requests of 65, 4 heads 5.3 / 7.2;  488 of 16, 4 heads 16.1 with 4, 18.9 with 16
+  //   one of 1,000 12.9 / 5.9 / 6.6 / 8.5, of 2,000 28 / 9.8 / 7.6 / 9.2, of 4,000 52 / 16.6 / 11.7 /
+  //   10.5, of 22,000 269 / 76 / 48 / 30
+  //   13 requests of 5,003 in all, 4 heads of 64 12.8 / 8.1 / 9.3 / 9.4
+  // and with 4 / 16 / 64: blocks of 64, one of 1,000 8.9 / 8.1 / 10.1, of 8,000 107 / 36 / 15;
+  // blocks of 128, one of 8,000 217 / 49 / 19, and 17 with 128.
   const int64_t each = tokens * ((cache->heads + heads_here - 1) / heads_here);
-  p.group = each <= 4096 ? 1 : each <= 32768 ? 4 : 16;
+  const int64_t ahead = tokens / requests;  // a request's on average
+  if (ahead < 16 || (each <= 4096 && ahead < 256))
+    p.group = each <= 4096 ? 1 : 4;
+  else if (each > 24576)
+    p.group = cache->block_size;
+  else if (each > 12288)
+    p.group = ahead >= 64 ? 16 : 4;
+  else
+    p.group = cache->block_size >= 64 && ahead >= 64 ? 16 : each > 4096 && ahead >= 1024 ? 8 : 4;
   if ((tokens + p.group - 1) / p.group > UINT32_MAX / (64 * waves))
     return mkv_fail(MKV_ERR_UNSUPPORTED, "%s: %lld tokens", who, (long long)tokens);
   const dim3 grid(static_cast<unsigned>((tokens + p.group - 1) / p.group),
