@@ -402,11 +402,14 @@ class ScaledShifts:
         pairs = list({(bytes(s.desc), bytes(d.desc)): (s, d) for s, d in zip(src, dst)}.values())
         src, dst = [s for s, _ in pairs], [d for _, d in pairs]
         self.src, self.dst, self.device, self.layers = src, dst, b.device, len(dst)
-        for i, c in enumerate(dst):
-            if any(_offset(c, other) is not None for other in dst[:i]):
-                raise ValueError("two layers of dst share memory")
         # where a source block n is the destination's block n + offset of some layer
-        offsets = {_offset(s, d) for s in src for d in dst} - {None}
+        offsets = set()
+        for i, j in _near(src + dst):
+            if i >= len(src) and _offset(dst[i - len(src)], dst[j - len(src)]) is not None:
+                raise ValueError("two layers of dst share memory")
+            if i < len(src) <= j:
+                offsets.add(_offset(src[i], dst[j - len(src)]))
+        offsets.discard(None)
         self.rotary = 0 if inv_freq is None else 2 * int(inv_freq.numel())
         if self.rotary % 32 or self.rotary > b.head_size:
             raise ValueError(f"rotary {self.rotary}: a multiple of 32, at most {b.head_size}")
@@ -517,6 +520,17 @@ class ScaledShifts:
     def _capturing(self) -> bool:
         with _on(self.device, _current(self.device)):
             return torch.cuda.is_current_stream_capturing()
+
+
+def _near(caches: list) -> set:
+    """The pairs of places, the lower first, of caches whose address ranges meet."""
+    ranges = sorted((r.base, r.end, i) for i, c in enumerate(caches) for r in (*c.rows, c.scale_rows))
+    pairs, open_ranges = set(), []
+    for base, end, i in ranges:
+        open_ranges = [r for r in open_ranges if r[0] > base]
+        pairs.update((min(i, j), max(i, j)) for _, j in open_ranges if i != j)
+        open_ranges.append((end, i))
+    return pairs
 
 
 def _offset(a: ScaledCache, b: ScaledCache) -> int | None:
