@@ -82,7 +82,8 @@ __device__ __forceinline__ void check_starts(const DevStep& s, int64_t tokens, b
   bool bad = false;
   for (int r = threadIdx.x; r < s.requests; r += blockDim.x) {
     const int64_t s0 = s.starts[r], s1 = s.starts[r + 1];
-    bad = bad || s0 < 0 || s1 < s0 || s1 > tokens || (rows_held && s.lens[r] < s1 - s0);
+    bad = bad || s0 < 0 || s1 < s0 || s1 > tokens ||
+          (rows_held && s1 > s0 && s.lens[r] < s1 - s0);
   }
   if (bad) raise(s.flags, MKV_FLAG_SPAN);
 }

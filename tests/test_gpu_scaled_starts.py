@@ -136,3 +136,19 @@ def test_starts_that_descend_are_flagged(gpu, starts):
     flags = i32([0], gpu)
     store_scaled(cache.dev, x, x, *args, error_flags=flags)
     assert flags.item() == _lib.MKV_FLAG_SPAN
+
+
+def test_a_request_of_no_new_tokens_holds_anything(gpu):
+    """Rows of a batch that no request has taken: empty, their length whatever it was."""
+    rng = np.random.default_rng(2)
+    cache = Cache(gpu, rng, 4, 1, 64, 16)
+    x = torch.from_numpy(loud(rng, (T, 1, 64))).to(gpu, torch.bfloat16)
+    tables = np.array([[0, 1], [2, 3], [-1, -1]], np.int32)
+    args = i32(tables, gpu), i32([0, 20, 20, 20], gpu), i32([20, -1, -2**31], gpu)
+    flags = i32([0], gpu)
+    store_scaled(cache.dev, x, x, *args, error_flags=flags)
+    attend_scaled(cache.dev, x, *args, error_flags=flags)
+    assert flags.item() == 0
+    x = x.double().cpu().numpy()
+    plain.store(cache.codes, cache.scales, x, x, tables[:1], [0, 20], [20], 16)
+    cache.check()
