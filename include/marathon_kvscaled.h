@@ -92,7 +92,9 @@ typedef struct mkv_scaled_cache {
  *   free_blocks   : int32 [free_len], ids of free blocks; those from free_at[0] on are free.
  *   starts, lens  : out, as above.
  *   slots         : out int64 [max_tokens]: block * block_size + row of every new token, -1
- *                   behind the last one.  positions: out int32 [max_tokens], 0 there.
+ *                   behind the last one and where a block's id is negative (ids are not checked
+ *                   otherwise: what takes them knows their cache).  positions: out int32
+ *                   [max_tokens], 0 behind the last one.
  *   free_at_out   : out int32 [1]: where the free list begins now.  Not free_at itself; nor
  *                   does another output share memory with an input.
  * All or nothing: where a length is negative, the new tokens exceed max_tokens, a request
@@ -183,7 +185,7 @@ int64_t mkv_attend_workspace_size(const mkv_attend_desc_t* desc);
  * the block's scale is the new rows': their values are undefined until they are written.
  * A block is written with all of its rows or, where a source block of one is out of range,
  * left as it was, its scales among it.
- * Destination blocks are distinct and no source blocks of the call.
+ * Destination blocks are distinct and no source blocks of the call, in any layer.
  *
  * mkv_scaled_units (a host function, no GPU call; every pointer a HOST one) resolves spans
  * into units, one for each destination block:

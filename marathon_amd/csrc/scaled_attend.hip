@@ -166,8 +166,8 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
 // the registers where the matrix instructions want them (16x16x32: a lane is a token of K or
 // 4, 8 or 16 dimensions of V, whose bytes are paired between tokens by v_perm), so nothing
 // passes through LDS but the waves' results at the end.  A token for each of 32 requests with
-// 8,270 on average, 8 KV heads of 128 (542 MB), takes 105 us, 5.2 TB/s; a bare linear read of
-// as many bytes 77 to 85.
+// 8,270 on average, 8 KV heads of 128 (542 MB), takes 106 us, 5.1 TB/s, and as long with its blocks
+// in order; a bare linear read of as many bytes 77 to 85.  Heads of 64 67 us, of 256 199.
 
 constexpr int kFewWaves = 4;
 
@@ -561,9 +561,11 @@ __global__ __launch_bounds__(64 * kFewWaves, (few_waves<D, RT>())) void attend_f
 // one column cover the 64 banks.
 // The next step's codes are loaded into registers before a step is computed and written to
 // the other of two buffers behind it: one barrier a step.  Two workgroups fit a CU, and one
-// computes while the other waits.  A chunk of 2,048 tokens over 22,141, 40 query heads of 128
-// (0.97 TFLOP), takes 1,040 to 1,070 us: 0.92 PFLOP/s, where a library product of 8,192^3
-// reaches 1.22.
+// computes while the other waits.  (Heads of 64 leave room for three, of 256 for one, which
+// spills 41 registers.)  A chunk of 2,048 tokens over 22,141, 40 query heads of 128 (0.97 TFLOP),
+// takes 1,050 to 1,130 us with the card: 0.86 to 0.93 PFLOP/s, where a library product of 8,192^3
+// reaches 1.22.  Heads of 64 run at 0.8 PFLOP/s, a score's softmax having half the products to
+// hide behind; of 256 at 0.5; fp16 queries, with a second product for p, at 0.69.
 
 constexpr int kManyWaves = 4;
 constexpr int kManyRows = 32 * kManyWaves;

@@ -217,7 +217,7 @@ def step_slots(held: torch.Tensor, new: torch.Tensor, block_tables: torch.Tensor
     step's tokens (the length of the slot map).  ``slots`` is what :func:`scatter_shifted` and
     a slot-addressed shift take, ``starts`` and ``lens`` what :func:`store_scaled` and
     :func:`attend_scaled` take; the next step's ``held`` is ``lens`` and its ``free_at``
-    the one returned.
+    the one returned.  Ids are taken as they are; a token whose block's id is negative gets slot -1.
 
     All or nothing: where the free list runs out, a request exceeds its table, the tokens
     exceed ``max_tokens`` or a length is negative, bit ``MKV_FLAG_DST_RANGE`` is set in
