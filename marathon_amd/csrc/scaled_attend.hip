@@ -1077,20 +1077,33 @@ Shape shape_for(const mkv_attend_desc_t& d, int64_t each, int32_t from, int32_t 
     want = groups >= 512 && (groups < 1024 || d.requests > 1) ? 1536 : 1024;
     per = per_of(want);
   } else if (s.rows == kManyRows) {
-    // One request: twice as many parts as run at once, by the kernel's registers and LDS; but half
-    // as many again where those would leave a tenth of the slots that they take in turns empty,
-    // if there are as many tiles as slots or the parts are long.  Twice / three times as many,
-    // heads of 128: 376 tiles over 22,000 tokens 705 / 653 us, over 2,000 113 / 125; 512 over
-    // 8,000 366 / 373; 572 over 556 183 / 162; 640 over 22,141 1,124 / 1,073; 856 over 8,000
-    // 666 / 635; 976 over 8,000 724 / 734; 1,080 over 8,000 879 / 840.  Of 256: 176 over 8,000
-    // 491 / 433, 512 over 8,000 1,109 / 1,243, 640 over 22,000 4,269 / 3,947; the exception
-    // 320 over 8,000, 747 / 784.
+    // One request: as few parts as fill nine tenths of the slots that they take in turns (as many as
+    // run at once, by the kernel's registers and LDS), one or two; otherwise twice as many parts as
+    // run at once, or three times where those fill less and are long.  Measured as 1,024 or (512 to
+    // 1,023 tiles) 1,536 wanted / this rule, heads of 128: 256 tiles over 2,000 tokens 92.2 / 83.1 us,
+    // over 22,000 465 / 445; 376 over 22,000 708 / 655; 512 over 2,000 173 / 135, over 8,000 379 /
+    // 343; 640 over 2,000 203 / 202; 856 over 8,000 630 / 633; 976 over 8,000 741 / 703; 1,080 over
+    // 22,000 2,143 / 1,899.  Of 256: 128 over 8,000 336 / 283, 512 over 8,000 1,292 / 1,108, 640 over
+    // 22,141 3,798 / 3,708.  Not where one turn takes long unequal tiles (two heads' 8,192 tokens
+    // from nothing: one part 218, two 204), nor, of more tiles than two turns take, where the history
+    // is short (1,256 over 1,000 tokens: one part 335, two 375).
     const int64_t resident = d.cache.head_size == 256 ? 256 : 512;
     want = 2 * resident;
     per = per_of(want);
-    const int64_t n = groups * parts_of(per), slots = (n + resident - 1) / resident * resident;
+    const int64_t fresh = each / (d.q_heads / d.cache.heads);
+    const bool wedge = 2 * fresh > longest && longest >= 4096;  // first tiles see little, last ones much
+    const auto fills = [&](int64_t n) {  // nine tenths of the slots that n parts a tile take in turns
+      const int64_t all = groups * n, turns = (all + resident - 1) / resident;
+      return 10 * all >= 9 * turns * resident && !(wedge && turns == 1);
+    };
     const int64_t shorter = per_of(3 * resident);
-    if (10 * n < 9 * slots && (groups >= resident || shorter >= 2048)) {
+    const bool cut = groups < 2 * resident || (longest >= 8192 && !wedge);
+    if (fills(1)) {
+      per = (longest + 64) / 64 * 64;
+    } else if (cut && fills(2)) {
+      per = ((longest + 1) / 2 + 63) / 64 * 64;
+      if (per < kMinSplit) per = kMinSplit;
+    } else if (cut && !fills(parts_of(per)) && (groups >= resident || shorter >= 2048)) {
       want = 3 * resident;
       per = shorter;
     }
@@ -1102,7 +1115,7 @@ Shape shape_for(const mkv_attend_desc_t& d, int64_t each, int32_t from, int32_t 
   const int64_t all = s.tiles * d.cache.heads;
   if (all * s.splits > kMostParts * want)
     s.splits = static_cast<int>(all < kMostParts * want ? kMostParts * want / all : 1);
-  s.per = static_cast<int>(per);
+  s.per = static_cast<int>(per < 1 << 30 ? per : 1 << 30);  // (no request has more tokens)
   return s;
 }
 

@@ -77,11 +77,11 @@ def test_a_small_hint_for_a_large_array_asks_for_a_bounded_workspace(tokens, req
 
 
 @pytest.mark.parametrize("d,tokens,parts", [
-    (256, 2048, 1),   # 512 tiles, 256 at once: two rounds
-    (256, 1024, 2), (256, 512, 4),
-    (256, 704, 5),    # 176 tiles: three parts each would leave a third of three rounds empty
-    (128, 4096, 1),   # 1,024 tiles, 512 at once
-    (128, 2048, 2), (128, 1024, 4),
+    (256, 2048, 1), (256, 1024, 1),  # 512 and 256 tiles, 256 at once
+    (256, 512, 2),    # 128
+    (256, 704, 5),    # 176: one or two parts each would leave a third of the slots empty
+    (128, 4096, 1), (128, 2048, 1),  # 1,024 and 512 tiles, 512 at once
+    (128, 1024, 2),
     (128, 2560, 3),   # 640
 ])
 def test_the_parts_of_a_chunk_fill_the_chip(d, tokens, parts):
