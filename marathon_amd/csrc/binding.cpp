@@ -359,7 +359,8 @@ PyObject* store(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (k->dim() != 3 || k->device() != dev || v->device() != dev || k->sizes() != v->sizes() ||
         k->scalar_type() != v->scalar_type() || (code != MKV_BF16 && code != MKV_F16 && code != MKV_F32) ||
         k->size(1) != cache->heads || k->size(2) != cache->head_size || k->stride(2) != 1 ||
-        v->stride(2) != 1 || needs_grad(*k) || needs_grad(*v) || !table_of(args[4], &dev, tab) || flags_of(args[7], dev, flags) != kUsual ||
+        v->stride(2) != 1 || needs_grad(*k) || needs_grad(*v) || !table_of(args[4], &dev, tab) ||
+        flags_of(args[7], dev, flags) != kUsual ||
         c10::hip::current_device() != dev.index())
       Py_RETURN_NONE;
     const int32_t* starts = vector_of(args[5], dev, tab.n + 1);

@@ -565,7 +565,7 @@ __global__ __launch_bounds__(64 * kFewWaves, (few_waves<D, RT>())) void attend_f
 // spills 41 registers.)  A chunk of 2,048 tokens over 22,141, 40 query heads of 128 (0.97 TFLOP),
 // takes 1,050 to 1,130 us with the card: 0.86 to 0.93 PFLOP/s, where a library product of 8,192^3
 // reaches 1.22.  Heads of 64 run at 0.8 PFLOP/s, a score's softmax having half the products to
-// hide behind; of 256 at 0.5; fp16 queries, with a second product for p, at 0.69.
+// hide behind; of 256 at 0.53; fp16 queries, with a second product for p, at 0.68.
 
 constexpr int kManyWaves = 4;
 constexpr int kManyRows = 32 * kManyWaves;

@@ -494,8 +494,8 @@ static_assert(sizeof(MoveParams) + sizeof(MoveWords) <= 4096, "a launch's argume
 
 // A workgroup makes one destination block of `heads_here` heads in one layer and ends.  What
 // it has to know is one record made on the host.  22,141 tokens x 40 layers of 8 heads of 128
-// (3.63 GB) take 628 to 652 us, 5.6 to 5.8 TB/s, where a copy of as many rows through shuffled block
-// tables takes 661, through ordered ones 584, and a linear one 542.  Found on the GPU instead
+// (3.63 GB) take 614 to 652 us, 5.6 to 5.9 TB/s, where a copy of as many rows through shuffled block
+// tables takes 653 to 661, through ordered ones 583, and a linear one 542.  Found on the GPU instead
 // (span, then tables, then rows), the chain of loads in front of the data made it 818; a loop over
 // layers behind one chain, whose loads wait for its stores, 755.
 template <int D, typename Words>

@@ -137,8 +137,8 @@ class ScaledCache:
         self.scale_rows = Rows(scales.data_ptr(), 2 * self.heads, ((2 * self.heads, kv.shape[0]),))
         # (an expanded cache, of stride 0, is one whose rows lie in one another)
         if not self.rows[0].apart():
-            raise ValueError(f"a cache of shape {tuple(kv.shape)} and strides {kv.stride()} has rows "
-                             "that overlap")
+            raise ValueError(f"a cache of shape {tuple(kv.shape)} and strides {kv.stride()} has "
+                             "rows that overlap")
         if v is not None and share(*self.rows):
             raise ValueError("kv and v_cache share memory")
         if any(s % 16 for s in strides[:3]) or kv.data_ptr() % 16 or (
@@ -524,7 +524,8 @@ class ScaledShifts:
 
 def _near(caches: list) -> set:
     """The pairs of places, the lower first, of caches whose address ranges meet."""
-    ranges = sorted((r.base, r.end, i) for i, c in enumerate(caches) for r in (*c.rows, c.scale_rows))
+    ranges = sorted((r.base, r.end, i) for i, c in enumerate(caches)
+                    for r in (*c.rows, c.scale_rows))
     pairs, open_ranges = set(), []
     for base, end, i in ranges:
         open_ranges = [r for r in open_ranges if r[0] > base]
