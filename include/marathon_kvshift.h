@@ -333,10 +333,10 @@ int mkv_rope_tables(const int32_t* deltas, int32_t n_spans, const float* inv_fre
 /* Human-readable reason for the last non-MKV_OK return on this thread ("" if none). */
 const char* mkv_last_error(void);
 
-/* ABI version of this header and marathon_kvscaled.h: (major << 16) | minor.  3.6 brought the
- * latter's entry points. */
+/* ABI version of this header, marathon_kvscaled.h and marathon_kvstep.h: (major << 16) | minor.
+ * 3.6 brought the second one's entry points, 3.7 the third one's. */
 int32_t mkv_abi_version(void);
-#define MKV_ABI_VERSION ((3 << 16) | 6)
+#define MKV_ABI_VERSION ((3 << 16) | 7)
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,117 @@
+/*
+ * marathon_kvstep.h -- C ABI of an engine step's operators around the block-scaled 8-bit KV
+ * cache on MI355X (gfx950): heads normalised and turned to their positions, the same on their
+ * way into the cache, and attention of a batch whose requests share what they begin with.
+ *
+ * Conventions are marathon_kvscaled.h's: device pointers, work enqueued on `stream`, nothing
+ * allocated or synchronised, strides in ELEMENTS, rows and their strides aligned to 16 bytes,
+ * MKV_OK or an MKV_ERR_* code with mkv_last_error(), indices in device memory checked on the
+ * device.  A step's requests are described by its starts, lens and block_tables.
+ *
+ * No counterpart in the reference, whose engine does these itself (the rotation that its keys
+ * come with is src/marathon/kvshift.py:44-61).
+ */
+#ifndef MARATHON_KVSTEP_H
+#define MARATHON_KVSTEP_H
+
+#include <stdint.h>
+
+#include "marathon_kvscaled.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/*
+ * Heads x[0..D) of a token at position p become
+ *     y = x / sqrt(mean(x^2) + eps) * weight            (norm 0: y = x)
+ *     out[i]     = y[i] cos(a_i) - y[i + R/2] sin(a_i),
+ *     out[i+R/2] = y[i+R/2] cos(a_i) + y[i] sin(a_i),    a_i = p * inv_freq[i],  i < R/2
+ *     out[i]     = y[i],                                                         i >= R
+ * (R = rotary) in fp32, the angles reduced in 64 bits (|a_i| below 2^50), rounded once.  The
+ * squares are summed in 32 bits: a head whose squares pass fp32's range comes out as zeros,
+ * or NaN where it holds an infinity.
+ *
+ *   inv_freq : fp32 [rotary / 2]; NULL for rotary 0.  rotary: a multiple of 32, at most
+ *              head_size.
+ *   q_weight, k_weight : [head_size] of weight_dtype (MKV_BF16, MKV_F16 or MKV_F32), 16-byte
+ *              aligned, or NULL: ones.  NULL for norm 0.
+ *   eps      : at least 0, finite.
+ */
+typedef struct mkv_turn {
+  const float* inv_freq;
+  const void* q_weight;
+  const void* k_weight;
+  int32_t rotary;
+  int32_t weight_dtype;
+  float eps;
+  int32_t norm;
+} mkv_turn_t;
+
+/* [tokens, heads, head_size] in, and out; contiguous in the last dimension. */
+typedef struct mkv_head_rows {
+  const void* x;
+  void* out;
+  int64_t token_stride, head_stride;
+  int64_t out_token_stride, out_head_stride;
+  int32_t heads;
+  int32_t reserved;
+} mkv_head_rows_t;
+
+/*
+ * Query and key heads of a step, one launch.
+ *   q, k      : of one dtype, MKV_BF16, MKV_F16 or MKV_F32; head_size 64, 128 or 256.  A row may
+ *               be written where it was read (out = x, equal strides); otherwise no row of an
+ *               output shares memory with another or with an input.
+ *   positions : [tokens] of int32 or int64 (position_bytes 4 or 8); NULL for rotary 0.
+ */
+typedef struct mkv_norm_rotate_desc {
+  mkv_head_rows_t q;
+  mkv_head_rows_t k;
+  mkv_turn_t turn;
+  const void* positions;
+  int64_t tokens;
+  int32_t position_bytes;
+  int32_t head_size;
+  int32_t dtype;
+  int32_t reserved;
+} mkv_norm_rotate_desc_t;
+
+int mkv_norm_rotate(const mkv_norm_rotate_desc_t* desc, void* stream);
+
+/*
+ * A step's projections: query heads normalised and turned as above, key heads too and, with the
+ * values, into their blocks as mkv_store_scaled stores them; one launch.  A token's position is
+ * its place in its request.  Keys are rounded once, from fp32 to their codes.
+ *   q    : heads and rows of the queries; out's rows share no memory with the cache, k, v or,
+ *          unless out = x with equal strides, with q.
+ *   k, v : [tokens, cache heads, head_size], all of q's dtype.
+ * Rows of no request are neither read nor written.
+ */
+typedef struct mkv_store_rotated_desc {
+  mkv_scaled_cache_t cache;
+  mkv_head_rows_t q;
+  mkv_turn_t turn;
+  const void* k;
+  const void* v;
+  int64_t k_token_stride, k_head_stride;
+  int64_t v_token_stride, v_head_stride;
+  const int32_t* block_tables;
+  const int32_t* starts;
+  const int32_t* lens;
+  int32_t* error_flags;
+  int64_t table_stride;
+  int64_t tokens;
+  int32_t table_width;
+  int32_t requests;
+  int32_t dtype;
+  int32_t reserved;
+} mkv_store_rotated_desc_t;
+
+int mkv_store_rotated(const mkv_store_rotated_desc_t* desc, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* MARATHON_KVSTEP_H */

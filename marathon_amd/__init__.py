@@ -21,6 +21,7 @@ from .scaled_cache import (
     step_slots,
     store_scaled,
 )
+from .scaled_step import norm_rotate, store_rotated
 from .shift_kernels import RopeShift, inv_freq_for, rope_shift, scatter_shifted, use_hip, warmup
 from .shift_store import (
     DEFAULT_STORE_TOKENS,
@@ -55,4 +56,6 @@ __all__ = [
     "attend_scaled",
     "step_slots",
     "store_scaled",
+    "norm_rotate",
+    "store_rotated",
 ]

@@ -1,5 +1,5 @@
-"""ctypes binding of ``libmarathon_kvshift.so`` (C ABI: include/marathon_kvshift.h and
-include/marathon_kvscaled.h).
+"""ctypes binding of ``libmarathon_kvshift.so`` (C ABI: include/marathon_kvshift.h,
+include/marathon_kvscaled.h and include/marathon_kvstep.h).
 
 The library is built in-tree by :func:`marathon_amd.build.build_library` and loaded
 from ``marathon_amd/_lib/``.  There is deliberately no fallback: if the library is
@@ -46,7 +46,7 @@ MKV_MAX_HEAD_SIZE = 512
 MKV_DIRECT_MAX_SPANS = 63
 MKV_SMALL_MAX_SPANS = 8
 MKV_SMALL_MAX_INDEX = 64
-MKV_ABI_VERSION = (3 << 16) | 6
+MKV_ABI_VERSION = (3 << 16) | 7
 MKV_ORDER_NONE = 0
 MKV_ORDER_DST_PAGE = 1
 MKV_NOALLOC_SCRATCH_BYTES = 16 << 20
@@ -80,6 +80,8 @@ EXPORTED = (
     "mkv_attend_workspace_size",
     "mkv_scaled_units",
     "mkv_shift_scaled",
+    "mkv_norm_rotate",
+    "mkv_store_rotated",
 )
 
 
@@ -234,6 +236,81 @@ assert ctypes.sizeof(ScaledCacheDesc) == 72 and ctypes.sizeof(AttendDesc) == 216
 assert ctypes.sizeof(ScaledShiftDesc) == 200
 
 
+class Turn(ctypes.Structure):
+    """mkv_turn_t (40 bytes)."""
+
+    _fields_ = [
+        ("inv_freq", ctypes.c_void_p),
+        ("q_weight", ctypes.c_void_p),
+        ("k_weight", ctypes.c_void_p),
+        ("rotary", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("norm", ctypes.c_int32),
+    ]
+
+
+class HeadRows(ctypes.Structure):
+    """mkv_head_rows_t (56 bytes)."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("token_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("out_token_stride", ctypes.c_int64),
+        ("out_head_stride", ctypes.c_int64),
+        ("heads", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class NormRotateDesc(ctypes.Structure):
+    """mkv_norm_rotate_desc_t (184 bytes)."""
+
+    _fields_ = [
+        ("q", HeadRows),
+        ("k", HeadRows),
+        ("turn", Turn),
+        ("positions", ctypes.c_void_p),
+        ("tokens", ctypes.c_int64),
+        ("position_bytes", ctypes.c_int32),
+        ("head_size", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class StoreRotatedDesc(ctypes.Structure):
+    """mkv_store_rotated_desc_t (280 bytes)."""
+
+    _fields_ = [
+        ("cache", ScaledCacheDesc),
+        ("q", HeadRows),
+        ("turn", Turn),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_token_stride", ctypes.c_int64),
+        ("k_head_stride", ctypes.c_int64),
+        ("v_token_stride", ctypes.c_int64),
+        ("v_head_stride", ctypes.c_int64),
+        ("block_tables", ctypes.c_void_p),
+        ("starts", ctypes.c_void_p),
+        ("lens", ctypes.c_void_p),
+        ("error_flags", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        ("table_width", ctypes.c_int32),
+        ("requests", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+assert ctypes.sizeof(Turn) == 40 and ctypes.sizeof(HeadRows) == 56
+assert ctypes.sizeof(NormRotateDesc) == 184 and ctypes.sizeof(StoreRotatedDesc) == 280
+
+
 def unit_words(src_bs: int, dst_bs: int) -> int:
     """MKV_UNIT_WORDS: int32 words of a unit of a block-scaled shift."""
     sources = dst_bs // src_bs + 1 if dst_bs > src_bs else 2
@@ -305,6 +382,12 @@ def _bind_scaled(cdll: ctypes.CDLL) -> ctypes.CDLL:
     f = cdll.mkv_shift_scaled
     f.restype = ctypes.c_int
     f.argtypes = [ctypes.POINTER(ScaledShiftDesc), vp]
+    f = cdll.mkv_norm_rotate
+    f.restype = ctypes.c_int
+    f.argtypes = [ctypes.POINTER(NormRotateDesc), vp]
+    f = cdll.mkv_store_rotated
+    f.restype = ctypes.c_int
+    f.argtypes = [ctypes.POINTER(StoreRotatedDesc), vp]
     return cdll
 
 

@@ -20,8 +20,10 @@ import sysconfig
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 SRC = os.path.join(HERE, "csrc", "kvshift.hip")
-#: The library's sources: the shift path, and the block-scaled cache's kernels.
-SRCS = [SRC, *(os.path.join(HERE, "csrc", n) for n in ("scaled_cache.hip", "scaled_attend.hip"))]
+#: The library's sources: the shift path, the block-scaled cache's kernels, and those of the
+#: step around it.
+SRCS = [SRC, *(os.path.join(HERE, "csrc", n)
+               for n in ("scaled_cache.hip", "scaled_attend.hip", "rotate_heads.hip"))]
 INCLUDE = os.path.join(ROOT, "include")
 OUT_DIR = os.path.join(HERE, "_lib")
 OUT = os.path.join(OUT_DIR, "libmarathon_kvshift.so")

@@ -1,0 +1,667 @@
+// rotate_heads.hip -- query and key heads normalised and turned to their positions for gfx950,
+// for any cache (norm_rotate) and on the way into the block-scaled one (store_rotated).
+//
+// Mathematics.  A head x of D values at position p:
+//     y = x * rsqrt(mean(x^2) + eps) * w
+//     (y_i, y_{i+R/2}) turned by a_i = p * inv_freq_i,  i < R/2
+// in fp32, rounded once.
+//
+// Layout.  Both sums and pairs stay within a few lanes: D / 16 lanes hold a head, each 8 values
+// at a_off and 8 at b_off, the two halves of 8 pairs (behind the first R values: 16 that are
+// not turned).  The sum of squares then takes 2 to 4 exchanges between neighbours by the vector
+// unit (DPP), a pair none, and every access moves 16 bytes a lane.
+//
+// Angles.  cos and sin are the same for all heads of a token, so a wave makes each once, a
+// frequency a lane, and hands them over through LDS.  p * inv_freq is taken in quarter turns
+// in 64 bits (a position of a million times an fp32 frequency loses 16 bits in 32), split
+// into the nearest whole one and what is left, |u| <= 1/2; of that fp32 holds enough, and the
+// Taylor series of sin and cos at u * pi/2 <= pi/4, to the terms of u^11 and u^12, are below
+// fp32's rounding.
+//
+// No matrix work, a dozen operations a value: bound by memory, small calls by their latency.
+
+#include "marathon_kvstep.h"
+#include "scaled_rows.h"
+
+#pragma clang fp contract(off)
+
+namespace {
+
+using namespace mkv_scaled;
+
+struct Turn {
+  const float* inv_freq;
+  const char* weight[2];  // q's, k's; null: ones
+  int32_t half;           // rotary / 2
+  int32_t weight_type;
+  float eps;
+  int32_t norm;
+};
+
+struct HeadRows {
+  const char* x;
+  char* out;
+  int64_t token, head, out_token, out_head;  // bytes
+  int32_t heads;
+};
+
+// Quarter turns of an angle a position, in 64 bits.
+__device__ __forceinline__ double quarters(float inv_freq) {
+  return static_cast<double>(inv_freq) * 0x1.45f306dc9c883p-1;
+}
+
+// (cos, sin) of `q` quarter turns, |q| < 2^51.
+__device__ __forceinline__ f32x2 cos_sin(double q) {
+  // 1.5 * 2^52 leaves no room for a fraction: the sum's last bits are the nearest whole number
+  constexpr double kWhole = 0x1.8p52;
+  const double sum = q + kWhole;
+  const uint32_t quadrant = static_cast<uint32_t>(__builtin_bit_cast(uint64_t, sum));
+  const float u = static_cast<float>(q - (sum - kWhole)), u2 = u * u;
+  // (pi/2)^n / n! with the signs of the series; pi/2 itself in two terms
+  float s = __builtin_fmaf(u2, -0x1.e307500000000p-19f, 0x1.5078340000000p-13f);
+  s = __builtin_fmaf(u2, s, -0x1.32d2cc0000000p-8f);
+  s = __builtin_fmaf(u2, s, 0x1.466bc60000000p-4f);
+  s = __builtin_fmaf(u2, s, -0x1.4abbce0000000p-1f);
+  s = __builtin_fmaf(u2, s, -0x1.777a5c0000000p-25f);
+  s = __builtin_fmaf(u, 0x1.921fb60000000p+0f, u * s);
+  float c = __builtin_fmaf(u2, 0x1.f9d38a0000000p-22f, -0x1.a6d1f20000000p-16f);
+  c = __builtin_fmaf(u2, c, 0x1.e1f5060000000p-11f);
+  c = __builtin_fmaf(u2, c, -0x1.55d3c80000000p-6f);
+  c = __builtin_fmaf(u2, c, 0x1.03c1f00000000p-2f);
+  c = __builtin_fmaf(u2, c, -0x1.3bd3cc0000000p+0f);
+  c = __builtin_fmaf(u2, c, 1.0f);
+  const bool odd = quadrant & 1;
+  const float x = odd ? s : c, y = odd ? c : s;
+  const uint32_t flip = quadrant << 30;  // bit 31: quadrants 2 and 3
+  return f32x2{__uint_as_float(__float_as_uint(x) ^ ((flip ^ (quadrant << 31)) & 0x80000000u)),
+               __uint_as_float(__float_as_uint(y) ^ (flip & 0x80000000u))};
+}
+
+// Where a lane's 16 values of a head lie.
+template <int D>
+struct Place {
+  static constexpr int kLanes = D / 16;         // lanes of a head
+  static constexpr int kHeads = 64 / kLanes;    // heads (or rows) a wave holds at once
+  int a, b;     // first values of the two eights
+  bool turned;
+  __device__ __forceinline__ Place(int piece, int half) {
+    turned = 8 * piece < half;
+    a = turned ? 8 * piece : 16 * piece;  // 2 half + 16 (piece - half / 8)
+    b = turned ? a + half : a + 8;
+  }
+};
+
+// The sum over a head's lanes, in each of them; the order is the same in every lane.
+template <int D>
+__device__ __forceinline__ float head_sum(float x) {
+#define MKV_DPP(ctrl) \
+  x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), ctrl, 0xF, 0xF, true))
+  MKV_DPP(0xB1);   // quad_perm 1 0 3 2
+  MKV_DPP(0x4E);   // quad_perm 2 3 0 1
+  if constexpr (D >= 128) MKV_DPP(0x141);  // row_half_mirror
+  if constexpr (D >= 256) MKV_DPP(0x140);  // row_mirror
+#undef MKV_DPP
+  return x;
+}
+
+// 8 weights; ones where there are none.
+__device__ __forceinline__ void weights8(const char* w, int type, int at, float* x) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = 1.0f;
+  if (w == nullptr) return;
+  if (type == MKV_F32) {
+    const u32x4* p = reinterpret_cast<const u32x4*>(w + 4 * at);
+    unpack8<MKV_F32>(Raw8<MKV_F32>{{p[0], p[1]}}, x);
+  } else {
+    const u32x4 p = *reinterpret_cast<const u32x4*>(w + 2 * at);
+    if (type == MKV_BF16)
+      unpack8<MKV_BF16>(Raw8<MKV_BF16>{{p}}, x);
+    else
+      unpack8<MKV_F16>(Raw8<MKV_F16>{{p}}, x);
+  }
+}
+
+template <int ET>
+__device__ __forceinline__ void put8(char* p, const float* x) {
+  if constexpr (ET == MKV_F32) {
+    reinterpret_cast<u32x4*>(p)[0] = u32x4{__float_as_uint(x[0]), __float_as_uint(x[1]),
+                                           __float_as_uint(x[2]), __float_as_uint(x[3])};
+    reinterpret_cast<u32x4*>(p)[1] = u32x4{__float_as_uint(x[4]), __float_as_uint(x[5]),
+                                           __float_as_uint(x[6]), __float_as_uint(x[7])};
+  } else {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    u32x4 w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (ET == MKV_BF16)
+        w[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x[2 * j], x[2 * j + 1]}), b2));
+      else
+        w[j] = __builtin_bit_cast(uint32_t, h2{static_cast<_Float16>(x[2 * j]), static_cast<_Float16>(x[2 * j + 1])});
+    }
+    *reinterpret_cast<u32x4*>(p) = w;
+  }
+}
+
+// A lane's 16 values of a head: normalised and weighted, then the pairs turned.
+template <int D>
+__device__ __forceinline__ void normalise(float* x, const float* w, const Turn& t) {
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) sum = __builtin_fmaf(x[i], x[i], sum);
+  const float r = rsqrtf(__builtin_fmaf(head_sum<D>(sum), 1.0f / D, t.eps));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = x[i] * r * w[i];
+}
+
+__device__ __forceinline__ void rotate(float* x, const f32x2* turn) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float a = x[i], b = x[8 + i], c = turn[i][0], s = turn[i][1];
+    x[i] = __builtin_fmaf(a, c, -(b * s));
+    x[8 + i] = __builtin_fmaf(b, c, a * s);
+  }
+}
+
+// The (cos, sin) of a lane's 8 pairs.
+template <int D>
+__device__ __forceinline__ void turns8(const f32x2* lds, const Place<D>& place, f32x2* turn) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) turn[i] = place.turned ? lds[place.a + i] : f32x2{1.0f, 0.0f};
+}
+
+// LDS that only this wave touches: its stores are done before its loads behind this.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// The heads [h0, h1) of one token and side, by one wave: the next heads' loads are in flight
+// while these are worked on.  `angles` makes the wave's (cos, sin) in LDS, once the first are.
+template <int ET, int D, typename F>
+__device__ __forceinline__ void turn_heads(const HeadRows& rows, const Turn& t, int side,
+                                           int64_t token, int h0, int h1, const f32x2* lds,
+                                           F angles) {
+  constexpr int kBytes = ET == MKV_F32 ? 4 : 2, kHeads = Place<D>::kHeads;
+  const int lane = threadIdx.x & 63, sub = lane / Place<D>::kLanes;
+  const Place<D> place(lane % Place<D>::kLanes, t.half);
+  const char* in = rows.x + token * rows.token;
+  char* out = rows.out + token * rows.out_token;
+  Raw8<ET> a{}, b{};
+  const auto fetch = [&](int h) {
+    const char* at = in + h * rows.head;
+    a = fetch8<ET>(at + place.a * kBytes);
+    b = fetch8<ET>(at + place.b * kBytes);
+  };
+  int h = h0 + sub;
+  if (h < h1) fetch(h);
+  float w[16];
+  if (t.norm) {
+    weights8(t.weight[side], t.weight_type, place.a, w);
+    weights8(t.weight[side], t.weight_type, place.b, w + 8);
+  }
+  angles();
+  f32x2 turn[8];
+  turns8(lds, place, turn);
+  for (int first = h0; first < h1; first += kHeads, h += kHeads) {
+    float x[16];
+    unpack8<ET>(a, x);
+    unpack8<ET>(b, x + 8);
+    if (h + kHeads < h1) fetch(h + kHeads);
+    if (t.norm) normalise<D>(x, w, t);
+    if (t.half > 0) rotate(x, turn);
+    if (h < h1) {
+      put8<ET>(out + h * rows.out_head + place.a * kBytes, x);
+      put8<ET>(out + h * rows.out_head + place.b * kBytes, x + 8);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------- norm and rotate
+
+struct RotateParams {
+  HeadRows side[2];  // q, k
+  Turn turn;
+  const void* positions;
+  int64_t tokens;
+  int32_t wide;      // positions of 64 bits
+  int32_t each;      // heads of a side that a wave takes
+  int32_t parts[2];  // waves of a side
+};
+
+constexpr int kWaves = 4;
+
+// A wave takes `each` heads of a token's queries or of its keys.
+template <int ET, int D>
+__global__ __launch_bounds__(64 * kWaves) void norm_rotate_kernel(RotateParams p) {
+  __shared__ f32x2 s_turn[kWaves][D / 2];
+  const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);
+  const int all = p.parts[0] + p.parts[1];
+  const uint32_t unit = blockIdx.x * kWaves + wave;
+  const int64_t token = unit / all;
+  if (token >= p.tokens) return;
+  int part = unit % all;
+  const int side = part >= p.parts[0];
+  if (side) part -= p.parts[0];
+  const HeadRows rows = side ? p.side[1] : p.side[0];
+  const int h0 = part * p.each, h1 = min(h0 + p.each, rows.heads);
+  f32x2* lds = s_turn[wave];
+  turn_heads<ET, D>(rows, p.turn, side, token, h0, h1, lds, [&]() {
+    if (p.turn.half == 0) return;
+    const double at = p.wide ? static_cast<double>(static_cast<const int64_t*>(p.positions)[token])
+                             : static_cast<double>(static_cast<const int32_t*>(p.positions)[token]);
+    for (int f = lane; f < p.turn.half; f += 64) lds[f] = cos_sin(at * quarters(p.turn.inv_freq[f]));
+    wave_fence();
+  });
+}
+
+// ------------------------------------------------------------- into the block-scaled cache
+
+struct PutParams {
+  DevCache c;
+  DevStep s;
+  HeadRows q;
+  Turn turn;
+  const char* k;
+  const char* v;
+  int64_t k_token, k_head, v_token, v_head;  // bytes
+  int64_t tokens;
+  int32_t group;   // tokens a workgroup looks through
+  int32_t planes;  // of the grid's y that store keys and values; those behind them turn queries
+  int32_t each;    // query heads that a wave takes
+};
+
+constexpr int kMaxWaves = 8;
+
+// Keys and values: a workgroup's waves take `heads_here` heads of the blocks that begin, for
+// their request and step, among `group` consecutive tokens, 16 rows of a block and head a wave,
+// as the cache's plain store does.  The block's angles are made by all of its waves together.
+template <int ET, int D>
+__device__ __forceinline__ void put_keys(const PutParams& p, f32x2* s_turn, uint32_t (*s_max)[2]) {
+  using R = Rows<D>;
+  constexpr int P = R::kPasses, kBytes = ET == MKV_F32 ? 4 : 2;
+  const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);
+  const int bs = 1 << p.c.bs_shift, parts = bs >> 4;
+  const int heads_here = (blockDim.x >> 6) / parts;
+  const int head = blockIdx.y * heads_here + wave / parts, part = wave % parts;
+  const bool active = head < p.c.heads;
+  const int piece = lane % R::kChunks, sub = lane / R::kChunks;
+  const Place<D> place(piece, p.turn.half);
+  const int half = p.turn.half;
+  if (blockIdx.x == 0 && blockIdx.y == 0) check_starts(p.s, p.tokens, true);
+  float w[16];
+  if (p.turn.norm) {
+    weights8(p.turn.weight[1], p.turn.weight_type, place.a, w);
+    weights8(p.turn.weight[1], p.turn.weight_type, place.b, w + 8);
+  }
+  int64_t t = static_cast<int64_t>(blockIdx.x) * p.group;
+  const int64_t end = min(t + p.group, p.tokens);
+  while (t < end) {  // the same steps in every wave of the workgroup
+    const int32_t* starts = p.s.starts;
+    const int r = last_at_most(p.s.requests, t, [starts](int i) { return starts[i]; });
+    if (r < 0) {  // before the first request
+      const int64_t first = p.s.requests > 0 ? starts[0] : end;
+      t = first > t ? first : end;
+      continue;
+    }
+    const int64_t s0 = starts[r], s1 = starts[r + 1];
+    if (t < s0 || t >= s1) break;  // behind the last request, or starts that descend
+    const int64_t first_pos = p.s.lens[r] - (s1 - s0);
+    const int64_t pos = first_pos + (t - s0);
+    if (s0 < 0 || s1 > p.tokens || first_pos < 0) {  // flagged by the first workgroup
+      t = s1;
+      continue;
+    }
+    const int off = static_cast<int>(pos & (bs - 1)), base = static_cast<int>(pos) - off;
+    if (t != s0 && off != 0) {  // a block that an earlier token leads
+      t = min(t + bs - off, s1);
+      continue;
+    }
+    const int n = static_cast<int>(min(static_cast<int64_t>(bs - off), s1 - t));
+    const int64_t col = pos >> p.c.bs_shift;
+    int64_t id = -1;
+    if (col < p.s.table_width) id = p.s.tables[r * p.s.table_stride + col];
+    if (id < 0 || id >= p.c.num_blocks) {
+      if (lane == 0 && wave == 0) raise(p.s.flags, MKV_FLAG_DST_RANGE);
+      t += n;
+      continue;
+    }
+    // this wave's new rows of the block
+    Raw8<ET> ka[P], kb[P], va[P], vb[P];
+#pragma unroll
+    for (int u = 0; u < P; ++u) {
+      const int row = part * 16 + u * R::kPerPass + sub;
+      const bool fresh = active && row >= off && row < off + n;
+      ka[u] = kb[u] = va[u] = vb[u] = Raw8<ET>{};
+      if (fresh) {
+        const int64_t at = t + row - off;
+        const char* k = p.k + at * p.k_token + head * p.k_head;
+        const char* v = p.v + at * p.v_token + head * p.v_head + piece * 16 * kBytes;
+        ka[u] = fetch8<ET>(k + place.a * kBytes);
+        kb[u] = fetch8<ET>(k + place.b * kBytes);
+        va[u] = fetch8<ET>(v);
+        vb[u] = fetch8<ET>(v + 8 * kBytes);
+      }
+    }
+    if (half > 0) {
+      __syncthreads();  // the last block's have been read
+      for (int f = lane; f < half; f += 64) {
+        const double each = quarters(p.turn.inv_freq[f]);
+        for (int row = off + wave; row < off + n; row += blockDim.x >> 6)
+          s_turn[row * half + f] = cos_sin(static_cast<double>(base + row) * each);
+      }
+      __syncthreads();
+    }
+    uint8_t* scale = p.c.scales + (id * p.c.heads + head) * 2;
+    const int64_t block = id * p.c.bstride + head * static_cast<int64_t>(p.c.hstride);
+    const int old = active && off > 0 ? *reinterpret_cast<const uint16_t*>(scale) : 0;
+    // rows [0, off) stay, under the larger scale
+    const auto keep = [&](char* at, int was, int e) {
+      if (e <= was) return;
+#pragma unroll
+      for (int u = 0; u < P; ++u) {
+        const int row = part * 16 + u * R::kPerPass + sub;
+        if (row >= off) continue;
+        u32x4* codes = reinterpret_cast<u32x4*>(at + row * p.c.tstride + piece * 16);
+        float x[16];
+        decode16(*codes, 1.0f, x);
+        *codes = encode16(x, min(e - was, 100), true);
+      }
+    };
+    int ek, ev;
+    {
+      float x[P][16];
+#pragma unroll
+      for (int u = 0; u < P; ++u) {
+        const int row = part * 16 + u * R::kPerPass + sub;
+        unpack8<ET>(ka[u], x[u]);
+        unpack8<ET>(kb[u], x[u] + 8);
+        if (p.turn.norm) normalise<D>(x[u], w, p.turn);
+        if (half > 0) {
+          f32x2 turn[8];
+          turns8(s_turn + row * half, place, turn);
+          rotate(x[u], turn);
+        }
+        if (!(active && row >= off && row < off + n)) {  // (eps 0 makes NaNs of no row at all)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[u][i] = 0.0f;
+        }
+      }
+      const Largest most = across(largest<16 * P>(x[0]), parts, s_max, wave);
+      ek = exponent_for(most.bits);
+      if (active) {
+        char* to = p.c.k + block;
+        if (off > 0) {
+          const int was = scale_exp(old & 0xFF);
+          keep(to, was, ek);
+          ek = max(ek, was);
+        }
+        // Neighbours exchange eights, so that each holds 16 values in a row: a lane of even
+        // number its own first eight and its neighbour's, one of odd number the second ones.
+        const bool odd = piece & 1;
+        const int at = place.turned && odd ? place.b - 8 : place.a;
+#pragma unroll
+        for (int u = 0; u < P; ++u) {
+          const int row = part * 16 + u * R::kPerPass + sub;
+          const auto other = [](uint32_t c) {
+            return static_cast<uint32_t>(
+                __builtin_amdgcn_update_dpp(0, static_cast<int>(c), 0xB1, 0xF, 0xF, true));
+          };
+          u32x4 c = encode16(x[u], ek, most.wild);
+          const uint32_t g0 = other(odd ? c[0] : c[2]), g1 = other(odd ? c[1] : c[3]);
+          if (place.turned) c = odd ? u32x4{g0, g1, c[2], c[3]} : u32x4{c[0], c[1], g0, g1};
+          if (row >= off && row < off + n)
+            __builtin_nontemporal_store(c, reinterpret_cast<u32x4*>(to + row * p.c.tstride + at));
+        }
+      }
+    }
+    {
+      float x[P][16];
+#pragma unroll
+      for (int u = 0; u < P; ++u) {
+        unpack8<ET>(va[u], x[u]);
+        unpack8<ET>(vb[u], x[u] + 8);
+      }
+      const Largest most = across(largest<16 * P>(x[0]), parts, s_max, wave);
+      ev = exponent_for(most.bits);
+      if (active) {
+        char* to = p.c.v + block;
+        if (off > 0) {
+          const int was = scale_exp(old >> 8);
+          keep(to, was, ev);
+          ev = max(ev, was);
+        }
+#pragma unroll
+        for (int u = 0; u < P; ++u) {
+          const int row = part * 16 + u * R::kPerPass + sub;
+          const u32x4 c = encode16(x[u], ev, most.wild);
+          if (row >= off && row < off + n)
+            __builtin_nontemporal_store(c, reinterpret_cast<u32x4*>(to + row * p.c.tstride + piece * 16));
+        }
+      }
+    }
+    if (parts > 1) __syncthreads();  // every wave has read the old scale
+    if (active && part == 0 && lane == 0)
+      *reinterpret_cast<uint16_t*>(scale) = static_cast<uint16_t>((ek + 127) | ((ev + 127) << 8));
+    t += n;
+  }
+}
+
+// Queries: the waves of a workgroup, and of the planes beside it, take turns at the tokens and
+// at their heads, `each` at a time.
+template <int ET, int D>
+__device__ __forceinline__ void put_queries(const PutParams& p, f32x2* s_turn) {
+  const int lane = threadIdx.x & 63, waves = blockDim.x >> 6, wave = uni(threadIdx.x >> 6);
+  const int slices = (p.q.heads + p.each - 1) / p.each;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.group;
+  const int here = static_cast<int>(min(static_cast<int64_t>(p.group), p.tokens - t0));
+  f32x2* lds = s_turn + wave * p.turn.half;
+  for (int i = (blockIdx.y - p.planes) * waves + wave; i < here * slices;
+       i += (gridDim.y - p.planes) * waves) {
+    const int64_t t = t0 + i / slices;
+    const int h0 = i % slices * p.each;
+    const int32_t* starts = p.s.starts;
+    const int r = last_at_most(p.s.requests, t, [starts](int j) { return starts[j]; });
+    if (r < 0) continue;
+    const int64_t s0 = starts[r], s1 = starts[r + 1];
+    const int64_t first_pos = p.s.lens[r] - (s1 - s0);
+    if (s0 < 0 || t < s0 || t >= s1 || s1 > p.tokens || first_pos < 0) continue;
+    turn_heads<ET, D>(p.q, p.turn, 0, t, h0, min(h0 + p.each, p.q.heads), lds, [&]() {
+      if (p.turn.half == 0) return;
+      const double at = static_cast<double>(first_pos + (t - s0));
+      wave_fence();  // the last token's have been read
+      for (int f = lane; f < p.turn.half; f += 64) lds[f] = cos_sin(at * quarters(p.turn.inv_freq[f]));
+      wave_fence();
+    });
+  }
+}
+
+template <int ET, int D>
+__global__ __launch_bounds__(64 * kMaxWaves) void put_kernel(PutParams p) {
+  extern __shared__ f32x2 s_turn[];  // [block size][half]: at least as many rows as waves
+  __shared__ uint32_t s_max[kMaxWaves][2];
+  if (static_cast<int>(blockIdx.y) < p.planes)
+    put_keys<ET, D>(p, s_turn, s_max);
+  else
+    put_queries<ET, D>(p, s_turn);
+}
+
+// ------------------------------------------------------------------------- host
+
+int check_turn(const char* who, const mkv_turn_t& t, int32_t head_size, Turn* out) {
+  if (t.rotary < 0 || t.rotary > head_size || t.rotary % 32 != 0)
+    return mkv_fail(MKV_ERR_ARG, "%s: rotary %d is not a multiple of 32 up to %d", who, t.rotary,
+                    head_size);
+  if (t.rotary > 0 && t.inv_freq == nullptr)
+    return mkv_fail(MKV_ERR_ARG, "%s: inv_freq is NULL", who);
+  if ((reinterpret_cast<uintptr_t>(t.inv_freq) & 3) != 0)
+    return mkv_fail(MKV_ERR_ALIGN, "%s: inv_freq is not 4-byte aligned", who);
+  if (t.norm && !(t.eps >= 0.0f && t.eps < __builtin_inff()))
+    return mkv_fail(MKV_ERR_ARG, "%s: eps %g", who, t.eps);
+  const bool weighted = t.q_weight != nullptr || t.k_weight != nullptr;
+  if (weighted && !t.norm) return mkv_fail(MKV_ERR_ARG, "%s: weights without a norm", who);
+  if (weighted && t.weight_dtype != MKV_BF16 && t.weight_dtype != MKV_F16 && t.weight_dtype != MKV_F32)
+    return mkv_fail(MKV_ERR_DTYPE, "%s: weight dtype %d is not bf16, fp16 or fp32", who,
+                    t.weight_dtype);
+  if (((reinterpret_cast<uintptr_t>(t.q_weight) | reinterpret_cast<uintptr_t>(t.k_weight)) & 15) != 0)
+    return mkv_fail(MKV_ERR_ALIGN, "%s: a weight is not 16-byte aligned", who);
+  out->inv_freq = t.inv_freq;
+  out->weight[0] = static_cast<const char*>(t.q_weight);
+  out->weight[1] = static_cast<const char*>(t.k_weight);
+  out->half = t.rotary / 2;
+  out->weight_type = t.weight_dtype;
+  out->eps = t.eps;
+  out->norm = t.norm != 0;
+  return MKV_OK;
+}
+
+// The rows that are read and written; those written lie apart.
+int check_rows(const char* who, const char* name, const mkv_head_rows_t& r, int64_t tokens,
+               int32_t head_size, int64_t eb, HeadRows* out) {
+  if (r.heads < 0 || r.heads > 65536)
+    return mkv_fail(MKV_ERR_ARG, "%s: %d heads of %s", who, r.heads, name);
+  const int64_t most = INT64_MAX / 64 / (tokens + r.heads + 1);
+  for (const int64_t s : {r.token_stride, r.head_stride, r.out_token_stride, r.out_head_stride})
+    if (s < 0 || s > most) return mkv_fail(MKV_ERR_ARG, "%s: a stride of %s is out of range", who, name);
+  *out = HeadRows{static_cast<const char*>(r.x), static_cast<char*>(r.out), r.token_stride * eb,
+                  r.head_stride * eb, r.out_token_stride * eb, r.out_head_stride * eb, r.heads};
+  if (tokens == 0 || r.heads == 0) return MKV_OK;
+  if (r.x == nullptr || r.out == nullptr) return mkv_fail(MKV_ERR_ARG, "%s: %s is NULL", who, name);
+  if (((reinterpret_cast<uintptr_t>(r.x) | reinterpret_cast<uintptr_t>(r.out) | out->token |
+        out->head | out->out_token | out->out_head) & 15) != 0)
+    return mkv_fail(MKV_ERR_ALIGN, "%s: %s is not 16-byte aligned", who, name);
+  // the smaller stride passes a row, the larger one all that the smaller reaches
+  const bool heads_first = r.out_head_stride <= r.out_token_stride;
+  int64_t reach = head_size;
+  for (const bool heads : {heads_first, !heads_first}) {
+    const int64_t n = heads ? r.heads : tokens, step = heads ? r.out_head_stride : r.out_token_stride;
+    if (n > 1 && step < reach) return mkv_fail(MKV_ERR_ARG, "%s: the rows of %s overlap", who, name);
+    reach += step * (n - 1);
+  }
+  return MKV_OK;
+}
+
+template <int ET>
+void rotate_launch(int d, dim3 grid, const RotateParams& p, hipStream_t s) {
+  if (d == 64)
+    norm_rotate_kernel<ET, 64><<<grid, 64 * kWaves, 0, s>>>(p);
+  else if (d == 128)
+    norm_rotate_kernel<ET, 128><<<grid, 64 * kWaves, 0, s>>>(p);
+  else
+    norm_rotate_kernel<ET, 256><<<grid, 64 * kWaves, 0, s>>>(p);
+}
+
+template <int ET>
+int put_launch(int d, dim3 grid, int threads, int lds, const PutParams& p, hipStream_t s) {
+  void (*kernel)(PutParams) =
+      d == 64 ? put_kernel<ET, 64> : d == 128 ? put_kernel<ET, 128> : put_kernel<ET, 256>;
+  if (lds > 65536) {  // heads of 256 in blocks of 128: more than a launch has unasked
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess)
+      return mkv_fail(MKV_ERR_HIP, "mkv_store_rotated: %d bytes of LDS: %s", lds, hipGetErrorString(e));
+  }
+  kernel<<<grid, threads, lds, s>>>(p);
+  return launched("mkv_store_rotated");
+}
+
+}  // namespace
+
+extern "C" int mkv_norm_rotate(const mkv_norm_rotate_desc_t* d, void* stream) {
+  const char* who = "mkv_norm_rotate";
+  if (d == nullptr) return mkv_fail(MKV_ERR_ARG, "%s: desc is NULL", who);
+  if (d->head_size != 64 && d->head_size != 128 && d->head_size != 256)
+    return mkv_fail(MKV_ERR_UNSUPPORTED, "%s: head_size %d is not 64, 128 or 256", who, d->head_size);
+  if (d->dtype != MKV_BF16 && d->dtype != MKV_F16 && d->dtype != MKV_F32)
+    return mkv_fail(MKV_ERR_DTYPE, "%s: dtype %d is not bf16, fp16 or fp32", who, d->dtype);
+  if (d->tokens < 0 || d->tokens > INT32_MAX)
+    return mkv_fail(MKV_ERR_ARG, "%s: tokens %lld", who, (long long)d->tokens);
+  RotateParams p;
+  const int64_t eb = d->dtype == MKV_F32 ? 4 : 2;
+  int rc = check_turn(who, d->turn, d->head_size, &p.turn);
+  if (rc == MKV_OK) rc = check_rows(who, "q", d->q, d->tokens, d->head_size, eb, &p.side[0]);
+  if (rc == MKV_OK) rc = check_rows(who, "k", d->k, d->tokens, d->head_size, eb, &p.side[1]);
+  if (rc != MKV_OK) return rc;
+  if (d->tokens == 0 || d->q.heads + d->k.heads == 0) return MKV_OK;
+  if (d->turn.rotary > 0) {
+    if (d->positions == nullptr) return mkv_fail(MKV_ERR_ARG, "%s: positions is NULL", who);
+    if (d->position_bytes != 4 && d->position_bytes != 8)
+      return mkv_fail(MKV_ERR_ARG, "%s: positions of %d bytes", who, d->position_bytes);
+    if ((reinterpret_cast<uintptr_t>(d->positions) & (d->position_bytes - 1)) != 0)
+      return mkv_fail(MKV_ERR_ALIGN, "%s: positions are not aligned", who);
+  }
+  p.positions = d->positions;
+  p.wide = d->position_bytes == 8;
+  p.tokens = d->tokens;
+  const int at_once = 64 / (d->head_size / 16);
+  const int passes = d->tokens * (d->q.heads + d->k.heads) / at_once >= 8192 ? 4 : 1;
+  p.each = at_once * passes;
+  for (int i = 0; i < 2; ++i) p.parts[i] = (p.side[i].heads + p.each - 1) / p.each;
+  const int64_t waves = d->tokens * (p.parts[0] + p.parts[1]);
+  if (waves > UINT32_MAX / 64)
+    return mkv_fail(MKV_ERR_UNSUPPORTED, "%s: %lld tokens", who, (long long)d->tokens);
+  const dim3 grid(static_cast<unsigned>((waves + kWaves - 1) / kWaves));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (d->dtype == MKV_BF16)
+    rotate_launch<MKV_BF16>(d->head_size, grid, p, s);
+  else if (d->dtype == MKV_F16)
+    rotate_launch<MKV_F16>(d->head_size, grid, p, s);
+  else
+    rotate_launch<MKV_F32>(d->head_size, grid, p, s);
+  return launched(who);
+}
+
+extern "C" int mkv_store_rotated(const mkv_store_rotated_desc_t* d, void* stream) {
+  const char* who = "mkv_store_rotated";
+  if (d == nullptr) return mkv_fail(MKV_ERR_ARG, "%s: desc is NULL", who);
+  PutParams p;
+  const mkv_scaled_cache_t& c = d->cache;
+  int rc = check_cache(who, c, true, &p.c);
+  if (rc == MKV_OK)
+    rc = check_step(who, c.block_size, d->block_tables, d->table_stride, d->table_width, d->starts,
+                    d->lens, d->requests, d->error_flags, &p.s);
+  if (rc != MKV_OK) return rc;
+  if (d->dtype != MKV_BF16 && d->dtype != MKV_F16 && d->dtype != MKV_F32)
+    return mkv_fail(MKV_ERR_DTYPE, "%s: dtype %d is not bf16, fp16 or fp32", who, d->dtype);
+  if (d->tokens < 0 || d->tokens > INT32_MAX)
+    return mkv_fail(MKV_ERR_ARG, "%s: tokens %lld", who, (long long)d->tokens);
+  const int64_t eb = d->dtype == MKV_F32 ? 4 : 2;
+  rc = check_turn(who, d->turn, c.head_size, &p.turn);
+  if (rc == MKV_OK) rc = check_rows(who, "q", d->q, d->tokens, c.head_size, eb, &p.q);
+  if (rc != MKV_OK) return rc;
+  if (d->tokens == 0 || d->requests == 0) return MKV_OK;
+  if (d->k == nullptr || d->v == nullptr) return mkv_fail(MKV_ERR_ARG, "%s: k or v is NULL", who);
+  const int64_t most = INT64_MAX / 16 / (d->tokens + c.heads);
+  for (const int64_t s : {d->k_token_stride, d->k_head_stride, d->v_token_stride, d->v_head_stride})
+    if (s < 0 || s > most)
+      return mkv_fail(MKV_ERR_ARG, "%s: a stride of k or v is out of range", who);
+  p.k = static_cast<const char*>(d->k);
+  p.v = static_cast<const char*>(d->v);
+  p.k_token = d->k_token_stride * eb;
+  p.k_head = d->k_head_stride * eb;
+  p.v_token = d->v_token_stride * eb;
+  p.v_head = d->v_head_stride * eb;
+  if (((reinterpret_cast<uintptr_t>(d->k) | reinterpret_cast<uintptr_t>(d->v) | p.k_token |
+        p.k_head | p.v_token | p.v_head) & 15) != 0)
+    return mkv_fail(MKV_ERR_ALIGN, "%s: k or v is not 16-byte aligned", who);
+  p.tokens = d->tokens;
+  const int parts = c.block_size / 16;
+  const int heads_here = 4 / parts < 1 ? 1 : c.heads < 4 / parts ? c.heads : 4 / parts;
+  const int waves = parts * heads_here;
+  p.planes = (c.heads + heads_here - 1) / heads_here;
+  const int64_t each = d->tokens * p.planes, ahead = d->tokens / d->requests;
+  p.group = ahead < 16 || each <= 4096 ? (each <= 4096 ? 1 : 4) : each > 12288 ? c.block_size : 4;
+  const int at_once = 64 / (c.head_size / 16);
+  p.each = at_once * (d->tokens * d->q.heads / at_once >= 8192 ? 4 : 1);
+  const int slices = (d->q.heads + p.each - 1) / p.each;
+  const int q_planes = (p.group * slices + waves * 4 - 1) / (waves * 4);
+  if ((d->tokens + p.group - 1) / p.group > UINT32_MAX / (64 * waves) || p.planes + q_planes > 65535)
+    return mkv_fail(MKV_ERR_UNSUPPORTED, "%s: %lld tokens", who, (long long)d->tokens);
+  const dim3 grid(static_cast<unsigned>((d->tokens + p.group - 1) / p.group),
+                  static_cast<unsigned>(p.planes + q_planes));
+  const int lds = c.block_size * p.turn.half * 8;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (d->dtype == MKV_BF16) return put_launch<MKV_BF16>(c.head_size, grid, 64 * waves, lds, p, s);
+  if (d->dtype == MKV_F16) return put_launch<MKV_F16>(c.head_size, grid, 64 * waves, lds, p, s);
+  return put_launch<MKV_F32>(c.head_size, grid, 64 * waves, lds, p, s);
+}
