@@ -110,6 +110,38 @@ typedef struct mkv_store_rotated_desc {
 
 int mkv_store_rotated(const mkv_store_rotated_desc_t* desc, void* stream);
 
+/*
+ * mkv_attend_scaled for a batch whose requests begin, in groups, with the same cached tokens.
+ *   groups : int32 [n_groups + 1], 0 <= n_groups <= MKV_MAX_REQUESTS: requests [groups[g],
+ *            groups[g + 1]) begin alike; groups[0] >= 0, not descending.  A request in no group
+ *            shares nothing.
+ *   shared : int32 [n_groups]: how many tokens; of them the whole blocks, shared[g] / block_size,
+ *            are read through block_tables' row groups[g] for the whole group, and its other
+ *            requests' entries for them are not read.  A row sees of them what stands before it.
+ *   attend : as mkv_attend_scaled takes it, but for
+ *            max_len    the most tokens that a request has behind what its group shares (0: not
+ *                       known), and
+ *            workspace  mkv_attend_shared_workspace_size() bytes.
+ *   max_shared : the most tokens that a group shares, where the caller knows it (0: not known).
+ * Where the tables of a group agree, the result is mkv_attend_scaled's but for the order of sums
+ * and p's roundings: over what is shared p is held in one bf16 term (off by 2^-8) where bf16
+ * queries take the kernel of more than 32 rows, here by the rows of a group.
+ * Groups that leave the requests or descend, and shared tokens below zero, raise MKV_FLAG_SPAN
+ * and share nothing; more shared tokens than a table has raise MKV_FLAG_SRC_RANGE, and are cut.
+ */
+typedef struct mkv_attend_shared_desc {
+  mkv_attend_desc_t attend;
+  const int32_t* groups;
+  const int32_t* shared;
+  int32_t n_groups;
+  int32_t max_shared;
+} mkv_attend_shared_desc_t;
+
+int mkv_attend_shared(const mkv_attend_shared_desc_t* desc, void* stream);
+
+/* Workspace bytes of that call (it reads no device memory); -1 where it would be refused. */
+int64_t mkv_attend_shared_workspace_size(const mkv_attend_shared_desc_t* desc);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,7 +21,7 @@ from .scaled_cache import (
     step_slots,
     store_scaled,
 )
-from .scaled_step import norm_rotate, store_rotated
+from .scaled_step import attend_shared, norm_rotate, store_rotated
 from .shift_kernels import RopeShift, inv_freq_for, rope_shift, scatter_shifted, use_hip, warmup
 from .shift_store import (
     DEFAULT_STORE_TOKENS,
@@ -58,4 +58,5 @@ __all__ = [
     "store_scaled",
     "norm_rotate",
     "store_rotated",
+    "attend_shared",
 ]

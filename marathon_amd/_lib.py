@@ -82,6 +82,8 @@ EXPORTED = (
     "mkv_shift_scaled",
     "mkv_norm_rotate",
     "mkv_store_rotated",
+    "mkv_attend_shared",
+    "mkv_attend_shared_workspace_size",
 )
 
 
@@ -307,6 +309,19 @@ class StoreRotatedDesc(ctypes.Structure):
     ]
 
 
+class AttendSharedDesc(ctypes.Structure):
+    """mkv_attend_shared_desc_t (240 bytes)."""
+
+    _fields_ = [
+        ("attend", AttendDesc),
+        ("groups", ctypes.c_void_p),
+        ("shared", ctypes.c_void_p),
+        ("n_groups", ctypes.c_int32),
+        ("max_shared", ctypes.c_int32),
+    ]
+
+
+assert ctypes.sizeof(AttendSharedDesc) == 240
 assert ctypes.sizeof(Turn) == 40 and ctypes.sizeof(HeadRows) == 56
 assert ctypes.sizeof(NormRotateDesc) == 184 and ctypes.sizeof(StoreRotatedDesc) == 280
 
@@ -388,6 +403,12 @@ def _bind_scaled(cdll: ctypes.CDLL) -> ctypes.CDLL:
     f = cdll.mkv_store_rotated
     f.restype = ctypes.c_int
     f.argtypes = [ctypes.POINTER(StoreRotatedDesc), vp]
+    f = cdll.mkv_attend_shared
+    f.restype = ctypes.c_int
+    f.argtypes = [ctypes.POINTER(AttendSharedDesc), vp]
+    f = cdll.mkv_attend_shared_workspace_size
+    f.restype = ctypes.c_int64
+    f.argtypes = [ctypes.POINTER(AttendSharedDesc)]
     return cdll
 
 

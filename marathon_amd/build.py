@@ -23,7 +23,8 @@ SRC = os.path.join(HERE, "csrc", "kvshift.hip")
 #: The library's sources: the shift path, the block-scaled cache's kernels, and those of the
 #: step around it.
 SRCS = [SRC, *(os.path.join(HERE, "csrc", n)
-               for n in ("scaled_cache.hip", "scaled_attend.hip", "rotate_heads.hip"))]
+               for n in ("scaled_cache.hip", "scaled_attend.hip", "rotate_heads.hip",
+                         "shared_attend.hip"))]
 INCLUDE = os.path.join(ROOT, "include")
 OUT_DIR = os.path.join(HERE, "_lib")
 OUT = os.path.join(OUT_DIR, "libmarathon_kvshift.so")

@@ -331,6 +331,22 @@ def attend_scaled(cache: ScaledCache, q: torch.Tensor, block_tables: torch.Tenso
         if type(got) is int:
             _lib.check(got)
         return got
+    desc, out = _attend_desc("attend_scaled", cache, q, block_tables, starts, lens, softmax_scale,
+                             max_new, max_len, out, error_flags)
+    device = cache.device
+    L = _lib.lib()
+    need = L.mkv_attend_workspace_size(ctypes.byref(desc))
+    with _on(device, _current(device)):
+        if need > 0:  # the allocator hands it on in stream order
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+            desc.workspace, desc.workspace_bytes = workspace.data_ptr(), need
+        _lib.check(L.mkv_attend_scaled(ctypes.byref(desc), current_stream(device)))
+    return out
+
+
+def _attend_desc(who: str, cache: ScaledCache, q, block_tables, starts, lens, softmax_scale, max_new,
+                 max_len, out, error_flags) -> tuple[_lib.AttendDesc, torch.Tensor]:
+    """An attention call's descriptor, but for its workspace, and its output."""
     device, d = cache.device, cache.head_size
     if q.dim() != 3 or q.shape[2] != d or q.shape[1] == 0 or q.shape[1] % cache.heads:
         raise ValueError(f"q {tuple(q.shape)}: [tokens, a multiple of {cache.heads}, {d}]")
@@ -338,7 +354,7 @@ def attend_scaled(cache: ScaledCache, q: torch.Tensor, block_tables: torch.Tenso
         raise TypeError(f"q {q.dtype}: one of {_QUERY_DTYPES}")
     if q.device != device:
         raise ValueError(f"q on {q.device}, the cache on {device}")
-    _no_gradient("attend_scaled", q=q, out=out)
+    _no_gradient(who, q=q, out=out)
     if q.stride(2) != 1:
         raise ValueError("q's rows must be contiguous in the last dimension")
     if out is None:
@@ -364,14 +380,7 @@ def attend_scaled(cache: ScaledCache, q: torch.Tensor, block_tables: torch.Tenso
     # (no request has more than 2^31 - 1 tokens, whatever the hints say)
     desc.max_new, desc.max_len = (max(-1, min(int(m or 0), 2**31 - 1)) for m in (max_new, max_len))
     desc.softmax_scale = d ** -0.5 if softmax_scale is None else float(softmax_scale)
-    L = _lib.lib()
-    need = L.mkv_attend_workspace_size(ctypes.byref(desc))
-    with _on(device, _current(device)):
-        if need > 0:  # the allocator hands it on in stream order
-            workspace = torch.empty(need, dtype=torch.uint8, device=device)
-            desc.workspace, desc.workspace_bytes = workspace.data_ptr(), need
-        _lib.check(L.mkv_attend_scaled(ctypes.byref(desc), current_stream(device)))
-    return out
+    return desc, out
 
 
 class ScaledShifts:

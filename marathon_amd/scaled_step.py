@@ -4,7 +4,10 @@
   each value) and turned to its token's position, in one pass; for a cache of any type;
 * :func:`store_rotated` -- the same for a step's projections with the keys and values written
   straight into a :class:`~marathon_amd.scaled_cache.ScaledCache`: what :func:`norm_rotate` and
-  :func:`~marathon_amd.scaled_cache.store_scaled` do, in one launch, the keys rounded once.
+  :func:`~marathon_amd.scaled_cache.store_scaled` do, in one launch, the keys rounded once;
+* :func:`attend_shared` -- :func:`~marathon_amd.scaled_cache.attend_scaled` for a batch whose
+  requests begin, in groups, with the same cached tokens (a system prompt, a document, one
+  history that several drafts continue): those are read once for all of a group's rows.
 
 A step's requests are described as in :mod:`marathon_amd.scaled_cache` (``block_tables``,
 ``starts``, ``lens``), all on the GPU; every call is asynchronous on the current stream and can
@@ -27,6 +30,7 @@ from .row_memory import share
 from .scaled_cache import (
     HEAD_SIZES,
     ScaledCache,
+    _attend_desc,
     _current,
     _flags,
     _int32,
@@ -208,3 +212,41 @@ def store_rotated(cache: ScaledCache, q: torch.Tensor, k: torch.Tensor, v: torch
     with _on(device, _current(device)):
         _lib.check(_lib.lib().mkv_store_rotated(ctypes.byref(desc), current_stream(device)))
     return out_q
+
+
+def attend_shared(cache: ScaledCache, q: torch.Tensor, block_tables: torch.Tensor,
+                  starts: torch.Tensor, lens: torch.Tensor, groups: torch.Tensor,
+                  shared: torch.Tensor, *, softmax_scale: float | None = None,
+                  max_new: int | None = None, max_shared: int | None = None,
+                  max_own: int | None = None, out: torch.Tensor | None = None,
+                  error_flags: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`~marathon_amd.scaled_cache.attend_scaled` where requests ``groups[g]`` to
+    ``groups[g + 1]`` (int32 ``[groups + 1]``) begin with the same ``shared[g]`` tokens (int32
+    ``[groups]``), both on the GPU.
+
+    Of the shared tokens whole blocks are read once for the group, through the block table of its
+    first request; the others' entries for them are not read.  Where a group's tables agree, as
+    those of requests that share blocks do, the result is ``attend_scaled``'s but for the order of
+    sums and the roundings of p named there, by the rows of a group in place of a request's.
+    Requests in no group share nothing.  Groups that leave the requests or descend, and negative
+    ``shared``, are flagged (``MKV_FLAG_SPAN``) and share nothing.
+
+    ``max_new``, ``max_shared`` and ``max_own``: the largest number of new tokens of a request, of
+    tokens that a group shares and of tokens that a request has behind them, where the host knows
+    them; they choose launch shapes only."""
+    desc = _lib.AttendSharedDesc()
+    desc.attend, out = _attend_desc("attend_shared", cache, q, block_tables, starts, lens,
+                                    softmax_scale, max_new, max_own, out, error_flags)
+    device = cache.device
+    desc.n_groups = shared.shape[0] if shared.dim() == 1 else 0
+    desc.shared = _int32("shared", shared, device, None)
+    desc.groups = _int32("groups", groups, device, desc.n_groups + 1)
+    desc.max_shared = max(-1, min(int(max_shared or 0), 2**31 - 1))
+    L = _lib.lib()
+    need = L.mkv_attend_shared_workspace_size(ctypes.byref(desc))
+    with _on(device, _current(device)):
+        if need > 0:  # the allocator hands it on in stream order
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+            desc.attend.workspace, desc.attend.workspace_bytes = workspace.data_ptr(), need
+        _lib.check(L.mkv_attend_shared(ctypes.byref(desc), current_stream(device)))
+    return out
