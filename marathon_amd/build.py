@@ -16,6 +16,8 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -63,10 +65,21 @@ def hipcc() -> str:
 
 
 def _compile(src: str | list, out: str, verbose: bool, extra: list | None = None) -> str:
+    """A library of one source, or of several that are compiled side by side."""
     os.makedirs(os.path.dirname(out), exist_ok=True)
     tmp = out + ".tmp"
-    srcs = [src] if isinstance(src, str) else src
-    cmd = [hipcc(), *HIPCC_FLAGS, *(extra or []), f"-I{INCLUDE}",
+    if isinstance(src, str) or len(src) == 1:
+        return _hipcc([src] if isinstance(src, str) else src, tmp, out, verbose, extra)
+    with tempfile.TemporaryDirectory() as objects, ThreadPoolExecutor(4) as pool:
+        made = [os.path.join(objects, os.path.basename(s) + ".o") for s in src]
+        flags = [*(extra or []), "-c"]
+        list(pool.map(lambda s, o: _hipcc([s], o + ".tmp", o, verbose, flags), src, made))
+        return _hipcc(made, tmp, out, verbose, extra)
+
+
+def _hipcc(srcs: list, tmp: str, out: str, verbose: bool, extra: list | None) -> str:
+    flags = [f for f in HIPCC_FLAGS if f != "-shared" or "-c" not in (extra or [])]
+    cmd = [hipcc(), *flags, *(extra or []), f"-I{INCLUDE}",
            f"-I{os.path.join(HERE, 'csrc')}", *srcs, "-o", tmp]
     if verbose:
         print(" ".join(cmd), flush=True)

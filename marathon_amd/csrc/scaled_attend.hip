@@ -9,6 +9,45 @@
 
 namespace {
 
+// ------------------------------------------------------------------ over whole histories
+
+template <int RT>
+struct Few {
+  typedef AttendParams Params;
+  static constexpr int kFew = RT;
+  static constexpr bool kMany = false, kGrouped = false;
+  static __device__ __forceinline__ const Params& params(const Params& p, Over) { return p; }
+  static __device__ __forceinline__ Section pick(const Params& p, unsigned& tile, int& head, int& part,
+                                                 Over&) {
+    head = blockIdx.y;
+    part = blockIdx.z;
+    // Workgroups go to the eight XCDs in turn: the tiles are turned by the part, so that a long
+    // request's parts do not all fall to one (32 ragged requests: 119 -> 112 us).
+    tile = (blockIdx.x + blockIdx.z) % gridDim.x;
+    if (part == p.splits) {  // (a part of its own: no register is held for it)
+      if (blockIdx.x + blockIdx.y == 0) check_starts(p.s, p.tokens, false);
+      return kNothing;
+    }
+    return kFewRows;
+  }
+};
+
+struct Many {
+  typedef AttendParams Params;
+  static constexpr int kFew = 0;
+  static constexpr bool kMany = true, kGrouped = false;
+  static __device__ __forceinline__ const Params& params(const Params& p, Over) { return p; }
+  static __device__ __forceinline__ Section pick(const Params& p, unsigned& tile, int& head, int& part,
+                                                 Over&) {
+    head = blockIdx.x;
+    part = blockIdx.z;
+    // the last tiles first: of one request they see the most
+    tile = gridDim.y - 1 - blockIdx.y;
+    if (blockIdx.x + blockIdx.y + blockIdx.z == 0) check_starts(p.s, p.tokens, false);
+    return kManyRowsTile;
+  }
+};
+
 // ------------------------------------------------------------------ the parts' results joined
 
 // A workgroup joins one row of a tile and KV head where there are many parts and few rows
@@ -21,7 +60,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p) {
   __shared__ float s_red[4];
   __shared__ f32x4 s_o[kGroups][kLanes];
   Tile t;
-  if (!find_tile<kHistory, BM>(p, blockIdx.x, t) || t.parts <= 1) return;
+  if (!find_tile<false, BM>(p, blockIdx.x, t) || t.parts <= 1) return;
   const int head = blockIdx.y, d = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
   const int64_t at = (static_cast<int64_t>(blockIdx.x) * p.c.heads + head) * p.splits;
   const int step = MANY ? gridDim.z : gridDim.z * kGroups;
@@ -135,7 +174,7 @@ template <bool F16, int D, int RT>
 void launch_few(const AttendParams& p, const Shape& s, int heads, hipStream_t stream) {
   // one part more, which looks through the starts
   const dim3 grid(static_cast<unsigned>(s.tiles), heads, s.splits + (p.s.flags != nullptr ? 1 : 0));
-  attend_few_kernel<kHistory, F16, D, RT><<<grid, 64 * kFewWaves, 0, stream>>>(p);
+  attend_kernel<Few<RT>, F16, D><<<grid, 64 * kFewWaves, 0, stream>>>(p);
   if (s.splits > 1) {
     const unsigned rows = static_cast<unsigned>(s.each < 16 * RT ? (s.each > 0 ? s.each : 1) : 16 * RT);
     attend_join_kernel<F16, D, 16 * RT, true>
@@ -148,7 +187,7 @@ void launch(const AttendParams& p, const Shape& s, int heads, hipStream_t stream
   if (s.rows == 16) return launch_few<F16, D, 1>(p, s, heads, stream);
   if (s.rows == 32) return launch_few<F16, D, 2>(p, s, heads, stream);
   const unsigned tiles = static_cast<unsigned>(s.tiles);
-  attend_many_kernel<kHistory, F16, D><<<dim3(heads, tiles, s.splits), 64 * kManyWaves, 0, stream>>>(p);
+  attend_kernel<Many, F16, D><<<dim3(heads, tiles, s.splits), 64 * kManyWaves, 0, stream>>>(p);
   if (s.splits > 1)
     attend_join_kernel<F16, D, kManyRows, false>
         <<<dim3(tiles, heads, kManyRows * D / 1024), 256, 0, stream>>>(p);

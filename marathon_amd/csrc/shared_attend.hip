@@ -20,10 +20,75 @@
 
 namespace {
 
+// ----------------------------------------------------------------- both ranges, one launch
+//
+// The two ranges' tiles run side by side: over what is shared a tile is bound by the matrix
+// instructions and, over own tokens, a few rows by memory's latency.
+
+struct BothParams {
+  GroupedParams own;
+  // of the tiles over what is shared
+  float* part_o;
+  float* part_ml;
+  int64_t shared_units, own_units;  // workgroups
+  int32_t shared_tiles, own_tiles;
+};
+
+// Tiles of SHARED rows over what is shared and of OWN rows over own tokens: 16 or 32 take the
+// section of few rows, 128 that of many.
+template <int SHARED, int OWN>
+struct Both {
+  typedef BothParams Params;
+  static constexpr bool kGrouped = true, kMany = SHARED == kManyRows;
+  static constexpr int kFew = OWN == kManyRows ? 0 : OWN / 16;
+  static_assert(kMany || SHARED == OWN, "one section of few rows");
+
+  static __device__ __forceinline__ Section pick(const Params& p, unsigned& tile, int& head, int& part,
+                                                 Over& over) {
+    uint32_t unit = blockIdx.x;
+    const uint32_t heads = p.own.c.heads;
+    if (unit < p.shared_units) {
+      // the tiles of one (part, head) go to one XCD, whose L2 then serves all of them but the first
+      const uint32_t in = unit % (8 * p.shared_tiles), pair = unit / (8 * p.shared_tiles) * 8 + in % 8;
+      tile = in / 8;
+      head = pair % heads;
+      part = pair / heads;
+      over = kShared;
+      if (part >= p.own.shared_splits) return kNothing;
+      return kMany ? kManyRowsTile : kFewRows;
+    }
+    unit -= p.shared_units;
+    if (unit >= p.own_units) {  // (a workgroup of its own: no register is held for it)
+      check_starts(p.own.s, p.own.tokens, false);
+      check_groups(p.own.s, p.own.g);
+      return kNothing;
+    }
+    const uint32_t tiles = p.own_tiles, y = unit / tiles;
+    head = y % heads;
+    part = y / heads;
+    tile = (unit + part) % tiles;  // turned by the part, as over whole histories
+    over = kOwn;
+    return OWN == kManyRows ? kManyRowsTile : kFewRows;
+  }
+
+  static __device__ __forceinline__ GroupedParams params(const Params& p, Over over) {
+    GroupedParams x = p.own;
+    if (over == kShared) {
+      x.part_o = p.part_o;
+      x.part_ml = p.part_ml;
+      x.splits = x.shared_splits;
+      x.per = x.shared_per;
+    }
+    return x;
+  }
+};
+
+// ------------------------------------------------------------------ the parts' results joined
+
 // Parts of a launch: results of `rows` rows a tile, tiles by KV heads by parts.
 struct PartSet {
-  const float* o;
-  const float* ml;
+  float* o;
+  float* ml;
   int32_t rows;
   int32_t splits;
   int64_t tiles;
@@ -40,71 +105,92 @@ struct JoinParams {
   int32_t heads, group;
 };
 
-constexpr int kJoinWaves = 4;
-
-// A wave joins a row: 64 parts' m and l at a time, one a lane, then their outputs, D / 4 lanes a
-// part.  What the places say is kept within the parts, whatever was changed between launches.
-template <bool F16, int D>
-__global__ __launch_bounds__(64 * kJoinWaves) void shared_join_kernel(JoinParams p) {
-  constexpr int kLanes = D / 4, kGroups = 64 / kLanes;
+// WAVES waves join a row, or one wave each of four rows: the parts' m and l, one a lane, then
+// their outputs, D / 4 lanes a part.  What the places say is kept within the parts, whatever was
+// changed between the launches.
+template <bool F16, int D, int WAVES>
+__global__ __launch_bounds__(256) void shared_join_kernel(JoinParams p) {
+  constexpr int kLanes = D / 4, kGroups = 64 / kLanes * WAVES;  // groups of lanes at a row's parts
+  __shared__ f32x4 s_o[WAVES][kLanes];
   const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);
   const int q_heads = p.heads * p.group;
-  const uint32_t unit = blockIdx.x * kJoinWaves + wave;
+  const uint32_t unit = WAVES > 1 ? blockIdx.x : blockIdx.x * 4 + wave;
   const int64_t token = unit / q_heads;
   if (token >= p.tokens) return;
   const int h = unit % q_heads, head = h / p.group;
-  RowPlace at = p.places[token * p.group + h % p.group];
+  const RowPlace at = p.places[token * p.group + h % p.group];
   const int32_t* starts = p.starts;
   const int r = last_at_most(p.requests, token, [starts](int i) { return starts[i]; });
   if (r < 0) return;
   const int64_t s0 = starts[r], s1 = starts[r + 1];
   if (s0 < 0 || token < s0 || token >= s1 || s1 > p.tokens) return;  // nobody's
-  const PartSet& mine = (at.own_parts >> 16) & 1 ? p.sets[2] : p.sets[1];
+  const PartSet shared = p.sets[0], mine = (at.own_parts >> 16) & 1 ? p.sets[2] : p.sets[1];
   const auto first_of = [&](const PartSet& s, int32_t place) {
     int64_t tile = place / s.rows;
     tile = tile < 0 ? 0 : tile < s.tiles ? tile : s.tiles - 1;
     const int row = place < 0 ? 0 : place % s.rows;
     return (tile * p.heads + head) * s.splits * s.rows + row;
   };
-  const int ns = min(max(at.shared_parts, 0), p.sets[0].splits);
+  const int ns = min(max(at.shared_parts, 0), shared.splits);
   const int no = min(max(at.own_parts & 0xFFFF, 0), mine.splits);
-  const int64_t from_s = ns > 0 ? first_of(p.sets[0], at.shared_at) : 0;
+  const int64_t from_s = ns > 0 ? first_of(shared, at.shared_at) : 0;
   const int64_t from_o = first_of(mine, at.own_at);
-  const int d = lane % kLanes, grp = lane / kLanes, n = ns + no;
+  const int d = lane % kLanes, grp = lane / kLanes + (WAVES > 1 ? wave * (64 / kLanes) : 0), n = ns + no;
   f32x4 o = {0, 0, 0, 0};
   float top = -kInf, sum = 0.0f;
   for (int base = 0; base < n; base += 64) {
-    const int i = base + lane;
+    const int i = base + lane, here = min(64, n - base);
     float m = -kInf, l = 0.0f;
     if (i < n) {
-      const PartSet& s = i < ns ? p.sets[0] : mine;
-      const int64_t row = i < ns ? from_s + static_cast<int64_t>(i) * s.rows
-                                 : from_o + static_cast<int64_t>(i - ns) * s.rows;
-      m = s.ml[2 * row];
-      l = s.ml[2 * row + 1];
+      const float* ml = i < ns ? shared.ml + 2 * (from_s + static_cast<int64_t>(i) * shared.rows)
+                               : mine.ml + 2 * (from_o + static_cast<int64_t>(i - ns) * mine.rows);
+      m = ml[0];
+      l = ml[1];
     }
+    // the first outputs are on their way while m and l are
+    const auto part_o = [&](int j) {
+      const int k = base + min(j, here - 1);
+      const float* x = k < ns ? shared.o + (from_s + static_cast<int64_t>(k) * shared.rows) * D
+                              : mine.o + (from_o + static_cast<int64_t>(k - ns) * mine.rows) * D;
+      return *reinterpret_cast<const f32x4*>(x + 4 * d);
+    };
+    f32x4 x[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) x[u] = part_o(grp + u * kGroups);
     float now = m;
-    for (int x = 32; x > 0; x >>= 1) now = fmaxf(now, __shfl_xor(now, x));
+    for (int y = 32; y > 0; y >>= 1) now = fmaxf(now, __shfl_xor(now, y));
     now = fmaxf(now, top);
     const float b = now == -kInf ? 0.0f : now, old = fast_exp2(top - b), f = fast_exp2(m - b);
     float part = l * f;
-    for (int x = 32; x > 0; x >>= 1) part += __shfl_xor(part, x);
+    for (int y = 32; y > 0; y >>= 1) part += __shfl_xor(part, y);
     sum = sum * old + part;
     o *= old;
     top = now;
-    const int here = min(64, n - base);
-    for (int j = grp; j < here; j += kGroups) {
-      const int k = base + j;
-      const float* x = k < ns ? p.sets[0].o + (from_s + static_cast<int64_t>(k) * p.sets[0].rows) * D
-                              : mine.o + (from_o + static_cast<int64_t>(k - ns) * mine.rows) * D;
-      o += *reinterpret_cast<const f32x4*>(x + 4 * d) * __shfl(f, j);
+    for (int j = grp; j - grp < here; j += 4 * kGroups) {  // (alike in every lane)
+      if (j != grp) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) x[u] = part_o(j + u * kGroups);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int k = j + u * kGroups;
+        const float w = __shfl(f, min(k, 63));
+        if (k < here) o += x[u] * w;
+      }
     }
   }
 #pragma unroll
   for (int x = kLanes; x < 64; x <<= 1)
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], x);
-  if (grp != 0) return;
+  if constexpr (WAVES > 1) {
+    if (lane < kLanes) s_o[wave][d] = o;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) o += s_o[w][d];
+  }
+  if (lane >= kLanes) return;
   o *= sum == 0.0f ? 0.0f : 1.0f / sum;
   *reinterpret_cast<u32x2*>(p.out + token * p.out_token + h * p.out_head + d * 8) =
       u32x2{out_pair<F16>(o[0], o[1]), out_pair<F16>(o[2], o[3])};
@@ -143,22 +229,23 @@ int check(const mkv_attend_shared_desc_t& d, GroupedParams* p, Plan* plan) {
     plan->own[0] = shape_for(a, each, 0, INT32_MAX);
     plan->owns = 1;
   }
-  plan->shared = Shape{};
-  if (d.n_groups > 0) {
-    mkv_attend_desc_t s = a;  // a group's rows as one request's
-    s.requests = d.n_groups;
-    s.max_len = d.max_shared;
-    const int64_t rows = (a.tokens * p->group + d.n_groups - 1) / d.n_groups;
-    plan->shared = shape_for(s, rows, 0, INT32_MAX);
+  mkv_attend_desc_t s = a;  // a group's rows as one request's
+  s.requests = d.n_groups > 0 ? d.n_groups : 1;
+  s.max_len = d.max_shared;
+  plan->shared = shape_for(s, (a.tokens * p->group + s.requests - 1) / s.requests, 0, INT32_MAX);
+  // one section of few rows, and many own rows beside many shared ones
+  Shape& own = plan->own[plan->owns - 1];
+  if (own.rows > plan->shared.rows)
+    plan->shared = shape_for(s, own.rows, 0, INT32_MAX);
+  else if (plan->shared.rows == 32 && own.rows == 16)
+    own = shape_for(a, 32, 0, INT32_MAX);
+  // the grid's limits, and 32 bits for a row's place
+  int64_t units = 1;
+  for (const Shape* x : {&plan->shared, &plan->own[0], &plan->own[plan->owns - 1]}) {
+    units += x->tiles * (a.cache.heads * x->splits + 7);
+    if (x->tiles * x->rows > INT32_MAX) units = INT64_MAX / 2;
   }
-  for (const Shape* s : {&plan->shared, &plan->own[0], &plan->own[1]}) {
-    if (s == &plan->own[1] && plan->owns < 2) continue;
-    if (s->tiles > (s->rows == kManyRows ? 65535 : UINT32_MAX / (64 * kFewWaves)) ||
-        s->tiles * s->rows > INT32_MAX)
-      return mkv_fail(MKV_ERR_UNSUPPORTED, "%s: %lld query rows", who,
-                      (long long)(a.tokens * p->group));
-  }
-  if (a.tokens * a.q_heads > UINT32_MAX / 64)
+  if (units > UINT32_MAX / 256 || a.tokens * a.q_heads > UINT32_MAX / 256)
     return mkv_fail(MKV_ERR_UNSUPPORTED, "%s: %lld query rows", who, (long long)(a.tokens * a.q_heads));
   return MKV_OK;
 }
@@ -166,63 +253,82 @@ int check(const mkv_attend_shared_desc_t& d, GroupedParams* p, Plan* plan) {
 // Every launch leaves parts, also where one is all.
 int64_t part_rows(const Shape& s, int heads) { return s.tiles * heads * s.splits * s.rows; }
 
+constexpr int64_t kFewJoins = 8192;  // rows that are joined by four waves each
+
 int64_t up16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 
 int64_t workspace_of(const mkv_attend_shared_desc_t& d, const Plan& plan) {
   const mkv_scaled_cache_t& c = d.attend.cache;
   int64_t rows = 0;
-  if (d.n_groups > 0) rows += part_rows(plan.shared, c.heads);
+  rows += part_rows(plan.shared, c.heads);
   for (int i = 0; i < plan.owns; ++i) rows += part_rows(plan.own[i], c.heads);
   return d.attend.tokens * (d.attend.q_heads / c.heads) * static_cast<int64_t>(sizeof(RowPlace)) +
          rows * (c.head_size + 2) * 4 + 64;
 }
 
-template <int OVER, bool F16, int D>
-void launch(const GroupedParams& p, const Shape& s, int heads, hipStream_t stream) {
-  const unsigned tiles = static_cast<unsigned>(s.tiles);
-  // (few rows: one part more looks through the starts)
-  const dim3 few(tiles, heads, s.splits + (OVER == kOwn && p.s.flags != nullptr ? 1 : 0));
-  if (s.rows == 16)
-    attend_few_kernel<OVER, F16, D, 1><<<few, 64 * kFewWaves, 0, stream>>>(p);
-  else if (s.rows == 32)
-    attend_few_kernel<OVER, F16, D, 2><<<few, 64 * kFewWaves, 0, stream>>>(p);
-  else
-    attend_many_kernel<OVER, F16, D><<<dim3(heads, tiles, s.splits), 64 * kManyWaves, 0, stream>>>(p);
+template <typename K, bool F16, int D>
+void launch(const BothParams& p, hipStream_t stream) {
+  const int64_t units = p.shared_units + p.own_units + (p.own.s.flags != nullptr ? 1 : 0);
+  attend_kernel<K, F16, D><<<static_cast<unsigned>(units), 256, 0, stream>>>(p);
 }
 
 template <bool F16, int D>
-void run(GroupedParams p, const Plan& plan, JoinParams j, char* room, hipStream_t stream) {
-  const int heads = j.heads;
-  const auto place = [&](const Shape& s, PartSet* set) {
-    const int64_t rows = part_rows(s, heads);
-    p.part_o = reinterpret_cast<float*>(room);
-    p.part_ml = p.part_o + rows * D;
-    p.splits = s.splits;
-    p.per = s.per;
-    p.rows_from = s.from;
-    p.rows_to = s.to;
-    room += up16(rows * (D + 2) * 4);
-    *set = PartSet{p.part_o, p.part_ml, s.rows, s.splits, s.tiles};
-  };
-  p.shared_rows = 16;
-  p.shared_splits = p.shared_per = 1;
-  if (p.g.count > 0) {
-    p.shared_rows = plan.shared.rows;
-    p.shared_per = plan.shared.per;
-    p.shared_splits = plan.shared.splits;
-    place(plan.shared, &j.sets[0]);
-    launch<kShared, F16, D>(p, plan.shared, heads, stream);
+void launch(int shared_rows, int own_rows, const BothParams& p, hipStream_t stream) {
+  if (shared_rows == kManyRows) {
+    if (own_rows == 16)
+      launch<Both<kManyRows, 16>, F16, D>(p, stream);
+    else if (own_rows == 32)
+      launch<Both<kManyRows, 32>, F16, D>(p, stream);
+    else
+      launch<Both<kManyRows, kManyRows>, F16, D>(p, stream);
+  } else if (shared_rows == 16) {
+    launch<Both<16, 16>, F16, D>(p, stream);
+  } else {
+    launch<Both<32, 32>, F16, D>(p, stream);
   }
-  for (int i = 0; i < plan.owns; ++i) {
-    p.launch = i;
-    place(plan.own[i], &j.sets[1 + i]);
-    launch<kOwn, F16, D>(p, plan.own[i], heads, stream);
+}
+
+template <bool F16, int D>
+void run(const GroupedParams& base, const Plan& plan, JoinParams j, char* room, hipStream_t stream) {
+  const int heads = j.heads;
+  const auto place = [&](const Shape& s, PartSet* set) {  // the parts of a launch's tiles
+    const int64_t rows = part_rows(s, heads);
+    float* o = reinterpret_cast<float*>(room);
+    room += up16(rows * (D + 2) * 4);
+    *set = PartSet{o, o + rows * D, s.rows, s.splits, s.tiles};
+  };
+  BothParams p = {};
+  p.own = base;
+  p.own.shared_rows = plan.shared.rows;
+  p.own.shared_per = plan.shared.per;
+  p.own.shared_splits = plan.shared.splits;
+  place(plan.shared, &j.sets[0]);
+  p.part_o = j.sets[0].o;
+  p.part_ml = j.sets[0].ml;
+  p.shared_tiles = static_cast<int32_t>(plan.shared.tiles);
+  for (int i = plan.owns - 1; i >= 0; --i) {  // the chunks beside what is shared
+    const Shape& own = plan.own[i];
+    PartSet& set = j.sets[1 + i];
+    place(own, &set);
+    p.own.part_o = set.o;
+    p.own.part_ml = set.ml;
+    p.own.splits = own.splits;
+    p.own.per = own.per;
+    p.own.rows_from = own.from;
+    p.own.rows_to = own.to;
+    p.own.launch = i;
+    p.own_tiles = static_cast<int32_t>(own.tiles);
+    p.own_units = own.tiles * heads * own.splits;
+    const bool with = i == plan.owns - 1 && base.g.count > 0;
+    p.shared_units = with ? plan.shared.tiles * ((heads * plan.shared.splits + 7) / 8 * 8) : 0;
+    launch<F16, D>(with ? plan.shared.rows : own.rows, own.rows, p, stream);
   }
   if (plan.owns == 1) j.sets[2] = j.sets[1];
-  if (p.g.count == 0) j.sets[0] = PartSet{nullptr, nullptr, 16, 0, 1};
   const int64_t rows = j.tokens * heads * j.group;
-  shared_join_kernel<F16, D><<<static_cast<unsigned>((rows + kJoinWaves - 1) / kJoinWaves),
-                               64 * kJoinWaves, 0, stream>>>(j);
+  if (rows <= kFewJoins)
+    shared_join_kernel<F16, D, 4><<<static_cast<unsigned>(rows), 256, 0, stream>>>(j);
+  else
+    shared_join_kernel<F16, D, 1><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, stream>>>(j);
 }
 
 template <bool F16>
