@@ -170,12 +170,6 @@ __device__ __forceinline__ void turns8(const f32x2* lds, const Place<D>& place, 
   for (int i = 0; i < 8; ++i) turn[i] = place.turned ? lds[place.a + i] : f32x2{1.0f, 0.0f};
 }
 
-// LDS that only this wave touches: its stores are done before its loads behind this.
-__device__ __forceinline__ void wave_fence() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-}
-
 // The heads [h0, h1) of one token and side, by one wave: the next heads' loads are in flight
 // while these are worked on.  `angles` makes the wave's (cos, sin) in LDS, once the first are.
 template <int ET, int D, typename F>

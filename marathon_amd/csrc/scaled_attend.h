@@ -147,11 +147,12 @@ __device__ __forceinline__ bool read_group(const DevCache& c, const DevStep& s, 
   out.index = g;
   out.a = d.groups[g];
   out.b = d.groups[g + 1];
+  const int shared = d.shared[g];
   if (out.a < 0 || out.b <= out.a || out.b > s.requests) return false;
   out.s0 = s.starts[out.a];
   out.s1 = s.starts[out.b];
   if (out.s0 < 0 || out.s1 < out.s0 || out.s1 > tokens) return false;
-  const int64_t n = within(c, s, d.shared[g]);
+  const int64_t n = within(c, s, shared);
   out.shared = n <= 0 ? 0 : static_cast<int>(n >> c.bs_shift << c.bs_shift);
   return true;
 }
@@ -165,11 +166,12 @@ __device__ __forceinline__ bool group_of(const DevCache& c, const DevStep& s, co
          s0 >= out.s0 && s1 <= out.s1;
 }
 
-// The first tile of group g in a launch of `rows` rows a tile: as for a request.
-__device__ __forceinline__ int64_t shared_begin(const DevStep& s, const DevGroups& d, int group,
-                                                int rows, int g) {
-  const int a = d.groups[g];
-  return a < 0 || a > s.requests ? g : static_cast<int64_t>(s.starts[a]) * group / rows + g;
+// The first tile of group g, whose rows begin at `row`, in a launch of `rows` rows a tile: rounded
+// up with the group's number, which leaves each group exactly as many as its rows may need and
+// one group none too many.  (An empty tile's workgroups end early, but where the chip is filled
+// once they leave others two to a CU: 32 parts of one tile 26.9 us, beside as many empty 37.4.)
+__device__ __forceinline__ int64_t shared_begin(int64_t row, int rows, int g) {
+  return (row + static_cast<int64_t>(g) * (rows - 1)) / rows;
 }
 
 // (GROUPED: over what `t.over` says; otherwise over histories.)
@@ -178,26 +180,22 @@ __device__ __forceinline__ bool find_tile(const P& p, int64_t tile, Tile& t) {
   const int32_t* starts = p.s.starts;
   const int group = p.group;
   if constexpr (GROUPED) if (t.over == kShared) {
-    const int g = last_at_most(p.g.count, tile, [&](int i) {
-      return shared_begin(p.s, p.g, group, BM, i);
+    const int32_t* groups = p.g.groups;
+    const int requests = p.s.requests;
+    const int g = p.g.count == 1 ? 0 : last_at_most(p.g.count, tile, [=](int i) {
+      const int a = groups[i];
+      return a < 0 || a > requests ? int64_t{0}
+                                   : shared_begin(static_cast<int64_t>(starts[a]) * group, BM, i);
     });
     Group of;
     if (g < 0 || !read_group(p.c, p.s, p.g, p.tokens, g, of)) return false;
     t.request = of.a;
     t.last = of.b - 1;
     t.s0 = of.s0;
-    t.row0 = (tile - shared_begin(p.s, p.g, group, BM, g)) * BM;
+    t.row0 = (tile - shared_begin(of.s0 * group, BM, g)) * BM;
     const int64_t rows = (of.s1 - of.s0) * group - t.row0;
     if (t.row0 < 0 || rows <= 0 || of.shared == 0) return false;
     t.rows = static_cast<int>(rows < BM ? rows : BM);
-    // nearly always every row stands behind what is shared
-    int64_t least = of.shared;
-    for (int r = of.a + (threadIdx.x & 63); r < of.b; r += 64) {
-      const int64_t n = static_cast<int64_t>(starts[r + 1]) - starts[r];
-      const int64_t sees = n > 0 ? p.s.lens[r] - n + 1 : of.shared;
-      least = sees < least ? sees : least;
-    }
-    t.full = __all(least >= of.shared) ? of.shared : 0;
     t.keys = of.shared;
     t.from = 0;
     t.first = 0;
@@ -237,7 +235,7 @@ __device__ __forceinline__ bool find_tile(const P& p, int64_t tile, Tile& t) {
     if (group_of(p.c, p.s, p.g, p.tokens, r, t.s0, s1, of) && of.shared > 0) {
       t.from = of.shared;
       t.shared_row = (t.s0 - of.s0) * group + t.row0;
-      t.shared_tile = shared_begin(p.s, p.g, group, p.shared_rows, of.index);
+      t.shared_tile = shared_begin(of.s0 * group, p.shared_rows, of.index);
       t.shared_parts = part_count(of.shared, part_size(of.shared, p.shared_splits, p.shared_per));
       if (t.keys < t.from) t.keys = t.full = t.from;  // nothing of its own
     }
@@ -245,6 +243,19 @@ __device__ __forceinline__ bool find_tile(const P& p, int64_t tile, Tile& t) {
   t.per = part_size(t.keys - t.from, p.splits, p.per);
   t.parts = part_count(t.keys - t.from, t.per);
   return true;
+}
+
+// Over what is shared: whether every row sees all of it, as nearly always, those that stand behind
+// it.  The requests' lengths are waited for here, not before the tile's table is looked up.
+template <typename P>
+__device__ __forceinline__ void find_full(const P& p, Tile& t) {
+  int64_t least = t.keys;
+  for (int r = t.request + (threadIdx.x & 63); r <= t.last; r += 64) {
+    const int64_t n = static_cast<int64_t>(p.s.starts[r + 1]) - p.s.starts[r];
+    const int64_t sees = n > 0 ? p.s.lens[r] - n + 1 : t.keys;
+    least = sees < least ? sees : least;
+  }
+  t.full = __all(least >= t.keys) ? t.keys : 0;
 }
 
 // Tokens that a row of the tile sees, at most t.keys.
@@ -395,7 +406,7 @@ enum Section { kNothing, kFewRows, kManyRowsTile };
 
 template <int D, int RT>
 struct FewLds {
-  float o[2][D * 16];
+  __attribute__((aligned(16))) float o[kFewWaves][D * 16];
   float ml[kFewWaves][16 * RT][2];
 };
 
@@ -476,6 +487,8 @@ __global__ __launch_bounds__(256, (min_waves<K, D>())) void attend_kernel(typena
     };
     const int first = k0 + 32 * wave;
     if (first < k1) look_up(first);
+    if constexpr (K::kGrouped)
+      if (t.over == kShared) find_full(p, t);
 
     // this lane's query rows: operand B of S^T = K Q^T
     u32x4 q[RT][KS];
@@ -700,25 +713,40 @@ __global__ __launch_bounds__(256, (min_waves<K, D>())) void attend_kernel(typena
 
     // One step's codes in registers, and other waves to hide its loads: keeping the next step's
     // as well takes the registers of one wave in three (119 us against 111, the same requests).
+    // Beside tiles of many rows the registers are there.
     constexpr int kStride = 32 * kFewWaves;
     for (int base = first; base < k1; base += 64 * kStride) {
       if (base != first) look_up(base);
       const int last = min(64, (k1 - base + kStride - 1) / kStride) - 1;
-      for (int n = 0; n <= last; ++n) {
-        FewRaw<D> x;
-        load(base + n * kStride, n, x);
-        step(base + n * kStride, n, x);
+      if constexpr (K::kMany) {
+        FewRaw<D> x, next;
+        load(base, 0, x);
+        for (int n = 0; n <= last; ++n) {
+          if (n < last) load(base + (n + 1) * kStride, n + 1, next);
+          step(base + n * kStride, n, x);
+          x = next;
+        }
+      } else {
+        for (int n = 0; n <= last; ++n) {
+          FewRaw<D> x;
+          load(base + n * kStride, n, x);
+          step(base + n * kStride, n, x);
+        }
       }
     }
 
     // the four waves' results: their largest, then the sums under it
+    // (places found anew: what the queries' addresses took is not kept in registers until here)
+    unsigned tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int cc = tid & 15, gg = tid >> 4 & 3;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       l[rt] += __shfl_xor(l[rt], 16);
       l[rt] += __shfl_xor(l[rt], 32);
-      if (g == 0) {
-        s_ml[wave][rt * 16 + c][0] = m[rt];
-        s_ml[wave][rt * 16 + c][1] = l[rt];
+      if (gg == 0) {
+        s_ml[wave][rt * 16 + cc][0] = m[rt];
+        s_ml[wave][rt * 16 + cc][1] = l[rt];
       }
     }
     __syncthreads();
@@ -731,68 +759,54 @@ __global__ __launch_bounds__(256, (min_waves<K, D>())) void attend_kernel(typena
     }
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      float top = -kInf, sum = 0.0f;
+      // the largest of a row and the sum under it
+      const auto row_sum = [&](int i, float& top) {
+        top = -kInf;
+        float sum = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kFewWaves; ++w) top = fmaxf(top, s_ml[w][rt * 16 + c][0]);
-      const float base = top == -kInf ? 0.0f : top;
+        for (int w = 0; w < kFewWaves; ++w) top = fmaxf(top, s_ml[w][i][0]);
+        const float base = top == -kInf ? 0.0f : top;
 #pragma unroll
-      for (int w = 0; w < kFewWaves; ++w)
-        sum += s_ml[w][rt * 16 + c][1] * fast_exp2(s_ml[w][rt * 16 + c][0] - base);
-      const float f = fast_exp2(m[rt] - base);
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= f;
-      const auto put = [&](int slot) {
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s_o[slot][(dt * 4 + r) * 64 + lane] = o[rt][dt][r];
+        for (int w = 0; w < kFewWaves; ++w) sum += s_ml[w][i][1] * fast_exp2(s_ml[w][i][0] - base);
+        return sum;
       };
-      const auto add = [&](int slot) {
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o[rt][dt][r] += s_o[slot][(dt * 4 + r) * 64 + lane];
-      };
+      float top;
+      row_sum(rt * 16 + cc, top);
+      const float f = fast_exp2(m[rt] - (top == -kInf ? 0.0f : top));
       if (rt > 0) __syncthreads();
-      if (wave >= 2) put(wave - 2);
+      // a row's quarters of a vector exchanged by its number, against bank conflicts
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int dt = 0; dt < DT; dt += 4)
+          *reinterpret_cast<f32x4*>(&s_o[wave][cc * D + 4 * (((D / 16) * (4 * gg + r) + dt) / 4 ^ cc)]) =
+              f32x4{o[rt][dt][r] * f, o[rt][dt + 1][r] * f, o[rt][dt + 2][r] * f, o[rt][dt + 3][r] * f};
       __syncthreads();
-      if (wave < 2) add(wave);
-      __syncthreads();
-      if (wave == 1) put(0);
-      __syncthreads();
-      if (wave == 0) {
-        add(0);
-        int i = rt * 16 + c, gg = g;
-        asm volatile("" : "+v"(i), "+v"(gg));  // found anew: what q's addresses took is not kept
-        if (i < t.rows) {
-          if (part_o != nullptr) {
-            if (gg == 0) {
-              part_ml[2 * i] = top;
-              part_ml[2 * i + 1] = sum;
-            }
+      constexpr int kLanes = D / 4;  // of a row
+      const int v = tid % kLanes;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              float* at = part_o + static_cast<int64_t>(i) * D + (D / 16) * (4 * gg + r);
+      for (int r = tid / kLanes; r < 16; r += 64 * kFewWaves / kLanes) {
+        const int i = rt * 16 + r;
+        if (i >= t.rows) break;
+        f32x4 x[kFewWaves];
 #pragma unroll
-              for (int dt = 0; dt < DT; dt += 4)
-                *reinterpret_cast<f32x4*>(at + dt) =
-                    f32x4{o[rt][dt][r], o[rt][dt + 1][r], o[rt][dt + 2][r], o[rt][dt + 3][r]};
-            }
-          } else {
-            const int64_t row = t.row0 + i;
-            char* at = p.out + (t.s0 + row / p.group) * p.out_token +
-                       (static_cast<int64_t>(head) * p.group + row % p.group) * p.out_head;
-            const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-#pragma unroll
-              for (int dt = 0; dt < DT; dt += 4) {
-                const u32x2 w = {out_pair<F16>(o[rt][dt][r] * by, o[rt][dt + 1][r] * by),
-                                 out_pair<F16>(o[rt][dt + 2][r] * by, o[rt][dt + 3][r] * by)};
-                *reinterpret_cast<u32x2*>(at + ((D / 16) * (4 * gg + r) + dt) * 2) = w;
-              }
-            }
+        for (int w = 0; w < kFewWaves; ++w)
+          x[w] = *reinterpret_cast<const f32x4*>(&s_o[w][r * D + 4 * (v ^ r)]);
+        const f32x4 all = (x[0] + x[2]) + (x[1] + x[3]);
+        const float sum = row_sum(i, top);
+        if (part_o != nullptr) {
+          *reinterpret_cast<f32x4*>(part_o + i * D + 4 * v) = all;
+          if (v == 0) {
+            part_ml[2 * i] = top;
+            part_ml[2 * i + 1] = sum;
           }
+        } else {
+          const int64_t row = t.row0 + i;
+          char* at = p.out + (t.s0 + row / p.group) * p.out_token +
+                     (static_cast<int64_t>(head) * p.group + row % p.group) * p.out_head;
+          const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+          *reinterpret_cast<u32x2*>(at + 8 * v) =
+              u32x2{out_pair<F16>(all[0] * by, all[1] * by), out_pair<F16>(all[2] * by, all[3] * by)};
         }
       }
     }
@@ -835,6 +849,10 @@ __global__ __launch_bounds__(256, (min_waves<K, D>())) void attend_kernel(typena
       }
       return x;
     };
+
+    Groups now = look_up(k0);
+    if constexpr (K::kGrouped)
+      if (t.over == kShared) find_full(p, t);
 
     // this wave's rows: operand B of S^T = K Q^T
     const int64_t row = t.row0 + wave * 32 + c;
@@ -1099,7 +1117,7 @@ __global__ __launch_bounds__(256, (min_waves<K, D>())) void attend_kernel(typena
     };
 
     if (k0 < k1) {
-      Groups now = look_up(k0), next = look_up(k0 + 1024);
+      Groups next = look_up(k0 + 1024);
       fetch(k0, now, 0);
       __syncthreads();  // s_odd is set
       stage(k0, now, 0, 0);
@@ -1123,23 +1141,32 @@ __global__ __launch_bounds__(256, (min_waves<K, D>())) void attend_kernel(typena
 
     l += __shfl_xor(l, 32);
     const int i = wave * 32 + c;
-    if (!there) return;
     if (K::kGrouped || t.parts > 1) {
       const int64_t at = (static_cast<int64_t>(tile) * p.c.heads + head) * p.splits + part;
-      if (h == 0) {
+      if (there && h == 0) {
         p.part_ml[(at * kManyRows + i) * 2] = m;
         p.part_ml[(at * kManyRows + i) * 2 + 1] = l;
       }
-      float* to = p.part_o + (at * kManyRows + i) * D;
+      // through LDS, so that rows leave whole, not 16 bytes of each at a time; a row's quarters of
+      // a vector are exchanged by its number, as the tiles' were
+      float* s_o = reinterpret_cast<float*>(s_k) + wave * 32 * D;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {  // dimensions W * d + 0..W-1, two of each mt
         const int d = 8 * (e >> 2) + 4 * h + (e & 3);
 #pragma unroll
         for (int mt = 0; mt < MT; mt += 2)
-          *reinterpret_cast<f32x4*>(to + W * d + 2 * mt) =
+          *reinterpret_cast<f32x4*>(s_o + c * D + 4 * ((W * d + 2 * mt) / 4 ^ (c & 15))) =
               f32x4{o[mt][e], o[mt][e + 8], o[mt + 1][e], o[mt + 1][e + 8]};
       }
-    } else {
+      wave_fence();
+      constexpr int kLanes = D / 4, kRows = 64 / kLanes;  // of a row; rows a store
+      const int v = lane % kLanes, last = min(32, t.rows - wave * 32);
+      float* to = p.part_o + (at * kManyRows + wave * 32) * D + 4 * v;
+#pragma unroll 8
+      for (int r = lane / kLanes; r < last; r += kRows)
+        *reinterpret_cast<f32x4*>(to + r * D) =
+            *reinterpret_cast<const f32x4*>(s_o + r * D + 4 * (v ^ (r & 15)));
+    } else if (there) {
       const float by = l == 0.0f ? 0.0f : 1.0f / l;
       char* to = p.out + (t.s0 + row / p.group) * p.out_token +
                  (static_cast<int64_t>(head) * p.group + row % p.group) * p.out_head;

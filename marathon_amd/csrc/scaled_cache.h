@@ -55,6 +55,12 @@ __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) <
 // A wave-uniform value as a scalar.
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// LDS that only this wave touches: its stores are done before its loads behind this.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // The last i in [0, n) whose value(i) is at most `at`, for values that do not descend; -1 if
 // there is none.  n <= 4096: at most two rounds of loads by the whole wave, where a binary
 // search takes log2(n) dependent ones (each some 300 ns).  Values that descend give some

@@ -232,13 +232,15 @@ int check(const mkv_attend_shared_desc_t& d, GroupedParams* p, Plan* plan) {
   mkv_attend_desc_t s = a;  // a group's rows as one request's
   s.requests = d.n_groups > 0 ? d.n_groups : 1;
   s.max_len = d.max_shared;
-  plan->shared = shape_for(s, (a.tokens * p->group + s.requests - 1) / s.requests, 0, INT32_MAX);
+  const int64_t rows = a.tokens * p->group;
+  plan->shared = shape_for(s, (rows + s.requests - 1) / s.requests, 0, INT32_MAX);
   // one section of few rows, and many own rows beside many shared ones
   Shape& own = plan->own[plan->owns - 1];
   if (own.rows > plan->shared.rows)
     plan->shared = shape_for(s, own.rows, 0, INT32_MAX);
   else if (plan->shared.rows == 32 && own.rows == 16)
     own = shape_for(a, 32, 0, INT32_MAX);
+  plan->shared.tiles = (rows + static_cast<int64_t>(s.requests) * (plan->shared.rows - 1)) / plan->shared.rows;
   // the grid's limits, and 32 bits for a row's place
   int64_t units = 1;
   for (const Shape* x : {&plan->shared, &plan->own[0], &plan->own[plan->owns - 1]}) {
