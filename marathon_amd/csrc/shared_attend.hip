@@ -16,6 +16,9 @@
 #include "marathon_kvstep.h"
 #include "scaled_attend.h"
 
+#include <algorithm>
+#include <cmath>
+
 #pragma clang fp contract(off)
 
 namespace {
@@ -206,6 +209,76 @@ struct Plan {
   int owns;
 };
 
+// What a kernel's steps take, in us: of `tokens` by a workgroup that is alone on its CU, and of a
+// CU's time where it has as many as fit; and how many workgroups run at once.  Measured on whole
+// calls, for 16 rows a tile, 32 and 128.
+struct Cost {
+  int tokens;
+  double alone, full;
+  int slots;
+};
+
+Cost cost_of(int rows, int head_size, bool f16) {
+  const int i = head_size == 64 ? 0 : head_size == 128 ? 1 : 2;
+  if (rows == kManyRows) {
+    constexpr double kAlone[] = {1.35, 1.6, 5.5}, kFull[] = {0.85, 1.06, 5.0};
+    constexpr int kSlots[] = {768, 512, 256};
+    const double more = f16 ? 1.4 : 1.0;  // p's second product
+    return {64, kAlone[i] * more, kFull[i] * more, kSlots[i]};
+  }
+  constexpr double kAlone[] = {1.1, 1.6, 3.4}, kFull[] = {0.8, 1.5, 3.4};
+  constexpr int kSlots[2][3] = {{1024, 1024, 512}, {768, 512, 256}};
+  const double more = rows == 32 ? 1.6 : 1.0;
+  return {32 * kFewWaves, kAlone[i] * more, kFull[i] * more, kSlots[rows == 32][i]};
+}
+
+// The parts of both ranges, by the time that they are expected to take: the longest workgroup of
+// either, or all of the work over the chip, whichever is more, and the join, which reads a row's
+// results once for each part.  Against a sweep of the parts over 16 batches (2 to 96 requests, 1 to 8
+// KV heads) its choice is within 8% of the best for 13 of them, and 10 to 30% off where groups differ
+// much in what they share, own histories are the longer ones, or heads are of 256.
+void choose_parts(const mkv_attend_shared_desc_t& d, int64_t shared_most, int64_t own_most, Shape* s,
+                  Shape* o) {
+  constexpr double kCus = 256, kStart = 5.0, kStartFull = 1.2, kJoin = 1.5e-6;  // (a value of a part)
+  const mkv_attend_desc_t& a = d.attend;
+  const bool f16 = a.dtype == MKV_F16;
+  const Cost cs = cost_of(s->rows, a.cache.head_size, f16), co = cost_of(o->rows, a.cache.head_size, f16);
+  const double heads = a.cache.heads;
+  const double part = 0.05 + kJoin * static_cast<double>(a.tokens) * a.q_heads * a.cache.head_size;
+  // tiles that have work, if groups and requests are alike; of lengths that differ, half the longest
+  const auto alike = [](const Shape& x, int64_t each, int64_t count) {
+    return static_cast<double>(std::min((each + x.rows - 1) / x.rows * count, x.tiles));
+  };
+  const double st = alike(*s, s->each, d.n_groups) * heads, ot = alike(*o, o->each, a.requests) * heads;
+  const double spare = 0.3 * (static_cast<double>(o->tiles) * heads - ot);  // (these end early)
+  const int64_t ss = (shared_most + cs.tokens - 1) / cs.tokens, os = (own_most + co.tokens - 1) / co.tokens;
+  const auto most = [](int64_t n) { return n < kMaxSplits ? n < 1 ? 1 : static_cast<int>(n) : kMaxSplits; };
+  const int most_s = d.n_groups > 0 ? most(shared_most / 128) : 1, most_o = most(own_most / 128);
+  double best = 1e30;
+  int n = 1, m = 1;
+  for (int i = 1; i <= most_s; i += (i + 3) / 4) {
+    const double units = st * i, steps = static_cast<double>((ss + i - 1) / i);
+    const double load = units <= kCus ? 1.0 : std::min(std::ceil(units / kCus), cs.slots / kCus);
+    const double path = ss > 0 ? kStart + steps * std::max(cs.alone, load * cs.full) : 0.0;
+    const double work = ss > 0 ? units * (kStartFull + steps * cs.full) : 0.0;
+    for (int j = 1; j <= most_o; j += (j + 3) / 4) {
+      const double own = ot * (j * kStartFull + 0.55 * static_cast<double>(os) * co.full);
+      const double own_path = kStart + static_cast<double>((os + j - 1) / j) * co.alone;
+      // where they do not all run at once, the chip waits for a quarter of a last one
+      const double wait = units > cs.slots ? path : units + (ot + spare) * j > cs.slots ? own_path : 0.0;
+      const double time = std::max(std::max(path, own_path), (work + own) / kCus + 0.25 * wait) + (i + j) * part;
+      if (time < best) best = time, n = i, m = j;
+    }
+  }
+  const auto cut = [](int64_t tokens, int parts, Shape* x) {
+    const int64_t per = (tokens / parts + 64) / 64 * 64;
+    x->per = static_cast<int>(per < 1 << 30 ? per : 1 << 30);
+    x->splits = static_cast<int>(tokens > per ? (tokens + per - 1) / per : 1);
+  };
+  cut(shared_most, n, s);
+  cut(own_most, m, o);
+}
+
 int check(const mkv_attend_shared_desc_t& d, GroupedParams* p, Plan* plan) {
   const char* who = "mkv_attend_shared";
   const mkv_attend_desc_t& a = d.attend;
@@ -237,10 +310,14 @@ int check(const mkv_attend_shared_desc_t& d, GroupedParams* p, Plan* plan) {
   // one section of few rows, and many own rows beside many shared ones
   Shape& own = plan->own[plan->owns - 1];
   if (own.rows > plan->shared.rows)
-    plan->shared = shape_for(s, own.rows, 0, INT32_MAX);
+    plan->shared.rows = own.rows;
   else if (plan->shared.rows == 32 && own.rows == 16)
     own = shape_for(a, 32, 0, INT32_MAX);
   plan->shared.tiles = (rows + static_cast<int64_t>(s.requests) * (plan->shared.rows - 1)) / plan->shared.rows;
+  const int64_t room = static_cast<int64_t>(a.table_width) * a.cache.block_size;
+  const auto known = [room](int32_t most) { return most > 0 && most < room ? most : room; };
+  if (plan->owns == 1)
+    choose_parts(d, d.n_groups > 0 ? known(d.max_shared) : 0, known(a.max_len), &plan->shared, &plan->own[0]);
   // the grid's limits, and 32 bits for a row's place
   int64_t units = 1;
   for (const Shape* x : {&plan->shared, &plan->own[0], &plan->own[plan->owns - 1]}) {
