@@ -472,6 +472,10 @@ def binding():
                     ctypes.cast(getattr(cdll, name), ctypes.c_void_p).value
                     for name in ("mkv_step_slots", "mkv_store_scaled", "mkv_attend_scaled",
                                  "mkv_attend_workspace_size")))
+                module.bind_step(*(
+                    ctypes.cast(getattr(cdll, name), ctypes.c_void_p).value
+                    for name in ("mkv_norm_rotate", "mkv_store_rotated", "mkv_attend_shared",
+                                 "mkv_attend_shared_workspace_size")))
                 _BINDING = module
     return _BINDING
 

@@ -16,7 +16,8 @@
 // slots, store and attend are scaled_cache.py's step_slots, store_scaled and attend_scaled in
 // the same way: a decode step's kernels run 4 to 20 us, and through Python methods and ctypes
 // the calls took 10 to 15 on the host.  They return their tensors (store: None on success
-// becomes True), the library's status as an int, or None for the general path.
+// becomes True), the library's status as an int, or None for the general path.  rotate, put and
+// attend_shared are scaled_step.py's calls in the same way: 20 us on the host became 4 to 6.
 
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
@@ -33,6 +34,7 @@
 
 #include "marathon_kvscaled.h"
 #include "marathon_kvshift.h"
+#include "marathon_kvstep.h"
 
 namespace {
 
@@ -385,6 +387,94 @@ PyObject* store(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   }
 }
 
+// An attention call's arguments, but for its workspace: cache descriptor's address, device index,
+// q, block_tables, starts, lens, scale, max_new, max_len, out, error_flags.
+int read_attend(PyObject* cache_at, PyObject* device, PyObject* q_o, PyObject* tables, PyObject* starts_o,
+                PyObject* lens_o, PyObject* scale, PyObject* max_new, PyObject* max_len, PyObject* out_o,
+                PyObject* flags_o, mkv_attend_desc_t& d, at::Device& dev, at::Tensor& out) {
+  if (at::impl::PythonTorchFunctionTLS::stack_len() != 0) return kOther;
+  const auto* cache = static_cast<const mkv_scaled_cache_t*>(PyLong_AsVoidPtr(cache_at));
+  if (cache == nullptr) return kError;
+  int64_t index, most_new = 0, most_len = 0;
+  const at::Tensor* q = plain(q_o);
+  if (!whole(device, 0, 127, index) || q == nullptr || !q->is_cuda()) return kOther;
+  dev = at::Device(at::kCUDA, static_cast<c10::DeviceIndex>(index));
+  Table tab;
+  int32_t* flags;
+  const int code = dtype_code(q->scalar_type());
+  if (q->dim() != 3 || q->device() != dev || (code != MKV_BF16 && code != MKV_F16) ||
+      cache->heads <= 0 || q->size(2) != cache->head_size || q->size(1) == 0 ||
+      q->size(1) % cache->heads != 0 || q->size(1) > INT32_MAX || q->stride(2) != 1 ||
+      needs_grad(*q) || !table_of(tables, &dev, tab) ||
+      flags_of(flags_o, dev, flags) != kUsual || c10::hip::current_device() != dev.index())
+    return kOther;
+  const int32_t* starts = vector_of(starts_o, dev, tab.n + 1);
+  const int32_t* lens = vector_of(lens_o, dev, tab.n);
+  if (starts == nullptr || lens == nullptr ||
+      (max_new != Py_None && !whole(max_new, 0, INT32_MAX, most_new)) ||
+      (max_len != Py_None && !whole(max_len, 0, INT32_MAX, most_len)))
+    return kOther;
+  if (scale == Py_None) {
+    d.softmax_scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(cache->head_size)));
+  } else {
+    if (!PyFloat_CheckExact(scale)) return kOther;
+    d.softmax_scale = static_cast<float>(PyFloat_AS_DOUBLE(scale));
+  }
+  if (out_o == Py_None) {
+    out = at::empty(q->sizes(), at::TensorOptions().dtype(q->dtype()).device(dev));
+  } else {
+    const at::Tensor* o = plain(out_o);
+    if (o == nullptr || o->device() != dev || o->scalar_type() != q->scalar_type() ||
+        o->sizes() != q->sizes() || o->stride(2) != 1 || needs_grad(*o))
+      return kOther;
+    // the general path tells rows that interleave from rows that share memory
+    const Range rows = range_of(*q), written = range_of(*o);
+    if (written.meets(rows.from, rows.to) || meets_cache(written, *cache)) return kOther;
+    out = *o;
+  }
+  const bool many = q->size(0) > 1, heads = q->size(1) > 1;
+  d.cache = *cache;
+  d.q = q->data_ptr();
+  d.out = out.data_ptr();
+  d.block_tables = tab.at;
+  d.starts = starts;
+  d.lens = lens;
+  d.error_flags = flags;
+  d.q_token_stride = many ? q->stride(0) : 0;
+  d.q_head_stride = heads ? q->stride(1) : 0;
+  d.out_token_stride = many ? out.stride(0) : 0;
+  d.out_head_stride = heads ? out.stride(1) : 0;
+  d.table_stride = tab.stride;
+  d.tokens = q->size(0);
+  d.table_width = static_cast<int32_t>(tab.width);
+  d.requests = static_cast<int32_t>(tab.n);
+  d.q_heads = static_cast<int32_t>(q->size(1));
+  d.dtype = code;
+  d.max_new = static_cast<int32_t>(most_new);
+  d.max_len = static_cast<int32_t>(most_len);
+  return kUsual;
+}
+
+// Launches the call with a workspace of `need` bytes, whose memory goes back in stream order.
+template <typename F>
+PyObject* launch_attend(mkv_attend_desc_t& d, int64_t need, const at::Device& dev, PyObject* out_o,
+                        const at::Tensor& out, F call) {
+  at::Tensor workspace;
+  if (need > 0) {
+    workspace = at::empty({need}, at::TensorOptions().dtype(at::kByte).device(dev));
+    d.workspace = workspace.data_ptr();
+    d.workspace_bytes = need;
+  }
+  void* stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = call(stream);
+  Py_END_ALLOW_THREADS
+  if (rc != MKV_OK) return PyLong_FromLong(rc);
+  if (out_o != Py_None) return (Py_INCREF(out_o), out_o);
+  return THPVariable_Wrap(out);
+}
+
 // attend(cache descriptor's address, device index, q, block_tables, starts, lens, scale,
 //        max_new, max_len, out, error_flags)
 PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -393,82 +483,228 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     return nullptr;
   }
   try {
+    mkv_attend_desc_t d{};
+    at::Device dev(at::kCPU);
+    at::Tensor out;
+    const int got = read_attend(args[0], args[1], args[2], args[3], args[4], args[5], args[6], args[7],
+                                args[8], args[9], args[10], d, dev, out);
+    if (got == kError) return nullptr;
+    if (got == kOther) Py_RETURN_NONE;
+    return launch_attend(d, g_attend_size(&d), dev, args[9], out,
+                         [&](void* stream) { return g_attend(&d, stream); });
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
+// ------------------------------------------------------- the step around the cache
+
+typedef decltype(&mkv_norm_rotate) rotate_fn;
+typedef decltype(&mkv_store_rotated) put_fn;
+typedef decltype(&mkv_attend_shared) shared_fn;
+typedef decltype(&mkv_attend_shared_workspace_size) shared_size_fn;
+rotate_fn g_rotate = nullptr;
+put_fn g_put = nullptr;
+shared_fn g_shared = nullptr;
+shared_size_fn g_shared_size = nullptr;
+
+// The heads' rows, and their output: a fresh one, or the rows themselves (kept in `out`).  Other
+// outputs are the general path's.
+bool rows_of(PyObject* x_o, PyObject* out_o, const at::Device& dev, int64_t d, int code,
+             mkv_head_rows_t& r, at::Tensor& out) {
+  const at::Tensor* x = plain(x_o);
+  if (x == nullptr || x->device() != dev || x->dim() != 3 || x->size(2) != d || x->stride(2) != 1 ||
+      dtype_code(x->scalar_type()) != code || x->size(1) > 65536 || needs_grad(*x))
+    return false;
+  if (out_o == Py_None) {
+    out = at::empty(x->sizes(), at::TensorOptions().dtype(x->dtype()).device(dev));
+  } else {
+    const at::Tensor* o = plain(out_o);
+    if (o == nullptr || o->device() != dev || o->scalar_type() != x->scalar_type() ||
+        o->sizes() != x->sizes() || o->strides() != x->strides() || o->data_ptr() != x->data_ptr() ||
+        needs_grad(*o))
+      return false;
+    out = *o;
+  }
+  const bool many = x->size(0) > 1, heads = x->size(1) > 1;
+  r.x = x->data_ptr();
+  r.out = out.data_ptr();
+  r.token_stride = many ? x->stride(0) : 0;
+  r.head_stride = heads ? x->stride(1) : 0;
+  r.out_token_stride = many ? out.stride(0) : 0;
+  r.out_head_stride = heads ? out.stride(1) : 0;
+  r.heads = static_cast<int32_t>(x->size(1));
+  return true;
+}
+
+// A contiguous vector on `dev` (of n values, unless n < 0) that needs no gradient, or null.
+const at::Tensor* values_of(PyObject* o, const at::Device& dev, int64_t n) {
+  const at::Tensor* t = plain(o);
+  return t == nullptr || t->device() != dev || t->dim() != 1 || !t->is_contiguous() ||
+                 (n >= 0 && t->size(0) != n) || needs_grad(*t)
+             ? nullptr
+             : t;
+}
+
+// inv_freq, q_weight, k_weight, eps.
+bool turn_of(PyObject* freq, PyObject* qw, PyObject* kw, PyObject* eps, const at::Device& dev, int64_t d,
+             mkv_turn_t& turn) {
+  if (freq != Py_None) {
+    const at::Tensor* f = values_of(freq, dev, -1);
+    if (f == nullptr || f->scalar_type() != at::kFloat || f->size(0) == 0 || f->size(0) % 16 != 0 ||
+        2 * f->size(0) > d)
+      return false;
+    turn.inv_freq = static_cast<const float*>(f->data_ptr());
+    turn.rotary = static_cast<int32_t>(2 * f->size(0));
+  }
+  if (!PyFloat_CheckExact(eps)) return eps == Py_None && qw == Py_None && kw == Py_None;
+  turn.norm = 1;
+  turn.eps = static_cast<float>(PyFloat_AS_DOUBLE(eps));
+  if (!(turn.eps >= 0.0f) || std::isinf(turn.eps)) return false;
+  int code = -1;
+  const void** to[2] = {&turn.q_weight, &turn.k_weight};
+  for (int i = 0; i < 2; ++i) {
+    PyObject* o = i == 0 ? qw : kw;
+    if (o == Py_None) continue;
+    const at::Tensor* w = values_of(o, dev, d);
+    if (w == nullptr) return false;
+    const int c = dtype_code(w->scalar_type());
+    if ((c != MKV_BF16 && c != MKV_F16 && c != MKV_F32) || (code >= 0 && c != code)) return false;
+    code = c;
+    *to[i] = w->data_ptr();
+  }
+  turn.weight_dtype = code < 0 ? 0 : code;
+  return true;
+}
+
+bool row_type(int code) { return code == MKV_BF16 || code == MKV_F16 || code == MKV_F32; }
+
+// rotate(q, k, positions, inv_freq, q_weight, k_weight, eps, out_q, out_k)
+PyObject* rotate(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 9 || g_rotate == nullptr) {
+    PyErr_SetString(PyExc_TypeError, "rotate takes 9 arguments, after bind_step()");
+    return nullptr;
+  }
+  try {
+    if (at::impl::PythonTorchFunctionTLS::stack_len() != 0) Py_RETURN_NONE;
+    const at::Tensor* q = plain(args[0]);
+    const at::Tensor* k = plain(args[1]);
+    if (q == nullptr || k == nullptr || !q->is_cuda() || q->dim() != 3 || k->dim() != 3 ||
+        q->size(0) != k->size(0) || c10::hip::current_device() != q->device().index())
+      Py_RETURN_NONE;
+    const at::Device dev = q->device();
+    const int64_t d = q->size(2), n = q->size(0);
+    const int code = dtype_code(q->scalar_type());
+    mkv_norm_rotate_desc_t desc{};
+    at::Tensor out_q, out_k;
+    if ((d != 64 && d != 128 && d != 256) || !row_type(code) ||
+        !turn_of(args[3], args[4], args[5], args[6], dev, d, desc.turn))
+      Py_RETURN_NONE;
+    if (desc.turn.rotary > 0) {
+      const at::Tensor* p = values_of(args[2], dev, n);
+      if (p == nullptr || (p->scalar_type() != at::kInt && p->scalar_type() != at::kLong)) Py_RETURN_NONE;
+      desc.positions = p->data_ptr();
+      desc.position_bytes = p->scalar_type() == at::kInt ? 4 : 8;
+    }
+    // (in place: q and k may be parts of one tensor, whose rows the general path tells apart)
+    if ((args[7] == Py_None) != (args[8] == Py_None) || (args[7] != Py_None && args[7] != args[0]) ||
+        (args[8] != Py_None && args[8] != args[1]))
+      Py_RETURN_NONE;
+    if (args[7] != Py_None) {
+      const Range a = range_of(*q), b = range_of(*k);
+      if (a.meets(b.from, b.to)) Py_RETURN_NONE;
+    }
+    if (!rows_of(args[0], args[7], dev, d, code, desc.q, out_q) ||
+        !rows_of(args[1], args[8], dev, d, code, desc.k, out_k))
+      Py_RETURN_NONE;
+    desc.tokens = n;
+    desc.head_size = static_cast<int32_t>(d);
+    desc.dtype = code;
+    void* stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_rotate(&desc, stream);
+    Py_END_ALLOW_THREADS
+    if (rc != MKV_OK) return PyLong_FromLong(rc);
+    PyObject* made = PyTuple_New(2);
+    if (made == nullptr) return nullptr;
+    for (int i = 0; i < 2; ++i) {
+      PyObject* given = args[7 + i];
+      PyObject* o = given != Py_None ? (Py_INCREF(given), given) : THPVariable_Wrap(i == 0 ? out_q : out_k);
+      if (o == nullptr) {
+        Py_DECREF(made);
+        return nullptr;
+      }
+      PyTuple_SET_ITEM(made, i, o);
+    }
+    return made;
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
+// put(cache descriptor's address, device index, q, k, v, block_tables, starts, lens, inv_freq,
+//     q_weight, k_weight, eps, out_q, error_flags)
+PyObject* put(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 14 || g_put == nullptr) {
+    PyErr_SetString(PyExc_TypeError, "put takes 14 arguments, after bind_step()");
+    return nullptr;
+  }
+  try {
     if (at::impl::PythonTorchFunctionTLS::stack_len() != 0) Py_RETURN_NONE;
     const auto* cache = static_cast<const mkv_scaled_cache_t*>(PyLong_AsVoidPtr(args[0]));
     if (cache == nullptr) return nullptr;
-    int64_t index, most_new = 0, most_len = 0;
+    int64_t index;
     const at::Tensor* q = plain(args[2]);
-    if (!whole(args[1], 0, 127, index) || q == nullptr || !q->is_cuda()) Py_RETURN_NONE;
+    const at::Tensor* k = plain(args[3]);
+    const at::Tensor* v = plain(args[4]);
+    // (an output of the caller's is told from k, v and the cache by the general path)
+    if (!whole(args[1], 0, 127, index) || q == nullptr || k == nullptr || v == nullptr || !q->is_cuda() ||
+        args[12] != Py_None)
+      Py_RETURN_NONE;
     const at::Device dev(at::kCUDA, static_cast<c10::DeviceIndex>(index));
+    const int code = dtype_code(q->scalar_type());
     Table tab;
     int32_t* flags;
-    const int code = dtype_code(q->scalar_type());
-    if (q->dim() != 3 || q->device() != dev || (code != MKV_BF16 && code != MKV_F16) ||
-        cache->heads <= 0 || q->size(2) != cache->head_size || q->size(1) == 0 ||
-        q->size(1) % cache->heads != 0 || q->size(1) > INT32_MAX || q->stride(2) != 1 ||
-        needs_grad(*q) || !table_of(args[3], &dev, tab) ||
-        flags_of(args[10], dev, flags) != kUsual || c10::hip::current_device() != dev.index())
-      Py_RETURN_NONE;
-    const int32_t* starts = vector_of(args[4], dev, tab.n + 1);
-    const int32_t* lens = vector_of(args[5], dev, tab.n);
-    if (starts == nullptr || lens == nullptr ||
-        (args[7] != Py_None && !whole(args[7], 0, INT32_MAX, most_new)) ||
-        (args[8] != Py_None && !whole(args[8], 0, INT32_MAX, most_len)))
-      Py_RETURN_NONE;
-    mkv_attend_desc_t d{};
-    if (args[6] == Py_None) {
-      d.softmax_scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(cache->head_size)));
-    } else {
-      if (!PyFloat_CheckExact(args[6])) Py_RETURN_NONE;
-      d.softmax_scale = static_cast<float>(PyFloat_AS_DOUBLE(args[6]));
-    }
+    mkv_store_rotated_desc_t d{};
     at::Tensor out;
-    if (args[9] == Py_None) {
-      out = at::empty(q->sizes(), at::TensorOptions().dtype(q->dtype()).device(dev));
-    } else {
-      const at::Tensor* o = plain(args[9]);
-      if (o == nullptr || o->device() != dev || o->scalar_type() != q->scalar_type() ||
-          o->sizes() != q->sizes() || o->stride(2) != 1 || needs_grad(*o))
-        Py_RETURN_NONE;
-      // the general path tells rows that interleave from rows that share memory
-      const Range rows = range_of(*q), written = range_of(*o);
-      if (written.meets(rows.from, rows.to) || meets_cache(written, *cache)) Py_RETURN_NONE;
-      out = *o;
-    }
-    const bool many = q->size(0) > 1, heads = q->size(1) > 1;
+    if (!row_type(code) || k->dim() != 3 || v->dim() != 3 || k->sizes() != v->sizes() ||
+        k->device() != dev || v->device() != dev || dtype_code(k->scalar_type()) != code ||
+        dtype_code(v->scalar_type()) != code || k->size(1) != cache->heads ||
+        k->size(2) != cache->head_size || k->stride(2) != 1 || v->stride(2) != 1 || needs_grad(*k) ||
+        needs_grad(*v) || c10::hip::current_device() != dev.index() || !table_of(args[5], &dev, tab) ||
+        flags_of(args[13], dev, flags) != kUsual || q->dim() != 3 || q->size(0) != k->size(0) ||
+        !turn_of(args[8], args[9], args[10], args[11], dev, cache->head_size, d.turn))
+      Py_RETURN_NONE;
+    const int32_t* starts = vector_of(args[6], dev, tab.n + 1);
+    const int32_t* lens = vector_of(args[7], dev, tab.n);
+    if (starts == nullptr || lens == nullptr || !rows_of(args[2], Py_None, dev, cache->head_size, code, d.q, out))
+      Py_RETURN_NONE;
+    const bool many = k->size(0) > 1, heads = k->size(1) > 1;
     d.cache = *cache;
-    d.q = q->data_ptr();
-    d.out = out.data_ptr();
+    d.k = k->data_ptr();
+    d.v = v->data_ptr();
+    d.k_token_stride = many ? k->stride(0) : 0;
+    d.k_head_stride = heads ? k->stride(1) : 0;
+    d.v_token_stride = many ? v->stride(0) : 0;
+    d.v_head_stride = heads ? v->stride(1) : 0;
     d.block_tables = tab.at;
     d.starts = starts;
     d.lens = lens;
     d.error_flags = flags;
-    d.q_token_stride = many ? q->stride(0) : 0;
-    d.q_head_stride = heads ? q->stride(1) : 0;
-    d.out_token_stride = many ? out.stride(0) : 0;
-    d.out_head_stride = heads ? out.stride(1) : 0;
     d.table_stride = tab.stride;
     d.tokens = q->size(0);
     d.table_width = static_cast<int32_t>(tab.width);
     d.requests = static_cast<int32_t>(tab.n);
-    d.q_heads = static_cast<int32_t>(q->size(1));
     d.dtype = code;
-    d.max_new = static_cast<int32_t>(most_new);
-    d.max_len = static_cast<int32_t>(most_len);
-    const int64_t need = g_attend_size(&d);
-    at::Tensor workspace;  // (its memory goes back in stream order)
-    if (need > 0) {
-      workspace = at::empty({need}, at::TensorOptions().dtype(at::kByte).device(dev));
-      d.workspace = workspace.data_ptr();
-      d.workspace_bytes = need;
-    }
     void* stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
     int rc;
     Py_BEGIN_ALLOW_THREADS
-    rc = g_attend(&d, stream);
+    rc = g_put(&d, stream);
     Py_END_ALLOW_THREADS
     if (rc != MKV_OK) return PyLong_FromLong(rc);
-    if (args[9] != Py_None) return (Py_INCREF(args[9]), args[9]);
     return THPVariable_Wrap(out);
   } catch (const std::exception& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
@@ -476,21 +712,70 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   }
 }
 
-// The addresses of mkv_step_slots, mkv_store_scaled, mkv_attend_scaled and
-// mkv_attend_workspace_size.
-PyObject* bind_scaled(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  void* p[4];
-  if (nargs != 4) {
-    PyErr_SetString(PyExc_TypeError, "bind_scaled takes 4 addresses");
+// attend_shared(cache descriptor's address, device index, q, block_tables, starts, lens, groups,
+//               shared, scale, max_new, max_shared, max_own, out, error_flags)
+PyObject* attend_shared(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 14 || g_shared == nullptr || g_shared_size == nullptr) {
+    PyErr_SetString(PyExc_TypeError, "attend_shared takes 14 arguments, after bind_step()");
     return nullptr;
+  }
+  try {
+    mkv_attend_shared_desc_t d{};
+    at::Device dev(at::kCPU);
+    at::Tensor out;
+    int64_t most = 0;
+    const int got = read_attend(args[0], args[1], args[2], args[3], args[4], args[5], args[8], args[9],
+                                args[11], args[12], args[13], d.attend, dev, out);
+    if (got == kError) return nullptr;
+    if (got == kOther || (args[10] != Py_None && !whole(args[10], 0, INT32_MAX, most))) Py_RETURN_NONE;
+    d.shared = vector_of(args[7], dev, -1);
+    if (d.shared == nullptr) Py_RETURN_NONE;
+    const int64_t n = THPVariable_Unpack(args[7]).size(0);
+    d.groups = n <= MKV_MAX_REQUESTS ? vector_of(args[6], dev, n + 1) : nullptr;
+    if (d.groups == nullptr) Py_RETURN_NONE;
+    d.n_groups = static_cast<int32_t>(n);
+    d.max_shared = static_cast<int32_t>(most);
+    return launch_attend(d.attend, g_shared_size(&d), dev, args[12], out,
+                         [&](void* stream) { return g_shared(&d, stream); });
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
+// The addresses that a bind takes; false with an exception set.
+bool addresses(PyObject* const* args, Py_ssize_t nargs, void* (&p)[4]) {
+  if (nargs != 4) {
+    PyErr_SetString(PyExc_TypeError, "4 addresses");
+    return false;
   }
   for (int i = 0; i < 4; ++i) {
     p[i] = PyLong_AsVoidPtr(args[i]);
     if (p[i] == nullptr) {
       if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "NULL function");
-      return nullptr;
+      return false;
     }
   }
+  return true;
+}
+
+// The addresses of mkv_norm_rotate, mkv_store_rotated, mkv_attend_shared and
+// mkv_attend_shared_workspace_size.
+PyObject* bind_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  void* p[4];
+  if (!addresses(args, nargs, p)) return nullptr;
+  g_rotate = reinterpret_cast<rotate_fn>(p[0]);
+  g_put = reinterpret_cast<put_fn>(p[1]);
+  g_shared = reinterpret_cast<shared_fn>(p[2]);
+  g_shared_size = reinterpret_cast<shared_size_fn>(p[3]);
+  Py_RETURN_NONE;
+}
+
+// The addresses of mkv_step_slots, mkv_store_scaled, mkv_attend_scaled and
+// mkv_attend_workspace_size.
+PyObject* bind_scaled(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  void* p[4];
+  if (!addresses(args, nargs, p)) return nullptr;
   g_slots = reinterpret_cast<slots_fn>(p[0]);
   g_store = reinterpret_cast<store_fn>(p[1]);
   g_attend = reinterpret_cast<attend_fn>(p[2]);
@@ -520,6 +805,14 @@ PyMethodDef methods[] = {
      "mkv_attend_scaled on torch tensors; None: take the general path"},
     {"bind_scaled", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind_scaled)),
      METH_FASTCALL, "the addresses that slots, store and attend call"},
+    {"rotate", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rotate)), METH_FASTCALL,
+     "mkv_norm_rotate on torch tensors; None: take the general path"},
+    {"put", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(put)), METH_FASTCALL,
+     "mkv_store_rotated on torch tensors; None: take the general path"},
+    {"attend_shared", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attend_shared)),
+     METH_FASTCALL, "mkv_attend_shared on torch tensors; None: take the general path"},
+    {"bind_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind_step)),
+     METH_FASTCALL, "the addresses that rotate, put and attend_shared call"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "marathon_binding", nullptr, -1, methods,

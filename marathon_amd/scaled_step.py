@@ -15,6 +15,8 @@ be captured into a graph.  The turn is the rotate-half one of the rest of this p
 first ``2 * len(inv_freq)`` values of each head: its keys are what :class:`ScaledShifts` and
 :func:`~marathon_amd.scatter_shifted` move (kvshift.py:44-61).
 
+The calls on tensors that need no conversion go through the CPython binding, as the cache's do.
+
 There is no CPU path and no gradient: tensors that are not on a HIP device raise, and so do
 rows that require a gradient or carry a tangent.  C ABI: ``include/marathon_kvstep.h``.
 """
@@ -38,6 +40,7 @@ from .scaled_cache import (
     _rows_of,
     _steps,
     _table,
+    _usual,
 )
 from .shift_kernels import current_stream, dtype_code
 from .spans import _on
@@ -143,6 +146,11 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor | None
 
     fp32 throughout and rounded once; angles are taken in 64 bits.  A head of zeros with eps 0 is
     NaN, as is one with an infinity."""
+    made = _usual.rotate(q, k, positions, inv_freq, q_weight, k_weight, eps, out_q, out_k)
+    if made is not None:
+        if type(made) is int:
+            _lib.check(made)
+        return made
     for name, t in (("q", q), ("k", k)):
         if not t.is_cuda:
             raise RuntimeError(f"norm_rotate: {name} is not on a HIP device; there is no CPU path")
@@ -188,6 +196,12 @@ def store_rotated(cache: ScaledCache, q: torch.Tensor, k: torch.Tensor, v: torch
     :func:`~marathon_amd.scaled_cache.store_scaled` does.  Keys are rounded once, to their codes.
     Rows of no request are not read, and of ``out_q`` left as they were (in a fresh one,
     undefined)."""
+    made = _usual.put(*cache.handle, q, k, v, block_tables, starts, lens, inv_freq, q_weight, k_weight,
+                      eps, out_q, error_flags)
+    if made is not None:
+        if type(made) is int:
+            _lib.check(made)
+        return made
     device, d = cache.device, cache.head_size
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.dim() != 3 or t.shape[2] != d or t.shape[0] != q.shape[0]:
@@ -234,6 +248,12 @@ def attend_shared(cache: ScaledCache, q: torch.Tensor, block_tables: torch.Tenso
     ``max_new``, ``max_shared`` and ``max_own``: the largest number of new tokens of a request, of
     tokens that a group shares and of tokens that a request has behind them, where the host knows
     them; they choose launch shapes only."""
+    made = _usual.attend_shared(*cache.handle, q, block_tables, starts, lens, groups, shared,
+                                softmax_scale, max_new, max_shared, max_own, out, error_flags)
+    if made is not None:
+        if type(made) is int:
+            _lib.check(made)
+        return made
     desc = _lib.AttendSharedDesc()
     desc.attend, out = _attend_desc("attend_shared", cache, q, block_tables, starts, lens,
                                     softmax_scale, max_new, max_own, out, error_flags)
