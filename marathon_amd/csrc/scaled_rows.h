@@ -191,4 +191,26 @@ __device__ __forceinline__ void load16(const char* p, float* x) {
   unpack8<ET>(b, x + 8);
 }
 
+// Host: the tokens that a workgroup of a store looks through, of `each` workgroups if it were one.
+// Decode steps want every token, and small stores every block, a workgroup of its own; large
+// stores few workgroups that lead nothing, up to one a block.  In us with 1 / 4 / 8 / 16 tokens a
+// workgroup, blocks of 16, 8 heads of 128 but where said:
+//   1,000 requests of one token 11.8 / 15.7 / 26 / 44, 4,096 39 / 39 / 36 / 52
+//   8 requests of 65, 4 heads 5.3 / 7.2;  488 of 16, 4 heads 16.1 with 4, 18.9 with 16
+//   one of 1,000 12.9 / 5.9 / 6.6 / 8.5, of 2,000 28 / 9.8 / 7.6 / 9.2, of 4,000 52 / 16.6 / 11.7 /
+//   10.5, of 22,000 269 / 76 / 48 / 30
+//   13 requests of 5,003 in all, 4 heads of 64 12.8 / 8.1 / 9.3 / 9.4
+// and with 4 / 16 / 64: blocks of 64, one of 1,000 8.9 / 8.1 / 10.1, of 8,000 107 / 36 / 15;
+// blocks of 128, one of 8,000 217 / 49 / 19, and 17 with 128.
+inline int store_group(int64_t tokens, int32_t requests, int64_t each, int32_t block_size) {
+  const int64_t ahead = tokens / requests;  // a request's on average
+  if (ahead < 16 || (each <= 4096 && ahead < 256))
+    return each <= 4096 ? 1 : 4;
+  if (each > 24576)
+    return block_size;
+  if (each > 12288)
+    return ahead >= 64 ? 16 : 4;
+  return block_size >= 64 && ahead >= 64 ? 16 : each > 4096 && ahead >= 1024 ? 8 : 4;
+}
+
 }  // namespace mkv_scaled
