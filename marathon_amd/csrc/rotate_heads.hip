@@ -207,7 +207,7 @@ __device__ __forceinline__ void turn_heads(const HeadRows& rows, const Turn& t, 
   if (owned == 0) return;
   const bool put = owned >> mine & 1;
   f32x2 turn[8];
-  turns8(lds + mine * t.half, place, turn);
+  turns8(lds + min(mine, s.count - 1) * t.half, place, turn);
   for (int first = s.h0; first < s.h1; first += kHeads, h += kHeads) {
     float x[16];
     unpack8<ET>(a, x);
