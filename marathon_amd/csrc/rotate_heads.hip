@@ -534,6 +534,8 @@ __device__ __forceinline__ void put_queries(const PutParams& p, f32x2* s_turn) {
         owned |= 1u << j;
         at = static_cast<int>(threadIdx.x & 63) == j ? static_cast<int>(t + shift) : at;
       }
+      // (a lane may ask another: `half` is a multiple of 16, so the last round of make_angles has at
+      // least 16 lanes, and no wave has more tokens)
       if (owned != 0 && p.turn.half > 0)
         make_angles(lds, p.turn, s.count, [&](int j) { return static_cast<double>(__shfl(at, j)); });
       return owned;

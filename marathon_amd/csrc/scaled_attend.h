@@ -183,9 +183,11 @@ __device__ __forceinline__ bool find_tile(const P& p, int64_t tile, Tile& t) {
     const int32_t* groups = p.g.groups;
     const int requests = p.s.requests;
     const int g = p.g.count == 1 ? 0 : last_at_most(p.g.count, tile, [=](int i) {
+      // (bad groups are come across where group_of() does, and by nobody else's tiles)
       const int a = groups[i];
-      return a < 0 || a > requests ? int64_t{0}
-                                   : shared_begin(static_cast<int64_t>(starts[a]) * group, BM, i);
+      return a < 0 ? int64_t{0}
+                   : a > requests ? INT64_MAX
+                                  : shared_begin(static_cast<int64_t>(starts[a]) * group, BM, i);
     });
     Group of;
     if (g < 0 || !read_group(p.c, p.s, p.g, p.tokens, g, of)) return false;
