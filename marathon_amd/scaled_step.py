@@ -57,6 +57,7 @@ def _vector(name: str, t: torch.Tensor, device, n: int) -> int:
 
 def _turn(who: str, device, head_size: int, inv_freq, q_weight, k_weight, eps) -> _lib.Turn:
     turn = _lib.Turn()
+    _no_gradient(who, inv_freq=inv_freq, q_weight=q_weight, k_weight=k_weight)
     if inv_freq is not None:
         if inv_freq.dtype != torch.float32:
             raise TypeError(f"inv_freq {inv_freq.dtype}: float32")
@@ -78,7 +79,6 @@ def _turn(who: str, device, head_size: int, inv_freq, q_weight, k_weight, eps) -
         if w.dtype not in _DTYPES or w.dtype != weights[0].dtype:
             raise TypeError(f"weights {[w.dtype for w in weights]}: of one type, one of {_DTYPES}")
         turn.weight_dtype = dtype_code(w.dtype)
-    _no_gradient(who, inv_freq=inv_freq, q_weight=q_weight, k_weight=k_weight)
     if q_weight is not None:
         turn.q_weight = _vector("q_weight", q_weight, device, head_size)
     if k_weight is not None:

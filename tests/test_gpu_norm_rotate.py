@@ -215,3 +215,11 @@ def test_refusals(gpu):
     with torch.no_grad():
         norm_rotate(q.clone().requires_grad_(), k, pos, inv)
     torch.cuda.synchronize()
+
+
+def test_frequencies_that_learn_are_refused_without_a_norm_too(gpu):
+    x = torch.randn(3, 2, 64, device=gpu)
+    pos, inv = torch.arange(3, device=gpu), torch.rand(32, device=gpu)
+    for eps in (None, 1e-6):
+        with pytest.raises(RuntimeError, match="backward"):
+            norm_rotate(x, x.clone(), pos, inv.clone().requires_grad_(), eps=eps)
