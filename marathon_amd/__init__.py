@@ -8,7 +8,9 @@ launches through :class:`marathon_amd.spans.ShiftPlan`; the worker-side load pat
 :mod:`marathon_amd.connector`.  The same for a cache held in 8 bits with a scale for each
 block of tokens and head (:mod:`marathon_amd.scaled_cache`): :class:`ScaledCache`, its step's
 tables and slots (:func:`step_slots`), :func:`store_scaled`, :func:`attend_scaled` and
-:class:`ScaledShifts`.  Everything that touches KV runs in hand-written gfx950 kernels
+:class:`ScaledShifts`; and what stands around them in a model's step
+(:mod:`marathon_amd.scaled_step`): :func:`norm_rotate`, :func:`store_rotated` and
+:func:`attend_shared`.  Everything that touches KV runs in hand-written gfx950 kernels
 (``csrc/*.hip``) behind the C ABI in ``include/``.
 """
 
