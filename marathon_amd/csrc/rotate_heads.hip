@@ -23,6 +23,10 @@
 #include "marathon_kvstep.h"
 #include "scaled_rows.h"
 
+#include <algorithm>
+#include <numeric>
+#include <type_traits>
+
 #pragma clang fp contract(off)
 
 namespace {
@@ -170,8 +174,8 @@ __device__ __forceinline__ void turns8(const f32x2* lds, const Place<D>& place, 
   for (int i = 0; i < 8; ++i) turn[i] = place.turned ? lds[place.a + i] : f32x2{1.0f, 0.0f};
 }
 
-// A wave's share of one side: heads [h0, h1) of one token, as many at once as a wave holds; or, of
-// heads fewer than that, all of `count` tokens from `token` on.
+// A wave's share of one side: heads [h0, h1) of one token; or (SEVERAL) all heads of `count` tokens
+// from `token` on.  As many at once as a wave holds, in the order (token, head).
 struct Share {
   int64_t token;
   int count, h0, h1;
@@ -180,24 +184,26 @@ struct Share {
 // The share's heads: the next heads' loads are in flight while these are worked on.  Behind the
 // first loads, `angles` makes the wave's (cos, sin) in LDS, [token][half], and says which of the
 // tokens are somebody's (a bit each): what finds positions is waited for beside the rows.
-template <int ET, int D, typename F>
+template <int ET, int D, bool SEVERAL, typename F>
 __device__ __forceinline__ void turn_heads(const HeadRows& rows, const Turn& t, int side,
                                            const Share& s, const f32x2* lds, F angles) {
   constexpr int kBytes = ET == MKV_F32 ? 4 : 2, kHeads = Place<D>::kHeads;
   const int lane = threadIdx.x & 63, sub = lane / Place<D>::kLanes;
   const Place<D> place(lane % Place<D>::kLanes, t.half);
-  const int heads = s.h1 - s.h0, mine = s.count > 1 ? sub / heads : 0;
-  int h = s.h0 + (s.count > 1 ? sub % heads : sub);
-  const char* in = rows.x + (s.token + mine) * rows.token;
-  char* out = rows.out + (s.token + mine) * rows.out_token;
-  const int end = mine < s.count ? s.h1 : 0;
+  const int heads = s.h1 - s.h0, count = SEVERAL ? s.count : 1;
+  const int skip = SEVERAL ? kHeads / heads : 0, step = kHeads - skip * heads;  // tokens, heads a round
+  int mine = SEVERAL ? sub / heads : 0, h = s.h0 + sub - mine * heads;
+  const char* in = rows.x + s.token * rows.token;
+  char* out = rows.out + s.token * rows.out_token;
   Raw8<ET> a{}, b{};
-  const auto fetch = [&](int h) {
+  const auto held = [&](int token, int h) { return token < count && h < s.h1; };
+  const auto fetch = [&](int token, int h) {
     const char* at = in + h * rows.head;
+    if constexpr (SEVERAL) at += token * rows.token;
     a = fetch8<ET>(at + place.a * kBytes);
     b = fetch8<ET>(at + place.b * kBytes);
   };
-  if (h < end) fetch(h);
+  if (held(mine, h)) fetch(mine, h);
   float w[16];
   if (t.norm) {
     weights8(t.weight[side], t.weight_type, place.a, w);
@@ -205,20 +211,26 @@ __device__ __forceinline__ void turn_heads(const HeadRows& rows, const Turn& t, 
   }
   const uint32_t owned = angles();
   if (owned == 0) return;
-  const bool put = owned >> mine & 1;
   f32x2 turn[8];
-  turns8(lds + min(mine, s.count - 1) * t.half, place, turn);
-  for (int first = s.h0; first < s.h1; first += kHeads, h += kHeads) {
+  if constexpr (!SEVERAL) turns8(lds, place, turn);
+  for (int first = 0; first < count * heads; first += kHeads) {
+    if constexpr (SEVERAL) turns8(lds + min(mine, count - 1) * t.half, place, turn);
     float x[16];
     unpack8<ET>(a, x);
     unpack8<ET>(b, x + 8);
-    if (h + kHeads < end) fetch(h + kHeads);
+    int next = mine + skip, h_next = h + step;
+    if (SEVERAL && h_next >= s.h1) ++next, h_next -= heads;
+    if (held(next, h_next)) fetch(next, h_next);
     if (t.norm) normalise<D>(x, w, t);
     if (t.half > 0) rotate(x, turn);
-    if (h < end && put) {
-      put8<ET>(out + h * rows.out_head + place.a * kBytes, x);
-      put8<ET>(out + h * rows.out_head + place.b * kBytes, x + 8);
+    if (held(mine, h) && (owned >> mine & 1)) {
+      char* to = out + h * rows.out_head;
+      if constexpr (SEVERAL) to += mine * rows.out_token;
+      put8<ET>(to + place.a * kBytes, x);
+      put8<ET>(to + place.b * kBytes, x + 8);
     }
+    mine = next;
+    h = h_next;
   }
 }
 
@@ -249,7 +261,12 @@ struct Cut {
 };
 
 Cut cut_heads(int heads, int at_once, int most) {
-  if (heads > 0 && 2 * heads <= at_once) return {at_once / heads, heads, 1};
+  // the fewest tokens whose heads leave no lane idle (at most as many as heads at once), against a
+  // token a wave or as many as fit in one round: 22,141 tokens of 5 + 1 heads of 128 19.6 to 24.4 us,
+  // of 10 + 2 29.5 to 34.6, of 5 + 1 into the cache 25.3 to 34.8; six rounds for all sides: 2,000
+  // tokens of 40 + 8 fp32 heads 27.6 to 22.5
+  const int tokens = heads > 0 ? std::min(at_once / std::gcd(heads, at_once), at_once * most / heads) : 1;
+  if (tokens > 1) return {tokens, heads, 1};
   const int passes = (heads + at_once - 1) / at_once, waves = (passes + most - 1) / most;
   const int each = at_once * (waves > 0 ? (passes + waves - 1) / waves : 1);
   return {1, each, (heads + each - 1) / each};
@@ -269,8 +286,9 @@ struct RotateParams {
 
 constexpr int kWaves = 4;
 
-// Queries' waves first, then the keys'.
-template <int ET, int D>
+// Queries' waves first, then the keys'.  SEVERAL: of one side or both, waves have several tokens (the
+// code for that costs the others 2%).
+template <int ET, int D, bool SEVERAL>
 __global__ __launch_bounds__(64 * kWaves) void norm_rotate_kernel(RotateParams p) {
   __shared__ f32x2 s_turn[kWaves][Place<D>::kHeads * D / 2];
   const int wave = uni(threadIdx.x >> 6);
@@ -285,14 +303,18 @@ __global__ __launch_bounds__(64 * kWaves) void norm_rotate_kernel(RotateParams p
   s.count = static_cast<int>(min(static_cast<int64_t>(cut.tokens), p.tokens - s.token));
   s.h0 = unit % cut.parts * cut.each;
   s.h1 = min(s.h0 + cut.each, rows.heads);
-  turn_heads<ET, D>(rows, p.turn, side, s, s_turn[wave], [&]() {
+  const auto angles = [&]() {
     if (p.turn.half > 0)
-      make_angles(s_turn[wave], p.turn, s.count, [&](int i) {
+      make_angles(s_turn[wave], p.turn, SEVERAL ? s.count : 1, [&](int i) {
         return p.wide ? static_cast<double>(static_cast<const int64_t*>(p.positions)[s.token + i])
                       : static_cast<double>(static_cast<const int32_t*>(p.positions)[s.token + i]);
       });
     return 0xFFFFFFFFu;
-  });
+  };
+  if (SEVERAL && cut.tokens > 1)
+    turn_heads<ET, D, SEVERAL>(rows, p.turn, side, s, s_turn[wave], angles);
+  else
+    turn_heads<ET, D, false>(rows, p.turn, side, s, s_turn[wave], angles);
 }
 
 // ------------------------------------------------------------- into the block-scaled cache
@@ -499,7 +521,7 @@ __device__ __forceinline__ void put_keys(const PutParams& p, f32x2* s_turn, uint
 
 // Queries: the waves of a workgroup, and of the planes beside it, take turns at the tokens and
 // at their heads.
-template <int ET, int D>
+template <int ET, int D, bool SEVERAL>
 __device__ __forceinline__ void put_queries(const PutParams& p, f32x2* s_turn) {
   const int waves = blockDim.x >> 6, wave = uni(threadIdx.x >> 6);
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.group;
@@ -513,7 +535,7 @@ __device__ __forceinline__ void put_queries(const PutParams& p, f32x2* s_turn) {
     s.count = min(p.cut.tokens, here - first);
     s.h0 = i % p.cut.parts * p.cut.each;
     s.h1 = min(s.h0 + p.cut.each, p.q.heads);
-    turn_heads<ET, D>(p.q, p.turn, 0, s, lds, [&]() {
+    turn_heads<ET, D, SEVERAL>(p.q, p.turn, 0, s, lds, [&]() {
       // each token's position, in the lane of its number; a request is looked up once for all of
       // its tokens
       uint32_t owned = 0;
@@ -549,8 +571,10 @@ __global__ __launch_bounds__(64 * kMaxWaves) void put_kernel(PutParams p) {
   __shared__ uint32_t s_max[kMaxWaves][2];
   if (static_cast<int>(blockIdx.y) < p.planes)
     put_keys<ET, D>(p, s_turn, s_max);
+  else if (p.cut.tokens > 1)
+    put_queries<ET, D, true>(p, s_turn);
   else
-    put_queries<ET, D>(p, s_turn);
+    put_queries<ET, D, false>(p, s_turn);
 }
 
 // ------------------------------------------------------------------------- host
@@ -610,12 +634,19 @@ int check_rows(const char* who, const char* name, const mkv_head_rows_t& r, int6
 
 template <int ET>
 void rotate_launch(int d, dim3 grid, const RotateParams& p, hipStream_t s) {
-  if (d == 64)
-    norm_rotate_kernel<ET, 64><<<grid, 64 * kWaves, 0, s>>>(p);
-  else if (d == 128)
-    norm_rotate_kernel<ET, 128><<<grid, 64 * kWaves, 0, s>>>(p);
+  const auto launch = [&](auto several) {
+    constexpr bool kSeveral = decltype(several)::value;
+    if (d == 64)
+      norm_rotate_kernel<ET, 64, kSeveral><<<grid, 64 * kWaves, 0, s>>>(p);
+    else if (d == 128)
+      norm_rotate_kernel<ET, 128, kSeveral><<<grid, 64 * kWaves, 0, s>>>(p);
+    else
+      norm_rotate_kernel<ET, 256, kSeveral><<<grid, 64 * kWaves, 0, s>>>(p);
+  };
+  if (p.cut[0].tokens > 1 || p.cut[1].tokens > 1)
+    launch(std::true_type());
   else
-    norm_rotate_kernel<ET, 256><<<grid, 64 * kWaves, 0, s>>>(p);
+    launch(std::false_type());
 }
 
 template <int ET>

@@ -197,3 +197,42 @@ def test_a_cache_beyond_4_gib(gpu):
     args = i32([0, 1, 2], gpu), i32([180, 190], gpu), i32([0, 2], gpu), i32([160], gpu)
     got = [attend_shared(cache, q, t, *args) for t in (near, near + blocks - 40)]
     assert torch.equal(*got)
+
+
+@pytest.mark.parametrize("qh,kh,d,rotary", [(5, 1, 128, 128), (10, 3, 128, 32), (3, 7, 64, 64), (40, 8, 64, 32),
+                                            (1, 1, 64, 64), (5, 2, 256, 256), (1, 3, 256, 64)])
+def test_a_large_call_does_what_small_ones_do(gpu, qh, kh, d, rotary):
+    """Bit for bit: waves that take several tokens and rounds, against those that take one, and the
+    queries of requests whose ends lie within a wave's tokens, beside rows of nobody."""
+    rng = np.random.default_rng(qh * d + kh)
+    n = 8192 * (1024 // d) // qh + 13
+    q, k, v = (torch.randn((n, h, d), device=gpu).to(torch.bfloat16) for h in (qh, kh, kh))
+    w = torch.randn(d, device=gpu, dtype=torch.bfloat16)
+    inv = freq(rotary).to(gpu)
+    new = rng.integers(0, 2 * n // 300, 300)
+    new[rng.integers(0, 300, 60)] = 1
+    starts = 5 + np.concatenate(([0], np.cumsum(new)))
+    assert starts[-1] > n // 2
+    new, starts = np.diff(np.minimum(starts, n - 3)), np.minimum(starts, n - 3)
+    held = rng.integers(0, 40, 300)
+    lens = held + new
+    at = np.zeros(n, np.int64)
+    for r in range(300):
+        at[starts[r]:starts[r + 1]] = held[r] + np.arange(new[r])
+    positions = i32(at, gpu)
+    all_q, all_k = norm_rotate(q, k, positions, inv, q_weight=w, k_weight=w)
+    for first in range(0, n, 997):
+        part = slice(first, first + 997)
+        some = norm_rotate(q[part], k[part], positions[part], inv, q_weight=w, k_weight=w)
+        assert torch.equal(some[0], all_q[part]) and torch.equal(some[1], all_k[part])
+    need = -(-lens // 16)
+    tables = np.zeros((300, need.max()), np.int32)
+    for r, b in enumerate(np.cumsum(need) - need):
+        tables[r, :need[r]] = b + np.arange(need[r])
+    cache = fresh_cache(gpu, int(need.sum()) + 1, kh, d)
+    out = torch.full_like(q, 77.0)
+    store_rotated(cache, q, k, v, i32(tables, gpu), i32(starts, gpu), i32(lens, gpu), inv, q_weight=w,
+                  k_weight=w, out_q=out)
+    a, b = int(starts[0]), int(starts[-1])
+    assert torch.equal(out[a:b], all_q[a:b])
+    assert (out[:a] == 77.0).all() and (out[b:] == 77.0).all()
