@@ -250,9 +250,11 @@ __device__ __forceinline__ void make_angles(f32x2* lds, const Turn& t, int count
 }
 
 // Host: how many times as many heads as it holds at once a wave takes, of `all` that there are: one
-// while that many waves fill the chip once, then as many as share a token's angles and have the next
-// heads' loads in flight (22,141 tokens of 40 + 8 heads of 128: 2 96.5 us, 3 91.8, 6 87.1).
-int passes_for(int64_t all) { return all >= 8192 ? 6 : 1; }
+// while so many waves fill the chip less than once, two while they fill it once or twice, then as
+// many as share a token's angles and have the next heads' loads in flight.  (With 1 / 2 / 6: 800
+// tokens of 32 + 8 heads of 128 5.1 / 5.1 / 5.8 us, 1,600 9.1 / 7.7 / 8.3, 4,000 20.5 / 18.6 / 17.3;
+// 22,141 of 40 + 8 109 / 93 / 87.)
+int passes_for(int64_t all) { return all >= 8192 ? 6 : all >= 3500 ? 2 : 1; }
 
 // Host: how a side's heads are shared out: tokens and heads that a wave takes, and waves of as many
 // tokens.
