@@ -47,6 +47,7 @@ struct HeadRows {
   char* out;
   int64_t token, head, out_token, out_head;  // bytes
   int32_t heads;
+  int32_t stream;  // the output past the caches
 };
 
 // Quarter turns of an angle a position, in 64 bits.
@@ -126,7 +127,7 @@ __device__ __forceinline__ void weights8(const char* w, int type, int at, float*
 }
 
 template <int ET>
-__device__ __forceinline__ void put8(char* p, const float* x) {
+__device__ __forceinline__ void put8(char* p, const float* x, bool stream) {
   if constexpr (ET == MKV_F32) {
     reinterpret_cast<u32x4*>(p)[0] = u32x4{__float_as_uint(x[0]), __float_as_uint(x[1]),
                                            __float_as_uint(x[2]), __float_as_uint(x[3])};
@@ -143,7 +144,13 @@ __device__ __forceinline__ void put8(char* p, const float* x) {
       else
         w[j] = __builtin_bit_cast(uint32_t, h2{static_cast<_Float16>(x[2 * j]), static_cast<_Float16>(x[2 * j + 1])});
     }
-    *reinterpret_cast<u32x4*>(p) = w;
+    if (stream) {
+      asm volatile("" ::: "memory");  // (else the two stores become one, an ordinary one)
+      __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(p));
+      asm volatile("" ::: "memory");
+    } else {
+      *reinterpret_cast<u32x4*>(p) = w;
+    }
   }
 }
 
@@ -226,8 +233,8 @@ __device__ __forceinline__ void turn_heads(const HeadRows& rows, const Turn& t, 
     if (held(mine, h) && (owned >> mine & 1)) {
       char* to = out + h * rows.out_head;
       if constexpr (SEVERAL) to += mine * rows.out_token;
-      put8<ET>(to + place.a * kBytes, x);
-      put8<ET>(to + place.b * kBytes, x + 8);
+      put8<ET>(to + place.a * kBytes, x, rows.stream);
+      put8<ET>(to + place.b * kBytes, x + 8, rows.stream);
     }
     mine = next;
     h = h_next;
@@ -617,7 +624,7 @@ int check_rows(const char* who, const char* name, const mkv_head_rows_t& r, int6
   for (const int64_t s : {r.token_stride, r.head_stride, r.out_token_stride, r.out_head_stride})
     if (s < 0 || s > most) return mkv_fail(MKV_ERR_ARG, "%s: a stride of %s is out of range", who, name);
   *out = HeadRows{static_cast<const char*>(r.x), static_cast<char*>(r.out), r.token_stride * eb,
-                  r.head_stride * eb, r.out_token_stride * eb, r.out_head_stride * eb, r.heads};
+                  r.head_stride * eb, r.out_token_stride * eb, r.out_head_stride * eb, r.heads, 0};
   if (tokens == 0 || r.heads == 0) return MKV_OK;
   if (r.x == nullptr || r.out == nullptr) return mkv_fail(MKV_ERR_ARG, "%s: %s is NULL", who, name);
   if (((reinterpret_cast<uintptr_t>(r.x) | reinterpret_cast<uintptr_t>(r.out) | out->token |
@@ -632,6 +639,16 @@ int check_rows(const char* who, const char* name, const mkv_head_rows_t& r, int6
     reach += step * (n - 1);
   }
   return MKV_OK;
+}
+
+// Whether outputs of `bytes` go past the caches: where they would not stay in them (256 MB) till they
+// are read, and a store of a wave writes whole lines of 128 bytes (other types, smaller heads and
+// parts of heads lose 2 to 13%).  Calls that write in turns to two outputs, without / with: 12,000
+// tokens of 40 + 8 heads of 128 (147 MB) 52.4 / 55.4 us, 14,000 67.0 / 64.3, 22,141 105 / 99; into the
+// cache 12,000 63.0 / 66.0, 16,000 89.6 / 86.6, 22,141 126 / 118.5.  (One output over and over, which
+// the caches absorb: 22,141 tokens 87 without.)
+int streams(int64_t bytes, int head_size, int rotary, int64_t eb) {
+  return bytes >= int64_t{150} << 20 && eb == 2 && head_size >= 128 && rotary == head_size;
 }
 
 template <int ET>
@@ -690,6 +707,8 @@ extern "C" int mkv_norm_rotate(const mkv_norm_rotate_desc_t* d, void* stream) {
     if ((reinterpret_cast<uintptr_t>(d->positions) & (d->position_bytes - 1)) != 0)
       return mkv_fail(MKV_ERR_ALIGN, "%s: positions are not aligned", who);
   }
+  p.side[0].stream = p.side[1].stream =
+      streams(d->tokens * (d->q.heads + d->k.heads) * d->head_size * eb, d->head_size, d->turn.rotary, eb);
   p.positions = d->positions;
   p.wide = d->position_bytes == 8;
   p.tokens = d->tokens;
@@ -759,6 +778,7 @@ extern "C" int mkv_store_rotated(const mkv_store_rotated_desc_t* d, void* stream
   p.planes = (c.heads + heads_here - 1) / heads_here;
   const int at_once = 64 / (c.head_size / 16);
   p.cut = cut_heads(d->q.heads, at_once, passes_for(d->tokens * d->q.heads / at_once));
+  p.q.stream = streams(d->tokens * d->q.heads * c.head_size * eb, c.head_size, d->turn.rotary, eb);
   const int units = (p.group + p.cut.tokens - 1) / p.cut.tokens * p.cut.parts;
   const int q_planes = (units + waves - 1) / waves;
   if ((d->tokens + p.group - 1) / p.group > UINT32_MAX / (64 * waves) || p.planes + q_planes > 65535)

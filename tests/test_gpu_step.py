@@ -236,3 +236,22 @@ def test_a_large_call_does_what_small_ones_do(gpu, qh, kh, d, rotary):
     a, b = int(starts[0]), int(starts[-1])
     assert torch.equal(out[a:b], all_q[a:b])
     assert (out[:a] == 77.0).all() and (out[b:] == 77.0).all()
+
+
+def test_outputs_beyond_the_caches_are_the_same(gpu):
+    """Bit for bit: outputs that are streamed (150 MiB and more), in place and not, against small calls."""
+    n, qh, kh, d = 15500, 40, 8, 128
+    q, k, v = (torch.randn((n, h, d), device=gpu).to(torch.bfloat16) for h in (qh, kh, kh))
+    inv = freq(d).to(gpu)
+    positions = torch.arange(n, dtype=torch.int32, device=gpu) + 3
+    all_q, all_k = norm_rotate(q, k, positions, inv)
+    for first in range(0, n, 499):
+        part = slice(first, first + 499)
+        some = norm_rotate(q[part], k[part], positions[part], inv)
+        assert torch.equal(some[0], all_q[part]) and torch.equal(some[1], all_k[part])
+    cache = fresh_cache(gpu, n // 16 + 2, kh, d)
+    table = torch.arange(n // 16 + 2, dtype=torch.int32, device=gpu)[None]
+    into = store_rotated(cache, q, k, v, table, i32([0, n], gpu), i32([n + 3], gpu), inv)
+    assert torch.equal(into, all_q)
+    norm_rotate(q, k, positions, inv, out_q=q, out_k=k)
+    assert torch.equal(q, all_q) and torch.equal(k, all_k)
