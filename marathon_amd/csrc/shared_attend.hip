@@ -281,7 +281,8 @@ void choose_parts(const mkv_attend_shared_desc_t& d, int64_t shared_most, int64_
     x->splits = static_cast<int>(tokens > per ? (tokens + per - 1) / per : 1);
     // Every tile has room for its parts, also those that hints or a padded batch leave without
     // work: a workspace is bounded as that of whole histories is, by fewer and longer parts.
-    const int64_t all = x->tiles * static_cast<int64_t>(heads), most = kMostParts * (x->rows == kManyRows ? 1536 : kWantFew);
+    const int64_t all = x->tiles * static_cast<int64_t>(heads);
+    const int64_t most = kMostParts * (x->rows == kManyRows ? 1536 : kWantFew);
     if (all * x->splits > most) x->splits = static_cast<int>(all < most ? most / all : 1);
   };
   cut(shared_most, n, s);
