@@ -124,8 +124,11 @@ int mkv_store_rotated(const mkv_store_rotated_desc_t* desc, void* stream);
  *            workspace  mkv_attend_shared_workspace_size() bytes.
  *   max_shared : the most tokens that a group shares, where the caller knows it (0: not known).
  * Where the tables of a group agree, the result is mkv_attend_scaled's but for the order of sums
- * and p's roundings: over what is shared p is held in one bf16 term (off by 2^-8) where bf16
- * queries take the kernel of more than 32 rows, here by the rows of a group.
+ * and p's roundings: for fp16 queries, and for bf16 ones of at most 32 rows a request (rows: max_new,
+ * or without it the tokens, times the query heads of a KV head), p is held in two bf16 terms (off by
+ * at most 2^-17) over both ranges; of more, in one (off by 2^-8) over what is shared, by every row of
+ * the call, and over own tokens as in mkv_attend_scaled.  The hints change a result by this and by the
+ * order of sums alone.
  * Groups that leave the requests or descend, and shared tokens below zero, raise MKV_FLAG_SPAN
  * and share nothing; more shared tokens than a table has raise MKV_FLAG_SRC_RANGE, and are cut.
  */

@@ -17,8 +17,11 @@
 // it.)  The one rounding is p's.  The kernel of few rows cuts it into two bf16 terms, which leaves
 // 2^-17: the second product hides behind memory (a batch's next tokens 110.7 -> 111.2 us, one
 // request's 19.8 -> 19.9; of 17 to 32 rows 27.4 -> 30.9).  The kernel of many rows does so for
-// fp16 queries; for bf16 ones it rounds p to bf16, by half a step of it, 2^-8, as the output
-// itself is: a second product would take 2,048 tokens over 22,141 from 1,072 to 1,380 us.
+// fp16 queries, and beside tiles of few rows (K::kFew): requests of few rows that share tokens keep
+// what they have alone, however many they are (32 of them 34.1 -> 37.9 us, 96 99 -> 117, 32 of
+// heads of 64 28 -> 29, of 256 60 -> 64).  For other bf16 queries it rounds p to bf16, by half a
+// step of it, 2^-8, as the output itself is: a second product would take 2,048 tokens over 22,141
+// from 1,072 to 1,380 us.
 // fp16 queries multiply the bare codes (exact in fp16, where a scaled value may not be) and
 // the scale is applied to s_j.
 //
@@ -818,6 +821,7 @@ __global__ __launch_bounds__(256, (min_waves<K, D>())) void attend_kernel(typena
   if constexpr (K::kMany) {
     constexpr int KS = D / 16, MT = D / 32, W = D / 16, KC = D / 16;
     constexpr int kKLoads = 64 * D / 16 / 256;
+    constexpr bool kTwoTerms = F16 || K::kFew > 0;  // of p
     auto& s_k = lds.many.k;
     auto& s_v = lds.many.v;
     auto& s_odd = lds.many.odd;
@@ -1056,7 +1060,7 @@ __global__ __launch_bounds__(256, (min_waves<K, D>())) void attend_kernel(typena
           for (int i = 0; i < 16; ++i) o[mt][i] *= f;
       }
       const float base = m == -kInf ? 0.0f : m;
-      u32x4 ph[4], pl[4];  // P^T: 16 tokens each; and what bf16 leaves of it (F16)
+      u32x4 ph[4], pl[4];  // P^T: 16 tokens each; and what bf16 leaves of it (kTwoTerms)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         float y[8];
@@ -1068,7 +1072,7 @@ __global__ __launch_bounds__(256, (min_waves<K, D>())) void attend_kernel(typena
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           ph[g][j] = round_pair(y[2 * j], y[2 * j + 1]);
-          if constexpr (F16)
+          if constexpr (kTwoTerms)
             pl[g][j] = round_pair(y[2 * j] - __uint_as_float(ph[g][j] << 16),
                                   y[2 * j + 1] - __uint_as_float(ph[g][j] & 0xFFFF0000u));
         }
@@ -1087,7 +1091,7 @@ __global__ __launch_bounds__(256, (min_waves<K, D>())) void attend_kernel(typena
         for (int mt = 0; mt < MT; ++mt) {
           const u32x4 a = v_of(g, mt);
           o[mt] = times(a, ph[g], o[mt]);
-          if constexpr (F16) o[mt] = times(a, pl[g], o[mt]);
+          if constexpr (kTwoTerms) o[mt] = times(a, pl[g], o[mt]);
         }
       }
       if (masked && uni(s_odd[buf]) == at) {
