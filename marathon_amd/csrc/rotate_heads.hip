@@ -165,12 +165,15 @@ __device__ __forceinline__ void normalise(float* x, const float* w, const Turn& 
   for (int i = 0; i < 16; ++i) x[i] = x[i] * r * w[i];
 }
 
-__device__ __forceinline__ void rotate(float* x, const f32x2* turn) {
+// (Values that are not turned are left alone, not turned by nothing: an infinity or a NaN would
+// reach its neighbour as 0 * inf.  Chosen behind the products: a branch costs calls that turn all
+// of a head up to 4%.)
+__device__ __forceinline__ void rotate(float* x, const f32x2* turn, bool turned) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float a = x[i], b = x[8 + i], c = turn[i][0], s = turn[i][1];
-    x[i] = __builtin_fmaf(a, c, -(b * s));
-    x[8 + i] = __builtin_fmaf(b, c, a * s);
+    x[i] = turned ? __builtin_fmaf(a, c, -(b * s)) : a;
+    x[8 + i] = turned ? __builtin_fmaf(b, c, a * s) : b;
   }
 }
 
@@ -229,7 +232,7 @@ __device__ __forceinline__ void turn_heads(const HeadRows& rows, const Turn& t, 
     if (SEVERAL && h_next >= s.h1) ++next, h_next -= heads;
     if (held(next, h_next)) fetch(next, h_next);
     if (t.norm) normalise<D>(x, w, t);
-    if (t.half > 0) rotate(x, turn);
+    if (t.half > 0) rotate(x, turn, place.turned);
     if (held(mine, h) && (owned >> mine & 1)) {
       char* to = out + h * rows.out_head;
       if constexpr (SEVERAL) to += mine * rows.out_token;
@@ -459,7 +462,7 @@ __device__ __forceinline__ void put_keys(const PutParams& p, f32x2* s_turn, uint
         if (half > 0) {
           f32x2 turn[8];
           turns8(s_turn + row * half, place, turn);
-          rotate(x[u], turn);
+          rotate(x[u], turn, place.turned);
         }
         if (!(active && row >= off && row < off + n)) {  // (eps 0 makes NaNs of no row at all)
 #pragma unroll

@@ -145,7 +145,8 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor | None
     and ``k`` themselves; otherwise they share no memory with them or each other.
 
     fp32 throughout and rounded once; angles are taken in 64 bits.  A head of zeros with eps 0 is
-    NaN, as is one with an infinity."""
+    NaN.  An infinity under the norm is NaN itself and, where it is turned, in its pair; the rest of
+    its head is zeros."""
     made = _usual.rotate(q, k, positions, inv_freq, q_weight, k_weight, eps, out_q, out_k)
     if made is not None:
         if type(made) is int:
