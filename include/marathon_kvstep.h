@@ -130,7 +130,9 @@ int mkv_store_rotated(const mkv_store_rotated_desc_t* desc, void* stream);
  * the call, and over own tokens as in mkv_attend_scaled.  The hints change a result by this and by the
  * order of sums alone.
  * Groups that leave the requests or descend, and shared tokens below zero, raise MKV_FLAG_SPAN
- * and share nothing; more shared tokens than a table has raise MKV_FLAG_SRC_RANGE, and are cut.
+ * and share nothing: their requests' own tables are read from the first token on.  The others share
+ * what they share, but for those that a descending group reaches into.  More shared tokens than a
+ * table has raise MKV_FLAG_SRC_RANGE, and are cut.
  */
 typedef struct mkv_attend_shared_desc {
   mkv_attend_desc_t attend;

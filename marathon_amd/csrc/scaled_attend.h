@@ -144,6 +144,33 @@ struct Group {
   int64_t s0, s1;
 };
 
+// The last group with value(its first request, its number) at most `at`, as last_at_most finds it; -1 if
+// there is none.  Groups that begin behind or in front of the batch, and those with value -1, are
+// passed over wherever they stand, so that they lead nobody away from the others: where one is a
+// probe, the next that is none of them stands for its 64.
+template <typename F>
+__device__ __forceinline__ int last_group(const DevGroups& d, int requests, int64_t at, F value) {
+  const int lane = threadIdx.x & 63;
+  const auto value_of = [&](int i) {
+    const int a = d.groups[i];
+    return a >= 0 && a < requests ? value(a, i) : int64_t{-1};
+  };
+  int base = 0;
+  if (d.count > 64) {
+    int i = lane * 64;
+    const int end = min(i + 64, d.count);
+    int64_t x = -1;
+    while (i < end && (x = value_of(i)) < 0) ++i;
+    const uint64_t hit = __ballot(x >= 0 && x <= at);
+    if (hit == 0) return -1;
+    base = (63 - __builtin_clzll(hit)) * 64;
+  }
+  const int i = base + lane;
+  const int64_t x = i < d.count ? value_of(i) : -1;
+  const uint64_t hit = __ballot(x >= 0 && x <= at);
+  return hit == 0 ? -1 : base + 63 - __builtin_clzll(hit);
+}
+
 // Group `g`; what a valid one shares is 0 or more whole blocks.
 __device__ __forceinline__ bool read_group(const DevCache& c, const DevStep& s, const DevGroups& d,
                                            int64_t tokens, int g, Group& out) {
@@ -163,8 +190,7 @@ __device__ __forceinline__ bool read_group(const DevCache& c, const DevStep& s, 
 // The group of request r with the rows [s0, s1), one wave; false where it is in none.
 __device__ __forceinline__ bool group_of(const DevCache& c, const DevStep& s, const DevGroups& d,
                                          int64_t tokens, int r, int64_t s0, int64_t s1, Group& out) {
-  const int32_t* groups = d.groups;
-  const int g = last_at_most(d.count, r, [groups](int i) { return groups[i]; });
+  const int g = last_group(d, s.requests, r, [](int a, int) { return static_cast<int64_t>(a); });
   return g >= 0 && read_group(c, s, d, tokens, g, out) && r >= out.a && r < out.b &&
          s0 >= out.s0 && s1 <= out.s1;
 }
@@ -177,21 +203,24 @@ __device__ __forceinline__ int64_t shared_begin(int64_t row, int rows, int g) {
   return (row + static_cast<int64_t>(g) * (rows - 1)) / rows;
 }
 
+// The group that a tile over what is shared may be of.
+template <typename P>
+__device__ __forceinline__ int shared_group(const P& p, int64_t tile, int rows) {
+  const int32_t* starts = p.s.starts;
+  const int64_t group = p.group, tokens = p.tokens;
+  return last_group(p.g, p.s.requests, tile, [=](int a, int i) {
+    const int64_t s0 = starts[a];
+    return s0 >= 0 && s0 <= tokens ? shared_begin(s0 * group, rows, i) : int64_t{-1};
+  });
+}
+
 // (GROUPED: over what `t.over` says; otherwise over histories.)
 template <bool GROUPED, int BM, typename P>
 __device__ __forceinline__ bool find_tile(const P& p, int64_t tile, Tile& t) {
   const int32_t* starts = p.s.starts;
   const int group = p.group;
   if constexpr (GROUPED) if (t.over == kShared) {
-    const int32_t* groups = p.g.groups;
-    const int requests = p.s.requests;
-    const int g = p.g.count == 1 ? 0 : last_at_most(p.g.count, tile, [=](int i) {
-      // (bad groups are come across where group_of() does, and by nobody else's tiles)
-      const int a = groups[i];
-      return a < 0 ? int64_t{0}
-                   : a > requests ? INT64_MAX
-                                  : shared_begin(static_cast<int64_t>(starts[a]) * group, BM, i);
-    });
+    const int g = p.g.count == 1 ? 0 : shared_group(p, tile, BM);
     Group of;
     if (g < 0 || !read_group(p.c, p.s, p.g, p.tokens, g, of)) return false;
     t.request = of.a;
@@ -237,10 +266,22 @@ __device__ __forceinline__ bool find_tile(const P& p, int64_t tile, Tile& t) {
   if constexpr (GROUPED) {
     Group of;
     t.shared_parts = 0;
-    if (group_of(p.c, p.s, p.g, p.tokens, r, t.s0, s1, of) && of.shared > 0) {
-      t.from = of.shared;
+    bool found = group_of(p.c, p.s, p.g, p.tokens, r, t.s0, s1, of) && of.shared > 0;
+    if (found) {
       t.shared_row = (t.s0 - of.s0) * group + t.row0;
       t.shared_tile = shared_begin(of.s0 * group, p.shared_rows, of.index);
+      if (p.g.count > 64) {
+        // Do the tiles that have the rows find the group?  With up to 64 groups always; beyond, starts
+        // that descend may hide it from them, and its parts would be read and never written.  (100
+        // groups of four requests 53.2 -> 55.1 us, 1,000 of two 127 -> 135.)
+        const int64_t first = t.shared_tile + t.shared_row / p.shared_rows;
+        const int64_t last = t.shared_tile + (t.shared_row + t.rows - 1) / p.shared_rows;
+        found = shared_group(p, first, p.shared_rows) == of.index &&
+                (last == first || shared_group(p, last, p.shared_rows) == of.index);
+      }
+    }
+    if (found) {
+      t.from = of.shared;
       t.shared_parts = part_count(of.shared, part_size(of.shared, p.shared_splits, p.shared_per));
       if (t.keys < t.from) t.keys = t.full = t.from;  // nothing of its own
     }
