@@ -695,9 +695,13 @@ template <int ET>
 int put_launch(int d, dim3 grid, int threads, int lds, const PutParams& p, hipStream_t s) {
   void (*kernel)(PutParams) =
       d == 64 ? put_kernel<ET, 64> : d == 128 ? put_kernel<ET, 128> : put_kernel<ET, 256>;
-  if (lds > 65536) {  // (heads of 256 in blocks of 128) more than a launch has unasked
+  // More than a launch has unasked, with the kernel's own: heads of 256 in blocks of 64 and of 128, of
+  // 128 in blocks of 128.  Asked for is always the most that heads of this size need, so that no call
+  // takes from another thread's what it has just asked for.
+  constexpr int kOwn = kMaxWaves * 2 * sizeof(uint32_t), kMostRows = 128;
+  if (lds + kOwn > 65536) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, kMostRows * d / 2 * 8);
     if (e != hipSuccess)
       return mkv_fail(MKV_ERR_HIP, "mkv_store_rotated: %d bytes of LDS: %s", lds, hipGetErrorString(e));
   }
