@@ -578,6 +578,20 @@ bool turn_of(PyObject* freq, PyObject* qw, PyObject* kw, PyObject* eps, const at
   return true;
 }
 
+// Whether any of some plain tensors, read as they lie in memory, has a byte among an output's rows.
+template <typename... T>
+bool reads_from(const Range& r, T... read) {
+  for (PyObject* o : {read...}) {
+    const at::Tensor* t = plain(o);
+    if (t == nullptr || t->numel() == 0) continue;
+    int64_t last = 1;
+    for (int64_t i = 0; i < t->dim(); ++i) last += (t->size(i) - 1) * t->stride(i);
+    const uintptr_t from = reinterpret_cast<uintptr_t>(t->data_ptr());
+    if (r.meets(from, from + static_cast<uintptr_t>(last) * t->element_size())) return true;
+  }
+  return false;
+}
+
 bool row_type(int code) { return code == MKV_BF16 || code == MKV_F16 || code == MKV_F32; }
 
 // rotate(q, k, positions, inv_freq, q_weight, k_weight, eps, out_q, out_k)
@@ -614,6 +628,8 @@ PyObject* rotate(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (args[7] != Py_None) {
       const Range a = range_of(*q), b = range_of(*k);
       if (a.meets(b.from, b.to)) Py_RETURN_NONE;
+      for (const Range& r : {a, b})
+        if (reads_from(r, args[2], args[3], args[4], args[5])) Py_RETURN_NONE;
     }
     if (!rows_of(args[0], args[7], dev, d, code, desc.q, out_q) ||
         !rows_of(args[1], args[8], dev, d, code, desc.k, out_k))

@@ -116,8 +116,10 @@ def _output(who: str, name: str, x: torch.Tensor, out, others: dict, inputs: tup
         if rows.base < r.end and r.base < rows.end:
             raise ValueError(f"out_{name} lies among the cache's rows")
     for t in inputs:
-        if t is not None and rows.base < t.data_ptr() + t.nbytes and t.data_ptr() < rows.end:
-            raise ValueError(f"out_{name} shares memory with an input")
+        if t is not None and t.numel():
+            last = 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+            if rows.base < t.data_ptr() + last * t.element_size() and t.data_ptr() < rows.end:
+                raise ValueError(f"out_{name} shares memory with an input")
     return out
 
 
