@@ -17,7 +17,8 @@
 // the same way: a decode step's kernels run 4 to 20 us, and through Python methods and ctypes
 // the calls took 10 to 15 on the host.  They return their tensors (store: None on success
 // becomes True), the library's status as an int, or None for the general path.  rotate, put and
-// attend_shared are scaled_step.py's calls in the same way: 20 us on the host became 4 to 6.
+// attend_shared are scaled_step.py's calls in the same way: 20 us on the host became 4 to 6 (into a
+// caller's outputs, in place among them, 27 to 39).
 
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
@@ -270,6 +271,21 @@ Range range_of(const at::Tensor& t) {
   return {from, from + static_cast<uintptr_t>(last) * t.element_size()};
 }
 
+// Whether two [tokens, heads, D] tensors' rows share no memory, as far as their ranges say it, or
+// that they are parts of one projection: the same step from token to token, and within it the one's
+// heads beside the other's.  (Others interleave in ways that the general path looks into.)
+bool apart(const at::Tensor& a, const at::Tensor& b) {
+  const Range x = range_of(a), y = range_of(b);
+  if (a.numel() == 0 || b.numel() == 0 || !x.meets(y.from, y.to)) return true;
+  const int64_t size = a.element_size(), step = a.stride(0) * size;
+  if (a.size(0) < 2 || b.size(0) < 2 || a.stride(0) != b.stride(0) || step <= 0) return false;
+  const auto span = [size](const at::Tensor& t) {
+    return ((t.size(1) - 1) * t.stride(1) + t.size(2)) * size;
+  };
+  const int64_t off = static_cast<int64_t>(y.from - x.from) % step, from = off < 0 ? off + step : off;
+  return from >= span(a) && from + span(b) <= step;
+}
+
 // Whether rows in `r` may lie in the cache.
 bool meets_cache(const Range& r, const mkv_scaled_cache_t& c) {
   if (c.num_blocks <= 0) return false;
@@ -509,8 +525,8 @@ put_fn g_put = nullptr;
 shared_fn g_shared = nullptr;
 shared_size_fn g_shared_size = nullptr;
 
-// The heads' rows, and their output: a fresh one, or the rows themselves (kept in `out`).  Other
-// outputs are the general path's.
+// The heads' rows, and their output, kept in `out`: a fresh one, the rows themselves, or the caller's
+// apart from them.
 bool rows_of(PyObject* x_o, PyObject* out_o, const at::Device& dev, int64_t d, int code,
              mkv_head_rows_t& r, at::Tensor& out) {
   const at::Tensor* x = plain(x_o);
@@ -522,8 +538,8 @@ bool rows_of(PyObject* x_o, PyObject* out_o, const at::Device& dev, int64_t d, i
   } else {
     const at::Tensor* o = plain(out_o);
     if (o == nullptr || o->device() != dev || o->scalar_type() != x->scalar_type() ||
-        o->sizes() != x->sizes() || o->strides() != x->strides() || o->data_ptr() != x->data_ptr() ||
-        needs_grad(*o))
+        o->sizes() != x->sizes() || o->stride(2) != 1 || needs_grad(*o) ||
+        !((o->data_ptr() == x->data_ptr() && o->strides() == x->strides()) || apart(*o, *x)))
       return false;
     out = *o;
   }
@@ -621,18 +637,14 @@ PyObject* rotate(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       desc.positions = p->data_ptr();
       desc.position_bytes = p->scalar_type() == at::kInt ? 4 : 8;
     }
-    // (in place: q and k may be parts of one tensor, whose rows the general path tells apart)
-    if ((args[7] == Py_None) != (args[8] == Py_None) || (args[7] != Py_None && args[7] != args[0]) ||
-        (args[8] != Py_None && args[8] != args[1]))
-      Py_RETURN_NONE;
-    if (args[7] != Py_None) {
-      const Range a = range_of(*q), b = range_of(*k);
-      if (a.meets(b.from, b.to)) Py_RETURN_NONE;
-      for (const Range& r : {a, b})
-        if (reads_from(r, args[2], args[3], args[4], args[5])) Py_RETURN_NONE;
-    }
     if (!rows_of(args[0], args[7], dev, d, code, desc.q, out_q) ||
         !rows_of(args[1], args[8], dev, d, code, desc.k, out_k))
+      Py_RETURN_NONE;
+    // a caller's outputs: apart from the other rows, from each other and from what is read
+    const bool mine[2] = {args[7] != Py_None, args[8] != Py_None};
+    if ((mine[0] && (!apart(out_q, *k) || reads_from(range_of(out_q), args[2], args[3], args[4], args[5]))) ||
+        (mine[1] && (!apart(out_k, *q) || reads_from(range_of(out_k), args[2], args[3], args[4], args[5]))) ||
+        (mine[0] && mine[1] && !apart(out_q, out_k)))
       Py_RETURN_NONE;
     desc.tokens = n;
     desc.head_size = static_cast<int32_t>(d);
@@ -676,9 +688,7 @@ PyObject* put(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const at::Tensor* q = plain(args[2]);
     const at::Tensor* k = plain(args[3]);
     const at::Tensor* v = plain(args[4]);
-    // (an output of the caller's is told from k, v and the cache by the general path)
-    if (!whole(args[1], 0, 127, index) || q == nullptr || k == nullptr || v == nullptr || !q->is_cuda() ||
-        args[12] != Py_None)
+    if (!whole(args[1], 0, 127, index) || q == nullptr || k == nullptr || v == nullptr || !q->is_cuda())
       Py_RETURN_NONE;
     const at::Device dev(at::kCUDA, static_cast<c10::DeviceIndex>(index));
     const int code = dtype_code(q->scalar_type());
@@ -696,8 +706,15 @@ PyObject* put(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       Py_RETURN_NONE;
     const int32_t* starts = vector_of(args[6], dev, tab.n + 1);
     const int32_t* lens = vector_of(args[7], dev, tab.n);
-    if (starts == nullptr || lens == nullptr || !rows_of(args[2], Py_None, dev, cache->head_size, code, d.q, out))
+    if (starts == nullptr || lens == nullptr ||
+        !rows_of(args[2], args[12], dev, cache->head_size, code, d.q, out))
       Py_RETURN_NONE;
+    if (args[12] != Py_None) {
+      const Range written = range_of(out);
+      if (!apart(out, *k) || !apart(out, *v) || meets_cache(written, *cache) ||
+          reads_from(written, args[5], args[6], args[7], args[8], args[9], args[10]))
+        Py_RETURN_NONE;
+    }
     const bool many = k->size(0) > 1, heads = k->size(1) > 1;
     d.cache = *cache;
     d.k = k->data_ptr();
@@ -721,7 +738,7 @@ PyObject* put(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     rc = g_put(&d, stream);
     Py_END_ALLOW_THREADS
     if (rc != MKV_OK) return PyLong_FromLong(rc);
-    return THPVariable_Wrap(out);
+    return args[12] != Py_None ? (Py_INCREF(args[12]), args[12]) : THPVariable_Wrap(out);
   } catch (const std::exception& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
     return nullptr;

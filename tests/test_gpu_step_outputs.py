@@ -1,4 +1,5 @@
-"""A caller's own outputs, told from what a call reads."""
+"""A caller's own outputs: taken by the calls' short path, told from what a call reads, and alike by
+both paths."""
 
 from __future__ import annotations
 
@@ -9,7 +10,7 @@ import torch
 from marathon_amd import norm_rotate, scaled_step, store_rotated
 from tests.test_gpu_norm_rotate import freq
 from tests.test_gpu_scaled import Cache, i32, requests_of
-from tests.test_gpu_step import Nothing
+from tests.test_gpu_step import Counted, Nothing
 
 pytestmark = pytest.mark.gpu
 
@@ -24,6 +25,58 @@ def step_of(gpu, tokens=21, heads=2, d=128):
 def projection(gpu, tokens=21, parts=(8, 2, 2), d=128):
     g = torch.Generator(device=gpu).manual_seed(1)
     return torch.randn((tokens, sum(parts), d), generator=g, device=gpu).to(torch.bfloat16).split(parts, 1)
+
+
+def taken(monkeypatch, short, call):
+    """The call by the short path, which has to take it, or by the general one."""
+    usual = Counted() if short else Nothing()
+    monkeypatch.setattr(scaled_step, "_usual", usual)
+    got = call()
+    assert not short or (usual.got and usual.got[-1] is not None)
+    return got
+
+
+@pytest.mark.parametrize("short", [True, False])
+@pytest.mark.parametrize("where", ["views", "apart", "other", "strided"])
+@pytest.mark.parametrize("tokens", [1, 21])
+def test_queries_of_a_store(gpu, short, where, tokens, monkeypatch):
+    cache, step = step_of(gpu, tokens)
+    q, k, v = projection(gpu, tokens)
+    inv = freq(128).to(gpu)
+    want = store_rotated(cache.dev, q, k, v, *step, inv)
+    codes = cache.planes[0].view(torch.uint8).clone()
+    whole = torch.full((tokens, 12, 128), 7.0, dtype=torch.bfloat16, device=gpu)
+    if where == "apart":
+        q = q.clone()
+    out = {"other": torch.empty(q.shape, dtype=q.dtype, device=gpu), "strided": whole[:, 2:10]}.get(where, q)
+    rest = [x.clone() for x in (k, v)]
+    got = taken(monkeypatch, short, lambda: store_rotated(cache.dev, q, k, v, *step, inv, out_q=out))
+    assert got is out and torch.equal(got, want)
+    assert torch.equal(cache.planes[0].view(torch.uint8), codes)
+    assert torch.equal(k, rest[0]) and torch.equal(v, rest[1])
+    if where == "strided":
+        assert (whole[:, :2] == 7).all() and (whole[:, 10:] == 7).all()
+
+
+@pytest.mark.parametrize("short", [True, False])
+@pytest.mark.parametrize("where", ["views", "apart", "other", "strided", "one"])
+@pytest.mark.parametrize("tokens", [1, 21])
+def test_queries_and_keys(gpu, short, where, tokens, monkeypatch):
+    q, k, v = projection(gpu, tokens)
+    pos, inv = torch.arange(tokens, device=gpu) + 3, freq(64).to(gpu)
+    want = norm_rotate(q, k, pos, inv)
+    whole = torch.full((tokens, 12, 128), 7.0, dtype=torch.bfloat16, device=gpu)
+    if where == "apart":
+        q, k = q.clone(), k.clone()
+    out = {"other": (torch.empty_like(q), torch.empty_like(k)), "strided": (whole[:, 3:11], whole[:, :2]),
+           "one": (None, k)}.get(where, (q, k))
+    rest = v.clone()
+    got = taken(monkeypatch, short, lambda: norm_rotate(q, k, pos, inv, out_q=out[0], out_k=out[1]))
+    for a, b, o in zip(got, want, out):
+        assert torch.equal(a, b) and (o is None or a is o)
+    assert torch.equal(v, rest)
+    if where == "strided":
+        assert (whole[:, 2:3] == 7).all() and (whole[:, 11:] == 7).all()
 
 
 @pytest.mark.parametrize("short", [True, False])
