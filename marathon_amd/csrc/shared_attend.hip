@@ -247,7 +247,10 @@ void choose_parts(const mkv_attend_shared_desc_t& d, int64_t shared_most, int64_
   const Cost cs = cost_of(s->rows, a.cache.head_size, f16), co = cost_of(o->rows, a.cache.head_size, f16);
   const double heads = a.cache.heads;
   const double part = 0.05 + kJoin * static_cast<double>(a.tokens) * a.q_heads * a.cache.head_size;
-  // tiles that have work, if groups and requests are alike; of lengths that differ, half the longest
+  // Tiles that have work, if groups and requests are alike.  Own histories, whose lengths only the GPU
+  // knows, are taken to be 0.55 of the longest on average: one of 8,000 tokens beside 31 of 200 77.6 us,
+  // where 0.8 or 1 took 98 or 143; the price is paid by those that are alike, 24 of 4,000 behind 2,000
+  // shared 55.8 (47.4 both), 8 of 8,000 behind 4,000 50.5 (50.5 and 40.2).
   const auto alike = [](const Shape& x, int64_t each, int64_t count) {
     return static_cast<double>(std::min((each + x.rows - 1) / x.rows * count, x.tiles));
   };
