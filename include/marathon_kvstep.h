@@ -124,11 +124,10 @@ int mkv_store_rotated(const mkv_store_rotated_desc_t* desc, void* stream);
  *            workspace  mkv_attend_shared_workspace_size() bytes.
  *   max_shared : the most tokens that a group shares, where the caller knows it (0: not known).
  * Where the tables of a group agree, the result is mkv_attend_scaled's but for the order of sums
- * and p's roundings: for fp16 queries, and for bf16 ones of at most 32 rows a request (rows: max_new,
- * or without it the tokens, times the query heads of a KV head), p is held in two bf16 terms (off by
- * at most 2^-17) over both ranges; of more, in one (off by 2^-8) over what is shared, by every row of
- * the call, and over own tokens as in mkv_attend_scaled.  The hints change a result by this and by the
- * order of sums alone.
+ * and p's roundings: over both ranges p is held in two bf16 terms (off by at most 2^-17) for every
+ * request whose p mkv_attend_scaled holds in two, by the same max_new, however many rows share; for
+ * the others in one (off by 2^-8) or two.  The hints change a result by this and by the order of sums
+ * alone.
  * Groups that leave the requests or descend, and shared tokens below zero, raise MKV_FLAG_SPAN
  * and share nothing: their requests' own tables are read from the first token on.  The others share
  * what they share, but for those that a descending group reaches into.  More shared tokens than a

@@ -35,7 +35,7 @@ struct Few {
 struct Many {
   typedef AttendParams Params;
   static constexpr int kFew = 0;
-  static constexpr bool kMany = true, kGrouped = false;
+  static constexpr bool kMany = true, kGrouped = false, kTwoTerms = false;
   static __device__ __forceinline__ const Params& params(const Params& p, Over) { return p; }
   static __device__ __forceinline__ Section pick(const Params& p, unsigned& tile, int& head, int& part,
                                                  Over&) {

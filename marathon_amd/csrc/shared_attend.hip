@@ -38,11 +38,11 @@ struct BothParams {
 };
 
 // Tiles of SHARED rows over what is shared and of OWN rows over own tokens: 16 or 32 take the
-// section of few rows, 128 that of many.
-template <int SHARED, int OWN>
+// section of few rows, 128 that of many, there with p of bf16 queries in two terms (TWO) or one.
+template <int SHARED, int OWN, bool TWO = (OWN < kManyRows)>
 struct Both {
   typedef BothParams Params;
-  static constexpr bool kGrouped = true, kMany = SHARED == kManyRows;
+  static constexpr bool kGrouped = true, kMany = SHARED == kManyRows, kTwoTerms = TWO;
   static constexpr int kFew = OWN == kManyRows ? 0 : OWN / 16;
   static_assert(kMany || SHARED == OWN, "one section of few rows");
 
@@ -85,6 +85,28 @@ struct Both {
     return x;
   }
 };
+
+// bf16 chunks beside another launch over the own tokens of requests of few rows, whose rows over what
+// is shared are here: their tiles take two terms of p, the chunks' one.
+template <int D>
+__global__ __launch_bounds__(256, (min_waves<Both<kManyRows, kManyRows>, D>())) void chunks_beside_kernel(
+    BothParams params) {
+  typedef Both<kManyRows, kManyRows, false> One;
+  __shared__ Lds<D, One::kFew, One::kMany> lds;
+  bool few = false;
+  if (blockIdx.x < params.shared_units) {
+    unsigned tile;
+    int head, part;
+    Tile t;
+    One::pick(params, tile, head, part, t.over);
+    const auto& p = One::params(params, t.over);
+    few = find_tile<true, kManyRows>(p, tile, t) && of_few_rows(p, t);
+  }
+  if (uni(few))
+    attend_tile<Both<kManyRows, kManyRows, true>, false, D>(params, lds);
+  else
+    attend_tile<One, false, D>(params, lds);
+}
 
 // ------------------------------------------------------------------ the parts' results joined
 
@@ -360,15 +382,21 @@ int64_t workspace_of(const mkv_attend_shared_desc_t& d, const Plan& plan) {
          rows * (c.head_size + 2) * 4 + 64;
 }
 
-template <typename K, bool F16, int D>
-void launch(const BothParams& p, hipStream_t stream) {
-  const int64_t units = p.shared_units + p.own_units + (p.own.s.flags != nullptr ? 1 : 0);
-  attend_kernel<K, F16, D><<<static_cast<unsigned>(units), 256, 0, stream>>>(p);
+unsigned units_of(const BothParams& p) {
+  return static_cast<unsigned>(p.shared_units + p.own_units + (p.own.s.flags != nullptr ? 1 : 0));
 }
 
+template <typename K, bool F16, int D>
+void launch(const BothParams& p, hipStream_t stream) {
+  attend_kernel<K, F16, D><<<units_of(p), 256, 0, stream>>>(p);
+}
+
+// (with_few: chunks beside another launch over the own tokens of requests of few rows)
 template <bool F16, int D>
-void launch(int shared_rows, int own_rows, const BothParams& p, hipStream_t stream) {
-  if (shared_rows == kManyRows) {
+void launch(int shared_rows, int own_rows, bool with_few, const BothParams& p, hipStream_t stream) {
+  if (with_few && !F16) {
+    chunks_beside_kernel<D><<<units_of(p), 256, 0, stream>>>(p);
+  } else if (shared_rows == kManyRows) {
     if (own_rows == 16)
       launch<Both<kManyRows, 16>, F16, D>(p, stream);
     else if (own_rows == 32)
@@ -415,7 +443,7 @@ void run(const GroupedParams& base, const Plan& plan, JoinParams j, char* room, 
     p.own_units = own.tiles * heads * own.splits;
     const bool with = i == plan.owns - 1 && base.g.count > 0;
     p.shared_units = with ? plan.shared.tiles * ((heads * plan.shared.splits + 7) / 8 * 8) : 0;
-    launch<F16, D>(with ? plan.shared.rows : own.rows, own.rows, p, stream);
+    launch<F16, D>(with ? plan.shared.rows : own.rows, own.rows, with && plan.owns == 2, p, stream);
   }
   if (plan.owns == 1) j.sets[2] = j.sets[1];
   const int64_t rows = j.tokens * heads * j.group;

@@ -244,11 +244,11 @@ def attend_shared(cache: ScaledCache, q: torch.Tensor, block_tables: torch.Tenso
     Of the shared tokens whole blocks are read once for the group, through the block table of its
     first request; the others' entries for them are not read.  Where a group's tables agree, as
     those of requests that share blocks do, the result is ``attend_scaled``'s but for the order of
-    sums and the roundings of p named there: 2^-17 of itself for fp16 queries and, however many rows
-    share, for bf16 ones of at most 32 rows a request (``max_new``, or without it the tokens, times the
-    query heads of a KV head); of more, 2^-8 for every row over what is shared.  Requests in no group
-    share nothing.  Groups that leave the requests or descend, and negative
-    ``shared``, are flagged (``MKV_FLAG_SPAN``) and share nothing.
+    sums and the roundings of p named there, by the rows of a request, however many share: 2^-17 of
+    itself for fp16 queries and for bf16 ones of at most 32 rows (``max_new``, or without it the tokens,
+    times the query heads of a KV head), 2^-8 of more.  Requests in no group share nothing.  Groups that
+    leave the requests or descend, and negative ``shared``, are flagged (``MKV_FLAG_SPAN``) and share
+    nothing.
 
     ``max_new``, ``max_shared`` and ``max_own``: the largest number of new tokens of a request, of
     tokens that a group shares and of tokens that a request has behind them, where the host knows

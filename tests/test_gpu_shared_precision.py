@@ -14,7 +14,7 @@ from tests.test_gpu_scaled import Cache
 pytestmark = pytest.mark.gpu
 
 
-def within(cache, q, tables, starts, lens, bs, got, p_rounding):
+def within(cache, q, tables, starts, lens, bs, got, p_rounding, requests=None):
     """Whether outputs are within the roundings of the exact ones, entry by entry.
 
     Of p where it meets V: ``p_rounding`` of each term.  Of a score: fp32 sums of D products and the
@@ -27,6 +27,8 @@ def within(cache, q, tables, starts, lens, bs, got, p_rounding):
     out, half = got.double().cpu().numpy(), torch.finfo(got.dtype).eps / 2
     worst = 0.0
     for r, last in enumerate(lens):
+        if requests is not None and r not in requests:
+            continue
         x = plain.rows(cache.codes, cache.scales, tables[r], last, bs)
         for t in range(starts[r], starts[r + 1]):
             sees = last - (starts[r + 1] - t) + 1
@@ -43,9 +45,9 @@ def within(cache, q, tables, starts, lens, bs, got, p_rounding):
     return worst <= 1
 
 
-def batch_of(gpu, requests, new, heads, group, d, seed):
+def batch_of(gpu, requests, new, heads, group, d, seed, more=()):
     rng = np.random.default_rng(seed)
-    batch = Batch(rng, [(512, [(int(n), new) for n in rng.integers(0, 60, requests)])], [], 16)
+    batch = Batch(rng, [(512, [(int(n), new) for n in rng.integers(0, 60, requests)] + list(more))], [], 16)
     cache = Cache(gpu, rng, batch.blocks, heads, d, 16, fill="any")
     # values of about one and scores of about a half: p's rounding stands out from the scores'
     cache.codes[:] = plain.encode(rng.standard_normal(cache.codes.shape) * 2.0 ** 4)
@@ -53,7 +55,8 @@ def batch_of(gpu, requests, new, heads, group, d, seed):
     x = cache.codes.transpose(0, 2, 1, 3, 4)
     cache.planes[0].view(torch.uint8).copy_(torch.from_numpy(x.reshape(*x.shape[:3], 2 * d).copy()))
     cache.dev_scales.view(torch.uint8).fill_(127 - 4)
-    q = torch.from_numpy(rng.standard_normal((requests * new, heads * group, d)) / 2).to(gpu, torch.bfloat16)
+    tokens = requests * new + sum(n for _, n in more)
+    q = torch.from_numpy(rng.standard_normal((tokens, heads * group, d)) / 2).to(gpu, torch.bfloat16)
     return batch, cache, q
 
 
@@ -83,3 +86,15 @@ def test_without_hints_p_may_be_one_term(gpu, requests, new, heads, group, d):
     batch, cache, q = batch_of(gpu, requests, new, heads, group, d, requests + d)
     got = run(gpu, batch, cache, q)
     assert within(cache, q, batch.tables, batch.starts, batch.lens, 16, got, 2.0 ** -8)
+
+
+@pytest.mark.parametrize("group,d", [(16, 128), (16, 64), (8, 256)])
+def test_decoding_requests_beside_a_long_chunk_keep_them_too(gpu, group, d):
+    """2,048 rows and more beside requests of up to 16: these have a launch of their own over their own
+    tokens, as in attend_scaled, and lose nothing over what is shared."""
+    chunk = 2048 // group
+    batch, cache, q = batch_of(gpu, 5, 1, 1, group, d, group + d, more=[(9, chunk)])
+    got = run(gpu, batch, cache, q, max_new=chunk, max_shared=512)
+    args = cache, q, batch.tables, batch.starts, batch.lens, 16, got
+    assert within(*args, 2.0 ** -17, requests=range(5))
+    assert within(*args, 2.0 ** -8, requests=[5])
