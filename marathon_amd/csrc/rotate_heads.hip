@@ -670,9 +670,9 @@ int check_rows(const char* who, const char* name, const mkv_head_rows_t& r, int6
 // tokens of 40 + 8 heads of 128 (147 MB) 52.4 / 55.4 us, 14,000 67.0 / 64.3, 16,000 74.4 / 71.6, 22,141
 // 102.5 / 97.5; into the cache 12,000 63.0 / 66.0, 16,000 89.6 / 87.5, 22,141 125 / 119; in place over
 // three projections 110 / 102 and 127 / 121.  One output over and over, which the caches absorb, is the
-// price: 16,000 62.6 / 71.6, 22,141 85 / 97.5, into the cache 111 / 119.  In a model's layer, a projection
-// in front and the attention behind, it comes to the same: 22,141 tokens 89 / 97 here and about as much
-// less in the attention, which finds nothing to be written back; 6.51 ms either way.
+// price: 16,000 62.6 / 71.6, 22,141 85 / 97.5, into the cache 111 / 119.  Between a projection and the
+// attention, as in a model's layer of 22,141 tokens, 89 / 97 us of 6.5 ms; the whole does not differ by
+// more than it varies (0.3%).
 int streams(int64_t bytes, int head_size, int rotary, int64_t eb) {
   return bytes >= int64_t{150} << 20 && eb == 2 && head_size >= 128 && rotary == head_size;
 }

@@ -439,7 +439,7 @@ constexpr int few_waves() {
 // The next step's codes are loaded into registers before a step is computed and written to
 // the other of two buffers behind it: one barrier a step.  Two workgroups fit a CU, and one
 // computes while the other waits.  (Heads of 64 leave room for three, of 256 for one, which
-// spills 41 registers.)  A chunk of 2,048 tokens over 22,141, 40 query heads of 128 (0.97 TFLOP),
+// spills 44 registers; beside tiles of few rows over own tokens 42 to 87.)  A chunk of 2,048 tokens over 22,141, 40 query heads of 128 (0.97 TFLOP),
 // takes 1,050 to 1,130 us with the card: 0.86 to 0.93 PFLOP/s, where a library product of 8,192^3
 // reaches 1.22.  Heads of 64 run at 0.8 PFLOP/s, a score's softmax having half the products to
 // hide behind; of 256 at 0.53; fp16 queries, with a second product for p, at 0.68.
