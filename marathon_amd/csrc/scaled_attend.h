@@ -304,7 +304,10 @@ __device__ __forceinline__ void find_full(const P& p, Tile& t) {
   t.full = __all(least >= t.keys) ? t.keys : 0;
 }
 
-// Over what is shared: whether a row of the tile is of a request of few rows.
+// Rows of a request beside a long chunk, at most, that has a launch of its own with others of so few.
+constexpr int kBesideRows = 16;
+
+// Over what is shared: whether a row of the tile is of such a request.
 template <typename P>
 __device__ __forceinline__ bool of_few_rows(const P& p, const Tile& t) {
   const int64_t from = t.s0 * p.group + t.row0, to = from + t.rows;
@@ -312,7 +315,7 @@ __device__ __forceinline__ bool of_few_rows(const P& p, const Tile& t) {
   for (int r = t.request + (threadIdx.x & 63); r <= t.last; r += 64) {
     const int64_t a = static_cast<int64_t>(p.s.starts[r]) * p.group;
     const int64_t b = static_cast<int64_t>(p.s.starts[r + 1]) * p.group;
-    few = few || (b - a <= 16 && a < to && b > from);
+    few = few || (b - a <= kBesideRows && a < to && b > from);
   }
   return __any(few);
 }

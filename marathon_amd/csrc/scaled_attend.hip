@@ -153,9 +153,9 @@ int check(const mkv_attend_desc_t& d, AttendParams* p, Plan* plan) {
   // 400 / 348, 1,000 beside one at 16,000 314 / 306, 512 beside 3 143 / 145; with a chunk of
   // 129 beside 31 149 / 173, of 13 beside one 41 / 59: there the one launch has room for both.
   const int64_t rest = (d.tokens - new_most) * p->group;
-  if (each >= 2048 && d.requests > 1 && rest <= 16 * static_cast<int64_t>(d.requests - 1)) {
-    plan->shape[0] = shape_for(d, 16, 0, 16);
-    plan->shape[1] = shape_for(d, each, 17, INT32_MAX);
+  if (each >= 2048 && d.requests > 1 && rest <= kBesideRows * static_cast<int64_t>(d.requests - 1)) {
+    plan->shape[0] = shape_for(d, kBesideRows, 0, kBesideRows);
+    plan->shape[1] = shape_for(d, each, kBesideRows + 1, INT32_MAX);
     plan->count = 2;
   } else {
     plan->shape[0] = shape_for(d, each, 0, INT32_MAX);

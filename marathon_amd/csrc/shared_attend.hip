@@ -331,9 +331,9 @@ int check(const mkv_attend_shared_desc_t& d, GroupedParams* p, Plan* plan) {
   const int64_t new_most = a.max_new > 0 && a.max_new < a.tokens ? a.max_new : a.tokens;
   const int64_t each = new_most * p->group;
   const int64_t rest = (a.tokens - new_most) * p->group;
-  if (each >= 2048 && a.requests > 1 && rest <= 16 * static_cast<int64_t>(a.requests - 1)) {
-    plan->own[0] = shape_for(a, 16, 0, 16);
-    plan->own[1] = shape_for(a, each, 17, INT32_MAX);
+  if (each >= 2048 && a.requests > 1 && rest <= kBesideRows * static_cast<int64_t>(a.requests - 1)) {
+    plan->own[0] = shape_for(a, kBesideRows, 0, kBesideRows);
+    plan->own[1] = shape_for(a, each, kBesideRows + 1, INT32_MAX);
     plan->owns = 2;
   } else {
     plan->own[0] = shape_for(a, each, 0, INT32_MAX);
